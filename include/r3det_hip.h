@@ -620,6 +620,39 @@ int r3det_set_option(const char* name, int value);
  * kernels, their gap included) is the figure that agrees with the profiler's sum. */
 int r3det_fr_profile_read(float* records, int capacity);
 
+/* ---------------------------------------------------------------------------------------
+ * Training: the classification loss of a softmax head
+ * ------------------------------------------------------------------------------------- */
+
+/* element types of the entry points that take more than fp32 */
+#define R3DET_F32 0
+#define R3DET_F16 1
+#define R3DET_BF16 2
+
+/* For each of `rows` rows of `classes` logits (rows `row_stride` elements apart, a row contiguous, 1 <= classes < 2^31):
+ *   log_prob (rows)  the log softmax at the row's label, `labels` int64 (rows) or NULL (then log_prob is not written);
+ *                    0 where has_ignore != 0 and the label is ignore_index; NaN where a label is outside [0, classes);
+ *   entropy (rows) or NULL: -sum p log p;
+ *   top_log_prob, top_index (rows, top_k): the top_k <= min(classes, 64) greatest, best first, ties to the lowest index;
+ *   stats (rows, 2) or NULL: what the gradient needs (the maximum and the log of the sum behind it).
+ * All results fp32 / int64.  A logit of -inf is a class that is not offered; a row with no class left has log_prob and
+ * top_log_prob -inf, entropy 0 and the gradient 0.  A row with NaN or +inf has NaN in place of its numbers (top_index then
+ * holds valid places).
+ * The workspace (r3det_label_log_probs_workspace_bytes; 0 for all but few, long rows) need not be initialised. */
+size_t r3det_label_log_probs_workspace_bytes(int64_t rows, int64_t classes, int top_k);
+int r3det_label_log_probs(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t row_stride,
+                          const int64_t* labels, int64_t ignore_index, int has_ignore, int top_k, float* log_prob,
+                          float* entropy, float* top_log_prob, int64_t* top_index, float* stats, void* ws, size_t ws_bytes,
+                          void* stream);
+
+/* d_logits (rows, classes), contiguous, of the logits' type, from the gradients of log_prob (d_log_prob, needs labels),
+ * entropy (d_entropy, needs entropy) and top_log_prob (d_top (rows, top_k), needs top_index); each may be NULL. */
+int r3det_label_log_probs_backward(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t row_stride,
+                                   const int64_t* labels, int64_t ignore_index, int has_ignore, int top_k,
+                                   const float* stats, const float* entropy, const int64_t* top_index,
+                                   const float* d_log_prob, const float* d_entropy, const float* d_top, void* d_logits,
+                                   void* stream);
+
 #if defined(__GNUC__) || defined(__clang__)
 #pragma GCC visibility pop
 #endif

@@ -841,4 +841,27 @@ int r3det_set_option(const char* name, int value) {
   return R3DET_OK;
 }
 
+size_t r3det_label_log_probs_workspace_bytes(int64_t rows, int64_t classes, int top_k) {
+  return r3k_logprob_workspace_bytes(rows, classes, top_k < 0 ? 0 : top_k);
+}
+
+int r3det_label_log_probs(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t row_stride,
+                          const int64_t* labels, int64_t ignore_index, int has_ignore, int top_k, float* log_prob,
+                          float* entropy, float* top_log_prob, int64_t* top_index, float* stats, void* ws, size_t ws_bytes,
+                          void* stream) {
+  const DeviceGuard guard(stream);
+  return rc(r3k_logprob(logits, dtype, rows, classes, row_stride, labels, ignore_index, has_ignore, top_k, log_prob, entropy,
+                        top_log_prob, top_index, stats, ws, ws_bytes, S(stream)));
+}
+
+int r3det_label_log_probs_backward(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t row_stride,
+                                   const int64_t* labels, int64_t ignore_index, int has_ignore, int top_k,
+                                   const float* stats, const float* entropy, const int64_t* top_index,
+                                   const float* d_log_prob, const float* d_entropy, const float* d_top, void* d_logits,
+                                   void* stream) {
+  const DeviceGuard guard(stream);
+  return rc(r3k_logprob_backward(logits, dtype, rows, classes, row_stride, labels, ignore_index, has_ignore, top_k, stats,
+                                 entropy, top_index, d_log_prob, d_entropy, d_top, d_logits, S(stream)));
+}
+
 }  // extern "C"

@@ -252,3 +252,14 @@ extern R3Option g_r3_iou_qcap;  // 0 default; > 0 caps the IoU pipeline's global
 extern R3Option g_r3_iou_small; // 0 default (513); > 0: column count from which the pipeline runs
 extern R3Option g_r3_nms_impl;  // 0 auto (queue pipeline), 1 tile kernels
 extern R3Option g_r3_nms_qcap;  // 0 default; > 0 caps the global pair queue (tests the overflow path)
+
+// log probabilities of given labels, entropies and best alternatives of rows of logits, and their gradient
+// (train/r3_logprob.hip).  dtype: 0 fp32, 1 fp16, 2 bf16
+size_t r3k_logprob_workspace_bytes(int64_t rows, int64_t classes, int k);
+int r3k_logprob(const void* x, int dtype, int64_t rows, int64_t classes, int64_t stride, const int64_t* labels, int64_t ignore,
+                int has_ignore, int k, float* log_prob, float* entropy, float* top_lp, int64_t* top_ix, float* stats, void* ws,
+                size_t ws_bytes, hipStream_t st);
+int r3k_logprob_backward(const void* x, int dtype, int64_t rows, int64_t classes, int64_t stride, const int64_t* labels,
+                         int64_t ignore, int has_ignore, int k, const float* stats, const float* entropy,
+                         const int64_t* top_ix, const float* d_lp, const float* d_h, const float* d_top, void* dx,
+                         hipStream_t st);

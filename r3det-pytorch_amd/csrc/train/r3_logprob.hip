@@ -1,0 +1,664 @@
+// r3_logprob.hip -- log probabilities of given labels, with the entropy and the best alternatives of every row, and their
+// gradient: what a softmax classification loss is made of.
+//
+// For a row x of `classes` logits, with m = max x:
+//   S = sum_j e^(x_j - m),   T = sum_j e^(x_j - m) (x_j - m)
+//   log p_j = (x_j - m) - log S,   H = -sum_j p_j log p_j = log S - T / S
+//   d x_j = dl [j = label] + sum_k dtop_k [j = top_k] - p_j (dl + sum_k dtop_k + dH (log p_j + H))
+// One pass over the logits forward and one backward: (m, S, T) of two parts join as
+//   m = max(m1, m2),  S = sum_i S_i e^(m_i - m),  T = sum_i e^(m_i - m) (T_i + S_i (m_i - m)),
+// so a lane keeps a running triple and lanes, wavefronts and workgroups join theirs.  Both directions are bound by HBM.
+//
+// All of it in 32 bits.  A difference is held above -150 where it is a FACTOR (e^-150 is 0 in fp32): 0 * -inf would make the
+// entropy NaN for every masked class.  The exponential itself sees the plain difference, so NaN and +inf reach S and T.
+#include <hip/hip_runtime.h>
+
+#include "../r3_kernels.h"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int TOP_MAX = 64;  // a wavefront holds the list of its best, one a lane
+
+template <typename T, int N>
+struct Pack {
+  T v[N];
+};
+// 16 bytes from an address that is aligned to one element only (the row of an odd number of classes): global accesses need
+// no more, and the compiler makes one wide load of it
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
+  Pack<T, N> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+
+// an order of the floats as unsigned numbers; no float is 0 (the key of "nothing"); -0 is +0
+__device__ __forceinline__ unsigned ord(float x) {
+  const unsigned b = __float_as_uint(x + 0.0f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float unord(unsigned u) {
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+// greater = better: by value, then the lowest index
+__device__ __forceinline__ unsigned long long make_key(float x, unsigned index) {
+  return ((unsigned long long)ord(x) << 32) | (unsigned)~index;
+}
+
+struct Stat {  // of the values seen so far
+  float m = -3.402823466e38f, s = 0.f, t = 0.f;
+  __device__ __forceinline__ void raise(float to) {  // the reference point moves up to `to`
+    const float d = m - to;
+    const float r = __builtin_amdgcn_exp2f(d * LOG2E);
+    t = r * (t + fmaxf(d, -150.f) * s);
+    s *= r;
+    m = to;
+  }
+  __device__ __forceinline__ void add(float x) {  // (x <= m)
+    const float d = x - m;
+    const float e = __builtin_amdgcn_exp2f(d * LOG2E);
+    s += e;
+    t = fmaf(e, fmaxf(d, -150.f), t);
+  }
+  __device__ __forceinline__ void join(float m2, float s2, float t2) {
+    Stat o;
+    o.m = m2, o.s = s2, o.t = t2;
+    const float top = fmaxf(m, m2);
+    raise(top);
+    o.raise(top);
+    s += o.s;
+    t += o.t;
+  }
+};
+template <int LANES>
+__device__ __forceinline__ void join_lanes(Stat& a) {
+#pragma unroll
+  for (int o = 1; o < LANES; o <<= 1) a.join(__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.t, o));
+}
+
+struct Out {
+  const int64_t* labels;
+  int64_t ignore;
+  int has_ignore;
+  int k;
+  float* log_prob;
+  float* entropy;
+  float* top_lp;
+  int64_t* top_ix;
+  float* stats;  // (rows, 2): m, log S
+};
+
+// One thread per row: what the row's triple says.  S = 0 only where every class is -inf: log p is -inf there and the
+// entropy 0 (nothing is left to be uncertain about); the backward pass knows such a row by its log S = -inf.
+template <typename T>
+__device__ __forceinline__ void finish_row(const Stat& a, int64_t row, const T* x, int64_t classes, const Out& o, float& m,
+                                           float& ls) {
+  m = a.m;
+  ls = logf(a.s);
+  if (o.stats) {
+    o.stats[2 * row] = m;
+    o.stats[2 * row + 1] = ls;
+  }
+  if (o.entropy) o.entropy[row] = a.s == 0.f ? 0.f : ls - a.t / a.s;
+  if (o.labels) {
+    const int64_t y = o.labels[row];
+    float lp;
+    if (o.has_ignore && y == o.ignore) lp = 0.f;
+    else if (y < 0 || y >= classes) lp = __uint_as_float(0x7fc00000u);  // (a label that is none: NaN, and no read)
+    else lp = a.s == 0.f ? -__builtin_inff() : ((float)x[y] - m) - ls;
+    o.log_prob[row] = lp;
+  }
+}
+__device__ __forceinline__ float top_value(float x, float m, float ls) {
+  return ls == -__builtin_inff() ? -__builtin_inff() : (x - m) - ls;
+}
+
+// ---------------------------------------------------------------------------------------------- few classes
+// LANES neighbouring lanes hold a row in registers, E values a lane.  VEC: 16-byte loads (aligned rows of whole packs).
+// At 16 classes a row is one lane's four 16-byte loads, without an exchange between lanes.
+template <typename T, int LANES, int E, bool VEC>
+__device__ __forceinline__ void load_row(const T* x, int lane, int64_t classes, float (&v)[E], int (&at)[E]) {
+  constexpr int W = VEC ? (E * (int)sizeof(T) < 16 ? E : 16 / (int)sizeof(T)) : 1;
+#pragma unroll
+  for (int c = 0; c < E / W; ++c) {
+    const int i = (c * LANES + lane) * W;
+    if constexpr (VEC) {
+      if (i < classes) {
+        const Pack<T, W> p = load_pack<T, W>(x + i);
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[c * W + j] = (float)p.v[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[c * W + j] = 0.f;
+      }
+    } else {
+      v[c] = i < classes ? (float)x[i] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) at[c * W + j] = i + j;
+  }
+}
+
+template <typename T, int LANES, int E, bool VEC, bool TOP>
+__global__ __launch_bounds__(256) void logprob_small_kernel(const T* __restrict__ logits, int64_t rows, int classes,
+                                                            int64_t stride, Out o) {
+  const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = g / LANES;
+  const int lane = (int)(g % LANES);
+  if (row >= rows) return;  // (whole groups: the exchanges below stay inside a group)
+  const T* x = logits + row * stride;
+  float v[E];
+  int at[E];
+  load_row<T, LANES, E, VEC>(x, lane, classes, v, at);
+  float top = -3.402823466e38f;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (at[e] < classes) top = fmaxf(top, v[e]);
+#pragma unroll
+  for (int d = 1; d < LANES; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  Stat a;
+  a.m = top;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (at[e] < classes) a.add(v[e]);
+#pragma unroll
+  for (int d = 1; d < LANES; d <<= 1) {  // (one reference point for the group: plain sums)
+    a.s += __shfl_xor(a.s, d);
+    a.t += __shfl_xor(a.t, d);
+  }
+  float m = 0.f, ls = 0.f;
+  if (lane == 0) finish_row(a, row, x, classes, o, m, ls);
+  if constexpr (TOP) {
+    unsigned u[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) u[e] = at[e] < classes ? ord(v[e]) : 0u;
+    for (int k = 0; k < o.k; ++k) {
+      unsigned best = 0u;
+      int which = 0x7fffffff;
+#pragma unroll
+      for (int e = 0; e < E; ++e)  // (a lane's places rise with e: the first of equals is the lowest)
+        if (u[e] > best) best = u[e], which = at[e];
+#pragma unroll
+      for (int d = 1; d < LANES; d <<= 1) {
+        const unsigned b2 = __shfl_xor(best, d);
+        const int w2 = __shfl_xor(which, d);
+        if (b2 > best || (b2 == best && w2 < which)) best = b2, which = w2;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (at[e] == which) u[e] = 0u;
+      if (lane == 0) {
+        o.top_lp[row * o.k + k] = top_value(unord(best), m, ls);
+        o.top_ix[row * o.k + k] = which;
+      }
+    }
+  }
+}
+
+template <typename T, int LANES, int E, bool VEC>
+__global__ __launch_bounds__(256) void logprob_small_backward_kernel(const T* __restrict__ logits, int64_t rows, int classes,
+                                                                     int64_t stride, Out o, const float* __restrict__ d_lp,
+                                                                     const float* __restrict__ d_h,
+                                                                     const float* __restrict__ d_top, T* __restrict__ dx) {
+  constexpr int W = VEC ? (E * (int)sizeof(T) < 16 ? E : 16 / (int)sizeof(T)) : 1;
+  const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = g / LANES;
+  const int lane = (int)(g % LANES);
+  if (row >= rows) return;
+  float v[E];
+  int at[E];
+  load_row<T, LANES, E, VEC>(logits + row * stride, lane, classes, v, at);
+  const float m = o.stats[2 * row], ls = o.stats[2 * row + 1];
+  const bool empty = ls == -__builtin_inff();
+  int64_t y = -1;
+  float dl = 0.f, sum = 0.f, dh = 0.f, h = 0.f;
+  if (d_lp) {
+    y = o.labels[row];
+    dl = d_lp[row];
+    if (o.has_ignore && y == o.ignore) y = -1, dl = 0.f;
+    else if (y < 0 || y >= classes) y = -1, dl = __uint_as_float(0x7fc00000u);
+    sum = dl;
+  }
+  if (d_h) dh = d_h[row], h = o.entropy[row];
+  if (d_top)
+    for (int k = 0; k < o.k; ++k) sum += d_top[row * o.k + k];
+  float r[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float lp = (v[e] - m) - ls, p = __builtin_amdgcn_exp2f(lp * LOG2E);
+    r[e] = (at[e] == y ? dl : 0.f) - p * (sum + dh * (fmaxf(lp, -150.f) + h));
+  }
+  if (d_top)
+    for (int k = 0; k < o.k; ++k) {
+      const int64_t ix = o.top_ix[row * o.k + k];
+      const float d = d_top[row * o.k + k];
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (at[e] == ix) r[e] += d;
+    }
+  T* out = dx + row * (int64_t)classes;
+#pragma unroll
+  for (int c = 0; c < E / W; ++c) {
+    if (at[c * W] < classes) {
+      Pack<T, W> p;
+#pragma unroll
+      for (int j = 0; j < W; ++j) p.v[j] = (T)(empty ? 0.f : r[c * W + j]);
+      __builtin_memcpy(out + at[c * W], &p, sizeof(p));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- many classes
+// The best keys a wavefront has seen, sorted, one a lane.
+struct Best {
+  unsigned long long key = 0;
+  unsigned long long least = 0;  // the k-th best (uniform): what a key has to pass
+  float floor = -__builtin_inff();  // its value
+  __device__ __forceinline__ void insert(unsigned long long in, int k) {  // `in` uniform
+    const unsigned lo = (unsigned)key, hi = (unsigned)(key >> 32);
+    // lane i takes lane i - 1's (wave_shr:1); lane 0 keeps its own, which the comparison below sees as "not better"
+    const unsigned plo = __builtin_amdgcn_update_dpp(0xffffffffu, lo, 0x138, 0xf, 0xf, false);
+    const unsigned phi = __builtin_amdgcn_update_dpp(0xffffffffu, hi, 0x138, 0xf, 0xf, false);
+    const unsigned long long prev = ((unsigned long long)phi << 32) | plo;
+    key = key > in ? key : (prev > in ? in : prev);
+    lo_hi(k);
+  }
+  __device__ __forceinline__ void lo_hi(int k) {
+    const unsigned lo = __builtin_amdgcn_readlane((unsigned)key, k - 1);
+    const unsigned hi = __builtin_amdgcn_readlane((unsigned)(key >> 32), k - 1);
+    least = ((unsigned long long)hi << 32) | lo;
+    floor = hi ? unord(hi) : -__builtin_inff();
+  }
+  // every lane offers one key (0: none); all lanes of the wavefront call
+  __device__ __forceinline__ void offer(unsigned long long in, int k) {
+    unsigned long long who = __ballot(in > least);
+    while (who) {
+      const int l = __builtin_ctzll(who);
+      const unsigned lo = __builtin_amdgcn_readlane((unsigned)in, l), hi = __builtin_amdgcn_readlane((unsigned)(in >> 32), l);
+      insert(((unsigned long long)hi << 32) | lo, k);
+      if ((int)__lane_id() == l) in = 0;
+      who = __ballot(in > least);
+    }
+  }
+};
+
+// The wavefronts' lists in shared memory: each key that is among the k best goes to its rank (keys differ: each holds its
+// place in the row).  k <= 64 and at most 16 lists: at most 1024 comparisons a thread, all reading one address.
+template <int THREADS, typename F>
+__device__ __forceinline__ void write_best(const unsigned long long* lists, int n, int k, const F& write) {
+  for (int q = threadIdx.x; q < n; q += THREADS) {
+    const unsigned long long mine = lists[q];
+    if (mine == 0) continue;
+    int rank = 0;
+    for (int r = 0; r < n; ++r) rank += lists[r] > mine;
+    if (rank < k) write(rank, mine);
+  }
+}
+
+constexpr int UNROLL = 4;  // packs of a lane in flight
+
+// WAVES wavefronts walk [from, to) of a row together (WAVES = 1: four rows a workgroup, a wavefront each).
+// split > 1: a row is walked by `split` workgroups, whose triples and keys go to `part` for logprob_join_kernel.
+template <typename T, int WAVES, bool TOP>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprob_row_kernel(const T* __restrict__ logits, int64_t rows,
+                                                                                    int64_t classes, int64_t stride, int split,
+                                                                                    int64_t span, float* __restrict__ part,
+                                                                                    unsigned long long* __restrict__ part_keys,
+                                                                                    Out o) {
+  constexpr int W = 16 / (int)sizeof(T);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  int64_t row;
+  int s = 0;
+  if constexpr (WAVES == 1) {
+    row = (int64_t)blockIdx.x * 4 + wave;
+    if (row >= rows) return;
+  } else {
+    row = blockIdx.x / (unsigned)split;
+    s = (int)(blockIdx.x % (unsigned)split);
+  }
+  const int64_t from = s * span, to = from + span < classes ? from + span : classes;
+  const T* x = logits + row * stride;
+  const int64_t packs = (to - from) / W;
+  const int first = WAVES == 1 ? 0 : wave * 64;
+  Stat a;
+  Best best;
+  for (int64_t c = first; c < packs; c += (int64_t)WAVES * 64 * UNROLL) {
+    Pack<T, W> p[UNROLL];
+    float top = a.m;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int64_t i = c + (int64_t)u * WAVES * 64 + lane;
+      if (i < packs) p[u] = load_pack<T, W>(x + from + i * W);
+      else
+#pragma unroll
+        for (int j = 0; j < W; ++j) p[u].v[j] = (T)-__builtin_inff();
+    }
+    float high[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      high[u] = (float)p[u].v[0];
+#pragma unroll
+      for (int j = 1; j < W; ++j) high[u] = fmaxf(high[u], (float)p[u].v[j]);
+      top = fmaxf(top, high[u]);
+    }
+    a.raise(top);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int j = 0; j < W; ++j) a.add((float)p[u].v[j]);
+    if constexpr (TOP) {
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const int64_t i = c + (int64_t)u * WAVES * 64 + lane;
+        if (__ballot(i < packs && !(high[u] < best.floor))) {  // (equal: a lower place may still come in)
+#pragma unroll
+          for (int j = 0; j < W; ++j)
+            best.offer(i < packs ? make_key((float)p[u].v[j], (unsigned)(from + i * W + j)) : 0ull, o.k);
+        }
+      }
+    }
+  }
+  {  // the elements behind the last whole pack: the first wavefront's
+    const int64_t i = from + packs * W + lane;
+    if (first == 0) {
+      const bool in = lane < W && i < to;
+      const float v = in ? (float)x[i] : 0.f;
+      if (in) {
+        a.raise(fmaxf(a.m, v));
+        a.add(v);
+      }
+      if constexpr (TOP) best.offer(in ? make_key(v, (unsigned)i) : 0ull, o.k);
+    }
+  }
+  join_lanes<64>(a);
+  if constexpr (WAVES == 1) {
+    float m = 0.f, ls = 0.f;
+    if (lane == 0) finish_row(a, row, x, classes, o, m, ls);
+    if constexpr (TOP) {
+      m = __shfl(m, 0);
+      ls = __shfl(ls, 0);
+      if (lane < o.k) {
+        o.top_lp[row * o.k + lane] = top_value(unord((unsigned)(best.key >> 32)), m, ls);
+        o.top_ix[row * o.k + lane] = (int64_t)(unsigned)~(unsigned)best.key;
+      }
+    }
+  } else {
+    __shared__ float sh[WAVES][3];
+    __shared__ float done[2];
+    __shared__ unsigned long long keys[TOP ? WAVES * TOP_MAX : 1];
+    if (lane == 0) sh[wave][0] = a.m, sh[wave][1] = a.s, sh[wave][2] = a.t;
+    if constexpr (TOP)
+      if (lane < o.k) keys[wave * o.k + lane] = best.key;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < WAVES; ++w) a.join(sh[w][0], sh[w][1], sh[w][2]);
+      if (split > 1) {
+        float* q = part + 3 * (row * split + s);
+        q[0] = a.m, q[1] = a.s, q[2] = a.t;
+      } else {
+        float m, ls;
+        finish_row(a, row, x, classes, o, m, ls);
+        done[0] = m, done[1] = ls;
+      }
+    }
+    if constexpr (TOP) {
+      __syncthreads();
+      write_best<WAVES * 64>(keys, WAVES * o.k, o.k, [&](int rank, unsigned long long mine) {
+        if (split > 1) part_keys[(row * split + s) * o.k + rank] = mine;
+        else {
+          o.top_lp[row * o.k + rank] = top_value(unord((unsigned)(mine >> 32)), done[0], done[1]);
+          o.top_ix[row * o.k + rank] = (int64_t)(unsigned)~(unsigned)mine;
+        }
+      });
+    }
+  }
+}
+
+// The parts of one row a workgroup: the triples in a fixed order; the keys through four wavefronts' lists, then by rank.
+// (Every part has at least TOP_MAX elements, so all its k keys were written.)
+template <typename T, bool TOP>
+__global__ __launch_bounds__(256) void logprob_join_kernel(const T* __restrict__ logits, int64_t rows, int64_t classes,
+                                                           int64_t stride, int split, const float* __restrict__ part,
+                                                           const unsigned long long* __restrict__ part_keys, Out o) {
+  __shared__ float done[2];
+  const int64_t row = blockIdx.x;
+  if (threadIdx.x < 64) {
+    Stat a;
+    for (int s = threadIdx.x; s < split; s += 64) {
+      const float* q = part + 3 * (row * split + s);
+      a.join(q[0], q[1], q[2]);
+    }
+    join_lanes<64>(a);
+    if (threadIdx.x == 0) {
+      float m, ls;
+      finish_row(a, row, logits + row * stride, classes, o, m, ls);
+      done[0] = m, done[1] = ls;
+    }
+  }
+  if constexpr (TOP) {
+    __shared__ unsigned long long lists[4 * TOP_MAX];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = split * o.k;
+    const unsigned long long* keys = part_keys + row * n;
+    Best best;
+    for (int q = wave * 64; q < n; q += 256) best.offer(q + lane < n ? keys[q + lane] : 0ull, o.k);
+    if (lane < o.k) lists[wave * o.k + lane] = best.key;
+    __syncthreads();
+    write_best<256>(lists, 4 * o.k, o.k, [&](int rank, unsigned long long mine) {
+      o.top_lp[row * o.k + rank] = top_value(unord((unsigned)(mine >> 32)), done[0], done[1]);
+      o.top_ix[row * o.k + rank] = (int64_t)(unsigned)~(unsigned)mine;
+    });
+  }
+}
+
+// LANES lanes walk a row's segment; the gradient's own pack holds what a lane read, so a row is read once and written once.
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void logprob_row_backward_kernel(const T* __restrict__ logits, int64_t rows, int64_t classes,
+                                                                   int64_t stride, int split, int64_t span, Out o,
+                                                                   const float* __restrict__ d_lp,
+                                                                   const float* __restrict__ d_h,
+                                                                   const float* __restrict__ d_top, T* __restrict__ dx) {
+  constexpr int W = 16 / (int)sizeof(T), ROWS = 256 / LANES;
+  const int lane = threadIdx.x % LANES;
+  const int64_t row = (int64_t)(blockIdx.x / (unsigned)split) * ROWS + threadIdx.x / LANES;
+  const int s = (int)(blockIdx.x % (unsigned)split);
+  if (row >= rows) return;
+  const int64_t from = s * span, to = from + span < classes ? from + span : classes;
+  const T* x = logits + row * stride;
+  T* out = dx + row * classes;
+  const float m = o.stats[2 * row], ls = o.stats[2 * row + 1];
+  const bool empty = ls == -__builtin_inff();
+  int64_t y = -1;
+  float dl = 0.f, sum = 0.f, dh = 0.f, h = 0.f;
+  if (d_lp) {
+    y = o.labels[row];
+    dl = d_lp[row];
+    if (o.has_ignore && y == o.ignore) y = -1, dl = 0.f;
+    else if (y < 0 || y >= classes) y = -1, dl = __uint_as_float(0x7fc00000u);
+    sum = dl;
+  }
+  if (d_h) dh = d_h[row], h = o.entropy[row];
+  if (d_top)
+    for (int k = 0; k < o.k; ++k) sum += d_top[row * o.k + k];
+  const auto one = [&](float v, int64_t at) {
+    const float lp = (v - m) - ls, p = __builtin_amdgcn_exp2f(lp * LOG2E);
+    float r = (at == y ? dl : 0.f) - p * (sum + dh * (fmaxf(lp, -150.f) + h));
+    if (d_top)
+      for (int k = 0; k < o.k; ++k)
+        if (o.top_ix[row * o.k + k] == at) r += d_top[row * o.k + k];
+    return (T)(empty ? 0.f : r);
+  };
+  const int64_t packs = (to - from) / W;
+  for (int64_t c = lane; c < packs; c += LANES * UNROLL) {
+    Pack<T, W> p[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (c + u * LANES < packs) p[u] = load_pack<T, W>(x + from + (c + u * LANES) * W);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (c + u * LANES < packs) {
+        const int64_t at = from + (c + u * LANES) * W;
+#pragma unroll
+        for (int j = 0; j < W; ++j) p[u].v[j] = one((float)p[u].v[j], at + j);
+        __builtin_memcpy(out + at, &p[u], sizeof(p[u]));
+      }
+  }
+  const int64_t i = from + packs * W + lane;
+  if (i < to) out[i] = one((float)x[i], i);  // (LANES >= W: one round)
+}
+
+// ---------------------------------------------------------------------------------------------- launches
+constexpr int SMALL_MAX = 128;     // classes whose row lanes hold in registers
+constexpr int WAVE_MAX = 4096;     // classes that one wavefront walks
+constexpr int64_t PART = 16384;    // classes a workgroup walks at least, where a row is split
+
+int row_split(int64_t rows, int64_t classes) {
+  if (classes <= WAVE_MAX) return 1;
+  const int64_t want = 2ll * r3_cu_count();  // workgroups that fill the card
+  int64_t s = want / rows;
+  if (s > classes / PART) s = classes / PART;
+  return s < 1 ? 1 : (s > 256 ? 256 : (int)s);
+}
+int64_t row_span(int64_t classes, int split) {  // (whole packs of 8)
+  return ((classes + split - 1) / split + 7) / 8 * 8;
+}
+
+template <typename T, int LANES, int E>
+int small_forward(const T* x, int64_t rows, int classes, int64_t stride, const Out& o, hipStream_t st) {
+  const int64_t blocks = (rows * LANES + 255) / 256;
+  if (blocks > 0x7fffffff) return -1;
+  const int w = E * (int)sizeof(T) < 16 ? E : 16 / (int)sizeof(T);
+  const bool vec = classes % w == 0;
+  const dim3 g((unsigned)blocks), b(256);
+  if (vec) {
+    if (o.k) hipLaunchKernelGGL((logprob_small_kernel<T, LANES, E, true, true>), g, b, 0, st, x, rows, classes, stride, o);
+    else hipLaunchKernelGGL((logprob_small_kernel<T, LANES, E, true, false>), g, b, 0, st, x, rows, classes, stride, o);
+  } else {
+    if (o.k) hipLaunchKernelGGL((logprob_small_kernel<T, LANES, E, false, true>), g, b, 0, st, x, rows, classes, stride, o);
+    else hipLaunchKernelGGL((logprob_small_kernel<T, LANES, E, false, false>), g, b, 0, st, x, rows, classes, stride, o);
+  }
+  return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+template <typename T, int LANES, int E>
+int small_backward(const T* x, int64_t rows, int classes, int64_t stride, const Out& o, const float* d_lp, const float* d_h,
+                   const float* d_top, T* dx, hipStream_t st) {
+  const int64_t blocks = (rows * LANES + 255) / 256;
+  if (blocks > 0x7fffffff) return -1;
+  const int w = E * (int)sizeof(T) < 16 ? E : 16 / (int)sizeof(T);
+  const dim3 g((unsigned)blocks), b(256);
+  if (classes % w == 0)
+    hipLaunchKernelGGL((logprob_small_backward_kernel<T, LANES, E, true>), g, b, 0, st, x, rows, classes, stride, o, d_lp, d_h,
+                       d_top, dx);
+  else
+    hipLaunchKernelGGL((logprob_small_backward_kernel<T, LANES, E, false>), g, b, 0, st, x, rows, classes, stride, o, d_lp, d_h,
+                       d_top, dx);
+  return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+
+template <typename T, int WAVES>
+int row_forward(const T* x, int64_t rows, int64_t classes, int64_t stride, int split, float* part, unsigned long long* keys,
+                const Out& o, hipStream_t st) {
+  const int64_t blocks = WAVES == 1 ? (rows + 3) / 4 : rows * split;
+  if (blocks > 0x7fffffff) return -1;
+  const dim3 g((unsigned)blocks), b(WAVES == 1 ? 256 : WAVES * 64);
+  const int64_t span = row_span(classes, split);
+  if (o.k)
+    hipLaunchKernelGGL((logprob_row_kernel<T, WAVES, true>), g, b, 0, st, x, rows, classes, stride, split, span, part, keys, o);
+  else
+    hipLaunchKernelGGL((logprob_row_kernel<T, WAVES, false>), g, b, 0, st, x, rows, classes, stride, split, span, part, keys, o);
+  if (hipGetLastError() != hipSuccess) return -2;
+  if (split > 1) {
+    if (o.k)
+      hipLaunchKernelGGL((logprob_join_kernel<T, true>), dim3((unsigned)rows), dim3(256), 0, st, x, rows, classes, stride,
+                         split, part, keys, o);
+    else
+      hipLaunchKernelGGL((logprob_join_kernel<T, false>), dim3((unsigned)rows), dim3(256), 0, st, x, rows, classes, stride,
+                         split, part, keys, o);
+    if (hipGetLastError() != hipSuccess) return -2;
+  }
+  return 0;
+}
+
+template <typename T>
+int forward(const T* x, int64_t rows, int64_t classes, int64_t stride, const Out& o, void* ws, hipStream_t st) {
+  const int c = (int)classes;
+  if (c <= 4) return small_forward<T, 1, 4>(x, rows, c, stride, o, st);
+  if (c <= 16) return small_forward<T, 1, 16>(x, rows, c, stride, o, st);
+  if (c <= 32) return small_forward<T, 2, 16>(x, rows, c, stride, o, st);
+  if (c <= 64) return small_forward<T, 4, 16>(x, rows, c, stride, o, st);
+  if (c <= SMALL_MAX) return small_forward<T, 8, 16>(x, rows, c, stride, o, st);
+  if (c <= WAVE_MAX) return row_forward<T, 1>(x, rows, classes, stride, 1, nullptr, nullptr, o, st);
+  const int split = row_split(rows, classes);
+  unsigned long long* keys = static_cast<unsigned long long*>(ws);
+  float* part = reinterpret_cast<float*>(keys + (size_t)rows * split * o.k);
+  if (rows * split <= r3_cu_count()) return row_forward<T, 16>(x, rows, classes, stride, split, part, keys, o, st);
+  return row_forward<T, 4>(x, rows, classes, stride, split, part, keys, o, st);
+}
+
+template <typename T>
+int backward(const T* x, int64_t rows, int64_t classes, int64_t stride, const Out& o, const float* d_lp, const float* d_h,
+             const float* d_top, T* dx, hipStream_t st) {
+  const int c = (int)classes;
+  if (c <= 4) return small_backward<T, 1, 4>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
+  if (c <= 16) return small_backward<T, 1, 16>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
+  if (c <= 32) return small_backward<T, 2, 16>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
+  if (c <= 64) return small_backward<T, 4, 16>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
+  if (c <= SMALL_MAX) return small_backward<T, 8, 16>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
+  if (c <= WAVE_MAX) {
+    const int64_t blocks = (rows + 3) / 4;
+    if (blocks > 0x7fffffff) return -1;
+    hipLaunchKernelGGL((logprob_row_backward_kernel<T, 64>), dim3((unsigned)blocks), dim3(256), 0, st, x, rows, classes, stride,
+                       1, classes, o, d_lp, d_h, d_top, dx);
+  } else {
+    int64_t split = (classes + 16383) / 16384;
+    if (rows * split > 0x7fffffff) split = 1;
+    if (rows > 0x7fffffff) return -1;
+    hipLaunchKernelGGL((logprob_row_backward_kernel<T, 256>), dim3((unsigned)(rows * split)), dim3(256), 0, st, x, rows,
+                       classes, stride, (int)split, row_span(classes, (int)split), o, d_lp, d_h, d_top, dx);
+  }
+  return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+
+}  // namespace
+
+size_t r3k_logprob_workspace_bytes(int64_t rows, int64_t classes, int k) {
+  if (rows <= 0 || classes <= WAVE_MAX) return 0;
+  const int split = row_split(rows, classes);
+  return split == 1 ? 0 : (size_t)rows * split * (3 * sizeof(float) + k * sizeof(unsigned long long));
+}
+
+int r3k_logprob(const void* x, int dtype, int64_t rows, int64_t classes, int64_t stride, const int64_t* labels, int64_t ignore,
+                int has_ignore, int k, float* log_prob, float* entropy, float* top_lp, int64_t* top_ix, float* stats, void* ws,
+                size_t ws_bytes, hipStream_t st) {
+  if (rows < 0 || classes < 1 || classes > 0x7fffffff || k < 0 || k > TOP_MAX || k > classes || dtype < 0 || dtype > 2) return -1;
+  if (rows == 0) return 0;
+  if (rows > (1ll << 40) || !x || stride < 0 || (labels && !log_prob) || (k && (!top_lp || !top_ix))) return -1;
+  const size_t need = r3k_logprob_workspace_bytes(rows, classes, k);
+  if (need && (!ws || ws_bytes < need)) return -3;
+  const Out o{labels, ignore, has_ignore, k, log_prob, entropy, top_lp, top_ix, stats};
+  switch (dtype) {
+    case 0: return forward(static_cast<const float*>(x), rows, classes, stride, o, ws, st);
+    case 1: return forward(static_cast<const _Float16*>(x), rows, classes, stride, o, ws, st);
+    default: return forward(static_cast<const __bf16*>(x), rows, classes, stride, o, ws, st);
+  }
+}
+
+int r3k_logprob_backward(const void* x, int dtype, int64_t rows, int64_t classes, int64_t stride, const int64_t* labels,
+                         int64_t ignore, int has_ignore, int k, const float* stats, const float* entropy,
+                         const int64_t* top_ix, const float* d_lp, const float* d_h, const float* d_top, void* dx,
+                         hipStream_t st) {
+  if (rows < 0 || classes < 1 || classes > 0x7fffffff || k < 0 || k > TOP_MAX || k > classes || dtype < 0 || dtype > 2) return -1;
+  if (rows == 0) return 0;
+  if (rows > (1ll << 40) || !x || stride < 0 || !stats || !dx || (d_lp && !labels) || (d_h && !entropy) || (d_top && (!k || !top_ix)))
+    return -1;
+  const Out o{labels, ignore, has_ignore, k, nullptr, const_cast<float*>(entropy), nullptr, const_cast<int64_t*>(top_ix),
+              const_cast<float*>(stats)};
+  switch (dtype) {
+    case 0:
+      return backward(static_cast<const float*>(x), rows, classes, stride, o, d_lp, d_h, d_top, static_cast<float*>(dx), st);
+    case 1:
+      return backward(static_cast<const _Float16*>(x), rows, classes, stride, o, d_lp, d_h, d_top, static_cast<_Float16*>(dx), st);
+    default:
+      return backward(static_cast<const __bf16*>(x), rows, classes, stride, o, d_lp, d_h, d_top, static_cast<__bf16*>(dx), st);
+  }
+}
