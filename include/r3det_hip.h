@@ -653,6 +653,30 @@ int r3det_label_log_probs_backward(const void* logits, int dtype, int64_t rows, 
                                    const float* d_log_prob, const float* d_entropy, const float* d_top, void* d_logits,
                                    void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Training: orthogonalised updates of weight matrices
+ * ------------------------------------------------------------------------------------- */
+
+/* Newton-Schulz products for `count` matrices at once.  For each matrix G (rows[i] x cols[i], contiguous, of type dtype;
+ * at least 1 x 1, at most 2^31 - 1 elements, the smaller side at most 32768):
+ *   X = G / (|G|_F + eps), then `steps` (1 .. 64) times  A = X X^t,  X <- a X + (b A + c A A) X   (for rows > cols: of G^t);
+ * dst[i] (rows x cols, contiguous, of the same type; may be src[i]) receives X.  All in fp32 accuracy whatever the type.
+ * The arrays of pointers and sizes are HOST arrays and are read before the call returns.  The coefficients have to keep
+ * the singular values, the entries of X, A and b A + c A A, below 15 for every s in [0, 1]
+ * (r3det_orthogonalize returns R3DET_EINVAL otherwise).  A workspace of r3det_orthogonalize_workspace_bytes (0: a shape that
+ * is not taken, or no matrix), 16-byte aligned, need not be initialised. */
+size_t r3det_orthogonalize_workspace_bytes(int count, const int* rows, const int* cols);
+int r3det_orthogonalize(int count, const void* const* src, void* const* dst, int dtype, const int* rows, const int* cols,
+                        int steps, float a, float b, float c, double eps, void* ws, size_t ws_bytes, void* stream);
+
+/* One optimiser step around it, per matrix:
+ *   buf <- momentum * buf + grad;   u = nesterov ? grad + momentum * buf : buf;
+ *   weight <- decay * weight - rates[i] * X(u)
+ * grads and weights of type dtype, buf fp32, all contiguous and alike in shape; no two of the pointers may overlap. */
+int r3det_orthogonal_update(int count, const void* const* grads, void* const* weights, float* const* bufs, int dtype,
+                            const int* rows, const int* cols, const float* rates, float decay, float momentum, int nesterov,
+                            int steps, float a, float b, float c, double eps, void* ws, size_t ws_bytes, void* stream);
+
 #if defined(__GNUC__) || defined(__clang__)
 #pragma GCC visibility pop
 #endif

@@ -864,4 +864,24 @@ int r3det_label_log_probs_backward(const void* logits, int dtype, int64_t rows, 
                                  entropy, top_index, d_log_prob, d_entropy, d_top, d_logits, S(stream)));
 }
 
+size_t r3det_orthogonalize_workspace_bytes(int count, const int* rows, const int* cols) {
+  return r3k_ortho_workspace_bytes(count, rows, cols);
+}
+
+int r3det_orthogonalize(int count, const void* const* src, void* const* dst, int dtype, const int* rows, const int* cols,
+                        int steps, float a, float b, float c, double eps, void* ws, size_t ws_bytes, void* stream) {
+  const DeviceGuard guard(stream);
+  return rc(r3k_ortho(count, src, dst, nullptr, dtype, rows, cols, nullptr, 1.f, 0.f, 0, steps, a, b, c, eps, ws, ws_bytes,
+                      S(stream)));
+}
+
+int r3det_orthogonal_update(int count, const void* const* grads, void* const* weights, float* const* bufs, int dtype,
+                            const int* rows, const int* cols, const float* rates, float decay, float momentum, int nesterov,
+                            int steps, float a, float b, float c, double eps, void* ws, size_t ws_bytes, void* stream) {
+  const DeviceGuard guard(stream);
+  if (count > 0 && (!bufs || !rates)) return R3DET_EINVAL;
+  return rc(r3k_ortho(count, grads, weights, bufs, dtype, rows, cols, rates, decay, momentum, nesterov, steps, a, b, c, eps,
+                      ws, ws_bytes, S(stream)));
+}
+
 }  // extern "C"

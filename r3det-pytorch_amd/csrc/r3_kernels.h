@@ -263,3 +263,9 @@ int r3k_logprob_backward(const void* x, int dtype, int64_t rows, int64_t classes
                          int64_t ignore, int has_ignore, int k, const float* stats, const float* entropy,
                          const int64_t* top_ix, const float* d_lp, const float* d_h, const float* d_top, void* dx,
                          hipStream_t st);
+
+// orthogonalised updates of a list of matrices (train/r3_ortho.hip); buf null: dst <- the orthogonalised src
+size_t r3k_ortho_workspace_bytes(int count, const int* rows, const int* cols);
+int r3k_ortho(int count, const void* const* src, void* const* dst, float* const* buf, int dtype, const int* rows,
+              const int* cols, const float* rates, float decay, float mu, int nesterov, int steps, float a, float b, float c,
+              double eps, void* ws, size_t ws_bytes, hipStream_t st);

@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("R3DET_HIP_LIB") or os.path.join(os.path.dirname(_HERE), "libr3det_hip.so")
 
 _vp, _i, _f, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
-_i64 = ctypes.c_int64
+_i64, _d = ctypes.c_int64, ctypes.c_double
 
 # name -> argtypes; the list doubles as the export table checked by tests/test_abi.py
 SIGNATURES = {
@@ -80,6 +80,8 @@ SIGNATURES = {
     "r3det_feature_refine_backward_levels_indexed": [_i, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _vp, _sz, _vp],
     "r3det_label_log_probs": [_vp, _i, _i64, _i64, _i64, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
     "r3det_label_log_probs_backward": [_vp, _i, _i64, _i64, _i64, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "r3det_orthogonalize": [_i, _vp, _vp, _i, _vp, _vp, _i, _f, _f, _f, _d, _vp, _sz, _vp],
+    "r3det_orthogonal_update": [_i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _f, _f, _i, _i, _f, _f, _f, _d, _vp, _sz, _vp],
     "r3det_set_option": [ctypes.c_char_p, _i],
     "r3det_fr_profile_read": [_vp, _i],
 }
@@ -140,6 +142,8 @@ def lib():
         L.r3det_iou_workspace_bytes.restype = _sz
         L.r3det_label_log_probs_workspace_bytes.argtypes = [_i64, _i64, _i]
         L.r3det_label_log_probs_workspace_bytes.restype = _sz
+        L.r3det_orthogonalize_workspace_bytes.argtypes = [_i, _vp, _vp]
+        L.r3det_orthogonalize_workspace_bytes.restype = _sz
         L.r3det_error_string.argtypes = [_i]
         L.r3det_error_string.restype = ctypes.c_char_p
         L.r3det_abi_version.restype = _i

@@ -1,0 +1,162 @@
+"""Orthogonalised updates of weight matrices by Newton-Schulz products (include/r3det_hip.h: r3det_orthogonalize,
+r3det_orthogonal_update), for a ragged list of matrices in one chain of launches.
+
+Not one of the reference's extension ops: it serves the training step's optimiser (``dist_train.Muon``).  A weight of more
+than two dimensions is the matrix of its first dimension against all others, as for a convolution's (out, in * kh * kw).
+"""
+import ctypes
+import math
+
+import torch
+
+from .. import _C
+from .log_probs import DTYPES
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+STEPS = 5
+
+
+def _numbers(steps, coefficients, eps):
+    if isinstance(steps, bool) or not isinstance(steps, int) or not 1 <= steps <= 64:
+        raise ValueError(f"steps must be an integer between 1 and 64, got {steps!r}")
+    a, b, c = (float(v) for v in coefficients)
+    if not float(eps) >= 0:
+        raise ValueError(f"eps must not be negative, got {eps!r}")
+    return steps, a, b, c, float(eps)
+
+
+def _check(t, name, like=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t)}")
+    if t.dim() < 2:
+        raise ValueError(f"{name} must have at least two dimensions, got {t.dim()}")
+    if like is not None and (t.shape != like.shape or t.device != like.device):
+        raise ValueError(f"{name} must match its weight: {tuple(t.shape)} on {t.device} against {tuple(like.shape)} on {like.device}")
+
+
+def _same(ts, name):
+    if ts and ts[0].dtype not in DTYPES:
+        raise RuntimeError(f"{name} must be fp32, fp16 or bf16, got {ts[0].dtype}")
+    for t in ts:
+        if t.dtype != ts[0].dtype or t.device != ts[0].device:
+            raise RuntimeError(f"{name} must be of one type and on one device")
+        rows, cols = t.size(0), t.numel() // max(t.size(0), 1)
+        if t.numel() >= 2 ** 31 or min(rows, cols) > 32768:
+            raise ValueError(f"{name}: a matrix of {rows} x {cols} is not taken (at most 2^31 - 1 elements, 32768 on the smaller side)")
+    for t in ts:
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must be CUDA tensors (HIP device tensors on ROCm)")
+
+
+def _pointers(ts):
+    return (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
+
+
+def _sizes(ts):
+    rows = [t.size(0) for t in ts]
+    make = ctypes.c_int * len(ts)
+    return make(*rows), make(*[t.numel() // r for t, r in zip(ts, rows)])
+
+
+def _workspace(count, rows, cols, device):
+    n = int(_C.lib().r3det_orthogonalize_workspace_bytes(count, rows, cols))
+    return torch.empty(n, dtype=torch.uint8, device=device), n
+
+
+@torch.no_grad()
+def orthogonalize(tensors, steps=STEPS, coefficients=COEFFICIENTS, eps=1e-7):
+    """One matrix or a list of matrices (fp32, fp16 or bf16, all alike; more than two dimensions: (size(0), rest)) ->
+    new, contiguous tensors of the same shapes and type: ``X = G / (|G| + eps)``, then ``steps`` times
+    ``X = a X + (b A + c A A) X`` with ``A = X X^t`` (of the transpose where there are more rows than columns), which moves
+    every singular value towards 1 and keeps the singular vectors.  Computed to fp32's accuracy whatever the type, and
+    rounded once.  A zero matrix stays zero; NaN or an infinity in a matrix makes that matrix NaN and no other.  The
+    coefficients must keep all iterates below 15 (RuntimeError otherwise).  No gradient flows through it.  Runs on the
+    current stream of the tensors' device, without a host synchronisation."""
+    one = isinstance(tensors, torch.Tensor)
+    ts = [tensors] if one else list(tensors)
+    steps, a, b, c, eps = _numbers(steps, coefficients, eps)
+    for t in ts:
+        _check(t, "tensors")
+    _same(ts, "tensors")
+    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in ts]
+    live = [(t.contiguous(), o) for t, o in zip(ts, outs) if t.numel()]
+    if live:
+        src, dst = [p[0] for p in live], [p[1] for p in live]
+        rows, cols = _sizes(src)
+        with torch.cuda.device(src[0].device):
+            ws, n = _workspace(len(src), rows, cols, src[0].device)
+            _C.check(_C.lib().r3det_orthogonalize(len(src), _pointers(src), _pointers(dst), DTYPES[src[0].dtype], rows, cols,
+                                                  steps, a, b, c, eps, _C.ptr(ws), n, _C.stream()), "r3det_orthogonalize")
+    return outs[0] if one else outs
+
+
+def _layout(t):
+    """The strides that say something (a dimension of size one has any)."""
+    return [s for s, n in zip(t.stride(), t.shape) if n > 1]
+
+
+def _dense(t):
+    """Whether the tensor's memory, read in order, is (size(0), rest) in some order of the rest -- contiguous, or a
+    channels_last convolution weight.  The order of the columns does not matter to the update as long as the weight,
+    its gradient and its momentum have the same one."""
+    if t.is_contiguous():
+        return True
+    return t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)
+
+
+@torch.no_grad()
+def orthogonal_update_(params, grads, buffers, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=STEPS,
+                       coefficients=COEFFICIENTS, eps=1e-7, scale="rms"):
+    """One optimiser step for a list of weights, in place, per weight W with gradient G and momentum M:
+
+        M = momentum * M + G;   U = G + momentum * M (nesterov) or M
+        W = (1 - lr * weight_decay) * W - lr * s * orthogonalize(U)
+
+    with ``s = 0.2 sqrt(max(rows, cols))`` for ``scale="rms"`` (the update's entries are then of about the size of an adaptive
+    optimiser's) or ``sqrt(max(1, rows / cols))`` for ``"spectral"``, or a number.  ``params`` and ``grads`` fp32, fp16 or bf16,
+    all alike; ``buffers`` fp32.  A weight must be contiguous or channels_last, its momentum laid out alike; a gradient
+    laid out otherwise is copied.  The same weight may not come twice.  ``lr`` and the other numbers are read when the
+    call is made (a captured graph keeps them)."""
+    params, grads, buffers = list(params), list(grads), list(buffers)
+    if not len(params) == len(grads) == len(buffers):
+        raise ValueError(f"{len(params)} params, {len(grads)} grads and {len(buffers)} buffers")
+    steps, a, b, c, eps = _numbers(steps, coefficients, eps)
+    lr, momentum, weight_decay = float(lr), float(momentum), float(weight_decay)
+    if not (lr >= 0 and momentum >= 0 and weight_decay >= 0):
+        raise ValueError("lr, momentum and weight_decay must not be negative")
+    if not (scale in ("rms", "spectral") if isinstance(scale, str) else isinstance(scale, (int, float))):
+        raise ValueError(f'scale must be "rms", "spectral" or a number, got {scale!r}')
+    for p, g, m in zip(params, grads, buffers):
+        _check(p, "params")
+        _check(g, "grads", p)
+        _check(m, "buffers", p)
+        if g.dtype != p.dtype:
+            raise RuntimeError(f"grads must be of their weight's type {p.dtype}, got {g.dtype}")
+        if m.dtype != torch.float32:
+            raise RuntimeError(f"buffers must be fp32, got {m.dtype}")
+        if not _dense(p) or (_layout(m) != _layout(p) and p.numel()):
+            raise RuntimeError("params must be contiguous or channels_last, and their buffers laid out alike")
+    if len({p.data_ptr() for p in params if p.numel()}) != sum(p.numel() > 0 for p in params) or \
+            len({m.data_ptr() for m in buffers if m.numel()}) != sum(m.numel() > 0 for m in buffers):
+        raise ValueError("the same weight or buffer comes twice")
+    _same(params, "params")
+    live = [(p, g, m) for p, g, m in zip(params, grads, buffers) if p.numel()]
+    if not live:
+        return
+    ps, ms = [t[0] for t in live], [t[2] for t in live]
+    gs = [g if _layout(g) == _layout(p) else torch.empty_like(p).copy_(g) for p, g, _ in live]
+    rows, cols = _sizes(ps)
+    if scale == "rms":
+        s = [0.2 * math.sqrt(max(r, k)) for r, k in zip(rows, cols)]
+    elif scale == "spectral":
+        s = [math.sqrt(max(1.0, r / k)) for r, k in zip(rows, cols)]
+    else:
+        s = [float(scale)] * len(ps)
+    rates = (ctypes.c_float * len(ps))(*[lr * v for v in s])
+    with torch.cuda.device(ps[0].device):
+        ws, n = _workspace(len(ps), rows, cols, ps[0].device)
+        _C.check(_C.lib().r3det_orthogonal_update(len(ps), _pointers(gs), _pointers(ps), _pointers(ms), DTYPES[ps[0].dtype],
+                                                  rows, cols, rates, 1.0 - lr * weight_decay, momentum, int(bool(nesterov)),
+                                                  steps, a, b, c, eps, _C.ptr(ws), n, _C.stream()), "r3det_orthogonal_update")
+    for t in ps + ms:
+        torch.autograd.graph.increment_version(t)

@@ -1,0 +1,94 @@
+"""CPU: what r3det.ops.orthogonalize refuses, at the Python boundary and at the C entries (which check before any launch)."""
+import ctypes
+
+import pytest
+import torch
+
+from r3det import _C
+from r3det.ops.orthogonalize import orthogonal_update_, orthogonalize
+
+W = torch.zeros(4, 6)
+
+
+def test_refusals_of_orthogonalize():
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        orthogonalize(W)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        orthogonalize([W, W])
+    with pytest.raises(TypeError, match="Tensor"):
+        orthogonalize([1.0])
+    with pytest.raises(ValueError, match="two dimensions"):
+        orthogonalize(torch.zeros(4))
+    with pytest.raises(RuntimeError, match="fp32, fp16 or bf16"):
+        orthogonalize(W.double())
+    with pytest.raises(RuntimeError, match="one type"):
+        orthogonalize([W, W.half()])
+    with pytest.raises(ValueError, match="not taken"):
+        orthogonalize(torch.empty(1, 1).expand(32769, 32769))
+    for steps in (0, 65, 2.5, True):
+        with pytest.raises(ValueError, match="steps"):
+            orthogonalize(W, steps=steps)
+    with pytest.raises(ValueError, match="eps"):
+        orthogonalize(W, eps=-1.0)
+    with pytest.raises(ValueError, match="eps"):
+        orthogonalize(W, eps=float("nan"))
+    assert orthogonalize([]) == []
+
+
+def test_refusals_of_the_update():
+    ok = dict(params=[W.clone()], grads=[W], buffers=[W.clone()], lr=0.1)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        orthogonal_update_(**ok)
+    for change, match in ((dict(grads=[]), "0 grads"), (dict(grads=[W[:2]]), "match its weight"),
+                          (dict(buffers=[W[:, :3]]), "match its weight"), (dict(lr=-1.0), "negative"),
+                          (dict(momentum=-0.1), "negative"), (dict(weight_decay=float("nan")), "negative"),
+                          (dict(scale="mean"), "scale"), (dict(scale=None), "scale"), (dict(steps=0), "steps")):
+        with pytest.raises(ValueError, match=match):
+            orthogonal_update_(**{**ok, **change})
+    for change, match in ((dict(grads=[W.half()]), "weight's type"), (dict(buffers=[W.half()]), "fp32"),
+                          (dict(params=[torch.zeros(6, 4).t()]), "channels_last"),
+                          (dict(buffers=[torch.zeros(6, 4).t()]), "laid out alike")):
+        with pytest.raises(RuntimeError, match=match):
+            orthogonal_update_(**{**ok, **change})
+    w = W.clone()
+    with pytest.raises(ValueError, match="twice"):
+        orthogonal_update_([w, w], [W, W], [W.clone(), W.clone()], lr=0.1)
+    with pytest.raises(ValueError, match="twice"):
+        orthogonal_update_([W.clone(), W.clone()], [W, W], [w, w], lr=0.1)
+    orthogonal_update_([], [], [], lr=0.1)
+
+
+def test_refusals_of_the_c_entries():
+    L = _C.lib()
+    ints = lambda *v: (ctypes.c_int * len(v))(*v)  # noqa: E731
+    ptrs = lambda *v: (ctypes.c_void_p * len(v))(*v)  # noqa: E731
+    far = 1 << 20  # (never followed: every call below ends at its checks)
+    size = L.r3det_orthogonalize_workspace_bytes
+    assert size(0, None, None) == 0
+    for rows, cols in ((0, 4), (4, 0), (-1, 4), (32769, 32769), (1 << 16, 1 << 16), (1, 65536 * 64)):
+        assert size(1, ints(rows), ints(cols)) == 0, (rows, cols)
+    assert size(-1, ints(1), ints(1)) == 0 and size(1, None, ints(1)) == 0
+    need = size(2, ints(4, 100), ints(6, 50))
+    assert need > 0
+
+    def run(count=2, src=ptrs(far, far), dst=ptrs(far, far), dtype=0, rows=ints(4, 100), cols=ints(6, 50), steps=5, a=3.4445,
+            b=-4.775, c=2.0315, eps=1e-7, ws=far, n=need):
+        return L.r3det_orthogonalize(count, src, dst, dtype, rows, cols, steps, a, b, c, eps, ws, n, None)
+    assert run(count=0) == 0
+    nan, inf = float("nan"), float("inf")
+    for bad in (dict(count=-1), dict(src=None), dict(dst=None), dict(src=ptrs(far, None)), dict(dst=ptrs(None, far)), dict(dtype=3),
+                dict(rows=ints(0, 100)), dict(cols=None), dict(steps=0), dict(steps=65), dict(a=nan), dict(b=inf), dict(c=nan),
+                dict(a=20.0), dict(a=4.0, b=0.0, c=0.0), dict(b=-20.0), dict(eps=-1.0), dict(eps=nan), dict(ws=far + 8)):
+        assert run(**bad) == -1, bad
+    assert run(a=2.0, b=0.0, c=0.0, steps=3) == -1  # |X| doubles: X = 4 before the third step, whose A = 16 is over 15
+    assert run(ws=None) == -3 and run(n=need - 1) == -3
+    # coefficients that keep the iterates bounded pass this check (and end at the workspace's)
+    for a, b, c, steps in ((1.5, -0.5, 0.0, 20), (2.0, -1.5, 0.5, 64), (15 / 8, -10 / 8, 3 / 8, 10), (3.4445, -4.7750, 2.0315, 10),
+                           (2.0, 0.0, 0.0, 2), (0.0, 0.0, 0.0, 1)):
+        assert run(a=a, b=b, c=c, steps=steps, n=0) == -3, (a, b, c)
+
+    def update(bufs=ptrs(far, far), rates=(ctypes.c_float * 2)(1, 1), ws=far, n=0):
+        return L.r3det_orthogonal_update(2, ptrs(far, far), ptrs(far, far), bufs, 0, ints(4, 100), ints(6, 50), rates, 1.0, 0.9,
+                                         1, 5, 3.4445, -4.775, 2.0315, 1e-7, ws, n, None)
+    assert update() == -3
+    assert update(bufs=None) == -1 and update(rates=None) == -1 and update(bufs=ptrs(far, None)) == -1
