@@ -6,14 +6,28 @@
 // Each singular value s goes to a s + b s^3 + c s^5 while the singular vectors stay.  With the usual coefficients a small one
 // grows by a = 3.44 a step, 485 in five, and so does every rounding of X: iterates rounded to 16 bits leave an error of
 // 2-3 % in the result where the spectrum is a few directions over noise (fp16; 20 % in bf16).  So an iterate is held as
-// TWO fp16 numbers, hi + lo, which together keep the 24 bits of fp32, and a product is three matrix products on the
-// matrix cores, hi hi + hi lo + lo hi, summed in fp32 (lo lo is below fp32's own rounding).  Stored values carry a factor
-// 2^12: |entries| <= the spectral norm <= 15 by the host's check of the coefficients, so hi does not overflow, and
-// lo keeps its bits for entries down to 2^-12 of the largest.
+// TWO fp16 numbers, hi + lo, 22 bits and lo's sign, and a product is three matrix products on the matrix cores,
+// hi hi + (hi lo + lo hi), summed in fp32 in two accumulators.
 //
-// Every product has both operands with the summed index contiguous: X X^t and A A (A is symmetric) as they are, B X from
-// X^t, which the kernel that makes X writes beside it.  X X^t and A A are symmetric: the tiles on and above the diagonal
-// are computed, and written twice.
+// Steps are taken in groups of two (the first of three where their number is odd) that touch X only twice.  Everything
+// inside a group is a polynomial of its first A, n x n and symmetric, written without cancellation: with the square
+// completed, t = -b / 2c and q = a - c t^2, a step multiplies X by
+//   F = a I + b A + c A A = q I + c (A - t I)^2,
+// which for the usual coefficients is 0.64 I and a positive matrix (the three terms cancel six to one where singular values
+// are near 1).  The next A is F (F A), and the group's steps together are X <- R X with R the product of the F.
+// For m = 9 n (a 3 x 3 convolution of equal width) that halves the operations and reads X twice instead of five times; a
+// square matrix needs as many operations as before.  Longer groups at the end lose digits (2 + 3 twice the error of 3 + 2).
+//
+// The symmetric matrices are mostly diagonal -- A is near I where it has converged, and far from it F is near a I -- and
+// the diagonal would decide where the matrix cores round.  It is kept apart, in fp32, and products take it apart:
+//   (G H)_ij = g_i H_ij + h_j G_ij + sum_k G_ik H_kj  with G and H without their diagonals,  (G H)_ii = g_i h_i + the sum.
+//
+// Stored values carry a power of two so that fp16 neither overflows -- spectral norms bound the entries, and the host checks
+// them for the given coefficients -- nor loses lo's bits: 2^12 for X, A, F, F A (norms below 15), 2^9 for R (below 120).
+//
+// Every product has both operands with the summed index contiguous: the symmetric matrices and X X^t as they are, R X from
+// X^t, which the kernel that makes X writes beside it.  Of a symmetric result the tiles on and above the diagonal are
+// computed, and written twice.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -24,10 +38,9 @@ namespace {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
-constexpr int TS = 64;           // tile of a product, and what matrices are padded to (with zeros, which stay zeros)
-constexpr int BK = 32;           // of the summed index a stage holds
 constexpr int NORM_CHUNK = 8192; // elements a workgroup of the norm's pass takes
 constexpr float SCALE = 4096.f;  // what stored values are multiplied by
+constexpr float R_SCALE = 512.f; // ... of R
 constexpr int WANT = 512;        // workgroups that fill the card
 
 struct Mat {  // one matrix, as the device's table holds it
@@ -37,33 +50,35 @@ struct Mat {  // one matrix, as the device's table holds it
   int rows, cols;    // as the caller has it
   float rate;        // weights <- decay * weights - rate * result
   int splits;        // parts of the sum of X X^t
-  unsigned tri0, rect0, norm0;  // first entries in the lists of triangle tiles (times splits), tiles, norm chunks
-  unsigned part0;    // first partial tile
+  unsigned gram0, tri0, rect0, fill0, norm0;  // first entries in the lists, see Lists
+  size_t part0;      // floats before this matrix's partial tiles
   size_t at;         // halves before this matrix's arrays
 };
-__host__ __device__ inline int up(int v) { return (v + TS - 1) / TS * TS; }
-struct Dim {
-  int n, m, np, mp, tn, tm;
-  __host__ __device__ Dim(int rows, int cols) {
+__host__ __device__ inline int up(int v, int to) { return (v + to - 1) / to * to; }
+enum { SQ_A, SQ_FA, SQ_F, SQ_R = SQ_F + 2, SQ = SQ_R + 2 };  // (two of F, two of R)
+struct Dim {  // padded to 64 or 128 -- a list has one of them -- with zeros, which stay zeros
+  int n, m, np, mp;
+  __host__ __device__ Dim(int rows, int cols, int pad) {
     n = rows < cols ? rows : cols;
     m = rows < cols ? cols : rows;
-    np = up(n), mp = up(m), tn = np / TS, tm = mp / TS;
+    np = up(n, pad), mp = up(m, pad);
   }
   __host__ __device__ size_t x() const { return (size_t)np * mp; }
   __host__ __device__ size_t a() const { return (size_t)np * np; }
-  // per matrix: X, X^t twice (read and written in the same pass), A, B; each hi then lo
-  __host__ __device__ size_t halves() const { return 2 * (3 * x() + 2 * a()); }
-  __host__ __device__ unsigned tri() const { return (unsigned)tn * (tn + 1) / 2; }
-  __host__ __device__ unsigned rect() const { return (unsigned)tn * tm; }
+  // per matrix: X, X^t twice (one read and one written in a pass), SQ n x n arrays, each hi then lo; SQ diagonals in fp32
+  __host__ __device__ size_t halves() const { return 2 * (3 * x() + SQ * a() + (size_t)SQ * np); }
+  __host__ __device__ unsigned tri(int ts) const { return (unsigned)(np / ts) * (np / ts + 1) / 2; }
+  __host__ __device__ unsigned rect(int ts) const { return (unsigned)(np / ts) * (mp / ts); }
   __host__ __device__ unsigned norms() const { return (unsigned)(((size_t)n * m + NORM_CHUNK - 1) / NORM_CHUNK); }
 };
 struct Area {  // where a matrix's arrays are
-  _Float16 *x, *xt, *a, *b;  // xt: two of them
+  _Float16 *x, *xt, *sq;  // xt: two, sq: SQ
+  float* diag;
   __device__ Area(_Float16* base, const Mat& t, const Dim& d) {
     x = base + t.at;
     xt = x + 2 * d.x();
-    a = xt + 4 * d.x();
-    b = a + 2 * d.a();
+    sq = xt + 4 * d.x();
+    diag = reinterpret_cast<float*>(sq + 2 * SQ * d.a());
   }
 };
 struct Tile {
@@ -71,16 +86,27 @@ struct Tile {
   unsigned short i, j;
   unsigned split;
 };
+struct Lists {  // one entry a workgroup
+  Mat* table;
+  Tile* gram;       // X X^t: triangle tiles times parts of the sum
+  Tile* tri;        // triangle tiles of the other n x n products
+  Tile* rect;       // tiles of X
+  Tile* fill;       // 64 x 64 pieces of X
+  uint2* norm_map;  // (matrix, chunk)
+  unsigned n_gram, n_tri, n_rect, n_fill, n_norm;
+  int count, pad, gram_ts, tri_ts, rect_ts;
+};
 
 // the whole workspace; every part is a multiple of 256 bytes
 struct Plan {
-  size_t table, tri, rect, norm_map, norms, counters, parts, halves, total;
-  unsigned n_tri, n_rect, n_norm, n_part;
-  int kc;  // the summed index of X X^t a workgroup takes at most
+  size_t table, gram, tri, rect, fill, norm_map, norms, parts, halves, total;
+  Lists l;    // (sizes only)
+  int kc;     // the summed index of X X^t a workgroup takes at most
+  bool split; // whether any matrix has more than one part
 };
 
 // ------------------------------------------------------------------------------------------------ the lists
-constexpr int BATCH = 48;
+constexpr int BATCH = 43;
 struct Batch {
   Mat m[BATCH];
 };
@@ -89,38 +115,49 @@ __global__ void ortho_table_kernel(Batch b, int count, Mat* table) {
   for (int i = threadIdx.x; i < count; i += blockDim.x) table[i] = b.m[i];
 }
 
-__device__ __forceinline__ unsigned find(const Mat* table, int count, unsigned Mat::* first, unsigned e) {
-  int lo = 0, hi = count - 1;  // the last matrix that begins at or before e
+__device__ __forceinline__ unsigned find(const Lists& l, unsigned Mat::* first, unsigned e) {
+  int lo = 0, hi = l.count - 1;  // the last matrix that begins at or before e
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
-    if (table[mid].*first <= e) lo = mid;
+    if (l.table[mid].*first <= e) lo = mid;
     else hi = mid - 1;
   }
   return lo;
 }
-__global__ void ortho_lists_kernel(const Mat* table, int count, Tile* tri, unsigned n_tri, Tile* rect, unsigned n_rect,
-                                   uint2* norm_map, unsigned n_norm, unsigned* counters, unsigned n_count) {
+__device__ __forceinline__ Tile triangle(unsigned mat, unsigned tile, unsigned wide, unsigned split) {
+  unsigned i = 0;
+  while (tile >= wide - i) tile -= wide - i, ++i;  // (row i has wide - i tiles)
+  return Tile{mat, (unsigned short)i, (unsigned short)(i + tile), split};
+}
+__global__ void ortho_lists_kernel(Lists l) {
   const unsigned g = blockIdx.x * blockDim.x + threadIdx.x, stride = gridDim.x * blockDim.x;
-  for (unsigned e = g; e < n_tri; e += stride) {
-    const unsigned k = find(table, count, &Mat::tri0, e);
-    const Mat& t = table[k];
-    const Dim d(t.rows, t.cols);
-    const unsigned local = e - t.tri0;
-    unsigned tile = local / t.splits, i = 0;
-    while (tile >= (unsigned)d.tn - i) tile -= d.tn - i, ++i;  // (row i has tn - i tiles)
-    tri[e] = Tile{k, (unsigned short)i, (unsigned short)(i + tile), local % t.splits};
+  for (unsigned e = g; e < l.n_gram; e += stride) {
+    const unsigned k = find(l, &Mat::gram0, e);
+    const Mat& t = l.table[k];
+    const unsigned local = e - t.gram0;
+    l.gram[e] = triangle(k, local / t.splits, Dim(t.rows, t.cols, l.pad).np / l.gram_ts, local % t.splits);
   }
-  for (unsigned e = g; e < n_rect; e += stride) {
-    const unsigned k = find(table, count, &Mat::rect0, e);
-    const Dim d(table[k].rows, table[k].cols);
-    const unsigned local = e - table[k].rect0;
-    rect[e] = Tile{k, (unsigned short)(local % d.tn), (unsigned short)(local / d.tn), 0};
+  for (unsigned e = g; e < l.n_tri; e += stride) {
+    const unsigned k = find(l, &Mat::tri0, e);
+    const Mat& t = l.table[k];
+    l.tri[e] = triangle(k, e - t.tri0, Dim(t.rows, t.cols, l.pad).np / l.tri_ts, 0);
   }
-  for (unsigned e = g; e < n_norm; e += stride) {
-    const unsigned k = find(table, count, &Mat::norm0, e);
-    norm_map[e] = make_uint2(k, e - table[k].norm0);
+  for (unsigned e = g; e < l.n_rect; e += stride) {
+    const unsigned k = find(l, &Mat::rect0, e);
+    const Mat& t = l.table[k];
+    const unsigned local = e - t.rect0, high = Dim(t.rows, t.cols, l.pad).np / l.rect_ts;
+    l.rect[e] = Tile{k, (unsigned short)(local % high), (unsigned short)(local / high), 0};
   }
-  for (unsigned e = g; e < n_count; e += stride) counters[e] = 0;
+  for (unsigned e = g; e < l.n_fill; e += stride) {
+    const unsigned k = find(l, &Mat::fill0, e);
+    const Mat& t = l.table[k];
+    const unsigned local = e - t.fill0, wide = Dim(t.rows, t.cols, l.pad).mp / 64;
+    l.fill[e] = Tile{k, (unsigned short)(local / wide), (unsigned short)(local % wide), 0};
+  }
+  for (unsigned e = g; e < l.n_norm; e += stride) {
+    const unsigned k = find(l, &Mat::norm0, e);
+    l.norm_map[e] = make_uint2(k, e - l.table[k].norm0);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ momentum, norm, X
@@ -140,11 +177,11 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
 // momentum <- mu momentum + gradient, and the squares of the direction summed in 64 bits (no scaling of the matrix is needed
 // against overflow, and the order of the sums is fixed)
 template <typename T>
-__global__ __launch_bounds__(256) void ortho_norm_kernel(const Mat* __restrict__ table, const uint2* __restrict__ map,
-                                                         double* __restrict__ norms, int update, float mu, int nesterov) {
+__global__ __launch_bounds__(256) void ortho_norm_kernel(Lists l, double* __restrict__ norms, int update, float mu,
+                                                         int nesterov) {
   __shared__ double sh[4];
-  const uint2 w = map[blockIdx.x];
-  const Mat t = table[w.x];
+  const uint2 w = l.norm_map[blockIdx.x];
+  const Mat t = l.table[w.x];
   const size_t all = (size_t)t.rows * t.cols, from = (size_t)w.y * NORM_CHUNK;
   const size_t to = from + NORM_CHUNK < all ? from + NORM_CHUNK : all;
   double s = 0;
@@ -161,202 +198,332 @@ __device__ __forceinline__ void split16(float v, _Float16& hi, _Float16& lo) {
   hi = (_Float16)v;
   lo = (_Float16)(v - (float)hi);
 }
-// A tile of fp32 in shared memory, E[r][c] -> hi / lo arrays; rows of `ld`.
-template <bool TURNED>
-__device__ __forceinline__ void store_tile(const float (*E)[TS + 1], _Float16* p, size_t lo, size_t ld, int r0, int c0) {
+__device__ __forceinline__ void store8(_Float16* at, size_t lo, const float (&v)[8]) {
+  half8 h, l;
 #pragma unroll
-  for (int q = threadIdx.x; q < TS * TS / 8; q += 256) {
-    const int r = q / (TS / 8), c = q % (TS / 8) * 8;
-    half8 h, l;
+  for (int k = 0; k < 8; ++k) {
+    _Float16 hh, ll;
+    split16(v[k], hh, ll);
+    h[k] = hh, l[k] = ll;
+  }
+  *reinterpret_cast<half8*>(at) = h;
+  *reinterpret_cast<half8*>(at + lo) = l;
+}
+__device__ __forceinline__ void add8(float (&v)[8], float f, const _Float16* at, size_t lo) {
+  const half8 h = *reinterpret_cast<const half8*>(at), l = *reinterpret_cast<const half8*>(at + lo);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      _Float16 hh, ll;
-      split16(TURNED ? E[c + k][r] : E[r][c + k], hh, ll);
-      h[k] = hh, l[k] = ll;
-    }
-    _Float16* at = p + (size_t)(r0 + r) * ld + c0 + c;
-    *reinterpret_cast<half8*>(at) = h;
-    *reinterpret_cast<half8*>(at + lo) = l;
+  for (int k = 0; k < 8; ++k) v[k] = fmaf(f, (float)h[k] + (float)l[k], v[k]);
+}
+// ROWS x COLS of fp32 in shared memory, rows of LD: f(row, column, eight values), which may change them; then `f`'s values
+// are in shared memory too.
+template <int ROWS, int COLS, int LD, typename F>
+__device__ __forceinline__ void rows8(float* E, const F& f) {
+#pragma unroll 2
+  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += 256) {
+    const int r = q / (COLS / 8), c = q % (COLS / 8) * 8;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = E[r * LD + c + k];
+    f(r, c, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) E[r * LD + c + k] = v[k];
+  }
+}
+// The transpose of ROWS x COLS in shared memory -> hi / lo arrays with rows of `ld`, at (r0, c0).
+template <int ROWS, int COLS, int LD>
+__device__ __forceinline__ void store_turned(const float* E, _Float16* p, size_t lo, size_t ld, int r0, int c0) {
+#pragma unroll 2
+  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += 256) {
+    const int r = q / (ROWS / 8), c = q % (ROWS / 8) * 8;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = E[(c + k) * LD + r];
+    store8(p + (size_t)(r0 + r) * ld + c0 + c, lo, v);
   }
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void ortho_start_kernel(const Mat* __restrict__ table, const Tile* __restrict__ rect,
-                                                          const double* __restrict__ norms, _Float16* __restrict__ base,
-                                                          int update, float mu, int nesterov, double eps) {
+__global__ __launch_bounds__(256) void ortho_start_kernel(Lists l, const double* __restrict__ norms,
+                                                          _Float16* __restrict__ base, int update, float mu, int nesterov,
+                                                          double eps) {
   __shared__ double sh[4];
-  __shared__ float E[TS][TS + 1];
-  const Tile w = rect[blockIdx.x];
-  const Mat t = table[w.mat];
-  const Dim d(t.rows, t.cols);
+  __shared__ float E[64 * 65];
+  const Tile w = l.fill[blockIdx.x];
+  const Mat t = l.table[w.mat];
+  const Dim d(t.rows, t.cols, l.pad);
   const Area o(base, t, d);
   double s = 0;
   for (unsigned i = threadIdx.x; i < d.norms(); i += 256) s += norms[t.norm0 + i];
   s = block_sum(s, sh);
   const double inv = (double)SCALE / (sqrt(s) + eps);
   const bool tall = t.rows > t.cols;
-  const int i0 = w.i * TS, j0 = w.j * TS;
-  for (int q = threadIdx.x; q < TS * TS; q += 256) {
+  const int i0 = w.i * 64, j0 = w.j * 64;
+  for (int q = threadIdx.x; q < 64 * 64; q += 256) {
     // (consecutive threads along the caller's rows)
-    const int r = tall ? q % TS : q / TS, c = tall ? q / TS : q % TS;
+    const int r = tall ? q % 64 : q / 64, c = tall ? q / 64 : q % 64;
     const int i = i0 + r, j = j0 + c;
     float v = 0.f;
     if (i < d.n && j < d.m) {
       const size_t at = tall ? (size_t)j * t.cols + i : (size_t)i * t.cols + j;
       v = (float)((double)direction<T>(t, at, update, mu, nesterov) * inv);
     }
-    E[r][c] = v;
+    E[r * 65 + c] = v;
   }
   __syncthreads();
-  store_tile<false>(E, o.x, d.x(), d.mp, i0, j0);
-  store_tile<true>(E, o.xt, d.x(), d.np, j0, i0);
+  rows8<64, 64, 65>(E, [&](int r, int c, float (&v)[8]) { store8(o.x + (size_t)(i0 + r) * d.mp + j0 + c, d.x(), v); });
+  store_turned<64, 64, 65>(E, o.xt, d.x(), d.np, j0, i0);
 }
 
 // ------------------------------------------------------------------------------------------------ the products
-// One 64 x 64 tile of P Q^t by 4 wavefronts, 32 x 32 each: P, Q (hi, lo) with rows of ldp / ldq, the summed index
-// [k0, k1).  A stage of 32 of it is 4 x 4 KB of shared memory, written by the loads themselves, two stages in turn.  A
-// 16-byte piece c of row r sits at c ^ (r / 2 % 4): eight rows that are read together then lie in different banks.
+// One TS x TS tile of P Q^t by 4 wavefronts, a quarter each: P, Q (hi, lo) with the summed index [k0, k1) contiguous, rows of
+// ldp / ldq.  A stage is 4 x 8 KB of shared memory -- 32 of the summed index at tiles of 128, 64 at tiles of 64 -- and comes
+// through registers: its loads are issued a stage ahead and have a stage's products to arrive in.  (Loads straight into
+// shared memory do not overlap here: before a stage is read, the compiler waits for every such load in flight, the next
+// stage's too.)  The 16-byte piece c of row r sits at c ^ (r / 2 % 4) or c ^ (r % 8): eight rows that are read together then
+// lie in different banks.
 struct Stage {
-  half8 v[4][TS * BK / 8];
+  half8 v[4][512];
 };
-__device__ __forceinline__ void load_stage(Stage& s, const _Float16* p, size_t plo, size_t ldp, const _Float16* q, size_t qlo,
-                                           size_t ldq, int k) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const _Float16* src = wave < 2 ? p + (wave & 1) * plo : q + (wave & 1) * qlo;
-  const size_t ld = wave < 2 ? ldp : ldq;
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int slot = t * 64 + lane, r = slot / 4, c = (slot % 4) ^ (r / 2 % 4);
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + (size_t)r * ld + k + c * 8),
-                                     (__attribute__((address_space(3))) void*)&s.v[wave][t * 64], 16, 0, 0);
+template <int TS>
+struct Core {
+  static constexpr int BK = TS == 128 ? 32 : 64, PIECES = BK / 8, M = TS / 64;
+  static constexpr int LD = TS + 1;
+  static __device__ __forceinline__ int place(int r, int c) {
+    return r * PIECES + (c ^ (PIECES == 4 ? r / 2 % 4 : r % 8));
   }
-}
-__device__ __forceinline__ void product(float16v& acc, Stage* st, const _Float16* p, size_t plo, size_t ldp, const _Float16* q,
-                                        size_t qlo, size_t ldq, int k0, int k1) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int pr = (wave >> 1) * 32 + (lane & 31), qr = (wave & 1) * 32 + (lane & 31), kc = lane >> 5;
-  load_stage(st[0], p, plo, ldp, q, qlo, ldq, k0);
-  int cur = 0;
-  for (int k = k0; k < k1; k += BK) {
-    __syncthreads();  // this stage's loads are in, and everyone is done with the other stage
-    if (k + BK < k1) load_stage(st[cur ^ 1], p, plo, ldp, q, qlo, ldq, k + BK);
-    const Stage& s = st[cur];
+  float16v hh[M][M], hl[M][M];  // hi hi, and the two others
+  half8 next[8];
+
+  __device__ __forceinline__ void fetch(const _Float16* p, size_t plo, size_t ldp, const _Float16* q, size_t qlo, size_t ldq,
+                                        int k) {
 #pragma unroll
-    for (int kk = 0; kk < BK / 16; ++kk) {
-      const int ps = pr * 4 + ((kk * 2 + kc) ^ (pr / 2 % 4)), qs = qr * 4 + ((kk * 2 + kc) ^ (qr / 2 % 4));
-      const half8 ph = s.v[0][ps], pl = s.v[1][ps], qh = s.v[2][qs], ql = s.v[3][qs];
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+    for (int t = 0; t < 2; ++t) {
+      const int slot = t * 256 + threadIdx.x, r = slot / PIECES, c = slot % PIECES;
+      const _Float16 *a = p + (size_t)r * ldp + k + c * 8, *b = q + (size_t)r * ldq + k + c * 8;
+      next[t] = *reinterpret_cast<const half8*>(a);
+      next[2 + t] = *reinterpret_cast<const half8*>(a + plo);
+      next[4 + t] = *reinterpret_cast<const half8*>(b);
+      next[6 + t] = *reinterpret_cast<const half8*>(b + qlo);
     }
-    cur ^= 1;
   }
-  __syncthreads();  // (the stages' memory is the epilogue's too)
-}
+  __device__ __forceinline__ void put(Stage& s) const {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int slot = t * 256 + threadIdx.x, at = place(slot / PIECES, slot % PIECES);
+#pragma unroll
+      for (int a = 0; a < 4; ++a) s.v[a][at] = next[2 * a + t];
+    }
+  }
+  __device__ __forceinline__ void run(Stage* st, const _Float16* p, size_t plo, size_t ldp, const _Float16* q, size_t qlo,
+                                      size_t ldq, int k0, int k1) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int pr = (wave >> 1) * (TS / 2) + (lane & 31), qr = (wave & 1) * (TS / 2) + (lane & 31), kc = lane >> 5;
+    fetch(p, plo, ldp, q, qlo, ldq, k0);
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int j = 0; j < M; ++j) hh[i][j] = float16v{}, hl[i][j] = float16v{};
+    put(st[0]);
+    if (k0 + BK < k1) fetch(p, plo, ldp, q, qlo, ldq, k0 + BK);
+    __syncthreads();
+    int cur = 0;
+    for (int k = k0; k < k1; k += BK) {
+      const Stage& s = st[cur];
+#pragma unroll
+      for (int kk = 0; kk < BK / 16; ++kk) {
+        half8 ph[M], pl[M], qh[M], ql[M];
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+          const int ps = place(pr + 32 * i, kk * 2 + kc), qs = place(qr + 32 * i, kk * 2 + kc);
+          ph[i] = s.v[0][ps], pl[i] = s.v[1][ps], qh[i] = s.v[2][qs], ql[i] = s.v[3][qs];
+        }
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+#pragma unroll
+          for (int j = 0; j < M; ++j) {
+            hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], hl[i][j], 0, 0, 0);
+            hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], hl[i][j], 0, 0, 0);
+            hh[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], hh[i][j], 0, 0, 0);
+          }
+      }
+      cur ^= 1;
+      if (k + BK < k1) {
+        put(st[cur]);  // (everyone left this stage before the last barrier)
+        if (k + 2 * BK < k1) fetch(p, plo, ldp, q, qlo, ldq, k + 2 * BK);
+      }
+      __syncthreads();  // (behind the last stage: the stages' memory is the epilogue's too)
+    }
+  }
+  // lane l of the matrix instruction holds column l % 32 and rows 8 (r / 4) + 4 (l / 32) + r % 4
+  template <typename F>
+  __device__ __forceinline__ void each(const F& f) const {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int j = 0; j < M; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          f((wave >> 1) * (TS / 2) + 32 * i + 8 * (r / 4) + 4 * (lane >> 5) + r % 4,
+            (wave & 1) * (TS / 2) + 32 * j + (lane & 31), hh[i][j][r] + hl[i][j][r]);
+  }
+  // ... times f, into shared memory
+  __device__ __forceinline__ void spill(float* E, float f) const {
+    each([&](int r, int c, float v) { E[r * LD + c] = v * f; });
+    __syncthreads();
+  }
+};
+template <int TS>
 union Shared {
   Stage st[2];
-  float E[TS][TS + 1];
+  float E[TS * (TS + 1)];
 };
-// lane l of the matrix instruction holds column l % 32 and rows 8 (r / 4) + 4 (l / 32) + r % 4
-template <typename F>
-__device__ __forceinline__ void each(const float16v& acc, const F& f) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-#pragma unroll
-  for (int r = 0; r < 16; ++r)
-    f((wave >> 1) * 32 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4, (wave & 1) * 32 + (lane & 31), acc[r]);
-}
 
-// A = X X^t: a tile on or above the diagonal, or one part of its sum.  The workgroup that ends a tile last adds the parts in
-// their order, whoever it is, so results do not depend on the order of arrival.
-__global__ __launch_bounds__(256) void ortho_gram_kernel(const Mat* __restrict__ table, const Tile* __restrict__ tri,
-                                                         _Float16* base, float* parts, unsigned* counters, int kc) {
-  __shared__ Shared sh;
-  __shared__ unsigned last;
-  const Tile w = tri[blockIdx.x];
-  const Mat t = table[w.mat];
-  const Dim d(t.rows, t.cols);
+// A from ROWS rows of a tile in shared memory
+template <int ROWS, int TS>
+__device__ __forceinline__ void store_gram(float* E, const Dim& d, const Area& o, int i0, int j0, bool diagonal) {
+  _Float16* a = o.sq + SQ_A * 2 * d.a();
+  rows8<ROWS, TS, TS + 1>(E, [&](int r, int c, float (&v)[8]) {
+    if (diagonal)
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i0 + r == j0 + c + k) o.diag[SQ_A * d.np + i0 + r] = v[k] * (1.f / SCALE), v[k] = 0.f;
+    store8(a + (size_t)(i0 + r) * d.np + j0 + c, d.a(), v);
+  });
+  if (!diagonal) {
+    __syncthreads();
+    store_turned<ROWS, TS, TS + 1>(E, a, d.a(), d.np, j0, i0);
+  }
+}
+// A = X X^t: a tile on or above the diagonal, or one part of its sum, which ortho_sum_kernel adds up in their order.
+// (Adding them in the workgroup that ends last needs the other workgroups' tiles flushed through the XCDs' caches: 160 us
+// where this and the launch behind it take 20, at eight 256 x 2304 matrices.)
+template <int TS>
+__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Lists l, _Float16* base, float* parts, int kc) {
+  __shared__ Shared<TS> sh;
+  const Tile w = l.gram[blockIdx.x];
+  const Mat t = l.table[w.mat];
+  const Dim d(t.rows, t.cols, l.pad);
   const Area o(base, t, d);
   const int i0 = w.i * TS, j0 = w.j * TS;
-  float16v acc = {};
   const int k0 = w.split * kc, k1 = k0 + kc < d.mp ? k0 + kc : d.mp;
-  product(acc, sh.st, o.x + (size_t)i0 * d.mp, d.x(), d.mp, o.x + (size_t)j0 * d.mp, d.x(), d.mp, k0, k1);
+  Core<TS> core;
+  core.run(sh.st, o.x + (size_t)i0 * d.mp, d.x(), d.mp, o.x + (size_t)j0 * d.mp, d.x(), d.mp, k0, k1);
   if (t.splits > 1) {
-    const unsigned tile = (blockIdx.x - t.tri0) / t.splits;
-    float* mine = parts + ((size_t)t.part0 + (size_t)tile * t.splits) * (TS * TS);
-    each(acc, [&](int r, int c, float v) { mine[(size_t)w.split * (TS * TS) + r * TS + c] = v; });
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0)
-      last = __hip_atomic_fetch_add(&counters[t.part0 + tile], 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
-             (unsigned)t.splits - 1;
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
-    for (int q = threadIdx.x; q < TS * TS; q += 256) {
-      float v = 0.f;
-      for (int s = 0; s < t.splits; ++s) v += mine[(size_t)s * (TS * TS) + q];
-      sh.E[q / TS][q % TS] = v * (1.f / SCALE);
+    float* mine = parts + t.part0 + (size_t)(blockIdx.x - t.gram0) * (TS * TS);
+    core.each([&](int r, int c, float v) { mine[r * TS + c] = v * (1.f / SCALE); });
+    return;
+  }
+  core.spill(sh.E, 1.f / SCALE);
+  store_gram<TS, TS>(sh.E, d, o, i0, j0, w.i == w.j);
+}
+// 32 rows of a tile of A from its parts
+template <int TS>
+__global__ __launch_bounds__(256) void ortho_sum_kernel(Lists l, _Float16* base, const float* __restrict__ parts) {
+  __shared__ float E[32 * (TS + 1)];
+  const Tile w = l.gram[blockIdx.x];
+  if (w.split) return;
+  const Mat t = l.table[w.mat];
+  if (t.splits == 1) return;
+  const Dim d(t.rows, t.cols, l.pad);
+  const Area o(base, t, d);
+  const int slice = blockIdx.y * 32;
+  const float* mine = parts + t.part0 + (size_t)(blockIdx.x - t.gram0) * (TS * TS) + slice * TS;
+#pragma unroll
+  for (int q = threadIdx.x * 4; q < 32 * TS; q += 1024) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < t.splits; ++s) {
+      const float4 u = *reinterpret_cast<const float4*>(mine + (size_t)s * (TS * TS) + q);
+      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
     }
-    if (threadIdx.x == 0) counters[t.part0 + tile] = 0;  // for the next step
-  } else {
-    each(acc, [&](int r, int c, float v) { sh.E[r][c] = v * (1.f / SCALE); });
+    float* e = E + q / TS * (TS + 1) + q % TS;
+    e[0] = v.x, e[1] = v.y, e[2] = v.z, e[3] = v.w;
   }
   __syncthreads();
-  store_tile<false>(sh.E, o.a, d.a(), d.np, i0, j0);
-  if (w.i != w.j) store_tile<true>(sh.E, o.a, d.a(), d.np, j0, i0);
+  store_gram<32, TS>(E, d, o, w.i * TS + slice, w.j * TS, w.i == w.j);
 }
 
-// B = b A + c A A
-__global__ __launch_bounds__(256) void ortho_poly_kernel(const Mat* __restrict__ table, const Tile* __restrict__ tri,
-                                                         _Float16* base, float b, float c) {
-  __shared__ Shared sh;
-  const Tile w = tri[blockIdx.x];
-  if (w.split) return;
-  const Mat t = table[w.mat];
-  const Dim d(t.rows, t.cols);
+// out = q I + l G + f (G - t I) (H - t I) of symmetric matrices that commute (all are polynomials of one): a tile on or above
+// the diagonal.  The scales of what is stored are in the factors: out_ij = fh g_i H_ij + (fg h_j + l) G_ij + fs sum.
+struct Op {
+  int out, g, h;  // which arrays
+  float t, q, l, f, fg, fh, fs, back;  // back: one over out's scale
+};
+template <int TS>
+__global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
+  __shared__ Shared<TS> sh;
+  const Tile w = l.tri[blockIdx.x];
+  const Mat t = l.table[w.mat];
+  const Dim d(t.rows, t.cols, l.pad);
   const Area o(base, t, d);
+  const Op op = blockIdx.y ? second : first;
   const int i0 = w.i * TS, j0 = w.j * TS;
-  float16v acc = {};
-  product(acc, sh.st, o.a + (size_t)i0 * d.np, d.a(), d.np, o.a + (size_t)j0 * d.np, d.a(), d.np, 0, d.np);
-  each(acc, [&](int r, int q, float v) {
-    const _Float16* p = o.a + (size_t)(i0 + r) * d.np + j0 + q;
-    sh.E[r][q] = fmaf(b, (float)p[0] + (float)p[d.a()], c * (v * (1.f / SCALE)));
+  const size_t lo = d.a(), step = 2 * lo;
+  const _Float16 *g = o.sq + op.g * step, *h = o.sq + op.h * step;
+  const float *gd = o.diag + op.g * d.np, *hd = o.diag + op.h * d.np;
+  Core<TS> core;
+  core.run(sh.st, g + (size_t)i0 * d.np, lo, d.np, h + (size_t)j0 * d.np, lo, d.np, 0, d.np);
+  core.spill(sh.E, 1.f);
+  _Float16* out = o.sq + op.out * step;
+  const bool diagonal = w.i == w.j;
+  rows8<TS, TS, TS + 1>(sh.E, [&](int r, int c, float (&v)[8]) {
+    const int i = i0 + r, j = j0 + c;
+    const size_t at = (size_t)i * d.np + j;
+    const half8 gh = *reinterpret_cast<const half8*>(g + at), gl = *reinterpret_cast<const half8*>(g + at + lo);
+    const half8 hh = *reinterpret_cast<const half8*>(h + at), hl = *reinterpret_cast<const half8*>(h + at + lo);
+    const float gi = op.fh * (gd[i] - op.t);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float hj = hd[j + k] - op.t;
+      float e = fmaf(fmaf(op.fg, hj, op.l), (float)gh[k] + (float)gl[k], op.fs * v[k]);
+      e = fmaf(gi, (float)hh[k] + (float)hl[k], e);
+      if (diagonal && i == j + k) {
+        o.diag[op.out * d.np + i] = fmaf(op.f * (gd[i] - op.t), hj, fmaf(op.l, gd[i], op.q)) + op.fs * op.back * v[k];
+        e = 0.f;
+      }
+      v[k] = e;
+    }
+    store8(out + at, lo, v);
   });
-  __syncthreads();
-  store_tile<false>(sh.E, o.b, d.a(), d.np, i0, j0);
-  if (w.i != w.j) store_tile<true>(sh.E, o.b, d.a(), d.np, j0, i0);
+  if (!diagonal) {
+    __syncthreads();
+    store_turned<TS, TS, TS + 1>(sh.E, out, lo, d.np, j0, i0);
+  }
 }
 
-// X <- a X + B X, from X^t; the last step's goes to the caller, as the result or into the weights
-template <typename T, bool LAST>
-__global__ __launch_bounds__(256) void ortho_apply_kernel(const Mat* __restrict__ table, const Tile* __restrict__ rect,
-                                                          _Float16* base, float a, int from, int update, float decay) {
-  __shared__ Shared sh;
-  const Tile w = rect[blockIdx.x];
-  const Mat t = table[w.mat];
-  const Dim d(t.rows, t.cols);
+// X <- R X, from X^t; the last group's goes to the caller, as the result or into the weights
+template <typename T, bool LAST, int TS>
+__global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* base, int R, float fs, int from, int update,
+                                                             float decay) {
+  __shared__ Shared<TS> sh;
+  const Tile w = l.rect[blockIdx.x];
+  const Mat t = l.table[w.mat];
+  const Dim d(t.rows, t.cols, l.pad);
   const Area o(base, t, d);
   const int i0 = w.i * TS, j0 = w.j * TS;
-  float16v acc = {};
-  const _Float16* xt = o.xt + (from ? 2 * d.x() : 0);
-  product(acc, sh.st, o.b + (size_t)i0 * d.np, d.a(), d.np, xt + (size_t)j0 * d.np, d.x(), d.np, 0, d.np);
-  each(acc, [&](int r, int q, float v) {
-    const _Float16* p = o.x + (size_t)(i0 + r) * d.mp + j0 + q;
-    sh.E[r][q] = fmaf(a, (float)p[0] + (float)p[d.x()], v * (1.f / SCALE));
+  const _Float16 *a = o.sq + R * 2 * d.a(), *xt = o.xt + (from ? 2 * d.x() : 0);
+  Core<TS> core;
+  core.run(sh.st, a + (size_t)i0 * d.np, d.a(), d.np, xt + (size_t)j0 * d.np, d.x(), d.np, 0, d.np);
+  core.spill(sh.E, fs);
+  rows8<TS, TS, TS + 1>(sh.E, [&](int r, int c, float (&v)[8]) {
+    _Float16* x = o.x + (size_t)(i0 + r) * d.mp + j0 + c;
+    add8(v, o.diag[R * d.np + i0 + r], x, d.x());
+    if constexpr (!LAST) store8(x, d.x(), v);
   });
   __syncthreads();
   if constexpr (!LAST) {
-    store_tile<false>(sh.E, o.x, d.x(), d.mp, i0, j0);
-    store_tile<true>(sh.E, o.xt + (from ? 0 : 2 * d.x()), d.x(), d.np, j0, i0);
+    store_turned<TS, TS, TS + 1>(sh.E, o.xt + (from ? 0 : 2 * d.x()), d.x(), d.np, j0, i0);
   } else {
     const bool tall = t.rows > t.cols;
     T* out = static_cast<T*>(t.dst);
+#pragma unroll 4
     for (int q = threadIdx.x; q < TS * TS; q += 256) {
       const int r = tall ? q % TS : q / TS, c = tall ? q / TS : q % TS;
       const int i = i0 + r, j = j0 + c;
       if (i < d.n && j < d.m) {
         const size_t at = tall ? (size_t)j * t.cols + i : (size_t)i * t.cols + j;
-        const float v = sh.E[r][c] * (1.f / SCALE);
+        const float v = sh.E[r * (TS + 1) + c] * (1.f / SCALE);
         out[at] = (T)(update ? fmaf(-t.rate, v, decay * (float)out[at]) : v);
       }
     }
@@ -372,30 +539,50 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   for (int i = 0; i < count; ++i) {
     if (rows[i] < 1 || cols[i] < 1 || (int64_t)rows[i] * cols[i] > 0x7fffffff) return -1;
     if ((rows[i] < cols[i] ? rows[i] : cols[i]) > 32768) return -1;
-    if ((rows[i] > cols[i] ? rows[i] : cols[i]) > 65535 * TS) return -1;
+    if ((rows[i] > cols[i] ? rows[i] : cols[i]) > 65535 * 64) return -1;  // (a tile's place has 16 bits)
   }
+  Lists& l = p.l;
+  l = Lists{};
+  l.count = count;
+  // Tiles: 128 needs half the reads of two operands that 64 does, and is taken for a pass that fills the card with such
+  // tiles, unless it pads much further.
+  uint64_t tri128 = 0, rect64 = 0, rect128 = 0, gram128 = 0;
+  for (int i = 0; i < count; ++i) {
+    const Dim s(rows[i], cols[i], 64), w(rows[i], cols[i], 128);
+    tri128 += w.tri(128), rect64 += s.rect(64), rect128 += w.rect(128);
+    gram128 += (uint64_t)w.tri(128) * ((w.mp + 255) / 256);
+  }
+  const bool tight = rect128 * 4 <= rect64 * 3 / 2;
+  l.gram_ts = tight && gram128 >= WANT / 2 ? 128 : 64;
+  l.tri_ts = tight && tri128 >= WANT / 2 ? 128 : 64;
+  l.rect_ts = tight && rect128 >= WANT / 2 ? 128 : 64;
+  l.pad = l.gram_ts == 128 || l.tri_ts == 128 || l.rect_ts == 128 ? 128 : 64;
   // X X^t: the longest parts of the sum that still fill the card.  A part is a workgroup's time, so the parts of a ragged
   // list are of like length, and a short list of wide matrices is spread.
   for (p.kc = 4096; p.kc > 256; p.kc /= 2) {
     uint64_t blocks = 0;
     for (int i = 0; i < count; ++i) {
-      const Dim d(rows[i], cols[i]);
-      blocks += (uint64_t)d.tri() * ((d.mp + p.kc - 1) / p.kc);
+      const Dim d(rows[i], cols[i], l.pad);
+      blocks += (uint64_t)d.tri(l.gram_ts) * ((d.mp + p.kc - 1) / p.kc);
     }
     if (blocks >= WANT) break;
   }
-  uint64_t tri = 0, rect = 0, norm = 0, part = 0, halves = 0;
+  uint64_t gram = 0, tri = 0, rect = 0, fill = 0, norm = 0, part = 0, halves = 0;
+  p.split = false;
   for (int i = 0; i < count; ++i) {
-    const Dim d(rows[i], cols[i]);
+    const Dim d(rows[i], cols[i], l.pad);
     const unsigned s = (unsigned)((d.mp + p.kc - 1) / p.kc);
-    tri += (uint64_t)d.tri() * s;
-    rect += d.rect();
+    gram += (uint64_t)d.tri(l.gram_ts) * s;
+    tri += d.tri(l.tri_ts);
+    rect += d.rect(l.rect_ts);
+    fill += d.rect(64);
     norm += d.norms();
-    part += (uint64_t)d.tri() * s;
+    if (s > 1) part += (uint64_t)d.tri(l.gram_ts) * s * l.gram_ts * l.gram_ts, p.split = true;
     halves += d.halves();
   }
-  if (tri > 0x7fffffff || rect > 0x7fffffff || norm > 0x7fffffff) return -1;
-  p.n_tri = (unsigned)tri, p.n_rect = (unsigned)rect, p.n_norm = (unsigned)norm, p.n_part = (unsigned)part;
+  if (gram > 0x7fffffff || tri > 0x7fffffff || rect > 0x7fffffff || fill > 0x7fffffff || norm > 0x7fffffff) return -1;
+  l.n_gram = (unsigned)gram, l.n_tri = (unsigned)tri, l.n_rect = (unsigned)rect, l.n_fill = (unsigned)fill;
+  l.n_norm = (unsigned)norm;
   size_t at = 0;
   const auto take = [&](size_t bytes) {
     const size_t was = at;
@@ -403,94 +590,160 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
     return was;
   };
   p.table = take(sizeof(Mat) * (size_t)count);
+  p.gram = take(sizeof(Tile) * gram);
   p.tri = take(sizeof(Tile) * tri);
   p.rect = take(sizeof(Tile) * rect);
+  p.fill = take(sizeof(Tile) * fill);
   p.norm_map = take(sizeof(uint2) * norm);
   p.norms = take(sizeof(double) * norm);
-  p.counters = take(sizeof(unsigned) * part);
-  p.parts = take(sizeof(float) * TS * TS * part);
+  p.parts = take(sizeof(float) * part);
   p.halves = take(sizeof(_Float16) * halves);
   p.total = at;
   return 0;
 }
 
-// Whether every stored value stays below fp16's range: the spectral norms of X, A and B, from |X| <= 1 on, step by step, with
-// the polynomial's extremes in between.  (1 % over, for the roundings of the iterates.)
-bool bounded(int steps, double a, double b, double c) {
-  if (!(fabs(a) < 1e6) || !(fabs(b) < 1e6) || !(fabs(c) < 1e6)) return false;
+// How a step's polynomial is taken: F = q I + l A + c (A - t I)^2.  The square is completed (l = 0) unless that needs large
+// numbers (c near 0): then t = 0.
+struct Poly {
+  float c, t, q, l;
+  int longest;  // group; 0: an iterate might leave fp16's range
+};
+// Groups of steps: twos, the first a three where the number is odd; ones where R of a longer group might leave its range
+int group_length(int left, int steps) { return left == 1 ? 1 : (left == steps && left % 2 ? 3 : 2); }
+// The spectral norms of X, A, F A, F off the diagonal from |X| <= 1 on, step by step, with the polynomials' extremes in between (1 % over, for
+// the roundings).
+Poly polynomial(int steps, double a, double b, double c) {
+  Poly r{(float)c, 0.f, (float)a, (float)b, 0};
+  if (!(fabs(a) < 1e6) || !(fabs(b) < 1e6) || !(fabs(c) < 1e6)) return r;
   const double most = 65504.0 / SCALE / 1.05;
-  double top = 1;
+  double t = 0, q = a, f = b;
+  if (c != 0 && fabs(b) <= 14 * fabs(c)) {
+    // t and c as they will be multiplied; q makes up for their rounding (a is the factor of what is far from 1 already:
+    // 4.5 units of the last place off in every step otherwise)
+    c = (float)c;
+    t = (float)(-b / (2 * c)), q = a - c * t * t, f = 0;
+  }
+  double top = 1, high = 0;  // the largest |X|, and |F| so far
   for (int k = 0; k < steps; ++k) {
     const auto X = [&](double s) { return fabs(s * (a + s * s * (b + s * s * c))); };
-    const auto B = [&](double t) { return fabs(t * (b + t * c)); };
+    const auto Q = [&](double v) { return a + v * (b + v * c); };
     const double t1 = top * top;
-    double x = X(top), p = B(t1);
-    const double tb = c != 0 ? -b / (2 * c) : -1;  // where b + 2 c t = 0
-    if (tb > 0 && tb < t1) p = fmax(p, B(tb));
-    // where a + 3 b t + 5 c t t = 0
-    double t[2] = {-1, -1};
+    double x = X(top), now = fmax(fabs(Q(0)), fabs(Q(t1))), e = fmax(fabs(Q(0) - q), fabs(Q(t1) - q));
+    const double tb = c != 0 ? -b / (2 * c) : -1;  // where b + 2 c v = 0
+    if (tb > 0 && tb < t1) now = fmax(now, fabs(Q(tb))), e = fmax(e, fabs(Q(tb) - q));
+    // where a + 3 b v + 5 c v v = 0
+    double z[2] = {-1, -1};
     if (c != 0) {
-      const double q = 9 * b * b - 20 * a * c;
-      if (q >= 0) t[0] = (-3 * b + sqrt(q)) / (10 * c), t[1] = (-3 * b - sqrt(q)) / (10 * c);
+      const double w = 9 * b * b - 20 * a * c;
+      if (w >= 0) z[0] = (-3 * b + sqrt(w)) / (10 * c), z[1] = (-3 * b - sqrt(w)) / (10 * c);
     } else if (b != 0) {
-      t[0] = -a / (3 * b);
+      z[0] = -a / (3 * b);
     }
-    for (double v : t)
+    for (double v : z)
       if (v > 0 && v < t1) x = fmax(x, X(sqrt(v)));
-    if (!(t1 <= most) || !(p <= most) || !(x <= most)) return false;
+    high = fmax(high, now);
+    if (!(t1 <= most) || !(x <= most) || !(x * top <= most) || !(e <= most)) return r;
     top = 1.01 * x;
   }
-  return true;
+  r.t = (float)t, r.q = (float)q, r.l = (float)f;
+  const double room = 65504.0 / R_SCALE / 1.05;  // R off its diagonal: that of R - q^g I
+  q = fabs(q);
+  r.longest = high * high * high + q * q * q <= room ? 3 : high * high + q * q <= room ? 2 : 1;
+  return r;
 }
 
 template <typename T>
 int run(int count, const void* const* src, void* const* dst, float* const* buf, const int* rows, const int* cols,
-        const float* rates, float decay, float mu, int nesterov, int steps, float a, float b, float c, double eps,
-        const Plan& p, char* ws, hipStream_t st) {
-  Mat* table = reinterpret_cast<Mat*>(ws + p.table);
-  Tile* tri = reinterpret_cast<Tile*>(ws + p.tri);
-  Tile* rect = reinterpret_cast<Tile*>(ws + p.rect);
-  uint2* norm_map = reinterpret_cast<uint2*>(ws + p.norm_map);
+        const float* rates, float decay, float mu, int nesterov, int steps, const Poly& f, double eps, const Plan& p, char* ws,
+        hipStream_t st) {
+  Lists l = p.l;
+  l.table = reinterpret_cast<Mat*>(ws + p.table);
+  l.gram = reinterpret_cast<Tile*>(ws + p.gram);
+  l.tri = reinterpret_cast<Tile*>(ws + p.tri);
+  l.rect = reinterpret_cast<Tile*>(ws + p.rect);
+  l.fill = reinterpret_cast<Tile*>(ws + p.fill);
+  l.norm_map = reinterpret_cast<uint2*>(ws + p.norm_map);
   double* norms = reinterpret_cast<double*>(ws + p.norms);
-  unsigned* counters = reinterpret_cast<unsigned*>(ws + p.counters);
   float* parts = reinterpret_cast<float*>(ws + p.parts);
   _Float16* base = reinterpret_cast<_Float16*>(ws + p.halves);
   const int update = buf != nullptr;
-  unsigned n_tri = 0, n_rect = 0, n_norm = 0;
-  size_t halves = 0;
+  unsigned gram = 0, tri = 0, rect = 0, fill = 0, norm = 0;
+  size_t halves = 0, part = 0;
   for (int first = 0; first < count; first += BATCH) {
-    Batch batch;
+    Batch batch{};
     const int many = count - first < BATCH ? count - first : BATCH;
     for (int k = 0; k < many; ++k) {
       const int i = first + k;
-      const Dim d(rows[i], cols[i]);
+      const Dim d(rows[i], cols[i], l.pad);
       const unsigned s = (unsigned)((d.mp + p.kc - 1) / p.kc);
-      batch.m[k] = Mat{src[i], dst[i], update ? buf[i] : nullptr, rows[i], cols[i], rates ? rates[i] : 0.f, (int)s, n_tri,
-                       n_rect, n_norm, n_tri, halves};
-      n_tri += d.tri() * s;
-      n_rect += d.rect();
-      n_norm += d.norms();
+      batch.m[k] = Mat{src[i], dst[i], update ? buf[i] : nullptr, rows[i], cols[i], rates ? rates[i] : 0.f, (int)s, gram,
+                       tri, rect, fill, norm, part, halves};
+      gram += d.tri(l.gram_ts) * s;
+      tri += d.tri(l.tri_ts);
+      rect += d.rect(l.rect_ts);
+      fill += d.rect(64);
+      norm += d.norms();
+      if (s > 1) part += (size_t)d.tri(l.gram_ts) * s * l.gram_ts * l.gram_ts;
       halves += d.halves();
     }
-    hipLaunchKernelGGL(ortho_table_kernel, dim3(1), dim3(64), 0, st, batch, many, table + first);
+    hipLaunchKernelGGL(ortho_table_kernel, dim3(1), dim3(64), 0, st, batch, many, l.table + first);
     if (hipGetLastError() != hipSuccess) return -2;
   }
-  unsigned blocks = (n_rect > n_tri ? n_rect : n_tri) / 256 + 1;
+  unsigned blocks = (l.n_fill > l.n_gram ? l.n_fill : l.n_gram) / 256 + 1;
   if (blocks > 1024) blocks = 1024;
-  hipLaunchKernelGGL(ortho_lists_kernel, dim3(blocks), dim3(256), 0, st, table, count, tri, n_tri, rect, n_rect, norm_map,
-                     n_norm, counters, p.n_part);
-  hipLaunchKernelGGL((ortho_norm_kernel<T>), dim3(n_norm), dim3(256), 0, st, table, norm_map, norms, update, mu, nesterov);
-  hipLaunchKernelGGL((ortho_start_kernel<T>), dim3(n_rect), dim3(256), 0, st, table, rect, norms, base, update, mu, nesterov, eps);
+  const dim3 wg(256);
+  hipLaunchKernelGGL(ortho_lists_kernel, dim3(blocks), wg, 0, st, l);
+  hipLaunchKernelGGL((ortho_norm_kernel<T>), dim3(l.n_norm), wg, 0, st, l, norms, update, mu, nesterov);
+  hipLaunchKernelGGL((ortho_start_kernel<T>), dim3(l.n_fill), wg, 0, st, l, norms, base, update, mu, nesterov, eps);
   if (hipGetLastError() != hipSuccess) return -2;
-  for (int k = 0; k < steps; ++k) {
-    hipLaunchKernelGGL(ortho_gram_kernel, dim3(n_tri), dim3(256), 0, st, table, tri, base, parts, counters, p.kc);
-    hipLaunchKernelGGL(ortho_poly_kernel, dim3(n_tri), dim3(256), 0, st, table, tri, base, b, c);
-    if (k + 1 < steps)
-      hipLaunchKernelGGL((ortho_apply_kernel<T, false>), dim3(n_rect), dim3(256), 0, st, table, rect, base, a, k & 1, update,
-                         decay);
+  const auto square = [&](const Op& one, const Op* two) {
+    const dim3 g(l.n_tri, two ? 2 : 1);
+    if (l.tri_ts == 128) hipLaunchKernelGGL((ortho_square_kernel<128>), g, wg, 0, st, l, base, one, two ? *two : one);
+    else hipLaunchKernelGGL((ortho_square_kernel<64>), g, wg, 0, st, l, base, one, two ? *two : one);
+  };
+  // G H, stored 2^so times from 2^sg and 2^sh times
+  const auto times = [](int out, int g, int h, float so, float sg, float sh) {
+    return Op{out, g, h, 0.f, 0.f, 0.f, 1.f, so / sg, so / sh, so / (sg * sh), 1.f / so};
+  };
+  int from = 0;
+  for (int left = steps; left > 0;) {
+    int g = group_length(left, steps);
+    if (g > f.longest) g = f.longest;
+    if (l.gram_ts == 128) {
+      hipLaunchKernelGGL((ortho_gram_kernel<128>), dim3(l.n_gram), wg, 0, st, l, base, parts, p.kc);
+      if (p.split) hipLaunchKernelGGL((ortho_sum_kernel<128>), dim3(l.n_gram, 4), wg, 0, st, l, base, parts);
+    } else {
+      hipLaunchKernelGGL((ortho_gram_kernel<64>), dim3(l.n_gram), wg, 0, st, l, base, parts, p.kc);
+      if (p.split) hipLaunchKernelGGL((ortho_sum_kernel<64>), dim3(l.n_gram, 2), wg, 0, st, l, base, parts);
+    }
+    int R = SQ_F, spare = SQ_R;
+    float scale = SCALE;  // R's
+    for (int k = 0; k < g; ++k) {
+      const int F = SQ_F + (k & 1);
+      square(Op{F, SQ_A, SQ_A, f.t, f.q, f.l, f.c, f.c, f.c, f.c / SCALE, 1.f / SCALE}, nullptr);
+      const Op FA = times(SQ_FA, F, SQ_A, SCALE, SCALE, SCALE);
+      if (k) {
+        const Op next = times(spare, F, R, R_SCALE, SCALE, scale);
+        if (k + 1 < g) square(next, &FA);
+        else square(next, nullptr);
+        R = spare, spare = SQ_R + (R == SQ_R), scale = R_SCALE;
+      } else if (k + 1 < g) {
+        square(FA, nullptr);
+      }
+      if (k + 1 < g) square(times(SQ_A, F, SQ_FA, SCALE, SCALE, SCALE), nullptr);
+    }
+    left -= g;
+    const float fs = 1.f / scale;
+    const dim3 grid(l.n_rect);
+    if (left && l.rect_ts == 128)
+      hipLaunchKernelGGL((ortho_apply_kernel<T, false, 128>), grid, wg, 0, st, l, base, R, fs, from, update, decay);
+    else if (left)
+      hipLaunchKernelGGL((ortho_apply_kernel<T, false, 64>), grid, wg, 0, st, l, base, R, fs, from, update, decay);
+    else if (l.rect_ts == 128)
+      hipLaunchKernelGGL((ortho_apply_kernel<T, true, 128>), grid, wg, 0, st, l, base, R, fs, from, update, decay);
     else
-      hipLaunchKernelGGL((ortho_apply_kernel<T, true>), dim3(n_rect), dim3(256), 0, st, table, rect, base, a, k & 1, update,
-                         decay);
+      hipLaunchKernelGGL((ortho_apply_kernel<T, true, 64>), grid, wg, 0, st, l, base, R, fs, from, update, decay);
+    from ^= 1;
     if (hipGetLastError() != hipSuccess) return -2;
   }
   return 0;
@@ -507,9 +760,9 @@ int r3k_ortho(int count, const void* const* src, void* const* dst, float* const*
               const int* cols, const float* rates, float decay, float mu, int nesterov, int steps, float a, float b, float c,
               double eps, void* ws, size_t ws_bytes, hipStream_t st) {
   Plan p;
-  if (plan(count, rows, cols, p) != 0 || dtype < 0 || dtype > 2 || steps < 1 || steps > 64 || !(eps >= 0) ||
-      !bounded(steps, a, b, c))
-    return -1;
+  if (plan(count, rows, cols, p) != 0 || dtype < 0 || dtype > 2 || steps < 1 || steps > 64 || !(eps >= 0)) return -1;
+  const Poly f = polynomial(steps, a, b, c);
+  if (!f.longest) return -1;
   if (count == 0) return 0;
   if (!src || !dst || (buf && !rates)) return -1;
   for (int i = 0; i < count; ++i)
@@ -518,8 +771,8 @@ int r3k_ortho(int count, const void* const* src, void* const* dst, float* const*
   char* w = static_cast<char*>(ws);
   if (reinterpret_cast<uintptr_t>(w) & 15) return -1;
   switch (dtype) {
-    case 0: return run<float>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, a, b, c, eps, p, w, st);
-    case 1: return run<_Float16>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, a, b, c, eps, p, w, st);
-    default: return run<__bf16>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, a, b, c, eps, p, w, st);
+    case 0: return run<float>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, p, w, st);
+    case 1: return run<_Float16>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, p, w, st);
+    default: return run<__bf16>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, p, w, st);
   }
 }

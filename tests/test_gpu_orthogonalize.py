@@ -8,7 +8,12 @@ step's largest slope: the slopes a + 3 b s^2 + 5 c s^4, the quotients p(s) / s a
 polynomial lie below 4 on [0, 1.21] for the usual coefficients, so the error of `steps` steps is at most
 sum_k 4^(steps - k) e_k.  That holds for every spectrum; for the ones here the op-by-op form in fp32 says much more, so
 the result must also be no further from 64 bits than three times that form is (their roundings have like sizes and
-different signs).  A result of 16 bits adds half a step of its own."""
+different signs).  A result of 16 bits adds half a step of its own.
+
+The second bound says nothing for a matrix of equal rows (``alike``).  The op-by-op form rounds equal rows equally, so its
+error stays in the one direction the matrix has, where the slope is small; any form that sums an entry's terms in an order
+of its own (in blocks, or with the diagonal apart) has errors in the directions the matrix does not have, where a step
+multiplies them by a = 3.4445 exactly.  There the first bound holds alone, with the slope a."""
 import math
 
 import pytest
@@ -38,23 +43,23 @@ def iterate(g, steps=5, co=COEFFICIENTS, eps=1e-7, dtype=torch.float64):
     return (x.t() if tall else x).reshape(g.shape), norms
 
 
-def tolerances(g, norms, plain_error, steps, dtype, slope=4.0):
+def tolerances(g, norms, plain_error, steps, dtype, slope=4.0, alike=False):
     k = max(g.size(0), g.numel() // g.size(0))
     e = (32 + 10 * math.sqrt(k)) * U
     proven = sum(slope ** (steps - i) * e * norms[i] for i in range(steps)) + e * norms[-1]
-    yard = 3 * plain_error + 16 * U * norms[-1]
+    yard = math.inf if alike else 3 * plain_error + 16 * U * norms[-1]
     t = torch.finfo(dtype)
     own = 0.0 if dtype == torch.float32 else t.eps / 2 * norms[-1] + t.smallest_normal * t.eps / 2 * math.sqrt(g.numel())
     return min(proven, yard) + own
 
 
-def check(tensors, steps=5, co=COEFFICIENTS, eps=1e-7, slope=4.0):
+def check(tensors, steps=5, co=COEFFICIENTS, eps=1e-7, slope=4.0, alike=False):
     got = orthogonalize(tensors, steps=steps, coefficients=co, eps=eps)
     for g, o in zip(tensors, got):
         assert o.shape == g.shape and o.dtype == g.dtype and o.is_contiguous()
         want, norms = iterate(g, steps, co, eps)
         plain = iterate(g, steps, co, eps, torch.float32)[0]
-        tol = tolerances(g, norms, (plain.double() - want).norm().item(), steps, o.dtype, slope)
+        tol = tolerances(g, norms, (plain.double() - want).norm().item(), steps, o.dtype, slope, alike)
         off = (o.double() - want).norm().item()
         assert off <= tol, (tuple(g.shape), off, tol, norms[-1])
     return got
@@ -88,7 +93,10 @@ def test_shapes(shape, dtype):
 @pytest.mark.parametrize("kind", ["low", "rank1", "ones", "eye"])
 @pytest.mark.parametrize("shape", [(64, 64), (200, 130), (256, 1280), (512, 600)], ids=str)
 def test_spectra(shape, kind):
-    check([matrix(*shape, kind=kind)])
+    if kind == "ones":
+        check([matrix(*shape, kind=kind)], slope=COEFFICIENTS[0], alike=True)
+    else:
+        check([matrix(*shape, kind=kind)])
 
 
 def test_a_ragged_list_of_many():
@@ -134,7 +142,8 @@ def test_nan_and_inf_stay_in_their_matrix():
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_layouts(dtype):
     base = matrix(140, 200, dtype=dtype)
-    check([base.t(), base[::2], base[:, 1:], base[:, ::3], base[3:40, 5:9], base[:1].expand(30, 200)])
+    check([base.t(), base[::2], base[:, 1:], base[:, ::3], base[3:40, 5:9]])
+    check([base[:1].expand(30, 200)], slope=COEFFICIENTS[0], alike=True)
     conv = base.reshape(140, 8, 5, 5)
     got = check([conv, conv.contiguous(memory_format=torch.channels_last)])
     assert torch.equal(got[0], got[1])
