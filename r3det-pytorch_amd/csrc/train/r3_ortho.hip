@@ -31,6 +31,8 @@
 #include <hip/hip_runtime.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "../r3_kernels.h"
 
 namespace {
@@ -95,6 +97,7 @@ struct Lists {  // one entry a workgroup
   uint2* norm_map;  // (matrix, chunk)
   unsigned n_gram, n_tri, n_rect, n_fill, n_norm;
   int count, pad, gram_ts, tri_ts, rect_ts;
+  int gram_g, tri_g, rect_g;  // groups of wavefronts a workgroup
 };
 
 // the whole workspace; every part is a multiple of 256 bytes
@@ -198,7 +201,14 @@ __device__ __forceinline__ void split16(float v, _Float16& hi, _Float16& lo) {
   hi = (_Float16)v;
   lo = (_Float16)(v - (float)hi);
 }
-__device__ __forceinline__ void store8(_Float16* at, size_t lo, const float (&v)[8]) {
+// Arrays are kept in blocks of 64 rows by 32 columns, row by row of blocks: 4 KB of hi, 4 KB of lo, 8 KB in all, each row of a
+// block 64 bytes.  What a stage of a product reads is then whole blocks, one behind the other.  (Plain rows are read 64
+// bytes at a time, half a cache line, and at a power of two apart: 76 us for 2048 x 2048 against XX.)
+constexpr int LO = 64 * 32, BLOCK = 2 * LO;
+__device__ __forceinline__ size_t place(int r, int c, int ld) {
+  return ((size_t)(r / 64) * (ld / 32) + c / 32) * BLOCK + r % 64 * 32 + c % 32;
+}
+__device__ __forceinline__ void store8(_Float16* at, const float (&v)[8]) {
   half8 h, l;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
@@ -207,19 +217,19 @@ __device__ __forceinline__ void store8(_Float16* at, size_t lo, const float (&v)
     h[k] = hh, l[k] = ll;
   }
   *reinterpret_cast<half8*>(at) = h;
-  *reinterpret_cast<half8*>(at + lo) = l;
+  *reinterpret_cast<half8*>(at + LO) = l;
 }
-__device__ __forceinline__ void add8(float (&v)[8], float f, const _Float16* at, size_t lo) {
-  const half8 h = *reinterpret_cast<const half8*>(at), l = *reinterpret_cast<const half8*>(at + lo);
+__device__ __forceinline__ void add8(float (&v)[8], float f, const _Float16* at) {
+  const half8 h = *reinterpret_cast<const half8*>(at), l = *reinterpret_cast<const half8*>(at + LO);
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = fmaf(f, (float)h[k] + (float)l[k], v[k]);
 }
 // ROWS x COLS of fp32 in shared memory, rows of LD: f(row, column, eight values), which may change them; then `f`'s values
 // are in shared memory too.
-template <int ROWS, int COLS, int LD, typename F>
+template <int ROWS, int COLS, int LD, int THREADS, typename F>
 __device__ __forceinline__ void rows8(float* E, const F& f) {
 #pragma unroll 2
-  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += 256) {
+  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += THREADS) {
     const int r = q / (COLS / 8), c = q % (COLS / 8) * 8;
     float v[8];
 #pragma unroll
@@ -229,16 +239,16 @@ __device__ __forceinline__ void rows8(float* E, const F& f) {
     for (int k = 0; k < 8; ++k) E[r * LD + c + k] = v[k];
   }
 }
-// The transpose of ROWS x COLS in shared memory -> hi / lo arrays with rows of `ld`, at (r0, c0).
-template <int ROWS, int COLS, int LD>
-__device__ __forceinline__ void store_turned(const float* E, _Float16* p, size_t lo, size_t ld, int r0, int c0) {
+// The transpose of ROWS x COLS in shared memory -> an array of `ld` columns, at (r0, c0).
+template <int ROWS, int COLS, int LD, int THREADS>
+__device__ __forceinline__ void store_turned(const float* E, _Float16* p, int ld, int r0, int c0) {
 #pragma unroll 2
-  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += 256) {
+  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += THREADS) {
     const int r = q / (ROWS / 8), c = q % (ROWS / 8) * 8;
     float v[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = E[(c + k) * LD + r];
-    store8(p + (size_t)(r0 + r) * ld + c0 + c, lo, v);
+    store8(p + place(r0 + r, c0 + c, ld), v);
   }
 }
 
@@ -270,86 +280,102 @@ __global__ __launch_bounds__(256) void ortho_start_kernel(Lists l, const double*
     E[r * 65 + c] = v;
   }
   __syncthreads();
-  rows8<64, 64, 65>(E, [&](int r, int c, float (&v)[8]) { store8(o.x + (size_t)(i0 + r) * d.mp + j0 + c, d.x(), v); });
-  store_turned<64, 64, 65>(E, o.xt, d.x(), d.np, j0, i0);
+  rows8<64, 64, 65, 256>(E, [&](int r, int c, float (&v)[8]) { store8(o.x + place(i0 + r, j0 + c, d.mp), v); });
+  store_turned<64, 64, 65, 256>(E, o.xt, d.np, j0, i0);
 }
 
 // ------------------------------------------------------------------------------------------------ the products
-// One TS x TS tile of P Q^t by 4 wavefronts, a quarter each: P, Q (hi, lo) with the summed index [k0, k1) contiguous, rows of
-// ldp / ldq.  A stage is 4 x 8 KB of shared memory -- 32 of the summed index at tiles of 128, 64 at tiles of 64 -- and comes
-// through registers: its loads are issued a stage ahead and have a stage's products to arrive in.  (Loads straight into
-// shared memory do not overlap here: before a stage is read, the compiler waits for every such load in flight, the next
-// stage's too.)  The 16-byte piece c of row r sits at c ^ (r / 2 % 4) or c ^ (r % 8): eight rows that are read together then
-// lie in different banks.
+// One TS x TS tile of P Q^t: P, Q arrays of ldp / ldq columns, of which [k0, k1) are summed; the tile's first rows given.  A
+// group of 4 wavefronts takes a quarter of the tile each; G groups take the stages of the sum in turn and are added at the
+// end, so that a tile that has a compute unit to itself still has two wavefronts on each of its matrix cores.  A stage is 4
+// x 8 KB of shared memory -- 32 of the summed index at tiles of 128, 64 at tiles of 64 -- and comes through registers: the
+// next one's loads are on their way while one is computed.  (Loads straight into shared memory do not overlap: before any
+// of it is read, the compiler waits for every such load in flight.)  The 16-byte piece c of row r sits at c ^ (r / 4 % 4)
+// or c ^ (r / 2 % 8): sixteen rows that are read together then lie in different banks.
 struct Stage {
   half8 v[4][512];
 };
-template <int TS>
+template <int TS, int G>
+union Shared {
+  Stage st[2 * G];
+  float E[TS * (TS + 1)];
+};
+template <int TS, int G>
 struct Core {
   static constexpr int BK = TS == 128 ? 32 : 64, PIECES = BK / 8, M = TS / 64;
   static constexpr int LD = TS + 1;
-  static __device__ __forceinline__ int place(int r, int c) {
-    return r * PIECES + (c ^ (PIECES == 4 ? r / 2 % 4 : r % 8));
+  static __device__ __forceinline__ int spot(int r, int c) {
+    return r * PIECES + (c ^ (PIECES == 4 ? r / 4 % 4 : r / 2 % 8));
   }
   float16v hh[M][M], hl[M][M];  // hi hi, and the two others
   half8 next[8];
 
-  __device__ __forceinline__ void fetch(const _Float16* p, size_t plo, size_t ldp, const _Float16* q, size_t qlo, size_t ldq,
-                                        int k) {
+  struct Source {  // this thread's pieces of the first two blocks of a stage, and how far the next stage's are
+    const _Float16 *p[2], *q[2];
+  };
+  __device__ __forceinline__ void fetch(const Source& s, int stage) {
+    const size_t k = (size_t)stage * (BK / 32 * BLOCK);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int slot = t * 256 + threadIdx.x, r = slot / PIECES, c = slot % PIECES;
-      const _Float16 *a = p + (size_t)r * ldp + k + c * 8, *b = q + (size_t)r * ldq + k + c * 8;
-      next[t] = *reinterpret_cast<const half8*>(a);
-      next[2 + t] = *reinterpret_cast<const half8*>(a + plo);
-      next[4 + t] = *reinterpret_cast<const half8*>(b);
-      next[6 + t] = *reinterpret_cast<const half8*>(b + qlo);
+      next[t] = *reinterpret_cast<const half8*>(s.p[t] + k + threadIdx.x % 256 * 8);
+      next[2 + t] = *reinterpret_cast<const half8*>(s.p[t] + k + LO + threadIdx.x % 256 * 8);
+      next[4 + t] = *reinterpret_cast<const half8*>(s.q[t] + k + threadIdx.x % 256 * 8);
+      next[6 + t] = *reinterpret_cast<const half8*>(s.q[t] + k + LO + threadIdx.x % 256 * 8);
     }
   }
   __device__ __forceinline__ void put(Stage& s) const {
+    const int r = threadIdx.x % 256 / 4, c = threadIdx.x % 4;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int slot = t * 256 + threadIdx.x, at = place(slot / PIECES, slot % PIECES);
+      const int at = TS == 128 ? spot(t * 64 + r, c) : spot(r, t * 4 + c);
 #pragma unroll
       for (int a = 0; a < 4; ++a) s.v[a][at] = next[2 * a + t];
     }
   }
-  __device__ __forceinline__ void run(Stage* st, const _Float16* p, size_t plo, size_t ldp, const _Float16* q, size_t qlo,
-                                      size_t ldq, int k0, int k1) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  __device__ __forceinline__ void compute(const Stage& s) {
+    const int wave = threadIdx.x >> 6 & 3, lane = threadIdx.x & 63;
     const int pr = (wave >> 1) * (TS / 2) + (lane & 31), qr = (wave & 1) * (TS / 2) + (lane & 31), kc = lane >> 5;
-    fetch(p, plo, ldp, q, qlo, ldq, k0);
+#pragma unroll
+    for (int kk = 0; kk < BK / 16; ++kk) {
+      half8 ph[M], pl[M], qh[M], ql[M];
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        const int ps = spot(pr + 32 * i, kk * 2 + kc), qs = spot(qr + 32 * i, kk * 2 + kc);
+        ph[i] = s.v[0][ps], pl[i] = s.v[1][ps], qh[i] = s.v[2][qs], ql[i] = s.v[3][qs];
+      }
+#pragma unroll
+      for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int j = 0; j < M; ++j) {
+          hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], hl[i][j], 0, 0, 0);
+          hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], hl[i][j], 0, 0, 0);
+          hh[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], hh[i][j], 0, 0, 0);
+        }
+    }
+  }
+  __device__ __forceinline__ void run(Stage* all, const _Float16* p, int prow, int ldp, const _Float16* q, int qrow, int ldq,
+                                      int k0, int k1) {
+    const int group = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 256);
+    Stage* st = all + 2 * group;
+    Source src;
+    src.p[0] = p + place(prow, k0, ldp), src.p[1] = TS == 128 ? p + place(prow + 64, k0, ldp) : src.p[0] + BLOCK;
+    src.q[0] = q + place(qrow, k0, ldq), src.q[1] = TS == 128 ? q + place(qrow + 64, k0, ldq) : src.q[0] + BLOCK;
+    const int stages = (k1 - k0) / BK;
+    if (group < stages) fetch(src, group);
 #pragma unroll
     for (int i = 0; i < M; ++i)
 #pragma unroll
       for (int j = 0; j < M; ++j) hh[i][j] = float16v{}, hl[i][j] = float16v{};
-    put(st[0]);
-    if (k0 + BK < k1) fetch(p, plo, ldp, q, qlo, ldq, k0 + BK);
+    if (group < stages) put(st[0]);
+    if (group + G < stages) fetch(src, group + G);
     __syncthreads();
     int cur = 0;
-    for (int k = k0; k < k1; k += BK) {
-      const Stage& s = st[cur];
-#pragma unroll
-      for (int kk = 0; kk < BK / 16; ++kk) {
-        half8 ph[M], pl[M], qh[M], ql[M];
-#pragma unroll
-        for (int i = 0; i < M; ++i) {
-          const int ps = place(pr + 32 * i, kk * 2 + kc), qs = place(qr + 32 * i, kk * 2 + kc);
-          ph[i] = s.v[0][ps], pl[i] = s.v[1][ps], qh[i] = s.v[2][qs], ql[i] = s.v[3][qs];
-        }
-#pragma unroll
-        for (int i = 0; i < M; ++i)
-#pragma unroll
-          for (int j = 0; j < M; ++j) {
-            hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], hl[i][j], 0, 0, 0);
-            hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], hl[i][j], 0, 0, 0);
-            hh[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], hh[i][j], 0, 0, 0);
-          }
-      }
+    for (int s = group; s - group < stages; s += G) {  // (every group as often: the barrier is everyone's)
+      if (s < stages) compute(st[cur]);
       cur ^= 1;
-      if (k + BK < k1) {
-        put(st[cur]);  // (everyone left this stage before the last barrier)
-        if (k + 2 * BK < k1) fetch(p, plo, ldp, q, qlo, ldq, k + 2 * BK);
+      if (s + G < stages) {
+        put(st[cur]);  // (everyone left that stage before the last barrier)
+        if (s + 2 * G < stages) fetch(src, s + 2 * G);
       }
       __syncthreads();  // (behind the last stage: the stages' memory is the epilogue's too)
     }
@@ -357,7 +383,7 @@ struct Core {
   // lane l of the matrix instruction holds column l % 32 and rows 8 (r / 4) + 4 (l / 32) + r % 4
   template <typename F>
   __device__ __forceinline__ void each(const F& f) const {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = threadIdx.x >> 6 & 3, lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < M; ++i)
 #pragma unroll
@@ -367,55 +393,55 @@ struct Core {
           f((wave >> 1) * (TS / 2) + 32 * i + 8 * (r / 4) + 4 * (lane >> 5) + r % 4,
             (wave & 1) * (TS / 2) + 32 * j + (lane & 31), hh[i][j][r] + hl[i][j][r]);
   }
-  // ... times f, into shared memory
+  // the groups' sum times f, into shared memory
   __device__ __forceinline__ void spill(float* E, float f) const {
-    each([&](int r, int c, float v) { E[r * LD + c] = v * f; });
-    __syncthreads();
+#pragma unroll
+    for (int g = G - 1; g >= 0; --g) {
+      if (G == 1 || (int)(threadIdx.x / 256) == g)
+        each([&](int r, int c, float v) { E[r * LD + c] = g == G - 1 ? v * f : fmaf(v, f, E[r * LD + c]); });
+      __syncthreads();
+    }
   }
-};
-template <int TS>
-union Shared {
-  Stage st[2];
-  float E[TS * (TS + 1)];
 };
 
 // A from ROWS rows of a tile in shared memory
-template <int ROWS, int TS>
+template <int ROWS, int TS, int THREADS>
 __device__ __forceinline__ void store_gram(float* E, const Dim& d, const Area& o, int i0, int j0, bool diagonal) {
   _Float16* a = o.sq + SQ_A * 2 * d.a();
-  rows8<ROWS, TS, TS + 1>(E, [&](int r, int c, float (&v)[8]) {
+  rows8<ROWS, TS, TS + 1, THREADS>(E, [&](int r, int c, float (&v)[8]) {
     if (diagonal)
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         if (i0 + r == j0 + c + k) o.diag[SQ_A * d.np + i0 + r] = v[k] * (1.f / SCALE), v[k] = 0.f;
-    store8(a + (size_t)(i0 + r) * d.np + j0 + c, d.a(), v);
+    store8(a + place(i0 + r, j0 + c, d.np), v);
   });
   if (!diagonal) {
     __syncthreads();
-    store_turned<ROWS, TS, TS + 1>(E, a, d.a(), d.np, j0, i0);
+    store_turned<ROWS, TS, TS + 1, THREADS>(E, a, d.np, j0, i0);
   }
 }
 // A = X X^t: a tile on or above the diagonal, or one part of its sum, which ortho_sum_kernel adds up in their order.
 // (Adding them in the workgroup that ends last needs the other workgroups' tiles flushed through the XCDs' caches: 160 us
 // where this and the launch behind it take 20, at eight 256 x 2304 matrices.)
-template <int TS>
-__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Lists l, _Float16* base, float* parts, int kc) {
-  __shared__ Shared<TS> sh;
+template <int TS, int G>
+__global__ __launch_bounds__(256 * G, 2) void ortho_gram_kernel(Lists l, _Float16* base, float* parts, int kc) {
+  __shared__ Shared<TS, G> sh;
   const Tile w = l.gram[blockIdx.x];
   const Mat t = l.table[w.mat];
   const Dim d(t.rows, t.cols, l.pad);
   const Area o(base, t, d);
   const int i0 = w.i * TS, j0 = w.j * TS;
   const int k0 = w.split * kc, k1 = k0 + kc < d.mp ? k0 + kc : d.mp;
-  Core<TS> core;
-  core.run(sh.st, o.x + (size_t)i0 * d.mp, d.x(), d.mp, o.x + (size_t)j0 * d.mp, d.x(), d.mp, k0, k1);
+  Core<TS, G> core;
+  core.run(sh.st, o.x, i0, d.mp, o.x, j0, d.mp, k0, k1);
   if (t.splits > 1) {
     float* mine = parts + t.part0 + (size_t)(blockIdx.x - t.gram0) * (TS * TS);
-    core.each([&](int r, int c, float v) { mine[r * TS + c] = v * (1.f / SCALE); });
+    core.spill(sh.E, 1.f / SCALE);
+    for (int q = threadIdx.x; q < TS * TS; q += 256 * G) mine[q] = sh.E[q / TS * (TS + 1) + q % TS];
     return;
   }
   core.spill(sh.E, 1.f / SCALE);
-  store_gram<TS, TS>(sh.E, d, o, i0, j0, w.i == w.j);
+  store_gram<TS, TS, 256 * G>(sh.E, d, o, i0, j0, w.i == w.j);
 }
 // 32 rows of a tile of A from its parts
 template <int TS>
@@ -441,7 +467,7 @@ __global__ __launch_bounds__(256) void ortho_sum_kernel(Lists l, _Float16* base,
     e[0] = v.x, e[1] = v.y, e[2] = v.z, e[3] = v.w;
   }
   __syncthreads();
-  store_gram<32, TS>(E, d, o, w.i * TS + slice, w.j * TS, w.i == w.j);
+  store_gram<32, TS, 256>(E, d, o, w.i * TS + slice, w.j * TS, w.i == w.j);
 }
 
 // out = q I + l G + f (G - t I) (H - t I) of symmetric matrices that commute (all are polynomials of one): a tile on or above
@@ -450,28 +476,28 @@ struct Op {
   int out, g, h;  // which arrays
   float t, q, l, f, fg, fh, fs, back;  // back: one over out's scale
 };
-template <int TS>
-__global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
-  __shared__ Shared<TS> sh;
+template <int TS, int G>
+__global__ __launch_bounds__(256 * G, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
+  __shared__ Shared<TS, G> sh;
   const Tile w = l.tri[blockIdx.x];
   const Mat t = l.table[w.mat];
   const Dim d(t.rows, t.cols, l.pad);
   const Area o(base, t, d);
   const Op op = blockIdx.y ? second : first;
   const int i0 = w.i * TS, j0 = w.j * TS;
-  const size_t lo = d.a(), step = 2 * lo;
+  const size_t step = 2 * d.a();
   const _Float16 *g = o.sq + op.g * step, *h = o.sq + op.h * step;
   const float *gd = o.diag + op.g * d.np, *hd = o.diag + op.h * d.np;
-  Core<TS> core;
-  core.run(sh.st, g + (size_t)i0 * d.np, lo, d.np, h + (size_t)j0 * d.np, lo, d.np, 0, d.np);
+  Core<TS, G> core;
+  core.run(sh.st, g, i0, d.np, h, j0, d.np, 0, d.np);
   core.spill(sh.E, 1.f);
   _Float16* out = o.sq + op.out * step;
   const bool diagonal = w.i == w.j;
-  rows8<TS, TS, TS + 1>(sh.E, [&](int r, int c, float (&v)[8]) {
+  rows8<TS, TS, TS + 1, 256 * G>(sh.E, [&](int r, int c, float (&v)[8]) {
     const int i = i0 + r, j = j0 + c;
-    const size_t at = (size_t)i * d.np + j;
-    const half8 gh = *reinterpret_cast<const half8*>(g + at), gl = *reinterpret_cast<const half8*>(g + at + lo);
-    const half8 hh = *reinterpret_cast<const half8*>(h + at), hl = *reinterpret_cast<const half8*>(h + at + lo);
+    const size_t at = place(i, j, d.np);
+    const half8 gh = *reinterpret_cast<const half8*>(g + at), gl = *reinterpret_cast<const half8*>(g + at + LO);
+    const half8 hh = *reinterpret_cast<const half8*>(h + at), hl = *reinterpret_cast<const half8*>(h + at + LO);
     const float gi = op.fh * (gd[i] - op.t);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -484,41 +510,41 @@ __global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16*
       }
       v[k] = e;
     }
-    store8(out + at, lo, v);
+    store8(out + at, v);
   });
   if (!diagonal) {
     __syncthreads();
-    store_turned<TS, TS, TS + 1>(sh.E, out, lo, d.np, j0, i0);
+    store_turned<TS, TS, TS + 1, 256 * G>(sh.E, out, d.np, j0, i0);
   }
 }
 
 // X <- R X, from X^t; the last group's goes to the caller, as the result or into the weights
-template <typename T, bool LAST, int TS>
-__global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* base, int R, float fs, int from, int update,
+template <typename T, bool LAST, int TS, int G>
+__global__ __launch_bounds__(256 * G, 2) void ortho_apply_kernel(Lists l, _Float16* base, int R, float fs, int from, int update,
                                                              float decay) {
-  __shared__ Shared<TS> sh;
+  __shared__ Shared<TS, G> sh;
   const Tile w = l.rect[blockIdx.x];
   const Mat t = l.table[w.mat];
   const Dim d(t.rows, t.cols, l.pad);
   const Area o(base, t, d);
   const int i0 = w.i * TS, j0 = w.j * TS;
   const _Float16 *a = o.sq + R * 2 * d.a(), *xt = o.xt + (from ? 2 * d.x() : 0);
-  Core<TS> core;
-  core.run(sh.st, a + (size_t)i0 * d.np, d.a(), d.np, xt + (size_t)j0 * d.np, d.x(), d.np, 0, d.np);
+  Core<TS, G> core;
+  core.run(sh.st, a, i0, d.np, xt, j0, d.np, 0, d.np);
   core.spill(sh.E, fs);
-  rows8<TS, TS, TS + 1>(sh.E, [&](int r, int c, float (&v)[8]) {
-    _Float16* x = o.x + (size_t)(i0 + r) * d.mp + j0 + c;
-    add8(v, o.diag[R * d.np + i0 + r], x, d.x());
-    if constexpr (!LAST) store8(x, d.x(), v);
+  rows8<TS, TS, TS + 1, 256 * G>(sh.E, [&](int r, int c, float (&v)[8]) {
+    _Float16* x = o.x + place(i0 + r, j0 + c, d.mp);
+    add8(v, o.diag[R * d.np + i0 + r], x);
+    if constexpr (!LAST) store8(x, v);
   });
   __syncthreads();
   if constexpr (!LAST) {
-    store_turned<TS, TS, TS + 1>(sh.E, o.xt + (from ? 0 : 2 * d.x()), d.x(), d.np, j0, i0);
+    store_turned<TS, TS, TS + 1, 256 * G>(sh.E, o.xt + (from ? 0 : 2 * d.x()), d.np, j0, i0);
   } else {
     const bool tall = t.rows > t.cols;
     T* out = static_cast<T*>(t.dst);
 #pragma unroll 4
-    for (int q = threadIdx.x; q < TS * TS; q += 256) {
+    for (int q = threadIdx.x; q < TS * TS; q += 256 * G) {
       const int r = tall ? q % TS : q / TS, c = tall ? q / TS : q % TS;
       const int i = i0 + r, j = j0 + c;
       if (i < d.n && j < d.m) {
@@ -583,6 +609,10 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   if (gram > 0x7fffffff || tri > 0x7fffffff || rect > 0x7fffffff || fill > 0x7fffffff || norm > 0x7fffffff) return -1;
   l.n_gram = (unsigned)gram, l.n_tri = (unsigned)tri, l.n_rect = (unsigned)rect, l.n_fill = (unsigned)fill;
   l.n_norm = (unsigned)norm;
+  // Two groups where that ends earlier: a compute unit holds two workgroups of one group or one of two.  (2048 x 2048,
+  // tiles of 128, X <- R X: 256 workgroups, 76 us with one group, XX with two.)
+  const auto groups = [](uint64_t n) { return (n + WANT / 2 - 1) / (WANT / 2) < 2 * ((n + WANT - 1) / WANT) ? 2 : 1; };
+  l.gram_g = groups(gram), l.tri_g = groups(tri), l.rect_g = groups(rect);
   size_t at = 0;
   const auto take = [&](size_t bytes) {
     const size_t was = at;
@@ -652,6 +682,16 @@ Poly polynomial(int steps, double a, double b, double c) {
   return r;
 }
 
+// f(tile, groups) as constants
+template <typename F>
+void choose(int ts, int g, const F& f) {
+  using std::integral_constant;
+  if (ts == 128 && g == 2) f(integral_constant<int, 128>(), integral_constant<int, 2>());
+  else if (ts == 128) f(integral_constant<int, 128>(), integral_constant<int, 1>());
+  else if (g == 2) f(integral_constant<int, 64>(), integral_constant<int, 2>());
+  else f(integral_constant<int, 64>(), integral_constant<int, 1>());
+}
+
 template <typename T>
 int run(int count, const void* const* src, void* const* dst, float* const* buf, const int* rows, const int* cols,
         const float* rates, float decay, float mu, int nesterov, int steps, const Poly& f, double eps, const Plan& p, char* ws,
@@ -697,9 +737,10 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
   hipLaunchKernelGGL((ortho_start_kernel<T>), dim3(l.n_fill), wg, 0, st, l, norms, base, update, mu, nesterov, eps);
   if (hipGetLastError() != hipSuccess) return -2;
   const auto square = [&](const Op& one, const Op* two) {
-    const dim3 g(l.n_tri, two ? 2 : 1);
-    if (l.tri_ts == 128) hipLaunchKernelGGL((ortho_square_kernel<128>), g, wg, 0, st, l, base, one, two ? *two : one);
-    else hipLaunchKernelGGL((ortho_square_kernel<64>), g, wg, 0, st, l, base, one, two ? *two : one);
+    choose(l.tri_ts, l.tri_g, [&](auto TS, auto G) {
+      hipLaunchKernelGGL((ortho_square_kernel<TS(), G()>), dim3(l.n_tri, two ? 2 : 1), dim3(256 * G()), 0, st, l, base, one,
+                         two ? *two : one);
+    });
   };
   // G H, stored 2^so times from 2^sg and 2^sh times
   const auto times = [](int out, int g, int h, float so, float sg, float sh) {
@@ -709,13 +750,10 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
   for (int left = steps; left > 0;) {
     int g = group_length(left, steps);
     if (g > f.longest) g = f.longest;
-    if (l.gram_ts == 128) {
-      hipLaunchKernelGGL((ortho_gram_kernel<128>), dim3(l.n_gram), wg, 0, st, l, base, parts, p.kc);
-      if (p.split) hipLaunchKernelGGL((ortho_sum_kernel<128>), dim3(l.n_gram, 4), wg, 0, st, l, base, parts);
-    } else {
-      hipLaunchKernelGGL((ortho_gram_kernel<64>), dim3(l.n_gram), wg, 0, st, l, base, parts, p.kc);
-      if (p.split) hipLaunchKernelGGL((ortho_sum_kernel<64>), dim3(l.n_gram, 2), wg, 0, st, l, base, parts);
-    }
+    choose(l.gram_ts, l.gram_g, [&](auto TS, auto G) {
+      hipLaunchKernelGGL((ortho_gram_kernel<TS(), G()>), dim3(l.n_gram), dim3(256 * G()), 0, st, l, base, parts, p.kc);
+      if (p.split) hipLaunchKernelGGL((ortho_sum_kernel<TS()>), dim3(l.n_gram, TS() / 32), wg, 0, st, l, base, parts);
+    });
     int R = SQ_F, spare = SQ_R;
     float scale = SCALE;  // R's
     for (int k = 0; k < g; ++k) {
@@ -734,15 +772,13 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
     }
     left -= g;
     const float fs = 1.f / scale;
-    const dim3 grid(l.n_rect);
-    if (left && l.rect_ts == 128)
-      hipLaunchKernelGGL((ortho_apply_kernel<T, false, 128>), grid, wg, 0, st, l, base, R, fs, from, update, decay);
-    else if (left)
-      hipLaunchKernelGGL((ortho_apply_kernel<T, false, 64>), grid, wg, 0, st, l, base, R, fs, from, update, decay);
-    else if (l.rect_ts == 128)
-      hipLaunchKernelGGL((ortho_apply_kernel<T, true, 128>), grid, wg, 0, st, l, base, R, fs, from, update, decay);
-    else
-      hipLaunchKernelGGL((ortho_apply_kernel<T, true, 64>), grid, wg, 0, st, l, base, R, fs, from, update, decay);
+    choose(l.rect_ts, l.rect_g, [&](auto TS, auto G) {
+      const dim3 grid(l.n_rect), block(256 * G());
+      if (left)
+        hipLaunchKernelGGL((ortho_apply_kernel<T, false, TS(), G()>), grid, block, 0, st, l, base, R, fs, from, update, decay);
+      else
+        hipLaunchKernelGGL((ortho_apply_kernel<T, true, TS(), G()>), grid, block, 0, st, l, base, R, fs, from, update, decay);
+    });
     from ^= 1;
     if (hipGetLastError() != hipSuccess) return -2;
   }
