@@ -58,7 +58,7 @@ struct Mat {  // one matrix, as the device's table holds it
 };
 __host__ __device__ inline int up(int v, int to) { return (v + to - 1) / to * to; }
 enum { SQ_A, SQ_FA, SQ_F, SQ_R = SQ_F + 2, SQ = SQ_R + 2 };  // (two of F, two of R)
-struct Dim {  // padded to 64 or 128 -- a list has one of them -- with zeros, which stay zeros
+struct Dim {  // padded with zeros, which stay zeros
   int n, m, np, mp;
   __host__ __device__ Dim(int rows, int cols, int pad) {
     n = rows < cols ? rows : cols;
@@ -97,7 +97,6 @@ struct Lists {  // one entry a workgroup
   uint2* norm_map;  // (matrix, chunk)
   unsigned n_gram, n_tri, n_rect, n_fill, n_norm;
   int count, pad, gram_ts, tri_ts, rect_ts;
-  int gram_g, tri_g, rect_g;  // groups of wavefronts a workgroup
 };
 
 // the whole workspace; every part is a multiple of 256 bytes
@@ -285,105 +284,152 @@ __global__ __launch_bounds__(256) void ortho_start_kernel(Lists l, const double*
 }
 
 // ------------------------------------------------------------------------------------------------ the products
-// One TS x TS tile of P Q^t: P, Q arrays of ldp / ldq columns, of which [k0, k1) are summed; the tile's first rows given.  A
-// group of 4 wavefronts takes a quarter of the tile each; G groups take the stages of the sum in turn and are added at the
-// end, so that a tile that has a compute unit to itself still has two wavefronts on each of its matrix cores.  A stage is 4
-// x 8 KB of shared memory -- 32 of the summed index at tiles of 128, 64 at tiles of 64 -- and comes through registers: the
-// next one's loads are on their way while one is computed.  (Loads straight into shared memory do not overlap: before any
-// of it is read, the compiler waits for every such load in flight.)  The 16-byte piece c of row r sits at c ^ (r / 4 % 4)
-// or c ^ (r / 2 % 8): sixteen rows that are read together then lie in different banks.
+// One TS x TS tile of P Q^t by 4 wavefronts, a quarter each: P, Q arrays of ldp / ldq columns, of which [k0, k1) are summed, a
+// multiple of 128; the tile's first rows given.  A stage is 32 of the summed index.  One wavefront a matrix core has to
+// hide everything behind its own products, so all of it runs ahead of them: four stages of a thread's loads in registers
+// (a load takes about a microsecond, other XCDs have just written what it reads), three stages in shared memory, and the
+// next 16 of the summed index in registers.  While stage s is multiplied, s + 2 is put into shared memory and the first
+// piece of s + 1 read from it.  Nothing of this is conditional -- the last stage is loaded again where there is no next --
+// or the compiler could not count the loads in flight and would wait for all of them.  (Loads straight into shared memory
+// do not overlap: before any of it is read, the compiler waits for every such load in flight.)  The 16-byte piece c of
+// row r sits at c ^ (r / 4 % 4): sixteen rows that are read together then lie in different banks.
+template <int TS>
 struct Stage {
-  half8 v[4][512];
+  half8 v[4][TS * 4];
 };
-template <int TS, int G>
+template <int TS>
 union Shared {
-  Stage st[2 * G];
+  Stage<TS> st[TS == 128 ? 2 : 3];
   float E[TS * (TS + 1)];
 };
-template <int TS, int G>
+template <int TS>
 struct Core {
-  static constexpr int BK = TS == 128 ? 32 : 64, PIECES = BK / 8, M = TS / 64;
-  static constexpr int LD = TS + 1;
-  static __device__ __forceinline__ int spot(int r, int c) {
-    return r * PIECES + (c ^ (PIECES == 4 ? r / 4 % 4 : r / 2 % 8));
-  }
+  static constexpr int M = TS / 64, LD = TS + 1, AHEAD = TS == 128 ? 1 : 4, BUFS = TS == 128 ? 2 : 3;
+  static constexpr int MFMA = 8, VMEM_READ = 0x20, DS_READ = 0x100, DS_WRITE = 0x200;  // kinds of instructions to the scheduler
+  static __device__ __forceinline__ int spot(int r, int c) { return r * 4 + (c ^ (r / 4 % 4)); }
   float16v hh[M][M], hl[M][M];  // hi hi, and the two others
-  half8 next[8];
+  half8 next[AHEAD][4 * M];
+  struct Piece {
+    half8 ph[M], pl[M], qh[M], ql[M];
+  } piece[2];
 
-  struct Source {  // this thread's pieces of the first two blocks of a stage, and how far the next stage's are
-    const _Float16 *p[2], *q[2];
+  struct Source {  // the stage's blocks
+    const _Float16 *p[M], *q[M];
   };
-  __device__ __forceinline__ void fetch(const Source& s, int stage) {
-    const size_t k = (size_t)stage * (BK / 32 * BLOCK);
+  static __device__ __forceinline__ void fetch(half8 (&to)[4 * M], const Source& s, int stage) {
+    const size_t k = (size_t)stage * BLOCK + threadIdx.x * 8;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      next[t] = *reinterpret_cast<const half8*>(s.p[t] + k + threadIdx.x % 256 * 8);
-      next[2 + t] = *reinterpret_cast<const half8*>(s.p[t] + k + LO + threadIdx.x % 256 * 8);
-      next[4 + t] = *reinterpret_cast<const half8*>(s.q[t] + k + threadIdx.x % 256 * 8);
-      next[6 + t] = *reinterpret_cast<const half8*>(s.q[t] + k + LO + threadIdx.x % 256 * 8);
+    for (int t = 0; t < M; ++t) {
+      to[4 * t] = *reinterpret_cast<const half8*>(s.p[t] + k);
+      to[4 * t + 1] = *reinterpret_cast<const half8*>(s.p[t] + k + LO);
+      to[4 * t + 2] = *reinterpret_cast<const half8*>(s.q[t] + k);
+      to[4 * t + 3] = *reinterpret_cast<const half8*>(s.q[t] + k + LO);
     }
   }
-  __device__ __forceinline__ void put(Stage& s) const {
-    const int r = threadIdx.x % 256 / 4, c = threadIdx.x % 4;
+  static __device__ __forceinline__ void put(Stage<TS>& s, const half8 (&from)[4 * M]) {
+    const int r = threadIdx.x / 4, c = threadIdx.x % 4;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int at = TS == 128 ? spot(t * 64 + r, c) : spot(r, t * 4 + c);
+    for (int t = 0; t < M; ++t)
 #pragma unroll
-      for (int a = 0; a < 4; ++a) s.v[a][at] = next[2 * a + t];
-    }
+      for (int a = 0; a < 4; ++a) s.v[a][spot(t * 64 + r, c)] = from[4 * t + a];
   }
-  __device__ __forceinline__ void compute(const Stage& s) {
-    const int wave = threadIdx.x >> 6 & 3, lane = threadIdx.x & 63;
+  static __device__ __forceinline__ void read(Piece& f, const Stage<TS>& s, int kk) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int pr = (wave >> 1) * (TS / 2) + (lane & 31), qr = (wave & 1) * (TS / 2) + (lane & 31), kc = lane >> 5;
 #pragma unroll
-    for (int kk = 0; kk < BK / 16; ++kk) {
-      half8 ph[M], pl[M], qh[M], ql[M];
-#pragma unroll
-      for (int i = 0; i < M; ++i) {
-        const int ps = spot(pr + 32 * i, kk * 2 + kc), qs = spot(qr + 32 * i, kk * 2 + kc);
-        ph[i] = s.v[0][ps], pl[i] = s.v[1][ps], qh[i] = s.v[2][qs], ql[i] = s.v[3][qs];
-      }
-#pragma unroll
-      for (int i = 0; i < M; ++i)
-#pragma unroll
-        for (int j = 0; j < M; ++j) {
-          hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], hl[i][j], 0, 0, 0);
-          hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], hl[i][j], 0, 0, 0);
-          hh[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], hh[i][j], 0, 0, 0);
-        }
+    for (int i = 0; i < M; ++i) {
+      const int ps = spot(pr + 32 * i, kk * 2 + kc), qs = spot(qr + 32 * i, kk * 2 + kc);
+      f.ph[i] = s.v[0][ps], f.pl[i] = s.v[1][ps], f.qh[i] = s.v[2][qs], f.ql[i] = s.v[3][qs];
     }
   }
-  __device__ __forceinline__ void run(Stage* all, const _Float16* p, int prow, int ldp, const _Float16* q, int qrow, int ldq,
+  __device__ __forceinline__ void multiply(const Piece& f) {
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int j = 0; j < M; ++j) hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[i], f.ql[j], hl[i][j], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int j = 0; j < M; ++j) hh[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[i], f.qh[j], hh[i][j], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int j = 0; j < M; ++j) hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.pl[i], f.qh[j], hl[i][j], 0, 0, 0);
+  }
+  __device__ __forceinline__ void run(Stage<TS>* st, const _Float16* p, int prow, int ldp, const _Float16* q, int qrow, int ldq,
                                       int k0, int k1) {
-    const int group = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 256);
-    Stage* st = all + 2 * group;
     Source src;
-    src.p[0] = p + place(prow, k0, ldp), src.p[1] = TS == 128 ? p + place(prow + 64, k0, ldp) : src.p[0] + BLOCK;
-    src.q[0] = q + place(qrow, k0, ldq), src.q[1] = TS == 128 ? q + place(qrow + 64, k0, ldq) : src.q[0] + BLOCK;
-    const int stages = (k1 - k0) / BK;
-    if (group < stages) fetch(src, group);
+#pragma unroll
+    for (int t = 0; t < M; ++t) src.p[t] = p + place(prow + 64 * t, k0, ldp), src.q[t] = q + place(qrow + 64 * t, k0, ldq);
+    const int stages = (k1 - k0) / 32, end = stages - 1;
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) fetch(next[d], src, d);
 #pragma unroll
     for (int i = 0; i < M; ++i)
 #pragma unroll
       for (int j = 0; j < M; ++j) hh[i][j] = float16v{}, hl[i][j] = float16v{};
-    if (group < stages) put(st[0]);
-    if (group + G < stages) fetch(src, group + G);
+#pragma unroll
+    for (int d = 0; d < BUFS - 1; ++d) {
+      put(st[d], next[d]);
+      fetch(next[d], src, d + AHEAD < end ? d + AHEAD : end);
+    }
     __syncthreads();
-    int cur = 0;
-    for (int s = group; s - group < stages; s += G) {  // (every group as often: the barrier is everyone's)
-      if (s < stages) compute(st[cur]);
-      cur ^= 1;
-      if (s + G < stages) {
-        put(st[cur]);  // (everyone left that stage before the last barrier)
-        if (s + 2 * G < stages) fetch(src, s + 2 * G);
+    if constexpr (TS == 128) {
+      Stage<TS> *now = st, *then = st + 1;
+      for (int s = 0; s < stages; ++s) {
+        read(piece[0], *now, 0);
+        read(piece[1], *now, 1);
+        multiply(piece[0]);
+        put(*then, next[0]);
+        fetch(next[0], src, s + 2 < end ? s + 2 : end);
+        multiply(piece[1]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(DS_WRITE, 1, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(VMEM_READ, 1, 0);
+        }
+        __syncthreads();  // (behind the last stage: the stages' memory is the epilogue's too)
+        Stage<TS>* was = now;
+        now = then, then = was;
       }
-      __syncthreads();  // (behind the last stage: the stages' memory is the epilogue's too)
+    } else {
+      Stage<TS> *now = st, *then = st + 1, *spare = st + 2;
+      read(piece[0], *now, 0);
+      for (int s0 = 0; s0 < stages; s0 += AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          const int s = s0 + u, more = s + 2 + AHEAD;
+          read(piece[1], *now, 1);
+          put(*spare, next[(u + 2) % AHEAD]);  // (that stage was left before the last barrier)
+          fetch(next[(u + 2) % AHEAD], src, more < end ? more : end);
+          multiply(piece[0]);
+          read(piece[0], *then, 0);
+          multiply(piece[1]);
+          __syncthreads();  // (behind the last stage: the stages' memory is the epilogue's too)
+          Stage<TS>* was = now;
+          now = then, then = spare, spare = was;
+        }
+      }
     }
   }
   // lane l of the matrix instruction holds column l % 32 and rows 8 (r / 4) + 4 (l / 32) + r % 4
   template <typename F>
   __device__ __forceinline__ void each(const F& f) const {
-    const int wave = threadIdx.x >> 6 & 3, lane = threadIdx.x & 63;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < M; ++i)
 #pragma unroll
@@ -393,14 +439,10 @@ struct Core {
           f((wave >> 1) * (TS / 2) + 32 * i + 8 * (r / 4) + 4 * (lane >> 5) + r % 4,
             (wave & 1) * (TS / 2) + 32 * j + (lane & 31), hh[i][j][r] + hl[i][j][r]);
   }
-  // the groups' sum times f, into shared memory
+  // ... times f, into shared memory
   __device__ __forceinline__ void spill(float* E, float f) const {
-#pragma unroll
-    for (int g = G - 1; g >= 0; --g) {
-      if (G == 1 || (int)(threadIdx.x / 256) == g)
-        each([&](int r, int c, float v) { E[r * LD + c] = g == G - 1 ? v * f : fmaf(v, f, E[r * LD + c]); });
-      __syncthreads();
-    }
+    each([&](int r, int c, float v) { E[r * LD + c] = v * f; });
+    __syncthreads();
   }
 };
 
@@ -423,25 +465,25 @@ __device__ __forceinline__ void store_gram(float* E, const Dim& d, const Area& o
 // A = X X^t: a tile on or above the diagonal, or one part of its sum, which ortho_sum_kernel adds up in their order.
 // (Adding them in the workgroup that ends last needs the other workgroups' tiles flushed through the XCDs' caches: 160 us
 // where this and the launch behind it take 20, at eight 256 x 2304 matrices.)
-template <int TS, int G>
-__global__ __launch_bounds__(256 * G, 2) void ortho_gram_kernel(Lists l, _Float16* base, float* parts, int kc) {
-  __shared__ Shared<TS, G> sh;
+template <int TS>
+__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Lists l, _Float16* base, float* parts, int kc) {
+  __shared__ Shared<TS> sh;
   const Tile w = l.gram[blockIdx.x];
   const Mat t = l.table[w.mat];
   const Dim d(t.rows, t.cols, l.pad);
   const Area o(base, t, d);
   const int i0 = w.i * TS, j0 = w.j * TS;
   const int k0 = w.split * kc, k1 = k0 + kc < d.mp ? k0 + kc : d.mp;
-  Core<TS, G> core;
+  Core<TS> core;
   core.run(sh.st, o.x, i0, d.mp, o.x, j0, d.mp, k0, k1);
   if (t.splits > 1) {
     float* mine = parts + t.part0 + (size_t)(blockIdx.x - t.gram0) * (TS * TS);
     core.spill(sh.E, 1.f / SCALE);
-    for (int q = threadIdx.x; q < TS * TS; q += 256 * G) mine[q] = sh.E[q / TS * (TS + 1) + q % TS];
+    for (int q = threadIdx.x; q < TS * TS; q += 256) mine[q] = sh.E[q / TS * (TS + 1) + q % TS];
     return;
   }
   core.spill(sh.E, 1.f / SCALE);
-  store_gram<TS, TS, 256 * G>(sh.E, d, o, i0, j0, w.i == w.j);
+  store_gram<TS, TS, 256>(sh.E, d, o, i0, j0, w.i == w.j);
 }
 // 32 rows of a tile of A from its parts
 template <int TS>
@@ -476,9 +518,9 @@ struct Op {
   int out, g, h;  // which arrays
   float t, q, l, f, fg, fh, fs, back;  // back: one over out's scale
 };
-template <int TS, int G>
-__global__ __launch_bounds__(256 * G, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
-  __shared__ Shared<TS, G> sh;
+template <int TS>
+__global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
+  __shared__ Shared<TS> sh;
   const Tile w = l.tri[blockIdx.x];
   const Mat t = l.table[w.mat];
   const Dim d(t.rows, t.cols, l.pad);
@@ -488,12 +530,12 @@ __global__ __launch_bounds__(256 * G, 2) void ortho_square_kernel(Lists l, _Floa
   const size_t step = 2 * d.a();
   const _Float16 *g = o.sq + op.g * step, *h = o.sq + op.h * step;
   const float *gd = o.diag + op.g * d.np, *hd = o.diag + op.h * d.np;
-  Core<TS, G> core;
+  Core<TS> core;
   core.run(sh.st, g, i0, d.np, h, j0, d.np, 0, d.np);
   core.spill(sh.E, 1.f);
   _Float16* out = o.sq + op.out * step;
   const bool diagonal = w.i == w.j;
-  rows8<TS, TS, TS + 1, 256 * G>(sh.E, [&](int r, int c, float (&v)[8]) {
+  rows8<TS, TS, TS + 1, 256>(sh.E, [&](int r, int c, float (&v)[8]) {
     const int i = i0 + r, j = j0 + c;
     const size_t at = place(i, j, d.np);
     const half8 gh = *reinterpret_cast<const half8*>(g + at), gl = *reinterpret_cast<const half8*>(g + at + LO);
@@ -514,37 +556,37 @@ __global__ __launch_bounds__(256 * G, 2) void ortho_square_kernel(Lists l, _Floa
   });
   if (!diagonal) {
     __syncthreads();
-    store_turned<TS, TS, TS + 1, 256 * G>(sh.E, out, d.np, j0, i0);
+    store_turned<TS, TS, TS + 1, 256>(sh.E, out, d.np, j0, i0);
   }
 }
 
 // X <- R X, from X^t; the last group's goes to the caller, as the result or into the weights
-template <typename T, bool LAST, int TS, int G>
-__global__ __launch_bounds__(256 * G, 2) void ortho_apply_kernel(Lists l, _Float16* base, int R, float fs, int from, int update,
+template <typename T, bool LAST, int TS>
+__global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* base, int R, float fs, int from, int update,
                                                              float decay) {
-  __shared__ Shared<TS, G> sh;
+  __shared__ Shared<TS> sh;
   const Tile w = l.rect[blockIdx.x];
   const Mat t = l.table[w.mat];
   const Dim d(t.rows, t.cols, l.pad);
   const Area o(base, t, d);
   const int i0 = w.i * TS, j0 = w.j * TS;
   const _Float16 *a = o.sq + R * 2 * d.a(), *xt = o.xt + (from ? 2 * d.x() : 0);
-  Core<TS, G> core;
+  Core<TS> core;
   core.run(sh.st, a, i0, d.np, xt, j0, d.np, 0, d.np);
   core.spill(sh.E, fs);
-  rows8<TS, TS, TS + 1, 256 * G>(sh.E, [&](int r, int c, float (&v)[8]) {
+  rows8<TS, TS, TS + 1, 256>(sh.E, [&](int r, int c, float (&v)[8]) {
     _Float16* x = o.x + place(i0 + r, j0 + c, d.mp);
     add8(v, o.diag[R * d.np + i0 + r], x);
     if constexpr (!LAST) store8(x, v);
   });
   __syncthreads();
   if constexpr (!LAST) {
-    store_turned<TS, TS, TS + 1, 256 * G>(sh.E, o.xt + (from ? 0 : 2 * d.x()), d.np, j0, i0);
+    store_turned<TS, TS, TS + 1, 256>(sh.E, o.xt + (from ? 0 : 2 * d.x()), d.np, j0, i0);
   } else {
     const bool tall = t.rows > t.cols;
     T* out = static_cast<T*>(t.dst);
 #pragma unroll 4
-    for (int q = threadIdx.x; q < TS * TS; q += 256 * G) {
+    for (int q = threadIdx.x; q < TS * TS; q += 256) {
       const int r = tall ? q % TS : q / TS, c = tall ? q / TS : q % TS;
       const int i = i0 + r, j = j0 + c;
       if (i < d.n && j < d.m) {
@@ -570,19 +612,18 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   Lists& l = p.l;
   l = Lists{};
   l.count = count;
+  l.pad = 128;
   // Tiles: 128 needs half the reads of two operands that 64 does, and is taken for a pass that fills the card with such
-  // tiles, unless it pads much further.
-  uint64_t tri128 = 0, rect64 = 0, rect128 = 0, gram128 = 0;
+  // tiles.
+  uint64_t tri128 = 0, rect128 = 0, gram128 = 0;
   for (int i = 0; i < count; ++i) {
-    const Dim s(rows[i], cols[i], 64), w(rows[i], cols[i], 128);
-    tri128 += w.tri(128), rect64 += s.rect(64), rect128 += w.rect(128);
+    const Dim w(rows[i], cols[i], 128);
+    tri128 += w.tri(128), rect128 += w.rect(128);
     gram128 += (uint64_t)w.tri(128) * ((w.mp + 255) / 256);
   }
-  const bool tight = rect128 * 4 <= rect64 * 3 / 2;
-  l.gram_ts = tight && gram128 >= WANT / 2 ? 128 : 64;
-  l.tri_ts = tight && tri128 >= WANT / 2 ? 128 : 64;
-  l.rect_ts = tight && rect128 >= WANT / 2 ? 128 : 64;
-  l.pad = l.gram_ts == 128 || l.tri_ts == 128 || l.rect_ts == 128 ? 128 : 64;
+  l.gram_ts = gram128 >= WANT / 2 ? 128 : 64;
+  l.tri_ts = tri128 >= WANT / 2 ? 128 : 64;
+  l.rect_ts = rect128 >= WANT / 2 ? 128 : 64;
   // X X^t: the longest parts of the sum that still fill the card.  A part is a workgroup's time, so the parts of a ragged
   // list are of like length, and a short list of wide matrices is spread.
   for (p.kc = 4096; p.kc > 256; p.kc /= 2) {
@@ -609,10 +650,6 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   if (gram > 0x7fffffff || tri > 0x7fffffff || rect > 0x7fffffff || fill > 0x7fffffff || norm > 0x7fffffff) return -1;
   l.n_gram = (unsigned)gram, l.n_tri = (unsigned)tri, l.n_rect = (unsigned)rect, l.n_fill = (unsigned)fill;
   l.n_norm = (unsigned)norm;
-  // Two groups where that ends earlier: a compute unit holds two workgroups of one group or one of two.  (2048 x 2048,
-  // tiles of 128, X <- R X: 256 workgroups, 76 us with one group, XX with two.)
-  const auto groups = [](uint64_t n) { return (n + WANT / 2 - 1) / (WANT / 2) < 2 * ((n + WANT - 1) / WANT) ? 2 : 1; };
-  l.gram_g = groups(gram), l.tri_g = groups(tri), l.rect_g = groups(rect);
   size_t at = 0;
   const auto take = [&](size_t bytes) {
     const size_t was = at;
@@ -682,14 +719,10 @@ Poly polynomial(int steps, double a, double b, double c) {
   return r;
 }
 
-// f(tile, groups) as constants
 template <typename F>
-void choose(int ts, int g, const F& f) {
-  using std::integral_constant;
-  if (ts == 128 && g == 2) f(integral_constant<int, 128>(), integral_constant<int, 2>());
-  else if (ts == 128) f(integral_constant<int, 128>(), integral_constant<int, 1>());
-  else if (g == 2) f(integral_constant<int, 64>(), integral_constant<int, 2>());
-  else f(integral_constant<int, 64>(), integral_constant<int, 1>());
+void choose(int ts, const F& f) {  // f(tile) with the tile a constant
+  if (ts == 128) f(std::integral_constant<int, 128>());
+  else f(std::integral_constant<int, 64>());
 }
 
 template <typename T>
@@ -737,8 +770,8 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
   hipLaunchKernelGGL((ortho_start_kernel<T>), dim3(l.n_fill), wg, 0, st, l, norms, base, update, mu, nesterov, eps);
   if (hipGetLastError() != hipSuccess) return -2;
   const auto square = [&](const Op& one, const Op* two) {
-    choose(l.tri_ts, l.tri_g, [&](auto TS, auto G) {
-      hipLaunchKernelGGL((ortho_square_kernel<TS(), G()>), dim3(l.n_tri, two ? 2 : 1), dim3(256 * G()), 0, st, l, base, one,
+    choose(l.tri_ts, [&](auto TS) {
+      hipLaunchKernelGGL((ortho_square_kernel<TS()>), dim3(l.n_tri, two ? 2 : 1), wg, 0, st, l, base, one,
                          two ? *two : one);
     });
   };
@@ -750,8 +783,8 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
   for (int left = steps; left > 0;) {
     int g = group_length(left, steps);
     if (g > f.longest) g = f.longest;
-    choose(l.gram_ts, l.gram_g, [&](auto TS, auto G) {
-      hipLaunchKernelGGL((ortho_gram_kernel<TS(), G()>), dim3(l.n_gram), dim3(256 * G()), 0, st, l, base, parts, p.kc);
+    choose(l.gram_ts, [&](auto TS) {
+      hipLaunchKernelGGL((ortho_gram_kernel<TS()>), dim3(l.n_gram), wg, 0, st, l, base, parts, p.kc);
       if (p.split) hipLaunchKernelGGL((ortho_sum_kernel<TS()>), dim3(l.n_gram, TS() / 32), wg, 0, st, l, base, parts);
     });
     int R = SQ_F, spare = SQ_R;
@@ -772,12 +805,12 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
     }
     left -= g;
     const float fs = 1.f / scale;
-    choose(l.rect_ts, l.rect_g, [&](auto TS, auto G) {
-      const dim3 grid(l.n_rect), block(256 * G());
+    choose(l.rect_ts, [&](auto TS) {
+      const dim3 grid(l.n_rect);
       if (left)
-        hipLaunchKernelGGL((ortho_apply_kernel<T, false, TS(), G()>), grid, block, 0, st, l, base, R, fs, from, update, decay);
+        hipLaunchKernelGGL((ortho_apply_kernel<T, false, TS()>), grid, wg, 0, st, l, base, R, fs, from, update, decay);
       else
-        hipLaunchKernelGGL((ortho_apply_kernel<T, true, TS(), G()>), grid, block, 0, st, l, base, R, fs, from, update, decay);
+        hipLaunchKernelGGL((ortho_apply_kernel<T, true, TS()>), grid, wg, 0, st, l, base, R, fs, from, update, decay);
     });
     from ^= 1;
     if (hipGetLastError() != hipSuccess) return -2;
