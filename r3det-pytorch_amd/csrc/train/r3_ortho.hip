@@ -200,12 +200,14 @@ __device__ __forceinline__ void split16(float v, _Float16& hi, _Float16& lo) {
   hi = (_Float16)v;
   lo = (_Float16)(v - (float)hi);
 }
-// Arrays are kept in blocks of 64 rows by 32 columns, row by row of blocks: 4 KB of hi, 4 KB of lo, 8 KB in all, each row of a
-// block 64 bytes.  What a stage of a product reads is then whole blocks, one behind the other.  (Plain rows are read 64
-// bytes at a time, half a cache line, and at a power of two apart: 76 us for 2048 x 2048 against XX.)
+// Arrays are kept in blocks of 64 rows by 32 columns, row by row of blocks: 4 KB of hi, 4 KB of lo.  Inside, in the order of
+// the matrix instruction's operands: 16 columns, 32 rows, 8 columns, row, column, so that a wavefront's operand is 1 KB in
+// one piece.  What a stage of a product reads is then whole blocks, one behind the other.  (Plain rows are read 64 bytes at
+// a time, half a cache line, and at a power of two apart: 7.0 ms for 4096 x 4096 against 6.2.)
 constexpr int LO = 64 * 32, BLOCK = 2 * LO;
 __device__ __forceinline__ size_t place(int r, int c, int ld) {
-  return ((size_t)(r / 64) * (ld / 32) + c / 32) * BLOCK + r % 64 * 32 + c % 32;
+  return ((size_t)(r / 64) * (ld / 32) + c / 32) * BLOCK + c % 32 / 16 * 1024 + r % 64 / 32 * 512 + c % 16 / 8 * 256 + r % 32 * 8 +
+         c % 8;
 }
 __device__ __forceinline__ void store8(_Float16* at, const float (&v)[8]) {
   half8 h, l;
@@ -224,26 +226,31 @@ __device__ __forceinline__ void add8(float (&v)[8], float f, const _Float16* at)
   for (int k = 0; k < 8; ++k) v[k] = fmaf(f, (float)h[k] + (float)l[k], v[k]);
 }
 // ROWS x COLS of fp32 in shared memory, rows of LD: f(row, column, eight values), which may change them; then `f`'s values
-// are in shared memory too.
-template <int ROWS, int COLS, int LD, int THREADS, typename F>
+// are in shared memory too.  PARTS > 1: the values are the sum of so many such arrays.  (Neighbouring threads have
+// neighbouring rows: the arrays' order, and LD is odd.)
+template <int ROWS, int COLS, int LD, int PARTS, typename F>
 __device__ __forceinline__ void rows8(float* E, const F& f) {
 #pragma unroll 2
-  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += THREADS) {
-    const int r = q / (COLS / 8), c = q % (COLS / 8) * 8;
+  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += 256) {
+    const int r = q % ROWS, c = q / ROWS * 8;
     float v[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = E[r * LD + c + k];
+#pragma unroll
+    for (int s = 1; s < PARTS; ++s)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += E[s * ROWS * LD + r * LD + c + k];
     f(r, c, v);
 #pragma unroll
     for (int k = 0; k < 8; ++k) E[r * LD + c + k] = v[k];
   }
 }
 // The transpose of ROWS x COLS in shared memory -> an array of `ld` columns, at (r0, c0).
-template <int ROWS, int COLS, int LD, int THREADS>
+template <int ROWS, int COLS, int LD>
 __device__ __forceinline__ void store_turned(const float* E, _Float16* p, int ld, int r0, int c0) {
 #pragma unroll 2
-  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += THREADS) {
-    const int r = q / (ROWS / 8), c = q % (ROWS / 8) * 8;
+  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += 256) {
+    const int r = q % COLS, c = q / COLS * 8;
     float v[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = E[(c + k) * LD + r];
@@ -279,178 +286,196 @@ __global__ __launch_bounds__(256) void ortho_start_kernel(Lists l, const double*
     E[r * 65 + c] = v;
   }
   __syncthreads();
-  rows8<64, 64, 65, 256>(E, [&](int r, int c, float (&v)[8]) { store8(o.x + place(i0 + r, j0 + c, d.mp), v); });
-  store_turned<64, 64, 65, 256>(E, o.xt, d.np, j0, i0);
+  rows8<64, 64, 65, 1>(E, [&](int r, int c, float (&v)[8]) { store8(o.x + place(i0 + r, j0 + c, d.mp), v); });
+  store_turned<64, 64, 65>(E, o.xt, d.np, j0, i0);
 }
 
 // ------------------------------------------------------------------------------------------------ the products
-// One TS x TS tile of P Q^t by 4 wavefronts, a quarter each: P, Q arrays of ldp / ldq columns, of which [k0, k1) are summed, a
-// multiple of 128; the tile's first rows given.  A stage is 32 of the summed index.  One wavefront a matrix core has to
-// hide everything behind its own products, so all of it runs ahead of them: four stages of a thread's loads in registers
-// (a load takes about a microsecond, other XCDs have just written what it reads), three stages in shared memory, and the
-// next 16 of the summed index in registers.  While stage s is multiplied, s + 2 is put into shared memory and the first
-// piece of s + 1 read from it.  Nothing of this is conditional -- the last stage is loaded again where there is no next --
-// or the compiler could not count the loads in flight and would wait for all of them.  (Loads straight into shared memory
-// do not overlap: before any of it is read, the compiler waits for every such load in flight.)  The 16-byte piece c of
-// row r sits at c ^ (r / 4 % 4): sixteen rows that are read together then lie in different banks.
-template <int TS>
-struct Stage {
-  half8 v[4][TS * 4];
+// One TS x TS tile of P Q^t by 4 wavefronts: P, Q arrays of ldp / ldq columns, of which [k0, k1) are summed, a multiple of 128;
+// the tile's first rows given.  Three matrix instructions for two operands of hi and lo, in two accumulators.
+typedef float16v Acc[2][2];
+__device__ __forceinline__ void clear(Acc& a) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) a[i][j] = float16v{};
+}
+struct Piece {  // 64 rows of P and of Q, 16 of the summed index
+  half8 ph[2], pl[2], qh[2], ql[2];
 };
-template <int TS>
-union Shared {
-  Stage<TS> st[TS == 128 ? 2 : 3];
-  float E[TS * (TS + 1)];
-};
-template <int TS>
-struct Core {
-  static constexpr int M = TS / 64, LD = TS + 1, AHEAD = TS == 128 ? 1 : 4, BUFS = TS == 128 ? 2 : 3;
-  static constexpr int MFMA = 8, VMEM_READ = 0x20, DS_READ = 0x100, DS_WRITE = 0x200;  // kinds of instructions to the scheduler
-  static __device__ __forceinline__ int spot(int r, int c) { return r * 4 + (c ^ (r / 4 % 4)); }
-  float16v hh[M][M], hl[M][M];  // hi hi, and the two others
-  half8 next[AHEAD][4 * M];
-  struct Piece {
-    half8 ph[M], pl[M], qh[M], ql[M];
-  } piece[2];
+__device__ __forceinline__ void multiply(Acc& hh, Acc& hl, const Piece& f) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[i], f.ql[j], hl[i][j], 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) hh[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[i], f.qh[j], hh[i][j], 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.pl[i], f.qh[j], hl[i][j], 0, 0, 0);
+}
+// 64 x 64 of the sum, into shared memory with rows of LD, times f.  Lane l of the matrix instruction holds column l % 32 and
+// rows 8 (r / 4) + 4 (l / 32) + r % 4.
+template <int LD>
+__device__ __forceinline__ void spill(const Acc& hh, const Acc& hl, float* E, float f) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        E[(32 * i + 8 * (r / 4) + 4 * (lane >> 5) + r % 4) * LD + 32 * j + (lane & 31)] = (hh[i][j][r] + hl[i][j][r]) * f;
+}
 
-  struct Source {  // the stage's blocks
-    const _Float16 *p[M], *q[M];
+// A tile of 128: a quarter a wavefront.  A stage is 32 of the summed index, whole blocks; it comes through registers into
+// shared memory, two stages in turn, two workgroups a compute unit.  The next stage's loads, the writes of the one before
+// it and the reads of the second piece lie between the matrix instructions, in an order that the scheduler is told:
+// left alone it reads an operand where it is needed and waits (4096 x 4096, R X: 395 us, 387 with it; 2048: 74, 61).
+// Nothing is conditional -- the last stage is loaded again where there is no next -- or the compiler could not count the
+// loads in flight and would wait for all of them.  (Loads straight into shared memory do not overlap: before any of it is
+// read, the compiler waits for every such load in flight.)  The 16-byte piece c of row r sits at c ^ (r / 4 % 4): sixteen
+// rows that are read together then lie in different banks.
+struct Stage {
+  half8 v[4][512];
+};
+struct Core128 {
+  static constexpr int TS = 128, LD = 129, PARTS = 1;
+  static constexpr int MFMA = 8, VMEM_READ = 0x20, DS_READ = 0x100, DS_WRITE = 0x200;  // kinds of instructions
+  union Shared {
+    Stage st[2];
+    float E[TS * LD];
   };
-  static __device__ __forceinline__ void fetch(half8 (&to)[4 * M], const Source& s, int stage) {
+  struct Source {  // the stage's blocks
+    const _Float16 *p[2], *q[2];
+  };
+  static __device__ __forceinline__ int spot(int r, int c) { return r * 4 + (c ^ (r / 4 % 4)); }
+  static __device__ __forceinline__ void fetch(half8 (&to)[8], const Source& s, int stage) {
     const size_t k = (size_t)stage * BLOCK + threadIdx.x * 8;
 #pragma unroll
-    for (int t = 0; t < M; ++t) {
+    for (int t = 0; t < 2; ++t) {
       to[4 * t] = *reinterpret_cast<const half8*>(s.p[t] + k);
       to[4 * t + 1] = *reinterpret_cast<const half8*>(s.p[t] + k + LO);
       to[4 * t + 2] = *reinterpret_cast<const half8*>(s.q[t] + k);
       to[4 * t + 3] = *reinterpret_cast<const half8*>(s.q[t] + k + LO);
     }
   }
-  static __device__ __forceinline__ void put(Stage<TS>& s, const half8 (&from)[4 * M]) {
-    const int r = threadIdx.x / 4, c = threadIdx.x % 4;
+  static __device__ __forceinline__ void put(Stage& s, const half8 (&from)[8]) {
+    const int t4 = threadIdx.x, r = t4 / 64 % 2 * 32 + t4 % 32, c = t4 / 128 * 2 + t4 / 32 % 2;  // (the block's order)
 #pragma unroll
-    for (int t = 0; t < M; ++t)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int a = 0; a < 4; ++a) s.v[a][spot(t * 64 + r, c)] = from[4 * t + a];
   }
-  static __device__ __forceinline__ void read(Piece& f, const Stage<TS>& s, int kk) {
+  static __device__ __forceinline__ void read(Piece& f, const Stage& s, int kk) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int pr = (wave >> 1) * (TS / 2) + (lane & 31), qr = (wave & 1) * (TS / 2) + (lane & 31), kc = lane >> 5;
+    const int pr = (wave >> 1) * 64 + (lane & 31), qr = (wave & 1) * 64 + (lane & 31), kc = lane >> 5;
 #pragma unroll
-    for (int i = 0; i < M; ++i) {
+    for (int i = 0; i < 2; ++i) {
       const int ps = spot(pr + 32 * i, kk * 2 + kc), qs = spot(qr + 32 * i, kk * 2 + kc);
       f.ph[i] = s.v[0][ps], f.pl[i] = s.v[1][ps], f.qh[i] = s.v[2][qs], f.ql[i] = s.v[3][qs];
     }
   }
-  __device__ __forceinline__ void multiply(const Piece& f) {
-#pragma unroll
-    for (int i = 0; i < M; ++i)
-#pragma unroll
-      for (int j = 0; j < M; ++j) hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[i], f.ql[j], hl[i][j], 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < M; ++i)
-#pragma unroll
-      for (int j = 0; j < M; ++j) hh[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ph[i], f.qh[j], hh[i][j], 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < M; ++i)
-#pragma unroll
-      for (int j = 0; j < M; ++j) hl[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.pl[i], f.qh[j], hl[i][j], 0, 0, 0);
-  }
-  __device__ __forceinline__ void run(Stage<TS>* st, const _Float16* p, int prow, int ldp, const _Float16* q, int qrow, int ldq,
-                                      int k0, int k1) {
+  // the tile times f in shared memory
+  static __device__ __forceinline__ void run(Shared& sh, const _Float16* p, int prow, int ldp, const _Float16* q, int qrow,
+                                             int ldq, int k0, int k1, float f) {
     Source src;
 #pragma unroll
-    for (int t = 0; t < M; ++t) src.p[t] = p + place(prow + 64 * t, k0, ldp), src.q[t] = q + place(qrow + 64 * t, k0, ldq);
+    for (int t = 0; t < 2; ++t) src.p[t] = p + place(prow + 64 * t, k0, ldp), src.q[t] = q + place(qrow + 64 * t, k0, ldq);
     const int stages = (k1 - k0) / 32, end = stages - 1;
-#pragma unroll
-    for (int d = 0; d < AHEAD; ++d) fetch(next[d], src, d);
-#pragma unroll
-    for (int i = 0; i < M; ++i)
-#pragma unroll
-      for (int j = 0; j < M; ++j) hh[i][j] = float16v{}, hl[i][j] = float16v{};
-#pragma unroll
-    for (int d = 0; d < BUFS - 1; ++d) {
-      put(st[d], next[d]);
-      fetch(next[d], src, d + AHEAD < end ? d + AHEAD : end);
-    }
+    half8 next[8];
+    Piece one, two;
+    Acc hh, hl;
+    fetch(next, src, 0);
+    clear(hh), clear(hl);
+    put(sh.st[0], next);
+    fetch(next, src, 1);
     __syncthreads();
-    if constexpr (TS == 128) {
-      Stage<TS> *now = st, *then = st + 1;
-      for (int s = 0; s < stages; ++s) {
-        read(piece[0], *now, 0);
-        read(piece[1], *now, 1);
-        multiply(piece[0]);
-        put(*then, next[0]);
-        fetch(next[0], src, s + 2 < end ? s + 2 : end);
-        multiply(piece[1]);
+    Stage *now = sh.st, *then = sh.st + 1;
+    for (int s = 0; s < stages; ++s) {
+      read(one, *now, 0);
+      read(two, *now, 1);
+      multiply(hh, hl, one);
+      put(*then, next);  // (that stage was left before the last barrier)
+      fetch(next, src, s + 2 < end ? s + 2 : end);
+      multiply(hh, hl, two);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
-        }
+      for (int k = 0; k < 8; ++k) __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(DS_WRITE, 1, 0);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(VMEM_READ, 1, 0);
-        }
-        __syncthreads();  // (behind the last stage: the stages' memory is the epilogue's too)
-        Stage<TS>* was = now;
-        now = then, then = was;
+      for (int k = 0; k < 8; ++k) {
+        __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
       }
-    } else {
-      Stage<TS> *now = st, *then = st + 1, *spare = st + 2;
-      read(piece[0], *now, 0);
-      for (int s0 = 0; s0 < stages; s0 += AHEAD) {
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-          const int s = s0 + u, more = s + 2 + AHEAD;
-          read(piece[1], *now, 1);
-          put(*spare, next[(u + 2) % AHEAD]);  // (that stage was left before the last barrier)
-          fetch(next[(u + 2) % AHEAD], src, more < end ? more : end);
-          multiply(piece[0]);
-          read(piece[0], *then, 0);
-          multiply(piece[1]);
-          __syncthreads();  // (behind the last stage: the stages' memory is the epilogue's too)
-          Stage<TS>* was = now;
-          now = then, then = spare, spare = was;
-        }
+      for (int k = 0; k < 8; ++k) {
+        __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(DS_WRITE, 1, 0);
       }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(VMEM_READ, 1, 0);
+      }
+      __syncthreads();  // (behind the last stage: the stages' memory is the epilogue's too)
+      Stage* was = now;
+      now = then, then = was;
     }
-  }
-  // lane l of the matrix instruction holds column l % 32 and rows 8 (r / 4) + 4 (l / 32) + r % 4
-  template <typename F>
-  __device__ __forceinline__ void each(const F& f) const {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-#pragma unroll
-    for (int i = 0; i < M; ++i)
-#pragma unroll
-      for (int j = 0; j < M; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          f((wave >> 1) * (TS / 2) + 32 * i + 8 * (r / 4) + 4 * (lane >> 5) + r % 4,
-            (wave & 1) * (TS / 2) + 32 * j + (lane & 31), hh[i][j][r] + hl[i][j][r]);
-  }
-  // ... times f, into shared memory
-  __device__ __forceinline__ void spill(float* E, float f) const {
-    each([&](int r, int c, float v) { E[r * LD + c] = v * f; });
+    const int wave = threadIdx.x >> 6;
+    spill<LD>(hh, hl, sh.E + (wave >> 1) * 64 * LD + (wave & 1) * 64, f);
     __syncthreads();
   }
 };
 
+// A tile of 64, for where those of 128 are too few: the whole tile a wavefront, the summed index in turn, 16 of it at a time.
+// Operands come from memory straight into registers, each by one wavefront only, so shared memory has nothing to save and
+// nobody waits at a barrier before the end; there the four sums are added.
+struct Core64 {
+  static constexpr int TS = 64, LD = 65, PARTS = 4, AHEAD = 3;
+  union Shared {
+    float E[PARTS * TS * LD];
+  };
+  static __device__ __forceinline__ void fetch(Piece& f, const _Float16* p, const _Float16* q, int unit) {
+    const size_t k = (size_t)(unit / 2) * BLOCK + unit % 2 * 1024 + (threadIdx.x & 63) * 8;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f.ph[i] = *reinterpret_cast<const half8*>(p + k + i * 512);
+      f.pl[i] = *reinterpret_cast<const half8*>(p + k + i * 512 + LO);
+      f.qh[i] = *reinterpret_cast<const half8*>(q + k + i * 512);
+      f.ql[i] = *reinterpret_cast<const half8*>(q + k + i * 512 + LO);
+    }
+  }
+  static __device__ __forceinline__ void run(Shared& sh, const _Float16* p, int prow, int ldp, const _Float16* q, int qrow,
+                                             int ldq, int k0, int k1, float f) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    p += place(prow, k0, ldp), q += place(qrow, k0, ldq);
+    const int units = (k1 - k0) / 64, end = units - 1;  // of this wavefront
+    Piece piece[AHEAD];
+    Acc hh, hl;
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) fetch(piece[d], p, q, (d < end ? d : end) * 4 + wave);
+    clear(hh), clear(hl);
+    for (int s = 0; s < units; s += AHEAD) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (s + u < units) multiply(hh, hl, piece[u]);
+        fetch(piece[u], p, q, (s + u + AHEAD < end ? s + u + AHEAD : end) * 4 + wave);
+      }
+    }
+    spill<LD>(hh, hl, sh.E + wave * TS * LD, f);
+    __syncthreads();
+  }
+};
+template <int TS>
+using Core = std::conditional_t<TS == 128, Core128, Core64>;
+
 // A from ROWS rows of a tile in shared memory
-template <int ROWS, int TS, int THREADS>
+template <int ROWS, int TS, int PARTS>
 __device__ __forceinline__ void store_gram(float* E, const Dim& d, const Area& o, int i0, int j0, bool diagonal) {
   _Float16* a = o.sq + SQ_A * 2 * d.a();
-  rows8<ROWS, TS, TS + 1, THREADS>(E, [&](int r, int c, float (&v)[8]) {
+  rows8<ROWS, TS, TS + 1, PARTS>(E, [&](int r, int c, float (&v)[8]) {
     if (diagonal)
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -459,7 +484,7 @@ __device__ __forceinline__ void store_gram(float* E, const Dim& d, const Area& o
   });
   if (!diagonal) {
     __syncthreads();
-    store_turned<ROWS, TS, TS + 1, THREADS>(E, a, d.np, j0, i0);
+    store_turned<ROWS, TS, TS + 1>(E, a, d.np, j0, i0);
   }
 }
 // A = X X^t: a tile on or above the diagonal, or one part of its sum, which ortho_sum_kernel adds up in their order.
@@ -467,23 +492,26 @@ __device__ __forceinline__ void store_gram(float* E, const Dim& d, const Area& o
 // where this and the launch behind it take 20, at eight 256 x 2304 matrices.)
 template <int TS>
 __global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Lists l, _Float16* base, float* parts, int kc) {
-  __shared__ Shared<TS> sh;
+  __shared__ typename Core<TS>::Shared sh;
   const Tile w = l.gram[blockIdx.x];
   const Mat t = l.table[w.mat];
   const Dim d(t.rows, t.cols, l.pad);
   const Area o(base, t, d);
   const int i0 = w.i * TS, j0 = w.j * TS;
   const int k0 = w.split * kc, k1 = k0 + kc < d.mp ? k0 + kc : d.mp;
-  Core<TS> core;
-  core.run(sh.st, o.x, i0, d.mp, o.x, j0, d.mp, k0, k1);
+  Core<TS>::run(sh, o.x, i0, d.mp, o.x, j0, d.mp, k0, k1, 1.f / SCALE);
   if (t.splits > 1) {
     float* mine = parts + t.part0 + (size_t)(blockIdx.x - t.gram0) * (TS * TS);
-    core.spill(sh.E, 1.f / SCALE);
-    for (int q = threadIdx.x; q < TS * TS; q += 256) mine[q] = sh.E[q / TS * (TS + 1) + q % TS];
+#pragma unroll 4
+    for (int q = threadIdx.x; q < TS * TS; q += 256) {
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < Core<TS>::PARTS; ++k) v += sh.E[k * TS * (TS + 1) + q / TS * (TS + 1) + q % TS];
+      mine[q] = v;
+    }
     return;
   }
-  core.spill(sh.E, 1.f / SCALE);
-  store_gram<TS, TS, 256>(sh.E, d, o, i0, j0, w.i == w.j);
+  store_gram<TS, TS, Core<TS>::PARTS>(sh.E, d, o, i0, j0, w.i == w.j);
 }
 // 32 rows of a tile of A from its parts
 template <int TS>
@@ -509,7 +537,7 @@ __global__ __launch_bounds__(256) void ortho_sum_kernel(Lists l, _Float16* base,
     e[0] = v.x, e[1] = v.y, e[2] = v.z, e[3] = v.w;
   }
   __syncthreads();
-  store_gram<32, TS, 256>(E, d, o, w.i * TS + slice, w.j * TS, w.i == w.j);
+  store_gram<32, TS, 1>(E, d, o, w.i * TS + slice, w.j * TS, w.i == w.j);
 }
 
 // out = q I + l G + f (G - t I) (H - t I) of symmetric matrices that commute (all are polynomials of one): a tile on or above
@@ -520,7 +548,7 @@ struct Op {
 };
 template <int TS>
 __global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
-  __shared__ Shared<TS> sh;
+  __shared__ typename Core<TS>::Shared sh;
   const Tile w = l.tri[blockIdx.x];
   const Mat t = l.table[w.mat];
   const Dim d(t.rows, t.cols, l.pad);
@@ -530,12 +558,10 @@ __global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16*
   const size_t step = 2 * d.a();
   const _Float16 *g = o.sq + op.g * step, *h = o.sq + op.h * step;
   const float *gd = o.diag + op.g * d.np, *hd = o.diag + op.h * d.np;
-  Core<TS> core;
-  core.run(sh.st, g, i0, d.np, h, j0, d.np, 0, d.np);
-  core.spill(sh.E, 1.f);
+  Core<TS>::run(sh, g, i0, d.np, h, j0, d.np, 0, d.np, 1.f);
   _Float16* out = o.sq + op.out * step;
   const bool diagonal = w.i == w.j;
-  rows8<TS, TS, TS + 1, 256>(sh.E, [&](int r, int c, float (&v)[8]) {
+  rows8<TS, TS, TS + 1, Core<TS>::PARTS>(sh.E, [&](int r, int c, float (&v)[8]) {
     const int i = i0 + r, j = j0 + c;
     const size_t at = place(i, j, d.np);
     const half8 gh = *reinterpret_cast<const half8*>(g + at), gl = *reinterpret_cast<const half8*>(g + at + LO);
@@ -556,7 +582,7 @@ __global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16*
   });
   if (!diagonal) {
     __syncthreads();
-    store_turned<TS, TS, TS + 1, 256>(sh.E, out, d.np, j0, i0);
+    store_turned<TS, TS, TS + 1>(sh.E, out, d.np, j0, i0);
   }
 }
 
@@ -564,24 +590,22 @@ __global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16*
 template <typename T, bool LAST, int TS>
 __global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* base, int R, float fs, int from, int update,
                                                              float decay) {
-  __shared__ Shared<TS> sh;
+  __shared__ typename Core<TS>::Shared sh;
   const Tile w = l.rect[blockIdx.x];
   const Mat t = l.table[w.mat];
   const Dim d(t.rows, t.cols, l.pad);
   const Area o(base, t, d);
   const int i0 = w.i * TS, j0 = w.j * TS;
   const _Float16 *a = o.sq + R * 2 * d.a(), *xt = o.xt + (from ? 2 * d.x() : 0);
-  Core<TS> core;
-  core.run(sh.st, a, i0, d.np, xt, j0, d.np, 0, d.np);
-  core.spill(sh.E, fs);
-  rows8<TS, TS, TS + 1, 256>(sh.E, [&](int r, int c, float (&v)[8]) {
+  Core<TS>::run(sh, a, i0, d.np, xt, j0, d.np, 0, d.np, fs);
+  rows8<TS, TS, TS + 1, Core<TS>::PARTS>(sh.E, [&](int r, int c, float (&v)[8]) {
     _Float16* x = o.x + place(i0 + r, j0 + c, d.mp);
     add8(v, o.diag[R * d.np + i0 + r], x);
     if constexpr (!LAST) store8(x, v);
   });
   __syncthreads();
   if constexpr (!LAST) {
-    store_turned<TS, TS, TS + 1, 256>(sh.E, o.xt + (from ? 0 : 2 * d.x()), d.np, j0, i0);
+    store_turned<TS, TS, TS + 1>(sh.E, o.xt + (from ? 0 : 2 * d.x()), d.np, j0, i0);
   } else {
     const bool tall = t.rows > t.cols;
     T* out = static_cast<T*>(t.dst);
