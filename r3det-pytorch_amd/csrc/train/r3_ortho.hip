@@ -51,7 +51,8 @@ struct Mat {  // one matrix, as the device's table holds it
   float* buf;        // the momentum (update only)
   int rows, cols;    // as the caller has it
   float rate;        // weights <- decay * weights - rate * result
-  int splits;        // parts of the sum of X X^t
+  unsigned short splits;  // parts of the sum of X X^t
+  unsigned short wide;    // whether four elements of a row are read and written as one
   unsigned gram0, tri0, rect0, fill0, norm0;  // first entries in the lists, see Lists
   size_t part0;      // floats before this matrix's partial tiles
   size_t at;         // halves before this matrix's arrays
@@ -73,20 +74,24 @@ struct Dim {  // padded with zeros, which stay zeros
   __host__ __device__ unsigned rect(int ts) const { return (unsigned)(np / ts) * (mp / ts); }
   __host__ __device__ unsigned norms() const { return (unsigned)(((size_t)n * m + NORM_CHUNK - 1) / NORM_CHUNK); }
 };
+struct Tile {  // one workgroup's work, with all that it needs of its matrix to begin
+  size_t at;    // Mat::at
+  size_t part;  // X X^t in parts: where this one goes
+  int np, mp;
+  unsigned short i, j, split, splits;
+  unsigned mat;
+};
 struct Area {  // where a matrix's arrays are
   _Float16 *x, *xt, *sq;  // xt: two, sq: SQ
   float* diag;
-  __device__ Area(_Float16* base, const Mat& t, const Dim& d) {
+  size_t na, nx;  // one of sq's, one of xt's (hi and lo)
+  __device__ Area(_Float16* base, const Tile& t) {
+    na = 2 * (size_t)t.np * t.np, nx = 2 * (size_t)t.np * t.mp;
     x = base + t.at;
-    xt = x + 2 * d.x();
-    sq = xt + 4 * d.x();
-    diag = reinterpret_cast<float*>(sq + 2 * SQ * d.a());
+    xt = x + nx;
+    sq = xt + 2 * nx;
+    diag = reinterpret_cast<float*>(sq + SQ * na);
   }
-};
-struct Tile {
-  unsigned mat;
-  unsigned short i, j;
-  unsigned split;
 };
 struct Lists {  // one entry a workgroup
   Mat* table;
@@ -108,66 +113,107 @@ struct Plan {
 };
 
 // ------------------------------------------------------------------------------------------------ the lists
-constexpr int BATCH = 43;
+constexpr int BATCH = 40;
 struct Batch {
   Mat m[BATCH];
+  int count;
+  Mat end;  // behind the last: the lists' ends
 };
-static_assert(sizeof(Batch) <= 3900, "a kernel's arguments hold 4 KB");
-__global__ void ortho_table_kernel(Batch b, int count, Mat* table) {
-  for (int i = threadIdx.x; i < count; i += blockDim.x) table[i] = b.m[i];
-}
+static_assert(sizeof(Batch) <= 3800, "a kernel's arguments hold 4 KB");
 
-__device__ __forceinline__ unsigned find(const Lists& l, unsigned Mat::* first, unsigned e) {
-  int lo = 0, hi = l.count - 1;  // the last matrix that begins at or before e
+__device__ __forceinline__ unsigned find(const Batch& b, unsigned Mat::* first, unsigned e) {
+  int lo = 0, hi = b.count - 1;  // the last matrix that begins at or before e
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
-    if (l.table[mid].*first <= e) lo = mid;
+    if (b.m[mid].*first <= e) lo = mid;
     else hi = mid - 1;
   }
   return lo;
 }
-__device__ __forceinline__ Tile triangle(unsigned mat, unsigned tile, unsigned wide, unsigned split) {
+__device__ __forceinline__ void triangle(Tile& w, unsigned tile, unsigned wide) {
   unsigned i = 0;
   while (tile >= wide - i) tile -= wide - i, ++i;  // (row i has wide - i tiles)
-  return Tile{mat, (unsigned short)i, (unsigned short)(i + tile), split};
+  w.i = i, w.j = i + tile;
 }
-__global__ void ortho_lists_kernel(Lists l) {
+// the table's and the lists' entries of `b`'s matrices
+__global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
   const unsigned g = blockIdx.x * blockDim.x + threadIdx.x, stride = gridDim.x * blockDim.x;
-  for (unsigned e = g; e < l.n_gram; e += stride) {
-    const unsigned k = find(l, &Mat::gram0, e);
-    const Mat& t = l.table[k];
-    const unsigned local = e - t.gram0;
-    l.gram[e] = triangle(k, local / t.splits, Dim(t.rows, t.cols, l.pad).np / l.gram_ts, local % t.splits);
+  if (g < (unsigned)b.count) l.table[first + g] = b.m[g];
+  const auto begin = [&](unsigned k) {
+    const Mat& t = b.m[k];
+    const Dim d(t.rows, t.cols, l.pad);
+    return Tile{t.at, 0, d.np, d.mp, 0, 0, 0, (unsigned short)t.splits, first + k};
+  };
+  for (unsigned e = b.m[0].gram0 + g; e < b.end.gram0; e += stride) {
+    const unsigned k = find(b, &Mat::gram0, e), local = e - b.m[k].gram0;
+    Tile w = begin(k);
+    triangle(w, local / w.splits, w.np / l.gram_ts);
+    w.split = local % w.splits;
+    w.part = b.m[k].part0 + (size_t)local * l.gram_ts * l.gram_ts;
+    l.gram[e] = w;
   }
-  for (unsigned e = g; e < l.n_tri; e += stride) {
-    const unsigned k = find(l, &Mat::tri0, e);
-    const Mat& t = l.table[k];
-    l.tri[e] = triangle(k, e - t.tri0, Dim(t.rows, t.cols, l.pad).np / l.tri_ts, 0);
+  for (unsigned e = b.m[0].tri0 + g; e < b.end.tri0; e += stride) {
+    const unsigned k = find(b, &Mat::tri0, e);
+    Tile w = begin(k);
+    triangle(w, e - b.m[k].tri0, w.np / l.tri_ts);
+    l.tri[e] = w;
   }
-  for (unsigned e = g; e < l.n_rect; e += stride) {
-    const unsigned k = find(l, &Mat::rect0, e);
-    const Mat& t = l.table[k];
-    const unsigned local = e - t.rect0, high = Dim(t.rows, t.cols, l.pad).np / l.rect_ts;
-    l.rect[e] = Tile{k, (unsigned short)(local % high), (unsigned short)(local / high), 0};
+  for (unsigned e = b.m[0].rect0 + g; e < b.end.rect0; e += stride) {
+    const unsigned k = find(b, &Mat::rect0, e), local = e - b.m[k].rect0;
+    Tile w = begin(k);
+    const unsigned high = w.np / l.rect_ts;
+    w.i = local % high, w.j = local / high;
+    l.rect[e] = w;
   }
-  for (unsigned e = g; e < l.n_fill; e += stride) {
-    const unsigned k = find(l, &Mat::fill0, e);
-    const Mat& t = l.table[k];
-    const unsigned local = e - t.fill0, wide = Dim(t.rows, t.cols, l.pad).mp / 64;
-    l.fill[e] = Tile{k, (unsigned short)(local / wide), (unsigned short)(local % wide), 0};
+  for (unsigned e = b.m[0].fill0 + g; e < b.end.fill0; e += stride) {
+    const unsigned k = find(b, &Mat::fill0, e), local = e - b.m[k].fill0;
+    Tile w = begin(k);
+    const unsigned wide = w.mp / 64;
+    w.i = local / wide, w.j = local % wide;
+    l.fill[e] = w;
   }
-  for (unsigned e = g; e < l.n_norm; e += stride) {
-    const unsigned k = find(l, &Mat::norm0, e);
-    l.norm_map[e] = make_uint2(k, e - l.table[k].norm0);
+  for (unsigned e = b.m[0].norm0 + g; e < b.end.norm0; e += stride) {
+    const unsigned k = find(b, &Mat::norm0, e);
+    l.norm_map[e] = make_uint2(first + k, e - b.m[k].norm0);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ momentum, norm, X
 template <typename T>
-__device__ __forceinline__ float direction(const Mat& t, size_t i, bool update, float mu, bool nesterov) {
-  const float g = (float)static_cast<const T*>(t.src)[i];
-  if (!update) return g;
-  return nesterov ? fmaf(mu, t.buf[i], g) : t.buf[i];
+struct alignas(4 * sizeof(T)) Four {
+  T v[4];
+};
+// What is orthogonalised, N elements from i on (N = 4: as one, which Mat::wide allows): the matrix, or the gradient with the
+// momentum (new: after its update, which this is).
+struct Momentum {
+  int update, nesterov;
+  float mu;
+};
+template <typename T, int N, bool NEW>
+__device__ __forceinline__ void direction(float (&v)[N], const Mat& t, size_t i, const Momentum& m) {
+  if constexpr (N == 4) {
+    const Four<T> g = *reinterpret_cast<const Four<T>*>(static_cast<const T*>(t.src) + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (float)g.v[k];
+  } else {
+    v[0] = (float)static_cast<const T*>(t.src)[i];
+  }
+  if (!m.update) return;
+  float b[N];
+  if constexpr (N == 4) {
+    const float4 u = *reinterpret_cast<const float4*>(t.buf + i);
+    b[0] = u.x, b[1] = u.y, b[2] = u.z, b[3] = u.w;
+  } else {
+    b[0] = t.buf[i];
+  }
+  if constexpr (NEW) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) b[k] = fmaf(m.mu, b[k], v[k]);
+    if constexpr (N == 4) *reinterpret_cast<float4*>(t.buf + i) = make_float4(b[0], b[1], b[2], b[3]);
+    else t.buf[i] = b[0];
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = m.nesterov ? fmaf(m.mu, b[k], v[k]) : b[k];
 }
 __device__ __forceinline__ double block_sum(double v, double* sh) {
 #pragma unroll
@@ -179,21 +225,53 @@ __device__ __forceinline__ double block_sum(double v, double* sh) {
 // momentum <- mu momentum + gradient, and the squares of the direction summed in 64 bits (no scaling of the matrix is needed
 // against overflow, and the order of the sums is fixed)
 template <typename T>
-__global__ __launch_bounds__(256) void ortho_norm_kernel(Lists l, double* __restrict__ norms, int update, float mu,
-                                                         int nesterov) {
+__global__ __launch_bounds__(256) void ortho_norm_kernel(Lists l, double* __restrict__ norms, Momentum m) {
   __shared__ double sh[4];
   const uint2 w = l.norm_map[blockIdx.x];
   const Mat t = l.table[w.x];
   const size_t all = (size_t)t.rows * t.cols, from = (size_t)w.y * NORM_CHUNK;
-  const size_t to = from + NORM_CHUNK < all ? from + NORM_CHUNK : all;
+  const int many = (int)(from + NORM_CHUNK < all ? NORM_CHUNK : all - from);
   double s = 0;
-  for (size_t i = from + threadIdx.x; i < to; i += 256) {
-    if (update) t.buf[i] = fmaf(mu, t.buf[i], (float)static_cast<const T*>(t.src)[i]);
-    const double v = direction<T>(t, i, update, mu, nesterov);
-    s = fma(v, v, s);
+  int i = threadIdx.x;
+  if (t.wide) {
+#pragma unroll 4
+    for (int q = threadIdx.x; q < many / 4; q += 256) {
+      float v[4];
+      direction<T, 4, true>(v, t, from + 4 * q, m);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s = fma((double)v[k], (double)v[k], s);
+    }
+    i += many / 4 * 4;
+  }
+  for (; i < many; i += 256) {
+    float v[1];
+    direction<T, 1, true>(v, t, from + i, m);
+    s = fma((double)v[0], (double)v[0], s);
   }
   s = block_sum(s, sh);
   if (threadIdx.x == 0) norms[blockIdx.x] = s;
+}
+// f(row and column of the caller's matrix, row and column of the TS x TS tile at (i0, j0), which of N the first is):
+// N = 4 along the caller's rows where that is allowed, else 1; TALL: the tile is of the transpose
+template <int TS, typename F>
+__device__ __forceinline__ void callers(const Mat& t, int i0, int j0, const F& f) {
+  const bool tall = t.rows > t.cols;
+  const int r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;
+  if (t.wide && t.cols % 4 == 0) {
+#pragma unroll 4
+    for (int q = threadIdx.x; q < TS * TS / 4; q += 256) {
+      const int r = q / (TS / 4), c = q % (TS / 4) * 4;
+      f(std::integral_constant<int, 4>(), (size_t)(r0 + r) * t.cols + c0 + c, r0 + r < t.rows && c0 + c < t.cols, tall ? c : r,
+        tall ? r : c, tall);
+    }
+  } else {
+#pragma unroll 4
+    for (int q = threadIdx.x; q < TS * TS; q += 256) {
+      const int r = q / TS, c = q % TS;
+      f(std::integral_constant<int, 1>(), (size_t)(r0 + r) * t.cols + c0 + c, r0 + r < t.rows && c0 + c < t.cols, tall ? c : r,
+        tall ? r : c, tall);
+    }
+  }
 }
 
 __device__ __forceinline__ void split16(float v, _Float16& hi, _Float16& lo) {
@@ -260,34 +338,27 @@ __device__ __forceinline__ void store_turned(const float* E, _Float16* p, int ld
 
 template <typename T>
 __global__ __launch_bounds__(256) void ortho_start_kernel(Lists l, const double* __restrict__ norms,
-                                                          _Float16* __restrict__ base, int update, float mu, int nesterov,
-                                                          double eps) {
+                                                          _Float16* __restrict__ base, Momentum m, double eps) {
   __shared__ double sh[4];
   __shared__ float E[64 * 65];
   const Tile w = l.fill[blockIdx.x];
   const Mat t = l.table[w.mat];
-  const Dim d(t.rows, t.cols, l.pad);
-  const Area o(base, t, d);
+  const Area o(base, w);
   double s = 0;
-  for (unsigned i = threadIdx.x; i < d.norms(); i += 256) s += norms[t.norm0 + i];
+  const unsigned chunks = Dim(t.rows, t.cols, l.pad).norms();
+  for (unsigned i = threadIdx.x; i < chunks; i += 256) s += norms[t.norm0 + i];
   s = block_sum(s, sh);
   const double inv = (double)SCALE / (sqrt(s) + eps);
-  const bool tall = t.rows > t.cols;
   const int i0 = w.i * 64, j0 = w.j * 64;
-  for (int q = threadIdx.x; q < 64 * 64; q += 256) {
-    // (consecutive threads along the caller's rows)
-    const int r = tall ? q % 64 : q / 64, c = tall ? q / 64 : q % 64;
-    const int i = i0 + r, j = j0 + c;
-    float v = 0.f;
-    if (i < d.n && j < d.m) {
-      const size_t at = tall ? (size_t)j * t.cols + i : (size_t)i * t.cols + j;
-      v = (float)((double)direction<T>(t, at, update, mu, nesterov) * inv);
-    }
-    E[r * 65 + c] = v;
-  }
+  callers<64>(t, i0, j0, [&](auto N, size_t at, bool in, int r, int c, bool tall) {
+    float v[N()] = {};
+    if (in) direction<T, N(), false>(v, t, at, m);
+#pragma unroll
+    for (int k = 0; k < N(); ++k) E[(tall ? r + k : r) * 65 + (tall ? c : c + k)] = (float)((double)v[k] * inv);
+  });
   __syncthreads();
-  rows8<64, 64, 65, 1>(E, [&](int r, int c, float (&v)[8]) { store8(o.x + place(i0 + r, j0 + c, d.mp), v); });
-  store_turned<64, 64, 65>(E, o.xt, d.np, j0, i0);
+  rows8<64, 64, 65, 1>(E, [&](int r, int c, float (&v)[8]) { store8(o.x + place(i0 + r, j0 + c, w.mp), v); });
+  store_turned<64, 64, 65>(E, o.xt, w.np, j0, i0);
 }
 
 // ------------------------------------------------------------------------------------------------ the products
@@ -473,18 +544,18 @@ using Core = std::conditional_t<TS == 128, Core128, Core64>;
 
 // A from ROWS rows of a tile in shared memory
 template <int ROWS, int TS, int PARTS>
-__device__ __forceinline__ void store_gram(float* E, const Dim& d, const Area& o, int i0, int j0, bool diagonal) {
-  _Float16* a = o.sq + SQ_A * 2 * d.a();
+__device__ __forceinline__ void store_gram(float* E, int np, const Area& o, int i0, int j0, bool diagonal) {
+  _Float16* a = o.sq + SQ_A * o.na;
   rows8<ROWS, TS, TS + 1, PARTS>(E, [&](int r, int c, float (&v)[8]) {
     if (diagonal)
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (i0 + r == j0 + c + k) o.diag[SQ_A * d.np + i0 + r] = v[k] * (1.f / SCALE), v[k] = 0.f;
-    store8(a + place(i0 + r, j0 + c, d.np), v);
+        if (i0 + r == j0 + c + k) o.diag[SQ_A * np + i0 + r] = v[k] * (1.f / SCALE), v[k] = 0.f;
+    store8(a + place(i0 + r, j0 + c, np), v);
   });
   if (!diagonal) {
     __syncthreads();
-    store_turned<ROWS, TS, TS + 1>(E, a, d.np, j0, i0);
+    store_turned<ROWS, TS, TS + 1>(E, a, np, j0, i0);
   }
 }
 // A = X X^t: a tile on or above the diagonal, or one part of its sum, which ortho_sum_kernel adds up in their order.
@@ -494,14 +565,12 @@ template <int TS>
 __global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Lists l, _Float16* base, float* parts, int kc) {
   __shared__ typename Core<TS>::Shared sh;
   const Tile w = l.gram[blockIdx.x];
-  const Mat t = l.table[w.mat];
-  const Dim d(t.rows, t.cols, l.pad);
-  const Area o(base, t, d);
+  const Area o(base, w);
   const int i0 = w.i * TS, j0 = w.j * TS;
-  const int k0 = w.split * kc, k1 = k0 + kc < d.mp ? k0 + kc : d.mp;
-  Core<TS>::run(sh, o.x, i0, d.mp, o.x, j0, d.mp, k0, k1, 1.f / SCALE);
-  if (t.splits > 1) {
-    float* mine = parts + t.part0 + (size_t)(blockIdx.x - t.gram0) * (TS * TS);
+  const int k0 = w.split * kc, k1 = k0 + kc < w.mp ? k0 + kc : w.mp;
+  Core<TS>::run(sh, o.x, i0, w.mp, o.x, j0, w.mp, k0, k1, 1.f / SCALE);
+  if (w.splits > 1) {
+    float* mine = parts + w.part;
 #pragma unroll 4
     for (int q = threadIdx.x; q < TS * TS; q += 256) {
       float v = 0.f;
@@ -511,25 +580,22 @@ __global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Lists l, _Float16* b
     }
     return;
   }
-  store_gram<TS, TS, Core<TS>::PARTS>(sh.E, d, o, i0, j0, w.i == w.j);
+  store_gram<TS, TS, Core<TS>::PARTS>(sh.E, w.np, o, i0, j0, w.i == w.j);
 }
 // 32 rows of a tile of A from its parts
 template <int TS>
 __global__ __launch_bounds__(256) void ortho_sum_kernel(Lists l, _Float16* base, const float* __restrict__ parts) {
   __shared__ float E[32 * (TS + 1)];
   const Tile w = l.gram[blockIdx.x];
-  if (w.split) return;
-  const Mat t = l.table[w.mat];
-  if (t.splits == 1) return;
-  const Dim d(t.rows, t.cols, l.pad);
-  const Area o(base, t, d);
+  if (w.split || w.splits == 1) return;
+  const Area o(base, w);
   const int slice = blockIdx.y * 32;
-  const float* mine = parts + t.part0 + (size_t)(blockIdx.x - t.gram0) * (TS * TS) + slice * TS;
+  const float* mine = parts + w.part + slice * TS;
 #pragma unroll
   for (int q = threadIdx.x * 4; q < 32 * TS; q += 1024) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int s = 0; s < t.splits; ++s) {
+    for (int s = 0; s < w.splits; ++s) {
       const float4 u = *reinterpret_cast<const float4*>(mine + (size_t)s * (TS * TS) + q);
       v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
     }
@@ -537,7 +603,7 @@ __global__ __launch_bounds__(256) void ortho_sum_kernel(Lists l, _Float16* base,
     e[0] = v.x, e[1] = v.y, e[2] = v.z, e[3] = v.w;
   }
   __syncthreads();
-  store_gram<32, TS, 1>(E, d, o, w.i * TS + slice, w.j * TS, w.i == w.j);
+  store_gram<32, TS, 1>(E, w.np, o, w.i * TS + slice, w.j * TS, w.i == w.j);
 }
 
 // out = q I + l G + f (G - t I) (H - t I) of symmetric matrices that commute (all are polynomials of one): a tile on or above
@@ -550,20 +616,17 @@ template <int TS>
 __global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
   __shared__ typename Core<TS>::Shared sh;
   const Tile w = l.tri[blockIdx.x];
-  const Mat t = l.table[w.mat];
-  const Dim d(t.rows, t.cols, l.pad);
-  const Area o(base, t, d);
+  const Area o(base, w);
   const Op op = blockIdx.y ? second : first;
   const int i0 = w.i * TS, j0 = w.j * TS;
-  const size_t step = 2 * d.a();
-  const _Float16 *g = o.sq + op.g * step, *h = o.sq + op.h * step;
-  const float *gd = o.diag + op.g * d.np, *hd = o.diag + op.h * d.np;
-  Core<TS>::run(sh, g, i0, d.np, h, j0, d.np, 0, d.np, 1.f);
-  _Float16* out = o.sq + op.out * step;
+  const _Float16 *g = o.sq + op.g * o.na, *h = o.sq + op.h * o.na;
+  const float *gd = o.diag + op.g * w.np, *hd = o.diag + op.h * w.np;
+  Core<TS>::run(sh, g, i0, w.np, h, j0, w.np, 0, w.np, 1.f);
+  _Float16* out = o.sq + op.out * o.na;
   const bool diagonal = w.i == w.j;
   rows8<TS, TS, TS + 1, Core<TS>::PARTS>(sh.E, [&](int r, int c, float (&v)[8]) {
     const int i = i0 + r, j = j0 + c;
-    const size_t at = place(i, j, d.np);
+    const size_t at = place(i, j, w.np);
     const half8 gh = *reinterpret_cast<const half8*>(g + at), gl = *reinterpret_cast<const half8*>(g + at + LO);
     const half8 hh = *reinterpret_cast<const half8*>(h + at), hl = *reinterpret_cast<const half8*>(h + at + LO);
     const float gi = op.fh * (gd[i] - op.t);
@@ -573,7 +636,7 @@ __global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16*
       float e = fmaf(fmaf(op.fg, hj, op.l), (float)gh[k] + (float)gl[k], op.fs * v[k]);
       e = fmaf(gi, (float)hh[k] + (float)hl[k], e);
       if (diagonal && i == j + k) {
-        o.diag[op.out * d.np + i] = fmaf(op.f * (gd[i] - op.t), hj, fmaf(op.l, gd[i], op.q)) + op.fs * op.back * v[k];
+        o.diag[op.out * w.np + i] = fmaf(op.f * (gd[i] - op.t), hj, fmaf(op.l, gd[i], op.q)) + op.fs * op.back * v[k];
         e = 0.f;
       }
       v[k] = e;
@@ -582,7 +645,7 @@ __global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16*
   });
   if (!diagonal) {
     __syncthreads();
-    store_turned<TS, TS, TS + 1>(sh.E, out, d.np, j0, i0);
+    store_turned<TS, TS, TS + 1>(sh.E, out, w.np, j0, i0);
   }
 }
 
@@ -592,33 +655,36 @@ __global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* 
                                                              float decay) {
   __shared__ typename Core<TS>::Shared sh;
   const Tile w = l.rect[blockIdx.x];
-  const Mat t = l.table[w.mat];
-  const Dim d(t.rows, t.cols, l.pad);
-  const Area o(base, t, d);
+  const Area o(base, w);
   const int i0 = w.i * TS, j0 = w.j * TS;
-  const _Float16 *a = o.sq + R * 2 * d.a(), *xt = o.xt + (from ? 2 * d.x() : 0);
-  Core<TS>::run(sh, a, i0, d.np, xt, j0, d.np, 0, d.np, fs);
+  const _Float16 *a = o.sq + R * o.na, *xt = o.xt + (from ? o.nx : 0);
+  Core<TS>::run(sh, a, i0, w.np, xt, j0, w.np, 0, w.np, fs);
   rows8<TS, TS, TS + 1, Core<TS>::PARTS>(sh.E, [&](int r, int c, float (&v)[8]) {
-    _Float16* x = o.x + place(i0 + r, j0 + c, d.mp);
-    add8(v, o.diag[R * d.np + i0 + r], x);
+    _Float16* x = o.x + place(i0 + r, j0 + c, w.mp);
+    add8(v, o.diag[R * w.np + i0 + r], x);
     if constexpr (!LAST) store8(x, v);
   });
   __syncthreads();
   if constexpr (!LAST) {
-    store_turned<TS, TS, TS + 1>(sh.E, o.xt + (from ? 0 : 2 * d.x()), d.np, j0, i0);
+    store_turned<TS, TS, TS + 1>(sh.E, o.xt + (from ? 0 : o.nx), w.np, j0, i0);
   } else {
-    const bool tall = t.rows > t.cols;
+    const Mat t = l.table[w.mat];
     T* out = static_cast<T*>(t.dst);
-#pragma unroll 4
-    for (int q = threadIdx.x; q < TS * TS; q += 256) {
-      const int r = tall ? q % TS : q / TS, c = tall ? q / TS : q % TS;
-      const int i = i0 + r, j = j0 + c;
-      if (i < d.n && j < d.m) {
-        const size_t at = tall ? (size_t)j * t.cols + i : (size_t)i * t.cols + j;
-        const float v = sh.E[r * (TS + 1) + c] * (1.f / SCALE);
-        out[at] = (T)(update ? fmaf(-t.rate, v, decay * (float)out[at]) : v);
+    callers<TS>(t, i0, j0, [&](auto N, size_t at, bool in, int r, int c, bool tall) {
+      if (!in) return;
+      float v[N()];
+      alignas(16) T x[N()];
+#pragma unroll
+      for (int k = 0; k < N(); ++k) v[k] = sh.E[(tall ? r + k : r) * (TS + 1) + (tall ? c : c + k)] * (1.f / SCALE);
+      if (update) {
+        if constexpr (N() == 4) *reinterpret_cast<Four<T>*>(x) = *reinterpret_cast<const Four<T>*>(out + at);
+        else x[0] = out[at];
+#pragma unroll
+        for (int k = 0; k < N(); ++k) v[k] = fmaf(-t.rate, v[k], decay * (float)x[k]);
       }
-    }
+      if constexpr (N() == 4) *reinterpret_cast<Four<T>*>(out + at) = Four<T>{{(T)v[0], (T)v[1], (T)v[2], (T)v[3]}};
+      else out[at] = (T)v[0];
+    });
   }
 }
 
@@ -764,16 +830,21 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
   float* parts = reinterpret_cast<float*>(ws + p.parts);
   _Float16* base = reinterpret_cast<_Float16*>(ws + p.halves);
   const int update = buf != nullptr;
+  const Momentum m{update, nesterov, mu};
   unsigned gram = 0, tri = 0, rect = 0, fill = 0, norm = 0;
   size_t halves = 0, part = 0;
+  const dim3 wg(256);
   for (int first = 0; first < count; first += BATCH) {
     Batch batch{};
-    const int many = count - first < BATCH ? count - first : BATCH;
-    for (int k = 0; k < many; ++k) {
+    batch.count = count - first < BATCH ? count - first : BATCH;
+    const unsigned was = fill + gram;
+    for (int k = 0; k < batch.count; ++k) {
       const int i = first + k;
       const Dim d(rows[i], cols[i], l.pad);
       const unsigned s = (unsigned)((d.mp + p.kc - 1) / p.kc);
-      batch.m[k] = Mat{src[i], dst[i], update ? buf[i] : nullptr, rows[i], cols[i], rates ? rates[i] : 0.f, (int)s, gram,
+      const auto over = [](const void* q, size_t bytes) { return reinterpret_cast<uintptr_t>(q) % bytes != 0; };
+      const unsigned short wide = !over(src[i], 4 * sizeof(T)) && !over(dst[i], 4 * sizeof(T)) && (!update || !over(buf[i], 16));
+      batch.m[k] = Mat{src[i], dst[i], update ? buf[i] : nullptr, rows[i], cols[i], rates ? rates[i] : 0.f, (unsigned short)s, wide, gram,
                        tri, rect, fill, norm, part, halves};
       gram += d.tri(l.gram_ts) * s;
       tri += d.tri(l.tri_ts);
@@ -783,15 +854,14 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
       if (s > 1) part += (size_t)d.tri(l.gram_ts) * s * l.gram_ts * l.gram_ts;
       halves += d.halves();
     }
-    hipLaunchKernelGGL(ortho_table_kernel, dim3(1), dim3(64), 0, st, batch, many, l.table + first);
+    batch.end.gram0 = gram, batch.end.tri0 = tri, batch.end.rect0 = rect, batch.end.fill0 = fill, batch.end.norm0 = norm;
+    unsigned blocks = (fill + gram - was) / 256 + 1;
+    if (blocks > 512) blocks = 512;
+    hipLaunchKernelGGL(ortho_lists_kernel, dim3(blocks), wg, 0, st, l, batch, (unsigned)first);
     if (hipGetLastError() != hipSuccess) return -2;
   }
-  unsigned blocks = (l.n_fill > l.n_gram ? l.n_fill : l.n_gram) / 256 + 1;
-  if (blocks > 1024) blocks = 1024;
-  const dim3 wg(256);
-  hipLaunchKernelGGL(ortho_lists_kernel, dim3(blocks), wg, 0, st, l);
-  hipLaunchKernelGGL((ortho_norm_kernel<T>), dim3(l.n_norm), wg, 0, st, l, norms, update, mu, nesterov);
-  hipLaunchKernelGGL((ortho_start_kernel<T>), dim3(l.n_fill), wg, 0, st, l, norms, base, update, mu, nesterov, eps);
+  hipLaunchKernelGGL((ortho_norm_kernel<T>), dim3(l.n_norm), wg, 0, st, l, norms, m);
+  hipLaunchKernelGGL((ortho_start_kernel<T>), dim3(l.n_fill), wg, 0, st, l, norms, base, m, eps);
   if (hipGetLastError() != hipSuccess) return -2;
   const auto square = [&](const Op& one, const Op* two) {
     choose(l.tri_ts, [&](auto TS) {
