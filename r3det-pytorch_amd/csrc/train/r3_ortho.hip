@@ -688,6 +688,215 @@ __global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* 
   }
 }
 
+// ------------------------------------------------------------------------------------------------ small matrices
+// A matrix of at most 64 x 128 stays in one workgroup's shared memory from the first step to the last, so that a list of such
+// is one launch instead of two dozen that wait for each other (64 x 64: XX us against 64).  One step at a time: X and X^t, A
+// and F, each 32 x 32 of a product a wavefront.  A lane holds four neighbouring entries of a column of the product, which
+// are four of a row of X^t, or of A and F, which are symmetric.
+constexpr int SMALL_N = 64, SMALL_M = 128;
+__host__ __device__ inline bool is_small(int rows, int cols) {
+  return (rows < cols ? rows : cols) <= SMALL_N && (rows < cols ? cols : rows) <= SMALL_M;
+}
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+struct Small {
+  _Float16 x[SMALL_M / 32 * BLOCK], xt[SMALL_M / 32 * BLOCK], a[2 * BLOCK], f[2 * BLOCK];
+  float da[64], df[64];
+  double norm[4];
+};
+// 32 x 32 at (i, j) of P Q^t over K columns, which both have
+template <int K>
+__device__ __forceinline__ float16v small_product(const _Float16* p, int i, const _Float16* q, int j) {
+  float16v hh = {}, hl = {}, lh = {};
+  const int lane8 = (threadIdx.x & 63) * 8;
+  half8 ph[K / 16], pl[K / 16], qh[K / 16], ql[K / 16];
+#pragma unroll
+  for (int k = 0; k < K / 16; ++k) {
+    const _Float16 *u = p + place(i, k * 16, K) + lane8, *v = q + place(j, k * 16, K) + lane8;
+    ph[k] = *reinterpret_cast<const half8*>(u), pl[k] = *reinterpret_cast<const half8*>(u + LO);
+    qh[k] = *reinterpret_cast<const half8*>(v), ql[k] = *reinterpret_cast<const half8*>(v + LO);
+  }
+#pragma unroll
+  for (int k = 0; k < K / 16; ++k) {  // (three chains: a matrix instruction waits for the one before it on the same sum)
+    hh = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[k], qh[k], hh, 0, 0, 0);
+    hl = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[k], ql[k], hl, 0, 0, 0);
+    lh = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[k], qh[k], lh, 0, 0, 0);
+  }
+  return hh + (hl + lh);
+}
+// f(place among four, row, column) for the sixteen entries of a lane, four of a column at a time: each four then `done`
+template <typename F>
+__device__ __forceinline__ void small_fours(int i, int j, const F& f) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) f(g, i + 8 * g + 4 * (lane >> 5), j + (lane & 31));
+}
+__device__ __forceinline__ void put4(_Float16* at, const float (&v)[4]) {
+  half4 h, l;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    _Float16 hh, ll;
+    split16(v[k], hh, ll);
+    h[k] = hh, l[k] = ll;
+  }
+  *reinterpret_cast<half4*>(at) = h;
+  *reinterpret_cast<half4*>(at + LO) = l;
+}
+__device__ __forceinline__ void get4(float (&v)[4], const _Float16* at) {
+  const half4 h = *reinterpret_cast<const half4*>(at), l = *reinterpret_cast<const half4*>(at + LO);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = (float)h[k] + (float)l[k];
+}
+struct Step {  // F = q I + l A + c (A - t I)^2
+  float c, t, q, l;
+};
+template <typename T, int mp>
+__device__ __forceinline__ void small_matrix(Small& sh, const Mat& t, const Momentum& m, const Step& p, int steps, double eps,
+                                             float decay) {
+  const bool tall = t.rows > t.cols;
+  const int shift = tall || mp == 64 ? 6 : 7;  // of the columns of the padded matrix as the caller has it
+  const int wave = threadIdx.x >> 6;
+  {
+    constexpr int EACH = SMALL_N * mp / 256;
+    float v[EACH];
+    double s = 0;
+    const auto at = [&](int k, bool& in) {
+      const int e = k * 256 + threadIdx.x, r = e >> shift, c = e & ((1 << shift) - 1);
+      in = r < t.rows && c < t.cols;
+      return in ? (size_t)r * t.cols + c : 0;
+    };
+    const auto read = [&](auto many) {  // (every load before the first use, inside or not)
+      float g[many()], u[many()];
+      bool in;
+#pragma unroll
+      for (int k = 0; k < many(); ++k) g[k] = (float)static_cast<const T*>(t.src)[at(k, in)];
+      if (m.update) {
+#pragma unroll
+        for (int k = 0; k < many(); ++k) u[k] = t.buf[at(k, in)];
+      }
+#pragma unroll
+      for (int k = 0; k < many(); ++k) {
+        const size_t where = at(k, in);
+        if (m.update) {
+          u[k] = fmaf(m.mu, u[k], g[k]);
+          if (in) t.buf[where] = u[k];
+          g[k] = m.nesterov ? fmaf(m.mu, u[k], g[k]) : u[k];
+        }
+        v[k] = in ? g[k] : 0.f;
+        s = fma((double)v[k], (double)v[k], s);
+      }
+    };
+    read(std::integral_constant<int, EACH>());
+    s = block_sum(s, sh.norm);
+    const double inv = (double)SCALE / (sqrt(s) + eps);
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      const int e = k * 256 + threadIdx.x, r = e >> shift, c = e & ((1 << shift) - 1);
+      {
+        const int i = tall ? c : r, j = tall ? r : c;
+        _Float16 h, l;
+        split16((float)((double)v[k] * inv), h, l);
+        const size_t x = place(i, j, mp), y = place(j, i, 64);
+        sh.x[x] = h, sh.x[x + LO] = l, sh.xt[y] = h, sh.xt[y + LO] = l;
+      }
+    }
+  }
+  __syncthreads();
+  const int i = (wave >> 1) * 32, j = (wave & 1) * 32;
+  T* out = static_cast<T*>(t.dst);
+  const auto target = [&](int r, int c, bool& in) {
+    const int row = tall ? c : r, col = tall ? r : c;
+    in = row < t.rows && col < t.cols;
+    return in ? (size_t)row * t.cols + col : 0;
+  };
+  T was[mp / 64][4][4];  // the weights: on their way while the steps are taken
+  if (m.update) {
+#pragma unroll
+    for (int h = 0; h < mp / 64; ++h)
+        small_fours(i, j + 64 * h, [&](int g, int r, int c) {
+          bool in;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) was[h][g][k] = out[target(r + k, c, in)];
+        });
+  }
+  for (int step = 0; step < steps; ++step) {
+    {
+      const float16v acc = small_product<mp>(sh.x, i, sh.x, j);
+      small_fours(i, j, [&](int g, int r, int c) {
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[k] = acc[4 * g + k] * (1.f / SCALE);
+          if (r + k == c) sh.da[c] = v[k] * (1.f / SCALE), v[k] = 0.f;
+        }
+        put4(sh.a + place(c, r, 64), v);
+      });
+    }
+    __syncthreads();
+    {
+      const float16v acc = small_product<64>(sh.a, i, sh.a, j);
+      small_fours(i, j, [&](int g, int r, int c) {
+        float v[4], a[4];
+        get4(a, sh.a + place(c, r, 64));
+        const float dj = sh.da[c] - p.t;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float di = sh.da[r + k] - p.t;
+          v[k] = fmaf(fmaf(p.c, di + dj, p.l), a[k], p.c / SCALE * acc[4 * g + k]);
+          if (r + k == c) {
+            sh.df[c] = fmaf(p.c * di, di, fmaf(p.l, sh.da[c], p.q)) + p.c / (SCALE * SCALE) * acc[4 * g + k];
+            v[k] = 0.f;
+          }
+        }
+        put4(sh.f + place(c, r, 64), v);
+      });
+    }
+    __syncthreads();
+    float16v acc[mp / 64];
+#pragma unroll
+    for (int h = 0; h < mp / 64; ++h) acc[h] = small_product<64>(sh.f, i, sh.xt, j + 64 * h);
+    float v[mp / 64][4][4];
+#pragma unroll
+    for (int h = 0; h < mp / 64; ++h)
+        small_fours(i, j + 64 * h, [&](int g, int r, int c) {
+          float x[4];
+          get4(x, sh.xt + place(c, r, 64));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[h][g][k] = fmaf(sh.df[r + k], x[k], acc[h][4 * g + k] * (1.f / SCALE));
+        });
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < mp / 64; ++h)
+        small_fours(i, j + 64 * h, [&](int g, int r, int c) {
+          if (step + 1 < steps) {
+            put4(sh.xt + place(c, r, 64), v[h][g]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              _Float16 hi, lo;
+              split16(v[h][g][k], hi, lo);
+              const size_t at = place(r + k, c, mp);
+              sh.x[at] = hi, sh.x[at + LO] = lo;
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              bool in;
+              const size_t at = target(r + k, c, in);
+              const float y = v[h][g][k] * (1.f / SCALE);
+              if (in) out[at] = (T)(m.update ? fmaf(-t.rate, y, decay * (float)was[h][g][k]) : y);
+            }
+          }
+        });
+    __syncthreads();
+  }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void ortho_small_kernel(Batch b, Momentum m, Step p, int steps, double eps, float decay) {
+  __shared__ Small sh;
+  const Mat t = b.m[blockIdx.x];
+  if (t.rows <= 64 && t.cols <= 64) small_matrix<T, 64>(sh, t, m, p, steps, eps, decay);
+  else small_matrix<T, 128>(sh, t, m, p, steps, eps, decay);
+}
+
 // ------------------------------------------------------------------------------------------------ the host
 size_t round256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -701,12 +910,13 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   }
   Lists& l = p.l;
   l = Lists{};
-  l.count = count;
   l.pad = 128;
   // Tiles: 128 needs half the reads of two operands that 64 does, and is taken for a pass that fills the card with such
   // tiles.
   uint64_t tri128 = 0, rect128 = 0, gram128 = 0;
   for (int i = 0; i < count; ++i) {
+    if (is_small(rows[i], cols[i])) continue;
+    ++l.count;
     const Dim w(rows[i], cols[i], 128);
     tri128 += w.tri(128), rect128 += w.rect(128);
     gram128 += (uint64_t)w.tri(128) * ((w.mp + 255) / 256);
@@ -716,9 +926,10 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   l.rect_ts = rect128 >= WANT / 2 ? 128 : 64;
   // X X^t: the longest parts of the sum that still fill the card.  A part is a workgroup's time, so the parts of a ragged
   // list are of like length, and a short list of wide matrices is spread.
-  for (p.kc = 4096; p.kc > 256; p.kc /= 2) {
+  for (p.kc = 4096; p.kc > 512; p.kc /= 2) {
     uint64_t blocks = 0;
     for (int i = 0; i < count; ++i) {
+      if (is_small(rows[i], cols[i])) continue;
       const Dim d(rows[i], cols[i], l.pad);
       blocks += (uint64_t)d.tri(l.gram_ts) * ((d.mp + p.kc - 1) / p.kc);
     }
@@ -727,6 +938,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   uint64_t gram = 0, tri = 0, rect = 0, fill = 0, norm = 0, part = 0, halves = 0;
   p.split = false;
   for (int i = 0; i < count; ++i) {
+    if (is_small(rows[i], cols[i])) continue;
     const Dim d(rows[i], cols[i], l.pad);
     const unsigned s = (unsigned)((d.mp + p.kc - 1) / p.kc);
     gram += (uint64_t)d.tri(l.gram_ts) * s;
@@ -746,7 +958,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
     at += round256(bytes);
     return was;
   };
-  p.table = take(sizeof(Mat) * (size_t)count);
+  p.table = take(sizeof(Mat) * (size_t)l.count);
   p.gram = take(sizeof(Tile) * gram);
   p.tri = take(sizeof(Tile) * tri);
   p.rect = take(sizeof(Tile) * rect);
@@ -755,7 +967,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   p.norms = take(sizeof(double) * norm);
   p.parts = take(sizeof(float) * part);
   p.halves = take(sizeof(_Float16) * halves);
-  p.total = at;
+  p.total = at ? at : 256;  // (nothing but small matrices needs nothing)
   return 0;
 }
 
@@ -834,18 +1046,33 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
   unsigned gram = 0, tri = 0, rect = 0, fill = 0, norm = 0;
   size_t halves = 0, part = 0;
   const dim3 wg(256);
-  for (int first = 0; first < count; first += BATCH) {
+  const auto matrix = [&](int i) {
+    const auto over = [](const void* q, size_t bytes) { return reinterpret_cast<uintptr_t>(q) % bytes != 0; };
+    const bool wide = !over(src[i], 4 * sizeof(T)) && !over(dst[i], 4 * sizeof(T)) && (!update || !over(buf[i], 16));
+    return Mat{src[i], dst[i], update ? buf[i] : nullptr, rows[i], cols[i], rates ? rates[i] : 0.f, 1, wide};
+  };
+  if (l.count < count)
+    for (int i = 0; i < count;) {
+      Batch batch{};
+      for (; i < count && batch.count < BATCH; ++i)
+        if (is_small(rows[i], cols[i])) batch.m[batch.count++] = matrix(i);
+      if (batch.count)
+        hipLaunchKernelGGL((ortho_small_kernel<T>), dim3(batch.count), wg, 0, st, batch, m, Step{f.c, f.t, f.q, f.l}, steps, eps,
+                           decay);
+      if (hipGetLastError() != hipSuccess) return -2;
+    }
+  if (l.count == 0) return 0;
+  for (int i = 0, first = 0; first < l.count;) {
     Batch batch{};
-    batch.count = count - first < BATCH ? count - first : BATCH;
     const unsigned was = fill + gram;
-    for (int k = 0; k < batch.count; ++k) {
-      const int i = first + k;
+    for (; i < count && batch.count < BATCH; ++i) {
+      if (is_small(rows[i], cols[i])) continue;
       const Dim d(rows[i], cols[i], l.pad);
       const unsigned s = (unsigned)((d.mp + p.kc - 1) / p.kc);
-      const auto over = [](const void* q, size_t bytes) { return reinterpret_cast<uintptr_t>(q) % bytes != 0; };
-      const unsigned short wide = !over(src[i], 4 * sizeof(T)) && !over(dst[i], 4 * sizeof(T)) && (!update || !over(buf[i], 16));
-      batch.m[k] = Mat{src[i], dst[i], update ? buf[i] : nullptr, rows[i], cols[i], rates ? rates[i] : 0.f, (unsigned short)s, wide, gram,
-                       tri, rect, fill, norm, part, halves};
+      Mat& t = batch.m[batch.count++];
+      t = matrix(i);
+      t.splits = (unsigned short)s;
+      t.gram0 = gram, t.tri0 = tri, t.rect0 = rect, t.fill0 = fill, t.norm0 = norm, t.part0 = part, t.at = halves;
       gram += d.tri(l.gram_ts) * s;
       tri += d.tri(l.tri_ts);
       rect += d.rect(l.rect_ts);
@@ -859,6 +1086,7 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
     if (blocks > 512) blocks = 512;
     hipLaunchKernelGGL(ortho_lists_kernel, dim3(blocks), wg, 0, st, l, batch, (unsigned)first);
     if (hipGetLastError() != hipSuccess) return -2;
+    first += batch.count;
   }
   hipLaunchKernelGGL((ortho_norm_kernel<T>), dim3(l.n_norm), wg, 0, st, l, norms, m);
   hipLaunchKernelGGL((ortho_start_kernel<T>), dim3(l.n_fill), wg, 0, st, l, norms, base, m, eps);
@@ -916,7 +1144,7 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
 
 size_t r3k_ortho_workspace_bytes(int count, const int* rows, const int* cols) {
   Plan p;
-  return plan(count, rows, cols, p) == 0 ? p.total : 0;
+  return count > 0 && plan(count, rows, cols, p) == 0 ? p.total : 0;
 }
 
 int r3k_ortho(int count, const void* const* src, void* const* dst, float* const* buf, int dtype, const int* rows,
