@@ -754,7 +754,7 @@ __device__ __forceinline__ void small_matrix(Small& sh, const Mat& t, const Mome
                                              float decay) {
   const bool tall = t.rows > t.cols;
   const int shift = tall || mp == 64 ? 6 : 7;  // of the columns of the padded matrix as the caller has it
-  const int wave = threadIdx.x >> 6;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   {
     constexpr int EACH = SMALL_N * mp / 256;
     float v[EACH];
@@ -818,76 +818,89 @@ __device__ __forceinline__ void small_matrix(Small& sh, const Mat& t, const Mome
           for (int k = 0; k < 4; ++k) was[h][g][k] = out[target(r + k, c, in)];
         });
   }
-  for (int step = 0; step < steps; ++step) {
+  float v[mp / 64][4][4];
+  const int diagonal = i == j ? (lane & 31) - 4 * (lane >> 5) : -1;  // of this lane's column: its row less 4 (l / 32)
+  for (int step = 0;; ++step) {
     {
       const float16v acc = small_product<mp>(sh.x, i, sh.x, j);
+      float d = 0.f;
       small_fours(i, j, [&](int g, int r, int c) {
-        float v[4];
+        float a[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          v[k] = acc[4 * g + k] * (1.f / SCALE);
-          if (r + k == c) sh.da[c] = v[k] * (1.f / SCALE), v[k] = 0.f;
+          const bool on = diagonal == 8 * g + k;
+          a[k] = acc[4 * g + k] * (1.f / SCALE);
+          d = on ? a[k] : d;
+          a[k] = on ? 0.f : a[k];
         }
-        put4(sh.a + place(c, r, 64), v);
+        put4(sh.a + place(c, r, 64), a);
       });
+      if (diagonal >= 0 && diagonal % 8 < 4) sh.da[j + (lane & 31)] = d * (1.f / SCALE);
     }
     __syncthreads();
     {
       const float16v acc = small_product<64>(sh.a, i, sh.a, j);
+      const float aj = sh.da[j + (lane & 31)], dj = aj - p.t, cs = p.c / SCALE;
+      float d = 0.f;
       small_fours(i, j, [&](int g, int r, int c) {
-        float v[4], a[4];
+        float a[4];
         get4(a, sh.a + place(c, r, 64));
-        const float dj = sh.da[c] - p.t;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float di = sh.da[r + k] - p.t;
-          v[k] = fmaf(fmaf(p.c, di + dj, p.l), a[k], p.c / SCALE * acc[4 * g + k]);
-          if (r + k == c) {
-            sh.df[c] = fmaf(p.c * di, di, fmaf(p.l, sh.da[c], p.q)) + p.c / (SCALE * SCALE) * acc[4 * g + k];
-            v[k] = 0.f;
-          }
+          const bool on = diagonal == 8 * g + k;
+          const float sum = cs * acc[4 * g + k];
+          a[k] = fmaf(fmaf(p.c, sh.da[r + k] - p.t + dj, p.l), a[k], sum);
+          d = on ? sum : d;
+          a[k] = on ? 0.f : a[k];
         }
-        put4(sh.f + place(c, r, 64), v);
+        put4(sh.f + place(c, r, 64), a);
       });
+      if (diagonal >= 0 && diagonal % 8 < 4)
+        sh.df[j + (lane & 31)] = fmaf(p.c * dj, dj, fmaf(p.l, aj, p.q)) + d * (1.f / SCALE);
     }
     __syncthreads();
-    float16v acc[mp / 64];
 #pragma unroll
-    for (int h = 0; h < mp / 64; ++h) acc[h] = small_product<64>(sh.f, i, sh.xt, j + 64 * h);
-    float v[mp / 64][4][4];
+    for (int h = 0; h < mp / 64; ++h) {
+      const float16v acc = small_product<64>(sh.f, i, sh.xt, j + 64 * h);
+      small_fours(i, j + 64 * h, [&](int g, int r, int c) {
+        float x[4];
+        get4(x, sh.xt + place(c, r, 64));
 #pragma unroll
-    for (int h = 0; h < mp / 64; ++h)
-        small_fours(i, j + 64 * h, [&](int g, int r, int c) {
-          float x[4];
-          get4(x, sh.xt + place(c, r, 64));
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[h][g][k] = fmaf(sh.df[r + k], x[k], acc[h][4 * g + k] * (1.f / SCALE));
-        });
+        for (int k = 0; k < 4; ++k) v[h][g][k] = fmaf(sh.df[r + k], x[k], acc[4 * g + k] * (1.f / SCALE));
+      });
+    }
+    if (step + 1 == steps) break;
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < mp / 64; ++h)
-        small_fours(i, j + 64 * h, [&](int g, int r, int c) {
-          if (step + 1 < steps) {
-            put4(sh.xt + place(c, r, 64), v[h][g]);
+      small_fours(i, j + 64 * h, [&](int g, int r, int c) {
+        half4 hi, lo;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              _Float16 hi, lo;
-              split16(v[h][g][k], hi, lo);
-              const size_t at = place(r + k, c, mp);
-              sh.x[at] = hi, sh.x[at + LO] = lo;
-            }
-          } else {
+        for (int k = 0; k < 4; ++k) {
+          _Float16 u, w;
+          split16(v[h][g][k], u, w);
+          hi[k] = u, lo[k] = w;
+        }
+        _Float16* at = sh.xt + place(c, r, 64);
+        *reinterpret_cast<half4*>(at) = hi;
+        *reinterpret_cast<half4*>(at + LO) = lo;
+        at = sh.x + place(r, c, mp);  // (rows of eight columns lie behind each other: r + 1 is 8 further)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              bool in;
-              const size_t at = target(r + k, c, in);
-              const float y = v[h][g][k] * (1.f / SCALE);
-              if (in) out[at] = (T)(m.update ? fmaf(-t.rate, y, decay * (float)was[h][g][k]) : y);
-            }
-          }
-        });
+        for (int k = 0; k < 4; ++k) at[8 * k] = hi[k], at[8 * k + LO] = lo[k];
+      });
     __syncthreads();
   }
+#pragma unroll
+  for (int h = 0; h < mp / 64; ++h)
+    small_fours(i, j + 64 * h, [&](int g, int r, int c) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        bool in;
+        const size_t at = target(r + k, c, in);
+        const float y = v[h][g][k] * (1.f / SCALE);
+        if (in) out[at] = (T)(m.update ? fmaf(-t.rate, y, decay * (float)was[h][g][k]) : y);
+      }
+    });
 }
 template <typename T>
 __global__ __launch_bounds__(256) void ortho_small_kernel(Batch b, Momentum m, Step p, int steps, double eps, float decay) {
