@@ -177,6 +177,19 @@ def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def run_on(device, what, fn, *args):
+    """``fn(*args, stream)`` with the current stream of ``device``, checked.  Addresses are plain numbers and the device is
+    switched only where another one is current: a call of a small operator is mostly what happens here."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        code = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if code != 0:
+        check(code, what)
+
+
 def iou_workspace(n1, n2, device):
     """Scratch for the stream + drain IoU pipeline (worst-case sized, mostly untouched; the
     caching allocator makes the per-call allocation free)."""

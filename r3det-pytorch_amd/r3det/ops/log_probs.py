@@ -33,33 +33,44 @@ def _rows(logits):
         return logits.reshape(-1, classes)
 
 
+def _forward(logits, labels, top_k, want_entropy, ignore_index, want_stats):
+    x = _rows(logits)
+    rows, classes = x.shape
+    lead, dev = logits.shape[:-1], logits.device
+    f32 = torch.float32
+    log_prob = torch.empty(lead, dtype=f32, device=dev) if labels is not None else None
+    entropy = torch.empty(lead, dtype=f32, device=dev) if want_entropy else None
+    top_lp = top_ix = stats = ws = None
+    if top_k:
+        top_lp = torch.empty((*lead, top_k), dtype=f32, device=dev)
+        top_ix = torch.empty((*lead, top_k), dtype=torch.int64, device=dev)
+    if want_stats:
+        stats = torch.empty((rows, 2), dtype=f32, device=dev)
+    if labels is not None:
+        labels = labels.contiguous()
+    if rows:
+        L = _C.lib()
+        nbytes = L.r3det_label_log_probs_workspace_bytes(rows, classes, top_k)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _C.run_on(dev, "r3det_label_log_probs", L.r3det_label_log_probs, x.data_ptr(), DTYPES[x.dtype], rows, classes, x.stride(0),
+                  _at(labels), ignore_index or 0, int(ignore_index is not None), top_k, _at(log_prob), _at(entropy), _at(top_lp),
+                  _at(top_ix), _at(stats), _at(ws), nbytes)
+    return log_prob, entropy, top_lp, top_ix, labels, stats
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
 class _LabelLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, top_k, want_entropy, ignore_index):
-        x = _rows(logits.detach())
-        rows, classes = x.shape
-        lead, dev = logits.shape[:-1], logits.device
-        new = lambda *s, dtype=torch.float32: torch.empty(s, dtype=dtype, device=dev)  # noqa: E731
-        log_prob = new(*lead) if labels is not None else None
-        entropy = new(*lead) if want_entropy else None
-        top_lp = new(*lead, top_k) if top_k else None
-        top_ix = new(*lead, top_k, dtype=torch.int64) if top_k else None
-        stats = new(rows, 2) if ctx.needs_input_grad[0] else None
-        lab = labels.contiguous() if labels is not None else None
-        has_ignore, ignore = ignore_index is not None, ignore_index or 0
-        if rows:
-            L = _C.lib()
-            with torch.cuda.device(dev):
-                nbytes = int(L.r3det_label_log_probs_workspace_bytes(rows, classes, top_k))
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-                _C.check(L.r3det_label_log_probs(_C.ptr(x), DTYPES[x.dtype], rows, classes, x.stride(0), _C.ptr(lab), ignore,
-                                                 int(has_ignore), top_k, _C.ptr(log_prob), _C.ptr(entropy), _C.ptr(top_lp),
-                                                 _C.ptr(top_ix), _C.ptr(stats), _C.ptr(ws), nbytes, _C.stream()),
-                         "r3det_label_log_probs")
+        log_prob, entropy, top_lp, top_ix, labels, stats = _forward(logits.detach(), labels, top_k, want_entropy, ignore_index,
+                                                                    True)
         ctx.set_materialize_grads(False)
-        if stats is not None:
-            ctx.save_for_backward(logits, lab, stats, entropy, top_ix)
-            ctx.args = (top_k, ignore, has_ignore)
+        ctx.save_for_backward(logits, labels, stats, entropy, top_ix)
+        ctx.args = (top_k, ignore_index)
         if top_ix is not None:
             ctx.mark_non_differentiable(top_ix)
         return log_prob, entropy, top_lp, top_ix
@@ -67,20 +78,18 @@ class _LabelLogProbs(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_lp, d_h, d_top, _):
-        logits, lab, stats, entropy, top_ix = ctx.saved_tensors
-        top_k, ignore, has_ignore = ctx.args
         if d_lp is None and d_h is None and d_top is None:
             return None, None, None, None, None
-        x = _rows(logits.detach())
+        logits, labels, stats, entropy, top_ix = ctx.saved_tensors
+        top_k, ignore_index = ctx.args
+        x = _rows(logits)
         rows, classes = x.shape
         dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        d_lp, d_h, d_top = (None if d is None else d.to(torch.float32).contiguous() for d in (d_lp, d_h, d_top))
+        d_lp, d_h, d_top = (None if d is None else d.contiguous() for d in (d_lp, d_h, d_top))  # (fp32, as the outputs are)
         if rows:
-            with torch.cuda.device(logits.device):
-                _C.check(_C.lib().r3det_label_log_probs_backward(
-                    _C.ptr(x), DTYPES[x.dtype], rows, classes, x.stride(0), _C.ptr(lab), ignore, int(has_ignore), top_k,
-                    _C.ptr(stats), _C.ptr(entropy), _C.ptr(top_ix), _C.ptr(d_lp), _C.ptr(d_h), _C.ptr(d_top), _C.ptr(dx),
-                    _C.stream()), "r3det_label_log_probs_backward")
+            _C.run_on(logits.device, "r3det_label_log_probs_backward", _C.lib().r3det_label_log_probs_backward, x.data_ptr(),
+                      DTYPES[x.dtype], rows, classes, x.stride(0), _at(labels), ignore_index or 0, int(ignore_index is not None),
+                      top_k, _at(stats), _at(entropy), _at(top_ix), _at(d_lp), _at(d_h), _at(d_top), dx.data_ptr())
         return dx, None, None, None, None
 
 
@@ -115,4 +124,6 @@ def label_log_probs(logits, labels=None, top_k=0, entropy=True, ignore_index=Non
             raise ValueError(f"labels must have the shape {tuple(logits.shape[:-1])}, got {tuple(labels.shape)}")
     if not logits.is_cuda:
         raise RuntimeError("logits must be a CUDA tensor (HIP device tensor on ROCm)")
-    return LabelLogProbs(*_LabelLogProbs.apply(logits, labels, top_k, bool(entropy), ignore_index))
+    if logits.requires_grad and torch.is_grad_enabled():
+        return LabelLogProbs(*_LabelLogProbs.apply(logits, labels, top_k, bool(entropy), ignore_index))
+    return LabelLogProbs(*_forward(logits, labels, top_k, bool(entropy), ignore_index, False)[:4])

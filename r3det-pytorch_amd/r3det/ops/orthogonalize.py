@@ -59,7 +59,7 @@ def _sizes(ts):
 
 
 def _workspace(count, rows, cols, device):
-    n = int(_C.lib().r3det_orthogonalize_workspace_bytes(count, rows, cols))
+    n = _C.lib().r3det_orthogonalize_workspace_bytes(count, rows, cols)
     return torch.empty(n, dtype=torch.uint8, device=device), n
 
 
@@ -83,10 +83,9 @@ def orthogonalize(tensors, steps=STEPS, coefficients=COEFFICIENTS, eps=1e-7):
     if live:
         src, dst = [p[0] for p in live], [p[1] for p in live]
         rows, cols = _sizes(src)
-        with torch.cuda.device(src[0].device):
-            ws, n = _workspace(len(src), rows, cols, src[0].device)
-            _C.check(_C.lib().r3det_orthogonalize(len(src), _pointers(src), _pointers(dst), DTYPES[src[0].dtype], rows, cols,
-                                                  steps, a, b, c, eps, _C.ptr(ws), n, _C.stream()), "r3det_orthogonalize")
+        ws, n = _workspace(len(src), rows, cols, src[0].device)
+        _C.run_on(src[0].device, "r3det_orthogonalize", _C.lib().r3det_orthogonalize, len(src), _pointers(src), _pointers(dst),
+                  DTYPES[src[0].dtype], rows, cols, steps, a, b, c, eps, ws.data_ptr(), n)
     return outs[0] if one else outs
 
 
@@ -153,10 +152,9 @@ def orthogonal_update_(params, grads, buffers, lr, momentum=0.95, nesterov=True,
     else:
         s = [float(scale)] * len(ps)
     rates = (ctypes.c_float * len(ps))(*[lr * v for v in s])
-    with torch.cuda.device(ps[0].device):
-        ws, n = _workspace(len(ps), rows, cols, ps[0].device)
-        _C.check(_C.lib().r3det_orthogonal_update(len(ps), _pointers(gs), _pointers(ps), _pointers(ms), DTYPES[ps[0].dtype],
-                                                  rows, cols, rates, 1.0 - lr * weight_decay, momentum, int(bool(nesterov)),
-                                                  steps, a, b, c, eps, _C.ptr(ws), n, _C.stream()), "r3det_orthogonal_update")
+    ws, n = _workspace(len(ps), rows, cols, ps[0].device)
+    _C.run_on(ps[0].device, "r3det_orthogonal_update", _C.lib().r3det_orthogonal_update, len(ps), _pointers(gs), _pointers(ps),
+              _pointers(ms), DTYPES[ps[0].dtype], rows, cols, rates, 1.0 - lr * weight_decay, momentum, int(bool(nesterov)), steps,
+              a, b, c, eps, ws.data_ptr(), n)
     for t in ps + ms:
         torch.autograd.graph.increment_version(t)
