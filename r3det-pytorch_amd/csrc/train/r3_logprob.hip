@@ -33,8 +33,9 @@ __device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
   return r;
 }
 
-// an order of the floats as unsigned numbers; no float is 0 (the key of "nothing"); -0 is +0
+// an order of the floats as unsigned numbers; no float is 0 (the key of "nothing"); -0 is +0; every NaN is above +inf
 __device__ __forceinline__ unsigned ord(float x) {
+  if (x != x) return 0xffffffffu;
   const unsigned b = __float_as_uint(x + 0.0f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
@@ -44,6 +45,10 @@ __device__ __forceinline__ float unord(unsigned u) {
 // greater = better: by value, then the lowest index
 __device__ __forceinline__ unsigned long long make_key(float x, unsigned index) {
   return ((unsigned long long)ord(x) << 32) | (unsigned)~index;
+}
+
+__device__ __forceinline__ unsigned long long offered(float x, unsigned index) {
+  return x == -__builtin_inff() ? 0ull : make_key(x, index);
 }
 
 struct Stat {  // of the values seen so far
@@ -253,8 +258,25 @@ __global__ __launch_bounds__(256) void logprob_small_backward_kernel(const T* __
 // The best keys a wavefront has seen, sorted, one a lane.
 struct Best {
   unsigned long long key = 0;
-  unsigned long long least = 0;  // the k-th best (uniform): what a key has to pass
+  unsigned long long bound = 0;  // what k keys are known to pass, the list's or not (uniform)
+  unsigned long long least = 0;  // what a key has to pass: the k-th best, or `bound`
   float floor = -__builtin_inff();  // its value
+  // The j-th greatest of the lanes' `high`, by its upper 16 bits (0: fewer have `any`).
+  static __device__ __forceinline__ unsigned of_lanes(bool any, float high, int j) {
+    const unsigned mine = any ? ord(high) >> 16 : 0u;
+    unsigned t = 0;
+#pragma unroll
+    for (int b = 15; b >= 0; --b) {
+      const unsigned more = t | 1u << b;
+      if (__popcll(__ballot(mine >= more)) >= j) t = more;
+    }
+    return t;
+  }
+  __device__ __forceinline__ void seed(unsigned t) {  // k elements are known to reach these upper 16 bits
+    bound = t ? ((unsigned long long)(t << 16) << 32) - 1 : 0ull;
+    least = bound;
+    floor = t ? unord(t << 16) : -__builtin_inff();
+  }
   __device__ __forceinline__ void insert(unsigned long long in, int k) {  // `in` uniform
     const unsigned lo = (unsigned)key, hi = (unsigned)(key >> 32);
     // lane i takes lane i - 1's (wave_shr:1); lane 0 keeps its own, which the comparison below sees as "not better"
@@ -267,8 +289,11 @@ struct Best {
   __device__ __forceinline__ void lo_hi(int k) {
     const unsigned lo = __builtin_amdgcn_readlane((unsigned)key, k - 1);
     const unsigned hi = __builtin_amdgcn_readlane((unsigned)(key >> 32), k - 1);
-    least = ((unsigned long long)hi << 32) | lo;
-    floor = hi ? unord(hi) : -__builtin_inff();
+    const unsigned long long kth = ((unsigned long long)hi << 32) | lo;
+    if (kth > bound) {
+      least = kth;
+      floor = unord(hi);
+    }
   }
   // every lane offers one key (0: none); all lanes of the wavefront call
   __device__ __forceinline__ void offer(unsigned long long in, int k) {
@@ -296,6 +321,21 @@ __device__ __forceinline__ void write_best(const unsigned long long* lists, int 
   }
 }
 
+// A masked class (-inf) is no key: a row with fewer than k others has its lowest masked classes behind them, which one
+// wavefront looks for from the row's beginning -- at most 2 k elements on.
+template <typename T, typename F>
+__device__ __forceinline__ void fill_masked(const T* x, int64_t classes, int have, int k, const F& write) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t b = 0; have < k && b < classes; b += 64) {
+    const bool in = b + lane < classes && (float)x[b + lane] == -__builtin_inff();
+    const unsigned long long who = __ballot(in);
+    const int rank = have + __popcll(who & ((1ull << lane) - 1));
+    if (in && rank < k) write(rank, make_key(-__builtin_inff(), (unsigned)(b + lane)));
+    have += __popcll(who);
+  }
+}
+
+constexpr int FEW = 1024;  // keys that are ranked as they are
 constexpr int UNROLL = 4;  // packs of a lane in flight
 
 // WAVES wavefronts walk [from, to) of a row together (WAVES = 1: four rows a workgroup, a wavefront each).
@@ -323,7 +363,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprob_row_ker
   const int first = WAVES == 1 ? 0 : wave * 64;
   Stat a;
   Best best;
-  for (int64_t c = first; c < packs; c += (int64_t)WAVES * 64 * UNROLL) {
+  __shared__ unsigned reached[64];
+  for (int64_t c0 = 0; c0 < packs; c0 += (int64_t)WAVES * 64 * UNROLL) {
+    const int64_t c = c0 + first;
     Pack<T, W> p[UNROLL];
     float top = a.m;
 #pragma unroll
@@ -339,7 +381,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprob_row_ker
     for (int u = 0; u < UNROLL; ++u) {
       high[u] = (float)p[u].v[0];
 #pragma unroll
-      for (int j = 1; j < W; ++j) high[u] = fmaxf(high[u], (float)p[u].v[j]);
+      for (int j = 1; j < W; ++j) high[u] = __builtin_elementwise_maximum(high[u], (float)p[u].v[j]);  // (NaN stays)
       top = fmaxf(top, high[u]);
     }
     a.raise(top);
@@ -348,13 +390,37 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprob_row_ker
 #pragma unroll
       for (int j = 0; j < W; ++j) a.add((float)p[u].v[j]);
     if constexpr (TOP) {
+      if (c0 == 0) {
+        // A bound from the first block, which k elements reach: the k-th greatest of every wavefront's greatest few lanes.
+        // Of a block of 16384 some 25 reach it then, where each wavefront alone would collect 98 of its 1024 for a list
+        // of 20, and each costs what reading 150 cost (one row of 50001, the best 20: 11.8 us, 18.2 us without; 67 rows
+        // of 131072: 16.3 + 4.1 us, 28 + 6 us without).
+        float most = high[0];
+#pragma unroll
+        for (int u = 1; u < UNROLL; ++u) most = __builtin_elementwise_maximum(most, high[u]);  // (packs that are not there are -inf)
+        if constexpr (WAVES == 1) {
+          best.seed(Best::of_lanes(most != -__builtin_inff(), most, o.k));
+        } else {
+          constexpr int EACH = 64 / WAVES;
+          const int whole = packs / 64 < WAVES ? (int)(packs / 64) : WAVES;  // wavefronts with a pack for every lane
+          if (whole * EACH >= o.k) {
+            const unsigned mine = most != -__builtin_inff() ? ord(most) >> 16 : 0u, t = Best::of_lanes(mine != 0, most, EACH);
+            const unsigned long long in = __ballot(mine >= t);
+            const int rank = __popcll(in & ((1ull << lane) - 1));
+            if (mine >= t && rank < EACH) reached[wave * EACH + rank] = mine;  // (t = 0: zeros among them)
+            __syncthreads();
+            const unsigned best_of = lane < whole * EACH ? reached[lane] : 0u;
+            best.seed(Best::of_lanes(best_of != 0, unord(best_of << 16 | 0xffffu), o.k));
+          }
+        }
+      }
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
         const int64_t i = c + (int64_t)u * WAVES * 64 + lane;
-        if (__ballot(i < packs && !(high[u] < best.floor))) {  // (equal: a lower place may still come in)
+        if (__ballot(i < packs && !(high[u] < best.floor) && high[u] != -__builtin_inff())) {  // (equal: a lower place may come in)
 #pragma unroll
           for (int j = 0; j < W; ++j)
-            best.offer(i < packs ? make_key((float)p[u].v[j], (unsigned)(from + i * W + j)) : 0ull, o.k);
+            best.offer(i < packs ? offered((float)p[u].v[j], (unsigned)(from + i * W + j)) : 0ull, o.k);
         }
       }
     }
@@ -368,7 +434,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprob_row_ker
         a.raise(fmaxf(a.m, v));
         a.add(v);
       }
-      if constexpr (TOP) best.offer(in ? make_key(v, (unsigned)i) : 0ull, o.k);
+      if constexpr (TOP) best.offer(in ? offered(v, (unsigned)i) : 0ull, o.k);
     }
   }
   join_lanes<64>(a);
@@ -378,19 +444,31 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprob_row_ker
     if constexpr (TOP) {
       m = __shfl(m, 0);
       ls = __shfl(ls, 0);
-      if (lane < o.k) {
-        o.top_lp[row * o.k + lane] = top_value(unord((unsigned)(best.key >> 32)), m, ls);
-        o.top_ix[row * o.k + lane] = (int64_t)(unsigned)~(unsigned)best.key;
-      }
+      const auto write = [&](int rank, unsigned long long mine) {
+        o.top_lp[row * o.k + rank] = top_value(unord((unsigned)(mine >> 32)), m, ls);
+        o.top_ix[row * o.k + rank] = (int64_t)(unsigned)~(unsigned)mine;
+      };
+      if (lane < o.k && best.key != 0) write(lane, best.key);
+      fill_masked(x, classes, __popcll(__ballot(lane < o.k && best.key != 0)), o.k, write);
     }
   } else {
     __shared__ float sh[WAVES][3];
     __shared__ float done[2];
     __shared__ unsigned long long keys[TOP ? WAVES * TOP_MAX : 1];
+    __shared__ int lists[WAVES];
     if (lane == 0) sh[wave][0] = a.m, sh[wave][1] = a.s, sh[wave][2] = a.t;
-    if constexpr (TOP)
-      if (lane < o.k) keys[wave * o.k + lane] = best.key;
+    const unsigned long long kept = TOP ? __ballot(lane < o.k && best.key != 0) : 0;  // (the first of the lanes)
+    if (TOP && lane == 0) lists[wave] = __popcll(kept);
     __syncthreads();
+    int many = 0;
+    if constexpr (TOP) {
+      int before = 0;
+      for (int w = 0; w < WAVES; ++w) {
+        before += w < wave ? lists[w] : 0;
+        many += lists[w];
+      }
+      if (kept >> lane & 1) keys[before + lane] = best.key;
+    }
     if (threadIdx.x == 0) {
       for (int w = 1; w < WAVES; ++w) a.join(sh[w][0], sh[w][1], sh[w][2]);
       if (split > 1) {
@@ -404,19 +482,24 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprob_row_ker
     }
     if constexpr (TOP) {
       __syncthreads();
-      write_best<WAVES * 64>(keys, WAVES * o.k, o.k, [&](int rank, unsigned long long mine) {
+      const auto write = [&](int rank, unsigned long long mine) {
         if (split > 1) part_keys[(row * split + s) * o.k + rank] = mine;
         else {
           o.top_lp[row * o.k + rank] = top_value(unord((unsigned)(mine >> 32)), done[0], done[1]);
           o.top_ix[row * o.k + rank] = (int64_t)(unsigned)~(unsigned)mine;
         }
-      });
+      };
+      write_best<WAVES * 64>(keys, many, o.k, write);
+      if (split > 1) {
+        if ((int)threadIdx.x < o.k && (int)threadIdx.x >= many) write(threadIdx.x, 0ull);
+      } else if (wave == 0) {
+        fill_masked(x, classes, many, o.k, write);
+      }
     }
   }
 }
 
-// The parts of one row a workgroup: the triples in a fixed order; the keys through four wavefronts' lists, then by rank.
-// (Every part has at least TOP_MAX elements, so all its k keys were written.)
+// The parts of one row a workgroup: the triples in a fixed order; the keys by rank.  A key of 0: none.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(256) void logprob_join_kernel(const T* __restrict__ logits, int64_t rows, int64_t classes,
                                                            int64_t stride, int split, const float* __restrict__ part,
@@ -437,17 +520,31 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(const T* __restrict__
     }
   }
   if constexpr (TOP) {
-    __shared__ unsigned long long lists[4 * TOP_MAX];
+    __shared__ unsigned long long lists[FEW];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = split * o.k;
     const unsigned long long* keys = part_keys + row * n;
-    Best best;
-    for (int q = wave * 64; q < n; q += 256) best.offer(q + lane < n ? keys[q + lane] : 0ull, o.k);
-    if (lane < o.k) lists[wave * o.k + lane] = best.key;
+    int many = n;
+    if (n <= FEW) {
+      for (int q = threadIdx.x; q < n; q += 256) lists[q] = keys[q];
+    } else {  // through four wavefronts' lists
+      Best best;
+      for (int q = wave * 64; q < n; q += 256) best.offer(q + lane < n ? keys[q + lane] : 0ull, o.k);
+      if (lane < o.k) lists[wave * o.k + lane] = best.key;
+      many = 4 * o.k;
+    }
     __syncthreads();
-    write_best<256>(lists, 4 * o.k, o.k, [&](int rank, unsigned long long mine) {
+    const auto write = [&](int rank, unsigned long long mine) {
       o.top_lp[row * o.k + rank] = top_value(unord((unsigned)(mine >> 32)), done[0], done[1]);
       o.top_ix[row * o.k + rank] = (int64_t)(unsigned)~(unsigned)mine;
-    });
+    };
+    write_best<256>(lists, many, o.k, write);
+    if (wave == 0) {  // (every list is sorted, its empty places behind)
+      int have = 0;
+      for (int q = lane; q < many; q += 64) have += lists[q] != 0;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) have += __shfl_xor(have, d);
+      fill_masked(logits + row * stride, classes, have, o.k, write);
+    }
   }
 }
 
@@ -510,12 +607,11 @@ __global__ __launch_bounds__(256) void logprob_row_backward_kernel(const T* __re
 // ---------------------------------------------------------------------------------------------- launches
 constexpr int SMALL_MAX = 128;     // classes whose row lanes hold in registers
 constexpr int WAVE_MAX = 4096;     // classes that one wavefront walks
-constexpr int64_t PART = 16384;    // classes a workgroup walks at least, where a row is split
+constexpr int64_t PART = 32768;    // classes a workgroup walks at least, where a row is split
 
 int row_split(int64_t rows, int64_t classes) {
   if (classes <= WAVE_MAX) return 1;
-  const int64_t want = 2ll * r3_cu_count();  // workgroups that fill the card
-  int64_t s = want / rows;
+  int64_t s = r3_cu_count() / rows;
   if (s > classes / PART) s = classes / PART;
   return s < 1 ? 1 : (s > 256 ? 256 : (int)s);
 }

@@ -101,7 +101,7 @@ def label_log_probs(logits, labels=None, top_k=0, entropy=True, ignore_index=Non
     label is outside [0, classes) -- nothing here reads labels on the host), ``entropy`` the row's -sum p log p, the top
     ones its ``top_k`` <= min(classes, 64) best classes in order, ties to the lowest index.  Logits of -inf are classes
     that are not offered: a row with none left has log probabilities of -inf, the entropy 0 and no gradient.  NaN or +inf
-    in a row makes its numbers NaN.  Differentiable (once) through all but ``top_index``; the logits must stay as they
+    in a row makes its numbers NaN; NaN is ranked first.  Differentiable (once) through all but ``top_index``; the logits must stay as they
     are until the backward pass.  Rows may be any distance apart; other strides are copied first.  Works on the current
     stream of the logits' device; nothing synchronises with the host."""
     if not isinstance(logits, torch.Tensor) or logits.dim() < 1:
@@ -113,8 +113,10 @@ def label_log_probs(logits, labels=None, top_k=0, entropy=True, ignore_index=Non
         raise ValueError(f"logits must have between 1 and 2^31 - 1 classes, got {classes}")
     if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= min(classes, TOP_MAX):
         raise ValueError(f"top_k must be an integer between 0 and min(classes, {TOP_MAX}), got {top_k!r} for {classes} classes")
-    if ignore_index is not None and not isinstance(ignore_index, int):
+    if ignore_index is not None and (isinstance(ignore_index, bool) or not isinstance(ignore_index, int)):
         raise TypeError("ignore_index must be an integer or None")
+    if ignore_index is not None and not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError("ignore_index must fit 64 bits")
     if labels is not None:
         if not isinstance(labels, torch.Tensor) or labels.dtype != torch.int64:
             raise RuntimeError("labels must be an int64 tensor")

@@ -195,6 +195,40 @@ def test_nan_and_inf_stay_in_their_rows(classes):
     assert torch.isfinite(dx[clean]).all()
 
 
+@pytest.mark.parametrize("rows,classes", [(5, 1000), (5, 70001), (300, 6000), (2, 300000)])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_few_classes_left_for_the_best_ones(rows, classes, dtype):
+    """The masked classes that fill up the list are the lowest; what is left lies in one lane's pack, or far apart."""
+    x = torch.full((rows, classes), -math.inf, dtype=TYPES[dtype], device=DEV)
+    x[0, classes - 3:] = torch.tensor([1.0, 3.0, 1.0], device=DEV).to(x.dtype)
+    x[1, :3] = 2.0
+    x[1, classes // 2] = 4.0
+    if rows > 2:
+        x[2, ::classes // 40] = 0.5
+        x[3, 40:140] = torch.finfo(x.dtype).min
+        x[4, 1::2] = -1.0
+    for k in (1, 8, 64):
+        check(x, k=k, grads=False)
+
+
+@pytest.mark.parametrize("classes", [16, 100, 1000, 5000, 70001])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_nan_is_ranked_first_whatever_its_sign(classes, dtype):
+    x, _ = logits(5, classes, dtype)
+    x[0] = -torch.tensor(math.nan, dtype=x.dtype, device=DEV)
+    x[1] = torch.tensor(math.nan, dtype=x.dtype, device=DEV)
+    x[2, classes // 2] = -math.nan
+    x[2, classes - 1] = math.inf
+    x[3] = -math.inf
+    x[3, 1::3] = math.nan
+    x[4, classes - 2:] = -math.nan
+    k = min(classes, 20)
+    got = label_log_probs(x, top_k=k)
+    want = x.cpu().float().sort(dim=-1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(got.top_index.cpu(), want)
+    assert torch.isnan(got.top_log_prob).all()
+
+
 def test_labels_ignored_and_out_of_range():
     for classes in (16, 300, 6000):
         x, y = logits(9, classes, "fp32")

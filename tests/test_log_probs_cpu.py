@@ -32,6 +32,10 @@ def test_refusals_of_the_python_entry():
         label_log_probs(x, y[:2])
     with pytest.raises(TypeError, match="ignore_index"):
         label_log_probs(x, y, ignore_index=1.0)
+    with pytest.raises(TypeError, match="ignore_index"):
+        label_log_probs(x, y, ignore_index=True)
+    with pytest.raises(ValueError, match="64 bits"):
+        label_log_probs(x, y, ignore_index=2 ** 63)
 
 
 def test_refusals_of_the_c_entries():
