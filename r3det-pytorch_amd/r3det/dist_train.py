@@ -14,6 +14,7 @@ import torch.distributed as dist
 from torch.nn.parallel import DistributedDataParallel
 
 from .models.detectors import parse_losses
+from .ops.orthogonalize import COEFFICIENTS, DTYPES, STEPS, orthogonal_update_
 
 # xGMI is point to point (7 links x ~153 GB/s per GPU): a ring all-reduce is bound per link, and the
 # 168 MB of fp32 gradients of R3Det-R50 go out in few, large buckets -- 4 x ~48 MB instead of torch's
@@ -46,8 +47,109 @@ def train_step(model, optimizer, img, gt_bboxes, gt_labels, img_metas=None):
     return loss.detach(), log_vars
 
 
-def build_optimizer(model, lr=0.0025, momentum=0.9, weight_decay=0.0001):
+class Muon(torch.optim.Optimizer):
+    """Orthogonalised momentum for weights of two and more dimensions (ops/orthogonalize.py: all of a group's weights in
+    one chain of launches), SGD with momentum for the groups with ``orthogonal=False`` (biases, norms).
+
+        orthogonal:  M = momentum M + G;  U = G + momentum M (nesterov) or M
+                     W = (1 - lr weight_decay) W - lr s orthogonalize(U)     (s: ``scale``)
+        otherwise:   M = momentum M + G + weight_decay W;  U = G + weight_decay W + momentum M (nesterov) or M
+                     W = W - lr U
+
+    The momentum is fp32 whatever the weights' type and is laid out as its weight is.  The same gradients give the same
+    bits, so replicas that exchange gradients stay equal.  ``lr`` and the others are read from the group at every step
+    (schedulers work; a captured step keeps them).  Device tensors only."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, orthogonal=True, scale='rms',
+                 steps=STEPS, coefficients=COEFFICIENTS, eps=1e-7):
+        if not (lr >= 0 and momentum >= 0 and weight_decay >= 0):
+            raise ValueError('lr, momentum and weight_decay must not be negative')
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
+                                      orthogonal=orthogonal, scale=scale, steps=steps, coefficients=tuple(coefficients),
+                                      eps=eps))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        group = self.param_groups[-1]
+        for p in group['params']:
+            if p.dtype not in DTYPES or (group['orthogonal'] and p.dim() < 2):
+                self.param_groups.pop()
+                raise ValueError('Muon: weights are fp32, fp16 or bf16, and of two and more dimensions in an orthogonal '
+                                 'group; put the others into a group with orthogonal=False')
+
+    def _momentum(self, p):
+        state = self.state[p]
+        m = state.get('momentum_buffer')
+        if m is None:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError('Muon: take one step before the capture (a replay would begin without momentum again)')
+            m = torch.zeros_like(p, dtype=torch.float32)
+        elif m.stride() != p.stride() or m.device != p.device:  # (the weight was laid out anew, or the state loaded)
+            m = torch.empty_like(p, dtype=torch.float32).copy_(m)
+        state['momentum_buffer'] = m
+        return m
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for g in self.param_groups:
+            alike = {}  # (one call takes weights of one type on one device)
+            for p in g['params']:
+                if p.grad is not None:
+                    if p.grad.is_sparse:
+                        raise RuntimeError('Muon: sparse gradients are not taken')
+                    alike.setdefault((p.device, p.dtype), []).append(p)
+            for ps in alike.values():
+                grads, buffers = [p.grad for p in ps], [self._momentum(p) for p in ps]
+                if g['orthogonal']:
+                    orthogonal_update_(ps, grads, buffers, g['lr'], g['momentum'], g['nesterov'], g['weight_decay'], g['steps'],
+                                       g['coefficients'], g['eps'], g['scale'])
+                else:
+                    self._sgd(ps, grads, buffers, g)
+        return loss
+
+    @staticmethod
+    def _sgd(ps, grads, buffers, g):
+        wide = [p.float() for p in ps]  # (16-bit weights: every step rounds once; fp32 ones are themselves)
+        grads = [d.float() for d in grads]
+        if g['weight_decay']:
+            grads = torch._foreach_add(grads, wide, alpha=g['weight_decay'])
+        torch._foreach_mul_(buffers, g['momentum'])
+        torch._foreach_add_(buffers, grads)
+        update = torch._foreach_add(grads, buffers, alpha=g['momentum']) if g['nesterov'] else buffers
+        torch._foreach_add_(wide, update, alpha=-g['lr'])
+        if wide[0] is not ps[0]:
+            torch._foreach_copy_(ps, wide)
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # (the base class casts the state to the weights' type: the momentum stays 32 bits wide)
+        saved = [i for group in state_dict['param_groups'] for i in group['params']]
+        for i, p in zip(saved, (p for group in self.param_groups for p in group['params'])):
+            m = state_dict['state'].get(i, {}).get('momentum_buffer')
+            if m is not None:
+                self.state[p]['momentum_buffer'] = torch.empty_like(p, dtype=torch.float32).copy_(m)
+
+
+MUON_NUMBERS = {'lr', 'momentum', 'nesterov', 'weight_decay', 'scale', 'steps', 'coefficients', 'eps'}
+
+
+def build_optimizer(model, lr=0.0025, momentum=0.9, weight_decay=0.0001, type='SGD', **matrices):
     """configs/_base_/schedules/schedule_1x.py: SGD(lr=0.0025, momentum=0.9, weight_decay=0.0001)
-    over the trainable parameters (grad clipping max_norm=35 is applied by the caller if wanted)."""
-    return torch.optim.SGD([p for p in model.parameters() if p.requires_grad], lr=lr, momentum=momentum,
-                           weight_decay=weight_decay)
+    over the trainable parameters (grad clipping max_norm=35 is applied by the caller if wanted).
+    ``type='Muon'``: the weights of two and more dimensions take orthogonalised updates with ``matrices`` (``lr``,
+    ``momentum``, ``scale``, ... of ``Muon``, spelt ``matrix_lr`` and so on; its defaults and the same weight decay
+    otherwise), the rest the numbers above."""
+    params = [p for p in model.parameters() if p.requires_grad]
+    if type == 'SGD' and not matrices:
+        return torch.optim.SGD(params, lr=lr, momentum=momentum, weight_decay=weight_decay)
+    own = {k[len('matrix_'):]: v for k, v in matrices.items() if k.startswith('matrix_')}
+    if type != 'Muon' or len(own) != len(matrices) or not set(own) <= MUON_NUMBERS:
+        raise ValueError(f"type must be 'SGD', or 'Muon' with matrix_ numbers of it, got {type!r} with {sorted(matrices)}")
+    groups = [dict(dict(weight_decay=weight_decay), params=[p for p in params if p.dim() >= 2], **own),
+              dict(params=[p for p in params if p.dim() < 2], orthogonal=False, lr=lr, momentum=momentum, nesterov=False,
+                   weight_decay=weight_decay)]
+    return Muon([g for g in groups if g['params']])

@@ -381,6 +381,8 @@ def calibrate_score_bias(model, img, frac=0.01, per_class=False):
     DOTA-shaped pool; configs/r3det/r3det_r50_fpn_1x_dota_v1.py:99-104).  One common shift leaves ~90 % of a
     random-weight model's candidates in a single class -- an artefact of the random head, not of the dataset."""
     head = model.refine_head[-1] if isinstance(model, R3Det) else model.bbox_head
+    if not head.use_sigmoid_cls:
+        raise NotImplementedError('calibrate_score_bias: a shift of every class changes no softmax score')
     x = model.extract_feat(img)
     if isinstance(model, R3Det):
         cls, reg = model.bbox_head(x)

@@ -19,6 +19,7 @@ from ..core.bbox.coder import DeltaXYWHAOBBoxCoder
 from ..core.bbox.rtransforms import obb2hbb
 from ..core.post_processing import CapacityHint, multiclass_nms_rotated_batch
 from ..ops import fr_boxes
+from ..ops.log_probs import label_log_probs
 from .backbone import ConvModule
 from .coder import delta2bbox_v1
 from .losses import build_loss
@@ -93,14 +94,16 @@ class RRetinaHead(nn.Module):
         self.stacked_convs = stacked_convs
         loss_cls = _cfg_dict(loss_cls or dict(type='FocalLoss', use_sigmoid=True, gamma=2.0, alpha=0.25,
                                               loss_weight=1.0))
-        if not loss_cls.get('use_sigmoid', False):
-            raise NotImplementedError('softmax classification heads are not used by the rotated configs')
-        self.use_sigmoid_cls = True
-        self.cls_out_channels = num_classes  # use_sigmoid_cls
+        # (rotate_anchor_head.py:33-98) sigmoid: a score per class; softmax: the background's is the last channel, and the
+        # loss is averaged over all samples, not over the positives
+        self.use_sigmoid_cls = bool(loss_cls.get('use_sigmoid', False))
+        self.cls_out_channels = num_classes if self.use_sigmoid_cls else num_classes + 1
         self.test_cfg = _cfg_dict(test_cfg) if test_cfg is not None else dict(
             nms_pre=2000, min_bbox_size=0, score_thr=0.05, nms=dict(iou_thr=0.1), max_per_img=2000)
         # training side (rotate_anchor_head.py:33-98); defaults = configs/r3det/r3det_r50_fpn_1x_dota_v1.py
         self.train_cfg = _cfg_dict(train_cfg) if train_cfg is not None else dict(self._default_train_cfg())
+        if not self.use_sigmoid_cls and 'sampler' in self.train_cfg:
+            raise NotImplementedError('RRetinaHead: every assigned anchor is a sample; train_cfg.sampler is not restated')
         self.assign_by_circumhbbox = assign_by_circumhbbox
         self.assigner = build_assigner(self.train_cfg['assigner'])
         self.bbox_coder = build_from(BBOX_CODERS, _cfg_dict(bbox_coder or dict(type='DeltaXYWHAOBBoxCoder')))
@@ -113,7 +116,7 @@ class RRetinaHead(nn.Module):
             c = in_channels if i == 0 else feat_channels
             self.cls_convs.append(ConvModule(c, feat_channels, 3, padding=1, act=True))
             self.reg_convs.append(ConvModule(c, feat_channels, 3, padding=1, act=True))
-        self.retina_cls = nn.Conv2d(feat_channels, num_anchors * num_classes, 3, padding=1)
+        self.retina_cls = nn.Conv2d(feat_channels, num_anchors * self.cls_out_channels, 3, padding=1)
         self.retina_reg = nn.Conv2d(feat_channels, num_anchors * 5, 3, padding=1)
         self._anchor_cache = {}
         self.nms_hint = CapacityHint()  # this head's own workspace-size memory for the batched NMS
@@ -263,9 +266,25 @@ class RRetinaHead(nn.Module):
             return None  # rotate_anchor_head.py:469-470
         labels, label_w, bbox_t, bbox_w, num_total_pos = targets
         avg = num_total_pos.to(torch.float32)
+        if not self.use_sigmoid_cls:  # (:470-471) the negatives are counted too, at least one an image
+            neg = sum(((w > 0) & (la == self.num_classes)).sum(1) for la, w in zip(labels, label_w))
+            avg = avg + neg.clamp(min=1).sum()
         out = [self.loss_single(c.float(), r.float(), la, lw, bt, bw, avg)
                for c, r, la, lw, bt, bw in zip(cls_scores, bbox_preds, labels, label_w, bbox_t, bbox_w)]
         return dict(loss_cls=[o[0] for o in out], loss_bbox=[o[1] for o in out])
+
+    def _rows(self, cls):
+        """(N, A * C, H, W) class channels -> (N, H * W * A, C), a row per anchor."""
+        return cls.permute(0, 2, 3, 1).reshape(cls.size(0), -1, self.cls_out_channels)
+
+    def _foreground(self, rows):
+        """Softmax heads: the log probability of every row's best class that is not the background (the last).  It is
+        among the row's best two, so no distribution is written out (ops/log_probs.py)."""
+        if not rows.is_cuda:
+            return torch.log_softmax(rows.float(), -1)[..., :-1].max(-1)[0]
+        got = label_log_probs(rows, top_k=2, entropy=False)
+        first, second = got.top_log_prob.unbind(-1)
+        return torch.where(got.top_index[..., 0] < self.num_classes, first, second)
 
     @torch.no_grad()
     def filter_bboxes(self, cls_scores, bbox_preds):
@@ -278,7 +297,11 @@ class RRetinaHead(nn.Module):
         anchors = self.anchors([c.shape[-2:] for c in cls_scores], cls_scores[0].device)
         out = [[] for _ in range(N)]
         for cls, reg, anc in zip(cls_scores, bbox_preds, anchors):
-            boxes = fr_boxes.filter_bboxes(cls, reg, anc, self.num_anchors, self.cls_out_channels)
+            if self.use_sigmoid_cls:
+                boxes = fr_boxes.filter_bboxes(cls, reg, anc, self.num_anchors, self.cls_out_channels)
+            else:  # the anchor whose best class is most probable
+                best = self._foreground(self._rows(cls)).view(N, *cls.shape[-2:], self.num_anchors).permute(0, 3, 1, 2)
+                boxes = fr_boxes.filter_bboxes(best, reg, anc, self.num_anchors, 1)
             for i in range(N):
                 out[i].append(boxes[i])
         return out
@@ -290,8 +313,10 @@ class RRetinaHead(nn.Module):
         out = [[] for _ in range(N)]
         for cls, reg, anc in zip(cls_scores, bbox_preds, anchors):
             A, C = self.num_anchors, self.cls_out_channels
-            cls = cls.permute(0, 2, 3, 1).reshape(N, -1, A, C)
-            best = cls.max(dim=-1)[0].argmax(dim=-1)                            # (N, HW)
+            if self.use_sigmoid_cls:
+                best = cls.permute(0, 2, 3, 1).reshape(N, -1, A, C).max(dim=-1)[0].argmax(dim=-1)   # (N, HW)
+            else:
+                best = self._foreground(self._rows(cls)).view(N, -1, A).argmax(dim=-1)
             reg = reg.permute(0, 2, 3, 1).reshape(N, -1, A, 5)
             idx = best[..., None, None].expand(-1, -1, 1, 5)
             best_pred = reg.gather(2, idx).squeeze(2)                           # (N, HW, 5)
@@ -316,11 +341,11 @@ class RRetinaHead(nn.Module):
         HIP graph together with the network.  On the device one library call for all levels (r3det_levels_pool:
         sigmoid, per-image top-nms_pre in score order, decoding, straight into the pool arrays; level by level
         through r3det_level_pool / torch when a level is beyond the library's top-k); the op-by-op torch form is
-        ``decode_bboxes_torch``."""
+        ``decode_bboxes_torch``.  A softmax head's levels go one by one: its probabilities, the background's the last."""
         cfg = cfg or self.test_cfg
         nms_pre = cfg.get('nms_pre', -1)
         nms_pre = -1 if nms_pre is None else int(nms_pre)
-        if not cls_scores[0].is_cuda or cls_scores[0].dtype != torch.float32:
+        if not cls_scores[0].is_cuda or cls_scores[0].dtype != torch.float32 or not self.use_sigmoid_cls:
             return self.decode_bboxes_torch(cls_scores, bbox_preds, img_shape, cfg, rois)
         N = cls_scores[0].size(0)
         A, C = self.num_anchors, self.cls_out_channels
@@ -359,15 +384,20 @@ class RRetinaHead(nn.Module):
         return boxes, scores
 
     def _level_torch(self, cls, reg, anc, nms_pre, img_shape):
-        """One level of rotate_anchor_head.py:626-660 for the whole batch, op by op: (N, r, 5), (N, r, C)."""
+        """One level of rotate_anchor_head.py:626-660 for the whole batch, op by op: (N, r, 5), (N, r, C).  Softmax heads
+        rank their rows without writing the distributions out, which only the kept rows need."""
         N, C = cls.size(0), self.cls_out_channels
-        scores = cls.permute(0, 2, 3, 1).reshape(N, -1, C).sigmoid()
+        rows = self._rows(cls)
+        scores = rows.sigmoid() if self.use_sigmoid_cls else rows
         reg = reg.permute(0, 2, 3, 1).reshape(N, -1, 5)
         if 0 < nms_pre < scores.shape[1]:
-            top = scores.max(dim=2)[0].topk(nms_pre, dim=1)[1]             # (N, nms_pre)
+            rank = scores.max(dim=2)[0] if self.use_sigmoid_cls else self._foreground(rows)
+            top = rank.topk(nms_pre, dim=1)[1]                             # (N, nms_pre)
             anc = anc.gather(1, top[..., None].expand(-1, -1, 5))
             reg = reg.gather(1, top[..., None].expand(-1, -1, 5))
             scores = scores.gather(1, top[..., None].expand(-1, -1, C))
+        if not self.use_sigmoid_cls:
+            scores = scores.float().softmax(-1)
         return delta2bbox_v1(anc, reg, max_shape=img_shape), scores
 
     def decode_bboxes_torch(self, cls_scores, bbox_preds, img_shape, cfg=None, rois=None):
@@ -384,7 +414,8 @@ class RRetinaHead(nn.Module):
                for cls, reg, anc in zip(cls_scores, bbox_preds, lvl_anchors)]
         boxes = torch.cat([p[0] for p in per], 1)
         scores = torch.cat([p[1] for p in per], 1)
-        scores = torch.cat([scores, scores.new_zeros(N, scores.shape[1], 1)], 2)  # dummy background
+        if self.use_sigmoid_cls:
+            scores = torch.cat([scores, scores.new_zeros(N, scores.shape[1], 1)], 2)  # dummy background
         return boxes, scores
 
 

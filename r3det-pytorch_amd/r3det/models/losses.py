@@ -1,7 +1,8 @@
 """The two losses the r3det configs select (configs/r3det/r3det_r50_fpn_1x_dota_v1.py:37-43,62-68):
-``FocalLoss(use_sigmoid=True, gamma=2.0, alpha=0.25)`` and ``SmoothL1Loss(beta=0.11)``.
+``FocalLoss(use_sigmoid=True, gamma=2.0, alpha=0.25)`` and ``SmoothL1Loss(beta=0.11)``; beside them ``L1Loss`` and, for
+heads with a softmax over the classes and the background, ``CrossEntropyLoss(use_sigmoid=False)``.
 
-Both classes are mmdet 2.19's (third-party, not under the reference tree); their rules are restated:
+The classes are mmdet 2.19's (third-party, not under the reference tree); their rules are restated:
 elementwise loss, times the per-sample weight, reduced as ``sum / avg_factor`` when ``avg_factor`` is
 given with ``reduction='mean'`` (mmdet ``weight_reduce_loss``), times ``loss_weight``.  ``avg_factor``
 may be a tensor (the positive count stays on the device: no host synchronisation in the step).
@@ -9,6 +10,8 @@ may be a tensor (the positive count stays on the device: no host synchronisation
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from ..ops.log_probs import label_log_probs
 
 
 def weight_reduce_loss(loss, weight=None, reduction='mean', avg_factor=None):
@@ -36,6 +39,46 @@ def sigmoid_focal_loss(pred, target, weight=None, gamma=2.0, alpha=0.25, reducti
     if weight is not None and weight.shape != loss.shape:
         weight = weight.view(-1, 1) if weight.size(0) == loss.size(0) else weight.view(loss.size(0), -1)
     return weight_reduce_loss(loss, weight, reduction, avg_factor)
+
+
+def cross_entropy(pred, target, weight=None, class_weight=None, ignore_index=-100, reduction='mean', avg_factor=None):
+    """pred (n, C) logits, target (n,) class index.  Per sample ``-class_weight[target] log softmax(pred)[target]``, 0
+    where the target is ``ignore_index``.  On the device one pass over the logits and one in the backward pass
+    (ops/log_probs.py; a target that is no class makes its loss NaN there); op by op on the host."""
+    if pred.dim() != 2:
+        raise ValueError(f'pred must be (n, C), got {tuple(pred.shape)}')
+    if class_weight is not None and class_weight.numel() != pred.size(1):
+        raise ValueError(f'class_weight has {class_weight.numel()} entries for {pred.size(1)} classes')
+    if pred.is_cuda:
+        loss = -label_log_probs(pred, target, entropy=False, ignore_index=ignore_index).log_prob
+    else:
+        loss = F.cross_entropy(pred if pred.dtype == torch.float64 else pred.float(), target, reduction='none',
+                               ignore_index=ignore_index)
+    if class_weight is not None:
+        # (an ignored target's loss is 0 whatever it is multiplied with, that of one that is no class NaN)
+        loss = loss * class_weight[target.clamp(0, pred.size(1) - 1)]
+    return weight_reduce_loss(loss, weight, reduction, avg_factor)
+
+
+class CrossEntropyLoss(nn.Module):
+    """mmdet CrossEntropyLoss, its softmax form (``use_sigmoid=False, use_mask=False``).  A head with this loss has one
+    class channel more, the background's, at the end."""
+
+    def __init__(self, use_sigmoid=False, use_mask=False, reduction='mean', class_weight=None, ignore_index=None,
+                 loss_weight=1.0):
+        super().__init__()
+        if use_sigmoid or use_mask:
+            raise NotImplementedError('CrossEntropyLoss: only the softmax form (use_sigmoid=False, use_mask=False)')
+        self.use_sigmoid = False
+        self.reduction, self.loss_weight = reduction, loss_weight
+        self.ignore_index = -100 if ignore_index is None else ignore_index
+        if class_weight is not None:  # (moves with the module: no copy from the host in the step)
+            class_weight = torch.tensor([float(w) for w in class_weight])
+        self.register_buffer('class_weight', class_weight, persistent=False)
+
+    def forward(self, pred, target, weight=None, avg_factor=None, reduction_override=None):
+        return self.loss_weight * cross_entropy(pred, target, weight, self.class_weight, self.ignore_index,
+                                                reduction_override or self.reduction, avg_factor)
 
 
 class FocalLoss(nn.Module):
@@ -84,7 +127,7 @@ class L1Loss(nn.Module):
 
 from ..registry import LOSSES, build_from  # noqa: E402
 
-for _c in (FocalLoss, SmoothL1Loss, L1Loss):
+for _c in (FocalLoss, CrossEntropyLoss, SmoothL1Loss, L1Loss):
     if _c.__name__ not in LOSSES:
         LOSSES.register_module(module=_c)
 

@@ -4,6 +4,7 @@ r3det_orthogonal_update), for a ragged list of matrices in one chain of launches
 Not one of the reference's extension ops: it serves the training step's optimiser (``dist_train.Muon``).  A weight of more
 than two dimensions is the matrix of its first dimension against all others, as for a convolution's (out, in * kh * kw).
 """
+import bisect
 import ctypes
 import math
 
@@ -103,6 +104,21 @@ def _dense(t):
     return t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last)
 
 
+def _apart(params, buffers, grads):
+    """All matrices are updated at once: none may share memory with another, nor with a gradient."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in params + buffers]
+    spans.sort()
+    starts = [s[0] for s in spans]
+    shared = any(a[1] > b for a, b in zip(spans, starts[1:]))
+    for g in () if shared else grads:
+        at = g.data_ptr()
+        i = bisect.bisect_right(starts, at)
+        if (i and spans[i - 1][1] > at) or (i < len(starts) and starts[i] < at + g.numel() * g.element_size()):
+            shared = True
+    if shared:
+        raise ValueError("the same weight or buffer comes twice, or shares memory with another one or with a gradient")
+
+
 @torch.no_grad()
 def orthogonal_update_(params, grads, buffers, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=STEPS,
                        coefficients=COEFFICIENTS, eps=1e-7, scale="rms"):
@@ -114,7 +130,7 @@ def orthogonal_update_(params, grads, buffers, lr, momentum=0.95, nesterov=True,
     with ``s = 0.2 sqrt(max(rows, cols))`` for ``scale="rms"`` (the update's entries are then of about the size of an adaptive
     optimiser's) or ``sqrt(max(1, rows / cols))`` for ``"spectral"``, or a number.  ``params`` and ``grads`` fp32, fp16 or bf16,
     all alike; ``buffers`` fp32.  A weight must be contiguous or channels_last, its momentum laid out alike; a gradient
-    laid out otherwise is copied.  The same weight may not come twice.  ``lr`` and the other numbers are read when the
+    laid out otherwise is copied.  No weight or buffer may share memory with another or with a gradient.  ``lr`` and the other numbers are read when the
     call is made (a captured graph keeps them)."""
     params, grads, buffers = list(params), list(grads), list(buffers)
     if not len(params) == len(grads) == len(buffers):
@@ -135,15 +151,13 @@ def orthogonal_update_(params, grads, buffers, lr, momentum=0.95, nesterov=True,
             raise RuntimeError(f"buffers must be fp32, got {m.dtype}")
         if not _dense(p) or (_layout(m) != _layout(p) and p.numel()):
             raise RuntimeError("params must be contiguous or channels_last, and their buffers laid out alike")
-    if len({p.data_ptr() for p in params if p.numel()}) != sum(p.numel() > 0 for p in params) or \
-            len({m.data_ptr() for m in buffers if m.numel()}) != sum(m.numel() > 0 for m in buffers):
-        raise ValueError("the same weight or buffer comes twice")
+    live = [(p, g, m, _layout(g) == _layout(p)) for p, g, m in zip(params, grads, buffers) if p.numel()]
+    ps, ms = [t[0] for t in live], [t[2] for t in live]
+    _apart(ps, ms, [g for _, g, _, alike in live if alike])
     _same(params, "params")
-    live = [(p, g, m) for p, g, m in zip(params, grads, buffers) if p.numel()]
     if not live:
         return
-    ps, ms = [t[0] for t in live], [t[2] for t in live]
-    gs = [g if _layout(g) == _layout(p) else torch.empty_like(p).copy_(g) for p, g, _ in live]
+    gs = [g if alike else torch.empty_like(p).copy_(g) for p, g, _, alike in live]
     rows, cols = _sizes(ps)
     if scale == "rms":
         s = [0.2 * math.sqrt(max(r, k)) for r, k in zip(rows, cols)]

@@ -58,6 +58,22 @@ def test_refusals_of_the_update():
     orthogonal_update_([], [], [], lr=0.1)
 
 
+def test_weights_that_share_memory_are_refused():
+    big = torch.zeros(10, 6)
+    with pytest.raises(ValueError, match="shares memory"):
+        orthogonal_update_([big[:4], big[3:7]], [W, W], [W.clone(), W.clone()], lr=0.1)
+    with pytest.raises(ValueError, match="shares memory"):
+        orthogonal_update_([big[:4]], [W], [big[2:6]], lr=0.1)
+    with pytest.raises(ValueError, match="shares memory"):
+        orthogonal_update_([big[4:8]], [big[1:5]], [W.clone()], lr=0.1)
+    with pytest.raises(ValueError, match="shares memory"):
+        orthogonal_update_([big[4:8]], [big[6:10]], [W.clone()], lr=0.1)
+    for args in (([big[:4], big[4:8]], [W, W], [W.clone(), W.clone()]),   # neighbours, one gradient for two: nothing refused
+                 ([big[4:8]], [big[:4]], [W.clone()])):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            orthogonal_update_(*args, lr=0.1)
+
+
 def test_refusals_of_the_c_entries():
     L = _C.lib()
     ints = lambda *v: (ctypes.c_int * len(v))(*v)  # noqa: E731
