@@ -135,6 +135,17 @@ __device__ __forceinline__ void triangle(Tile& w, unsigned tile, unsigned wide) 
   while (tile >= wide - i) tile -= wide - i, ++i;  // (row i has wide - i tiles)
   w.i = i, w.j = i + tile;
 }
+// Workgroups go to the eight XCDs in turn, and each has an L2 of its own.  The u-th of n pieces of work is taken by that
+// workgroup which makes CHUNK neighbours share one: the tiles of a matrix read the same rows.
+constexpr unsigned XCDS = 8, CHUNK = 16;
+__device__ __forceinline__ unsigned entry(unsigned u, unsigned n) {
+  const unsigned first = u / (XCDS * CHUNK) * (XCDS * CHUNK), v = u - first;
+  const unsigned here = n - first < XCDS * CHUNK ? n - first : XCDS * CHUNK;  // (fewer at the end: as even as possible)
+  const unsigned q = here / XCDS, longer = here % XCDS * (q + 1);
+  const unsigned x = v < longer ? v / (q + 1) : here % XCDS + (v - longer) / q;
+  const unsigned c = v < longer ? v % (q + 1) : (v - longer) % q;
+  return first + c * XCDS + x;
+}
 // the table's and the lists' entries of `b`'s matrices
 __global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
   const unsigned g = blockIdx.x * blockDim.x + threadIdx.x, stride = gridDim.x * blockDim.x;
@@ -147,16 +158,17 @@ __global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
   for (unsigned e = b.m[0].gram0 + g; e < b.end.gram0; e += stride) {
     const unsigned k = find(b, &Mat::gram0, e), local = e - b.m[k].gram0;
     Tile w = begin(k);
-    triangle(w, local / w.splits, w.np / l.gram_ts);
-    w.split = local % w.splits;
-    w.part = b.m[k].part0 + (size_t)local * l.gram_ts * l.gram_ts;
-    l.gram[e] = w;
+    const unsigned high = w.np / l.gram_ts, tiles = high * (high + 1) / 2, tile = local % tiles;
+    triangle(w, tile, high);
+    w.split = local / tiles;
+    w.part = b.m[k].part0 + ((size_t)tile * w.splits + w.split) * (l.gram_ts * l.gram_ts);
+    l.gram[entry(e, l.n_gram)] = w;
   }
   for (unsigned e = b.m[0].tri0 + g; e < b.end.tri0; e += stride) {
     const unsigned k = find(b, &Mat::tri0, e);
     Tile w = begin(k);
     triangle(w, e - b.m[k].tri0, w.np / l.tri_ts);
-    l.tri[e] = w;
+    l.tri[entry(e, l.n_tri)] = w;
   }
   for (unsigned e = b.m[0].rect0 + g; e < b.end.rect0; e += stride) {
     const unsigned k = find(b, &Mat::rect0, e), local = e - b.m[k].rect0;
@@ -935,7 +947,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
     gram128 += (uint64_t)w.tri(128) * ((w.mp + 255) / 256);
   }
   l.gram_ts = gram128 >= WANT / 2 ? 128 : 64;
-  l.tri_ts = tri128 >= WANT / 2 ? 128 : 64;
+  l.tri_ts = tri128 >= WANT ? 128 : 64;
   l.rect_ts = rect128 >= WANT / 2 ? 128 : 64;
   // X X^t: the longest parts of the sum that still fill the card.  A part is a workgroup's time, so the parts of a ragged
   // list are of like length, and a short list of wide matrices is spread.
