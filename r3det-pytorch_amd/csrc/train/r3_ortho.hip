@@ -38,6 +38,7 @@
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr int NORM_CHUNK = 8192; // elements a workgroup of the norm's pass takes
@@ -68,8 +69,9 @@ struct Dim {  // padded with zeros, which stay zeros
   }
   __host__ __device__ size_t x() const { return (size_t)np * mp; }
   __host__ __device__ size_t a() const { return (size_t)np * np; }
-  // per matrix: X, X^t twice (one read and one written in a pass), SQ n x n arrays, each hi then lo; SQ diagonals in fp32
-  __host__ __device__ size_t halves() const { return 2 * (3 * x() + SQ * a() + (size_t)SQ * np); }
+  // per matrix: X twice (one read and one written in a pass), or X and X^t twice; SQ n x n arrays, each hi then lo; SQ
+  // diagonals in fp32
+  __host__ __device__ size_t halves(int rect_ts) const { return 2 * ((rect_ts == 64 ? 3 : 2) * x() + SQ * a() + (size_t)SQ * np); }
   __host__ __device__ unsigned tri(int ts) const { return (unsigned)(np / ts) * (np / ts + 1) / 2; }
   __host__ __device__ unsigned rect(int ts) const { return (unsigned)(np / ts) * (mp / ts); }
   __host__ __device__ unsigned norms() const { return (unsigned)(((size_t)n * m + NORM_CHUNK - 1) / NORM_CHUNK); }
@@ -82,15 +84,18 @@ struct Tile {  // one workgroup's work, with all that it needs of its matrix to 
   unsigned mat;
 };
 struct Area {  // where a matrix's arrays are
-  _Float16 *x, *xt, *sq;  // xt: two, sq: SQ
+  _Float16 *x, *next, *sq;  // X (or X^t) that a pass reads, and writes; sq: SQ
+  _Float16 *xt, *next_t;
   float* diag;
-  size_t na, nx;  // one of sq's, one of xt's (hi and lo)
-  __device__ Area(_Float16* base, const Tile& t) {
-    na = 2 * (size_t)t.np * t.np, nx = 2 * (size_t)t.np * t.mp;
-    x = base + t.at;
-    xt = x + nx;
-    sq = xt + 2 * nx;
+  size_t na;  // one of sq's (hi and lo)
+  __device__ Area(_Float16* base, const Tile& t, int rect_ts, int from) {
+    const size_t nx = 2 * (size_t)t.np * t.mp;
+    na = 2 * (size_t)t.np * t.np;
+    x = next = base + t.at;
+    sq = x + (rect_ts == 64 ? 3 : 2) * nx;
     diag = reinterpret_cast<float*>(sq + SQ * na);
+    if (rect_ts == 64) xt = x + (from ? 2 : 1) * nx, next_t = x + (from ? 1 : 2) * nx;
+    else xt = next_t = nullptr, x += from ? nx : 0, next += from ? 0 : nx;
   }
 };
 struct Lists {  // one entry a workgroup
@@ -355,7 +360,7 @@ __global__ __launch_bounds__(256) void ortho_start_kernel(Lists l, const double*
   __shared__ float E[64 * 65];
   const Tile w = l.fill[blockIdx.x];
   const Mat t = l.table[w.mat];
-  const Area o(base, w);
+  const Area o(base, w, l.rect_ts, 0);
   double s = 0;
   const unsigned chunks = Dim(t.rows, t.cols, l.pad).norms();
   for (unsigned i = threadIdx.x; i < chunks; i += 256) s += norms[t.norm0 + i];
@@ -370,7 +375,7 @@ __global__ __launch_bounds__(256) void ortho_start_kernel(Lists l, const double*
   });
   __syncthreads();
   rows8<64, 64, 65, 1>(E, [&](int r, int c, float (&v)[8]) { store8(o.x + place(i0 + r, j0 + c, w.mp), v); });
-  store_turned<64, 64, 65>(E, o.xt, w.np, j0, i0);
+  if (o.xt) store_turned<64, 64, 65>(E, o.xt, w.np, j0, i0);
 }
 
 // ------------------------------------------------------------------------------------------------ the products
@@ -432,63 +437,93 @@ struct Core128 {
     Stage st[2];
     float E[TS * LD];
   };
-  struct Source {  // the stage's blocks
+  struct Source {  // the first stage's blocks
     const _Float16 *p[2], *q[2];
+    size_t down;  // TURNED: 64 rows further in Q
   };
   static __device__ __forceinline__ int spot(int r, int c) { return r * 4 + (c ^ (r / 4 % 4)); }
+  // TURNED: Q's rows are the summed index.  32 of them lie in shared memory as they come, the 16-byte piece c of row k at
+  // this place, and are turned by the reads of it: of sixteen lanes, four each name sixteen columns of a row, and each
+  // receives four rows of a column.  Both ways go over all banks.
+  static __device__ __forceinline__ int turned_spot(int k, int c) { return k * 16 + (c / 4 ^ k % 4) * 4 + (c % 4 ^ k / 4 % 4); }
+  template <bool TURNED>
   static __device__ __forceinline__ void fetch(half8 (&to)[8], const Source& s, int stage) {
     const size_t k = (size_t)stage * BLOCK + threadIdx.x * 8;
+    const size_t kq = TURNED ? (size_t)(stage / 2) * s.down + stage % 2 * 512 + threadIdx.x % 64 * 8 : k;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       to[4 * t] = *reinterpret_cast<const half8*>(s.p[t] + k);
       to[4 * t + 1] = *reinterpret_cast<const half8*>(s.p[t] + k + LO);
-      to[4 * t + 2] = *reinterpret_cast<const half8*>(s.q[t] + k);
-      to[4 * t + 3] = *reinterpret_cast<const half8*>(s.q[t] + k + LO);
+      to[4 * t + 2] = *reinterpret_cast<const half8*>(s.q[t] + kq);
+      to[4 * t + 3] = *reinterpret_cast<const half8*>(s.q[t] + kq + LO);
     }
   }
+  template <bool TURNED>
   static __device__ __forceinline__ void put(Stage& s, const half8 (&from)[8]) {
     const int t4 = threadIdx.x, r = t4 / 64 % 2 * 32 + t4 % 32, c = t4 / 128 * 2 + t4 / 32 % 2;  // (the block's order)
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int a = 0; a < 4; ++a) s.v[a][spot(t * 64 + r, c)] = from[4 * t + a];
+    for (int t = 0; t < 2; ++t) {
+      const int ps = spot(t * 64 + r, c), qs = TURNED ? turned_spot(t4 % 32, t * 8 + t4 / 32) : ps;
+      s.v[0][ps] = from[4 * t], s.v[1][ps] = from[4 * t + 1], s.v[2][qs] = from[4 * t + 2], s.v[3][qs] = from[4 * t + 3];
+    }
   }
+  static __device__ __forceinline__ half4 turn(const half8* at, int half) {
+    typedef __attribute__((address_space(3))) decltype(__builtin_amdgcn_ds_read_tr16_b64_v4f16(nullptr)) Turned;
+    const auto v = __builtin_amdgcn_ds_read_tr16_b64_v4f16((Turned*)(reinterpret_cast<const half4*>(at) + half));
+    return __builtin_bit_cast(half4, v);
+  }
+  template <bool TURNED>
   static __device__ __forceinline__ void read(Piece& f, const Stage& s, int kk) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int pr = (wave >> 1) * 64 + (lane & 31), qr = (wave & 1) * 64 + (lane & 31), kc = lane >> 5;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int ps = spot(pr + 32 * i, kk * 2 + kc), qs = spot(qr + 32 * i, kk * 2 + kc);
-      f.ph[i] = s.v[0][ps], f.pl[i] = s.v[1][ps], f.qh[i] = s.v[2][qs], f.ql[i] = s.v[3][qs];
+      const int ps = spot(pr + 32 * i, kk * 2 + kc);
+      f.ph[i] = s.v[0][ps], f.pl[i] = s.v[1][ps];
+      if constexpr (TURNED) {
+        const int c = (wave & 1) * 8 + 4 * i + lane / 16 % 2 * 2 + lane % 4 / 2, k = kk * 16 + kc * 8 + lane % 16 / 4;
+        const int one = turned_spot(k, c), two = turned_spot(k + 4, c);
+        f.qh[i] = __builtin_shufflevector(turn(&s.v[2][one], lane & 1), turn(&s.v[2][two], lane & 1), 0, 1, 2, 3, 4, 5, 6, 7);
+        f.ql[i] = __builtin_shufflevector(turn(&s.v[3][one], lane & 1), turn(&s.v[3][two], lane & 1), 0, 1, 2, 3, 4, 5, 6, 7);
+      } else {
+        const int qs = spot(qr + 32 * i, kk * 2 + kc);
+        f.qh[i] = s.v[2][qs], f.ql[i] = s.v[3][qs];
+      }
     }
   }
-  // the tile times f in shared memory
+  // the tile times f in shared memory; TURNED: of P Q
+  template <bool TURNED = false>
   static __device__ __forceinline__ void run(Shared& sh, const _Float16* p, int prow, int ldp, const _Float16* q, int qrow,
                                              int ldq, int k0, int k1, float f) {
     Source src;
+    src.down = (size_t)(ldq / 32) * BLOCK;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) src.p[t] = p + place(prow + 64 * t, k0, ldp), src.q[t] = q + place(qrow + 64 * t, k0, ldq);
+    for (int t = 0; t < 2; ++t) {
+      src.p[t] = p + place(prow + 64 * t, k0, ldp);
+      src.q[t] = q + (TURNED ? place(k0, qrow + 64 * t + threadIdx.x / 64 * 16, ldq) : place(qrow + 64 * t, k0, ldq));
+    }
     const int stages = (k1 - k0) / 32, end = stages - 1;
     half8 next[8];
     Piece one, two;
     Acc hh, hl;
-    fetch(next, src, 0);
+    fetch<TURNED>(next, src, 0);
     clear(hh), clear(hl);
-    put(sh.st[0], next);
-    fetch(next, src, 1);
+    put<TURNED>(sh.st[0], next);
+    fetch<TURNED>(next, src, 1);
     __syncthreads();
     Stage *now = sh.st, *then = sh.st + 1;
     for (int s = 0; s < stages; ++s) {
-      read(one, *now, 0);
-      read(two, *now, 1);
+      read<TURNED>(one, *now, 0);
+      read<TURNED>(two, *now, 1);
       multiply(hh, hl, one);
-      put(*then, next);  // (that stage was left before the last barrier)
-      fetch(next, src, s + 2 < end ? s + 2 : end);
+      put<TURNED>(*then, next);  // (that stage was left before the last barrier)
+      fetch<TURNED>(next, src, s + 2 < end ? s + 2 : end);
       multiply(hh, hl, two);
+      constexpr int READS = TURNED ? 12 : 8, LOADS = TURNED ? 2 : 1;  // (24 matrix instructions)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
+      for (int k = 0; k < READS; ++k) __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < READS; ++k) {
         __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
         __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
       }
@@ -498,9 +533,9 @@ struct Core128 {
         __builtin_amdgcn_sched_group_barrier(DS_WRITE, 1, 0);
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 8 / LOADS; ++k) {
         __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(VMEM_READ, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(VMEM_READ, LOADS, 0);
       }
       __syncthreads();  // (behind the last stage: the stages' memory is the epilogue's too)
       Stage* was = now;
@@ -574,10 +609,10 @@ __device__ __forceinline__ void store_gram(float* E, int np, const Area& o, int 
 // (Adding them in the workgroup that ends last needs the other workgroups' tiles flushed through the XCDs' caches: 160 us
 // where this and the launch behind it take 20, at eight 256 x 2304 matrices.)
 template <int TS>
-__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Lists l, _Float16* base, float* parts, int kc) {
+__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Lists l, _Float16* base, float* parts, int kc, int from) {
   __shared__ typename Core<TS>::Shared sh;
   const Tile w = l.gram[blockIdx.x];
-  const Area o(base, w);
+  const Area o(base, w, l.rect_ts, from);
   const int i0 = w.i * TS, j0 = w.j * TS;
   const int k0 = w.split * kc, k1 = k0 + kc < w.mp ? k0 + kc : w.mp;
   Core<TS>::run(sh, o.x, i0, w.mp, o.x, j0, w.mp, k0, k1, 1.f / SCALE);
@@ -600,7 +635,7 @@ __global__ __launch_bounds__(256) void ortho_sum_kernel(Lists l, _Float16* base,
   __shared__ float E[32 * (TS + 1)];
   const Tile w = l.gram[blockIdx.x];
   if (w.split || w.splits == 1) return;
-  const Area o(base, w);
+  const Area o(base, w, l.rect_ts, 0);
   const int slice = blockIdx.y * 32;
   const float* mine = parts + w.part + slice * TS;
 #pragma unroll
@@ -628,7 +663,7 @@ template <int TS>
 __global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
   __shared__ typename Core<TS>::Shared sh;
   const Tile w = l.tri[blockIdx.x];
-  const Area o(base, w);
+  const Area o(base, w, l.rect_ts, 0);
   const Op op = blockIdx.y ? second : first;
   const int i0 = w.i * TS, j0 = w.j * TS;
   const _Float16 *g = o.sq + op.g * o.na, *h = o.sq + op.h * o.na;
@@ -661,24 +696,25 @@ __global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16*
   }
 }
 
-// X <- R X, from X^t; the last group's goes to the caller, as the result or into the weights
+// X <- R X; the last group's goes to the caller, as the result or into the weights
 template <typename T, bool LAST, int TS>
 __global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* base, int R, float fs, int from, int update,
                                                              float decay) {
   __shared__ typename Core<TS>::Shared sh;
   const Tile w = l.rect[blockIdx.x];
-  const Area o(base, w);
+  const Area o(base, w, TS, from);
   const int i0 = w.i * TS, j0 = w.j * TS;
-  const _Float16 *a = o.sq + R * o.na, *xt = o.xt + (from ? o.nx : 0);
-  Core<TS>::run(sh, a, i0, w.np, xt, j0, w.np, 0, w.np, fs);
+  const _Float16* a = o.sq + R * o.na;
+  if constexpr (TS == 128) Core128::run<true>(sh, a, i0, w.np, o.x, j0, w.mp, 0, w.np, fs);
+  else Core64::run(sh, a, i0, w.np, o.xt, j0, w.np, 0, w.np, fs);
   rows8<TS, TS, TS + 1, Core<TS>::PARTS>(sh.E, [&](int r, int c, float (&v)[8]) {
-    _Float16* x = o.x + place(i0 + r, j0 + c, w.mp);
-    add8(v, o.diag[R * w.np + i0 + r], x);
-    if constexpr (!LAST) store8(x, v);
+    const size_t at = place(i0 + r, j0 + c, w.mp);
+    add8(v, o.diag[R * w.np + i0 + r], o.x + at);
+    if constexpr (!LAST) store8(o.next + at, v);
   });
   __syncthreads();
   if constexpr (!LAST) {
-    store_turned<TS, TS, TS + 1>(sh.E, o.xt + (from ? 0 : o.nx), w.np, j0, i0);
+    if constexpr (TS == 64) store_turned<TS, TS, TS + 1>(sh.E, o.next_t, w.np, j0, i0);
   } else {
     const Mat t = l.table[w.mat];
     T* out = static_cast<T*>(t.dst);
@@ -709,7 +745,6 @@ constexpr int SMALL_N = 64, SMALL_M = 128;
 __host__ __device__ inline bool is_small(int rows, int cols) {
   return (rows < cols ? rows : cols) <= SMALL_N && (rows < cols ? cols : rows) <= SMALL_M;
 }
-typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 struct Small {
   _Float16 x[SMALL_M / 32 * BLOCK], xt[SMALL_M / 32 * BLOCK], a[2 * BLOCK], f[2 * BLOCK];
   float da[64], df[64];
@@ -972,7 +1007,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
     fill += d.rect(64);
     norm += d.norms();
     if (s > 1) part += (uint64_t)d.tri(l.gram_ts) * s * l.gram_ts * l.gram_ts, p.split = true;
-    halves += d.halves();
+    halves += d.halves(l.rect_ts);
   }
   if (gram > 0x7fffffff || tri > 0x7fffffff || rect > 0x7fffffff || fill > 0x7fffffff || norm > 0x7fffffff) return -1;
   l.n_gram = (unsigned)gram, l.n_tri = (unsigned)tri, l.n_rect = (unsigned)rect, l.n_fill = (unsigned)fill;
@@ -1104,7 +1139,7 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
       fill += d.rect(64);
       norm += d.norms();
       if (s > 1) part += (size_t)d.tri(l.gram_ts) * s * l.gram_ts * l.gram_ts;
-      halves += d.halves();
+      halves += d.halves(l.rect_ts);
     }
     batch.end.gram0 = gram, batch.end.tri0 = tri, batch.end.rect0 = rect, batch.end.fill0 = fill, batch.end.norm0 = norm;
     unsigned blocks = (fill + gram - was) / 256 + 1;
@@ -1131,7 +1166,7 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
     int g = group_length(left, steps);
     if (g > f.longest) g = f.longest;
     choose(l.gram_ts, [&](auto TS) {
-      hipLaunchKernelGGL((ortho_gram_kernel<TS()>), dim3(l.n_gram), wg, 0, st, l, base, parts, p.kc);
+      hipLaunchKernelGGL((ortho_gram_kernel<TS()>), dim3(l.n_gram), wg, 0, st, l, base, parts, p.kc, from);
       if (p.split) hipLaunchKernelGGL((ortho_sum_kernel<TS()>), dim3(l.n_gram, TS() / 32), wg, 0, st, l, base, parts);
     });
     int R = SQ_F, spare = SQ_R;
