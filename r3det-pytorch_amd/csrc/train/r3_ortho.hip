@@ -180,7 +180,7 @@ __global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
     Tile w = begin(k);
     const unsigned high = w.np / l.rect_ts;
     w.i = local % high, w.j = local / high;
-    l.rect[e] = w;
+    l.rect[entry(e, l.n_rect)] = w;
   }
   for (unsigned e = b.m[0].fill0 + g; e < b.end.fill0; e += stride) {
     const unsigned k = find(b, &Mat::fill0, e), local = e - b.m[k].fill0;
