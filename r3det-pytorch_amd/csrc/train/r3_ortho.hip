@@ -41,7 +41,6 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
-constexpr int NORM_CHUNK = 8192; // elements a workgroup of the norm's pass takes
 constexpr float SCALE = 4096.f;  // what stored values are multiplied by
 constexpr float R_SCALE = 512.f; // ... of R
 constexpr int WANT = 512;        // workgroups that fill the card
@@ -74,7 +73,7 @@ struct Dim {  // padded with zeros, which stay zeros
   __host__ __device__ size_t halves(int rect_ts) const { return 2 * ((rect_ts == 64 ? 3 : 2) * x() + SQ * a() + (size_t)SQ * np); }
   __host__ __device__ unsigned tri(int ts) const { return (unsigned)(np / ts) * (np / ts + 1) / 2; }
   __host__ __device__ unsigned rect(int ts) const { return (unsigned)(np / ts) * (mp / ts); }
-  __host__ __device__ unsigned norms() const { return (unsigned)(((size_t)n * m + NORM_CHUNK - 1) / NORM_CHUNK); }
+  __host__ __device__ unsigned norms(int chunk) const { return (unsigned)(((size_t)n * m + chunk - 1) / chunk); }
 };
 struct Tile {  // one workgroup's work, with all that it needs of its matrix to begin
   size_t at;    // Mat::at
@@ -107,6 +106,7 @@ struct Lists {  // one entry a workgroup
   uint2* norm_map;  // (matrix, chunk)
   unsigned n_gram, n_tri, n_rect, n_fill, n_norm;
   int count, pad, gram_ts, tri_ts, rect_ts;
+  int chunk;  // elements a workgroup of the norm's pass takes
 };
 
 // the whole workspace; every part is a multiple of 256 bytes
@@ -246,8 +246,8 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(Lists l, double* __rest
   __shared__ double sh[4];
   const uint2 w = l.norm_map[blockIdx.x];
   const Mat t = l.table[w.x];
-  const size_t all = (size_t)t.rows * t.cols, from = (size_t)w.y * NORM_CHUNK;
-  const int many = (int)(from + NORM_CHUNK < all ? NORM_CHUNK : all - from);
+  const size_t all = (size_t)t.rows * t.cols, from = (size_t)w.y * l.chunk;
+  const int many = (int)(from + l.chunk < all ? l.chunk : all - from);
   double s = 0;
   int i = threadIdx.x;
   if (t.wide) {
@@ -323,10 +323,10 @@ __device__ __forceinline__ void add8(float (&v)[8], float f, const _Float16* at)
 // ROWS x COLS of fp32 in shared memory, rows of LD: f(row, column, eight values), which may change them; then `f`'s values
 // are in shared memory too.  PARTS > 1: the values are the sum of so many such arrays.  (Neighbouring threads have
 // neighbouring rows: the arrays' order, and LD is odd.)
-template <int ROWS, int COLS, int LD, int PARTS, typename F>
+template <int ROWS, int COLS, int LD, int PARTS, int THREADS = 256, typename F>
 __device__ __forceinline__ void rows8(float* E, const F& f) {
 #pragma unroll 2
-  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += 256) {
+  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += THREADS) {
     const int r = q % ROWS, c = q / ROWS * 8;
     float v[8];
 #pragma unroll
@@ -341,10 +341,10 @@ __device__ __forceinline__ void rows8(float* E, const F& f) {
   }
 }
 // The transpose of ROWS x COLS in shared memory -> an array of `ld` columns, at (r0, c0).
-template <int ROWS, int COLS, int LD>
+template <int ROWS, int COLS, int LD, int THREADS = 256>
 __device__ __forceinline__ void store_turned(const float* E, _Float16* p, int ld, int r0, int c0) {
 #pragma unroll 2
-  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += 256) {
+  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += THREADS) {
     const int r = q % COLS, c = q / COLS * 8;
     float v[8];
 #pragma unroll
@@ -362,16 +362,16 @@ __global__ __launch_bounds__(256) void ortho_start_kernel(Lists l, const double*
   const Mat t = l.table[w.mat];
   const Area o(base, w, l.rect_ts, 0);
   double s = 0;
-  const unsigned chunks = Dim(t.rows, t.cols, l.pad).norms();
+  const unsigned chunks = Dim(t.rows, t.cols, l.pad).norms(l.chunk);
   for (unsigned i = threadIdx.x; i < chunks; i += 256) s += norms[t.norm0 + i];
   s = block_sum(s, sh);
   const double inv = (double)SCALE / (sqrt(s) + eps);
   const int i0 = w.i * 64, j0 = w.j * 64;
   callers<64>(t, i0, j0, [&](auto N, size_t at, bool in, int r, int c, bool tall) {
-    float v[N()] = {};
-    if (in) direction<T, N(), false>(v, t, at, m);
+    float v[N()];
+    direction<T, N(), false>(v, t, in ? at : 0, m);  // (inside or not, so that several are on their way)
 #pragma unroll
-    for (int k = 0; k < N(); ++k) E[(tall ? r + k : r) * 65 + (tall ? c : c + k)] = (float)((double)v[k] * inv);
+    for (int k = 0; k < N(); ++k) E[(tall ? r + k : r) * 65 + (tall ? c : c + k)] = in ? (float)((double)v[k] * inv) : 0.f;
   });
   __syncthreads();
   rows8<64, 64, 65, 1>(E, [&](int r, int c, float (&v)[8]) { store8(o.x + place(i0 + r, j0 + c, w.mp), v); });
@@ -431,7 +431,7 @@ struct Stage {
   half8 v[4][512];
 };
 struct Core128 {
-  static constexpr int TS = 128, LD = 129, PARTS = 1;
+  static constexpr int TS = 128, LD = 129, PARTS = 1, THREADS = 256;
   static constexpr int MFMA = 8, VMEM_READ = 0x20, DS_READ = 0x100, DS_WRITE = 0x200;  // kinds of instructions
   union Shared {
     Stage st[2];
@@ -549,9 +549,11 @@ struct Core128 {
 
 // A tile of 64, for where those of 128 are too few: the whole tile a wavefront, the summed index in turn, 16 of it at a time.
 // Operands come from memory straight into registers, each by one wavefront only, so shared memory has nothing to save and
-// nobody waits at a barrier before the end; there the four sums are added.
+// nobody waits at a barrier before the end; there the wavefronts' sums are added.  Two pieces are on their way (three, and
+// loads of the last one again where there is no next: 9 more where a wavefront has four; 64 x 64 of 256: 9.2 us, 8.4 so).
+template <int WAVES>
 struct Core64 {
-  static constexpr int TS = 64, LD = 65, PARTS = 4, AHEAD = 3;
+  static constexpr int TS = 64, LD = 65, PARTS = WAVES, THREADS = 64 * WAVES, AHEAD = 2;
   union Shared {
     float E[PARTS * TS * LD];
   };
@@ -569,25 +571,29 @@ struct Core64 {
                                              int ldq, int k0, int k1, float f) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     p += place(prow, k0, ldp), q += place(qrow, k0, ldq);
-    const int units = (k1 - k0) / 64, end = units - 1;  // of this wavefront
+    const int units = (k1 - k0) / (16 * WAVES), end = units - 1;  // of this wavefront
     Piece piece[AHEAD];
     Acc hh, hl;
 #pragma unroll
-    for (int d = 0; d < AHEAD; ++d) fetch(piece[d], p, q, (d < end ? d : end) * 4 + wave);
+    for (int d = 0; d < AHEAD; ++d) fetch(piece[d], p, q, (d < end ? d : end) * WAVES + wave);
     clear(hh), clear(hl);
-    for (int s = 0; s < units; s += AHEAD) {
+    int s = 0;
+    for (; s + AHEAD < units; s += AHEAD) {
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
-        if (s + u < units) multiply(hh, hl, piece[u]);
-        fetch(piece[u], p, q, (s + u + AHEAD < end ? s + u + AHEAD : end) * 4 + wave);
+        multiply(hh, hl, piece[u]);
+        fetch(piece[u], p, q, (s + u + AHEAD < end ? s + u + AHEAD : end) * WAVES + wave);
       }
     }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (s + u < units) multiply(hh, hl, piece[u]);
     spill<LD>(hh, hl, sh.E + wave * TS * LD, f);
     __syncthreads();
   }
 };
 template <int TS>
-using Core = std::conditional_t<TS == 128, Core128, Core64>;
+using Core = std::conditional_t<TS == 128, Core128, Core64<4>>;
 
 // A from ROWS rows of a tile in shared memory
 template <int ROWS, int TS, int PARTS>
@@ -659,19 +665,20 @@ struct Op {
   int out, g, h;  // which arrays
   float t, q, l, f, fg, fh, fs, back;  // back: one over out's scale
 };
-template <int TS>
-__global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
-  __shared__ typename Core<TS>::Shared sh;
+template <typename C>
+__global__ __launch_bounds__(C::THREADS, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
+  constexpr int TS = C::TS;
+  __shared__ typename C::Shared sh;
   const Tile w = l.tri[blockIdx.x];
   const Area o(base, w, l.rect_ts, 0);
   const Op op = blockIdx.y ? second : first;
   const int i0 = w.i * TS, j0 = w.j * TS;
   const _Float16 *g = o.sq + op.g * o.na, *h = o.sq + op.h * o.na;
   const float *gd = o.diag + op.g * w.np, *hd = o.diag + op.h * w.np;
-  Core<TS>::run(sh, g, i0, w.np, h, j0, w.np, 0, w.np, 1.f);
+  C::run(sh, g, i0, w.np, h, j0, w.np, 0, w.np, 1.f);
   _Float16* out = o.sq + op.out * o.na;
   const bool diagonal = w.i == w.j;
-  rows8<TS, TS, TS + 1, Core<TS>::PARTS>(sh.E, [&](int r, int c, float (&v)[8]) {
+  rows8<TS, TS, TS + 1, C::PARTS, C::THREADS>(sh.E, [&](int r, int c, float (&v)[8]) {
     const int i = i0 + r, j = j0 + c;
     const size_t at = place(i, j, w.np);
     const half8 gh = *reinterpret_cast<const half8*>(g + at), gl = *reinterpret_cast<const half8*>(g + at + LO);
@@ -692,7 +699,7 @@ __global__ __launch_bounds__(256, 2) void ortho_square_kernel(Lists l, _Float16*
   });
   if (!diagonal) {
     __syncthreads();
-    store_turned<TS, TS, TS + 1>(sh.E, out, w.np, j0, i0);
+    store_turned<TS, TS, TS + 1, C::THREADS>(sh.E, out, w.np, j0, i0);
   }
 }
 
@@ -706,7 +713,7 @@ __global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* 
   const int i0 = w.i * TS, j0 = w.j * TS;
   const _Float16* a = o.sq + R * o.na;
   if constexpr (TS == 128) Core128::run<true>(sh, a, i0, w.np, o.x, j0, w.mp, 0, w.np, fs);
-  else Core64::run(sh, a, i0, w.np, o.xt, j0, w.np, 0, w.np, fs);
+  else Core<TS>::run(sh, a, i0, w.np, o.xt, j0, w.np, 0, w.np, fs);
   rows8<TS, TS, TS + 1, Core<TS>::PARTS>(sh.E, [&](int r, int c, float (&v)[8]) {
     const size_t at = place(i0 + r, j0 + c, w.mp);
     add8(v, o.diag[R * w.np + i0 + r], o.x + at);
@@ -973,17 +980,20 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   l.pad = 128;
   // Tiles: 128 needs half the reads of two operands that 64 does, and is taken for a pass that fills the card with such
   // tiles.
-  uint64_t tri128 = 0, rect128 = 0, gram128 = 0;
+  uint64_t tri128 = 0, rect128 = 0, gram128 = 0, elements = 0;
   for (int i = 0; i < count; ++i) {
     if (is_small(rows[i], cols[i])) continue;
     ++l.count;
     const Dim w(rows[i], cols[i], 128);
+    elements += (uint64_t)rows[i] * cols[i];
     tri128 += w.tri(128), rect128 += w.rect(128);
     gram128 += (uint64_t)w.tri(128) * ((w.mp + 255) / 256);
   }
   l.gram_ts = gram128 >= WANT / 2 ? 128 : 64;
   l.tri_ts = tri128 >= WANT ? 128 : 64;
   l.rect_ts = rect128 >= WANT / 2 ? 128 : 64;
+  // The norms: each thread 32 elements, fewer where that would leave compute units without work (2.6 M elements: 20 us, 6 so).
+  for (l.chunk = 8192; l.chunk > 1024 && elements / l.chunk < 2 * WANT;) l.chunk /= 2;
   // X X^t: the longest parts of the sum that still fill the card.  A part is a workgroup's time, so the parts of a ragged
   // list are of like length, and a short list of wide matrices is spread.
   for (p.kc = 4096; p.kc > 512; p.kc /= 2) {
@@ -1005,7 +1015,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
     tri += d.tri(l.tri_ts);
     rect += d.rect(l.rect_ts);
     fill += d.rect(64);
-    norm += d.norms();
+    norm += d.norms(l.chunk);
     if (s > 1) part += (uint64_t)d.tri(l.gram_ts) * s * l.gram_ts * l.gram_ts, p.split = true;
     halves += d.halves(l.rect_ts);
   }
@@ -1137,7 +1147,7 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
       tri += d.tri(l.tri_ts);
       rect += d.rect(l.rect_ts);
       fill += d.rect(64);
-      norm += d.norms();
+      norm += d.norms(l.chunk);
       if (s > 1) part += (size_t)d.tri(l.gram_ts) * s * l.gram_ts * l.gram_ts;
       halves += d.halves(l.rect_ts);
     }
@@ -1151,11 +1161,18 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
   hipLaunchKernelGGL((ortho_norm_kernel<T>), dim3(l.n_norm), wg, 0, st, l, norms, m);
   hipLaunchKernelGGL((ortho_start_kernel<T>), dim3(l.n_fill), wg, 0, st, l, norms, base, m, eps);
   if (hipGetLastError() != hipSuccess) return -2;
+  const unsigned cus = (unsigned)r3_cu_count();
   const auto square = [&](const Op& one, const Op* two) {
-    choose(l.tri_ts, [&](auto TS) {
-      hipLaunchKernelGGL((ortho_square_kernel<TS()>), dim3(l.n_tri, two ? 2 : 1), wg, 0, st, l, base, one,
-                         two ? *two : one);
-    });
+    const dim3 grid(l.n_tri, two ? 2 : 1);
+    const auto launch = [&](auto core) {
+      typedef decltype(core) C;
+      hipLaunchKernelGGL((ortho_square_kernel<C>), grid, dim3(C::THREADS), 0, st, l, base, one, two ? *two : one);
+    };
+    // A tile a compute unit: eight wavefronts share its sum and its epilogue (eight of 256 x 256: 7.3 us, four 8.4; more
+    // tiles than that share the units anyway: 2048 x 2048, 56 against 53).
+    if (l.tri_ts == 128) launch(Core128());
+    else if (grid.x * grid.y <= cus) launch(Core64<8>());
+    else launch(Core64<4>());
   };
   // G H, stored 2^so times from 2^sg and 2^sh times
   const auto times = [](int out, int g, int h, float so, float sg, float sh) {
