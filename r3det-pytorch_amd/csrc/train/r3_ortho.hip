@@ -151,16 +151,25 @@ __device__ __forceinline__ unsigned entry(unsigned u, unsigned n) {
   const unsigned c = v < longer ? v % (q + 1) : (v - longer) % q;
   return first + c * XCDS + x;
 }
-// the table's and the lists' entries of `b`'s matrices
+// the table's and the lists' entries of `b`'s matrices: a thread an entry, list behind list
 __global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
-  const unsigned g = blockIdx.x * blockDim.x + threadIdx.x, stride = gridDim.x * blockDim.x;
-  if (g < (unsigned)b.count) l.table[first + g] = b.m[g];
+  unsigned e = blockIdx.x * blockDim.x + threadIdx.x;
+  if (e < (unsigned)b.count) l.table[first + e] = b.m[e];
+  const auto within = [&](unsigned Mat::* member) {  // of this list: the entry, and the matrix in front of which it begins
+    const unsigned from = b.m[0].*member, many = b.end.*member - from;
+    if (e < many) {
+      e += from;
+      return true;
+    }
+    e -= many;
+    return false;
+  };
   const auto begin = [&](unsigned k) {
     const Mat& t = b.m[k];
     const Dim d(t.rows, t.cols, l.pad);
     return Tile{t.at, 0, d.np, d.mp, 0, 0, 0, (unsigned short)t.splits, first + k};
   };
-  for (unsigned e = b.m[0].gram0 + g; e < b.end.gram0; e += stride) {
+  if (within(&Mat::gram0)) {
     const unsigned k = find(b, &Mat::gram0, e), local = e - b.m[k].gram0;
     Tile w = begin(k);
     const unsigned high = w.np / l.gram_ts, tiles = high * (high + 1) / 2, tile = local % tiles;
@@ -168,28 +177,24 @@ __global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
     w.split = local / tiles;
     w.part = b.m[k].part0 + ((size_t)tile * w.splits + w.split) * (l.gram_ts * l.gram_ts);
     l.gram[entry(e, l.n_gram)] = w;
-  }
-  for (unsigned e = b.m[0].tri0 + g; e < b.end.tri0; e += stride) {
+  } else if (within(&Mat::tri0)) {
     const unsigned k = find(b, &Mat::tri0, e);
     Tile w = begin(k);
     triangle(w, e - b.m[k].tri0, w.np / l.tri_ts);
     l.tri[entry(e, l.n_tri)] = w;
-  }
-  for (unsigned e = b.m[0].rect0 + g; e < b.end.rect0; e += stride) {
+  } else if (within(&Mat::rect0)) {
     const unsigned k = find(b, &Mat::rect0, e), local = e - b.m[k].rect0;
     Tile w = begin(k);
     const unsigned high = w.np / l.rect_ts;
     w.i = local % high, w.j = local / high;
     l.rect[entry(e, l.n_rect)] = w;
-  }
-  for (unsigned e = b.m[0].fill0 + g; e < b.end.fill0; e += stride) {
+  } else if (within(&Mat::fill0)) {
     const unsigned k = find(b, &Mat::fill0, e), local = e - b.m[k].fill0;
     Tile w = begin(k);
     const unsigned wide = w.mp / 64;
     w.i = local / wide, w.j = local % wide;
     l.fill[e] = w;
-  }
-  for (unsigned e = b.m[0].norm0 + g; e < b.end.norm0; e += stride) {
+  } else if (within(&Mat::norm0)) {
     const unsigned k = find(b, &Mat::norm0, e);
     l.norm_map[e] = make_uint2(first + k, e - b.m[k].norm0);
   }
@@ -1020,6 +1025,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
     halves += d.halves(l.rect_ts);
   }
   if (gram > 0x7fffffff || tri > 0x7fffffff || rect > 0x7fffffff || fill > 0x7fffffff || norm > 0x7fffffff) return -1;
+  if (gram + tri + rect + fill + norm > 0xffffff00) return -1;  // (the lists' threads)
   l.n_gram = (unsigned)gram, l.n_tri = (unsigned)tri, l.n_rect = (unsigned)rect, l.n_fill = (unsigned)fill;
   l.n_norm = (unsigned)norm;
   size_t at = 0;
@@ -1134,7 +1140,7 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
   if (l.count == 0) return 0;
   for (int i = 0, first = 0; first < l.count;) {
     Batch batch{};
-    const unsigned was = fill + gram;
+    const uint64_t was = (uint64_t)gram + tri + rect + fill + norm;
     for (; i < count && batch.count < BATCH; ++i) {
       if (is_small(rows[i], cols[i])) continue;
       const Dim d(rows[i], cols[i], l.pad);
@@ -1152,9 +1158,8 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
       halves += d.halves(l.rect_ts);
     }
     batch.end.gram0 = gram, batch.end.tri0 = tri, batch.end.rect0 = rect, batch.end.fill0 = fill, batch.end.norm0 = norm;
-    unsigned blocks = (fill + gram - was) / 256 + 1;
-    if (blocks > 512) blocks = 512;
-    hipLaunchKernelGGL(ortho_lists_kernel, dim3(blocks), wg, 0, st, l, batch, (unsigned)first);
+    const uint64_t entries = (uint64_t)gram + tri + rect + fill + norm - was;
+    hipLaunchKernelGGL(ortho_lists_kernel, dim3((unsigned)((entries + 255) / 256)), wg, 0, st, l, batch, (unsigned)first);
     if (hipGetLastError() != hipSuccess) return -2;
     first += batch.count;
   }
