@@ -636,8 +636,8 @@ int r3det_fr_profile_read(float* records, int capacity);
  *   top_log_prob, top_index (rows, top_k): the top_k <= min(classes, 64) greatest, best first, ties to the lowest index;
  *   stats (rows, 2) or NULL: what the gradient needs (the maximum and the log of the sum behind it).
  * All results fp32 / int64.  A logit of -inf is a class that is not offered; a row with no class left has log_prob and
- * top_log_prob -inf, entropy 0 and the gradient 0.  A row with NaN or +inf has NaN in place of its numbers (top_index then
- * holds valid places).
+ * top_log_prob -inf, entropy 0 and the gradient 0.  A row with NaN or +inf has NaN in place of its numbers; NaN is ranked
+ * first.
  * The workspace (r3det_label_log_probs_workspace_bytes; 0 for all but few, long rows) need not be initialised. */
 size_t r3det_label_log_probs_workspace_bytes(int64_t rows, int64_t classes, int top_k);
 int r3det_label_log_probs(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t row_stride,
@@ -661,10 +661,11 @@ int r3det_label_log_probs_backward(const void* logits, int dtype, int64_t rows, 
  * at least 1 x 1, at most 2^31 - 1 elements, the smaller side at most 32768):
  *   X = G / (|G|_F + eps), then `steps` (1 .. 64) times  A = X X^t,  X <- a X + (b A + c A A) X   (for rows > cols: of G^t);
  * dst[i] (rows x cols, contiguous, of the same type; may be src[i]) receives X.  All in fp32 accuracy whatever the type.
- * The arrays of pointers and sizes are HOST arrays and are read before the call returns.  The coefficients have to keep
- * the singular values, the entries of X, A and b A + c A A, below 15 for every s in [0, 1]
- * (r3det_orthogonalize returns R3DET_EINVAL otherwise).  A workspace of r3det_orthogonalize_workspace_bytes (0: a shape that
- * is not taken, or no matrix), 16-byte aligned, need not be initialised. */
+ * A zero matrix stays zero where eps > 0.  The arrays of pointers and sizes are HOST arrays and are read before the call
+ * returns.  With P = a I + b A + c A A, the coefficients have to keep the spectral norms of X, A, P A and of P less its
+ * vertex a - b b / (4 c) (less a, where |b| > 14 |c|) below 15 in every step, for singular values of up to 1 at first
+ * (R3DET_EINVAL otherwise).  A workspace of r3det_orthogonalize_workspace_bytes (0: a shape that is not taken, or no
+ * matrix), 16-byte aligned, need not be initialised. */
 size_t r3det_orthogonalize_workspace_bytes(int count, const int* rows, const int* cols);
 int r3det_orthogonalize(int count, const void* const* src, void* const* dst, int dtype, const int* rows, const int* cols,
                         int steps, float a, float b, float c, double eps, void* ws, size_t ws_bytes, void* stream);

@@ -25,9 +25,16 @@
 // Stored values carry a power of two so that fp16 neither overflows -- spectral norms bound the entries, and the host checks
 // them for the given coefficients -- nor loses lo's bits: 2^12 for X, A, F, F A (norms below 15), 2^9 for R (below 120).
 //
-// Every product has both operands with the summed index contiguous: the symmetric matrices and X X^t as they are, R X from
-// X^t, which the kernel that makes X writes beside it.  Of a symmetric result the tiles on and above the diagonal are
-// computed, and written twice.
+// The matrix instructions want both operands with the summed index contiguous.  The symmetric matrices and X X^t have it;
+// for R X, X is turned on its way out of shared memory (tiles of 128), or X^t is kept beside it (tiles of 64, which come
+// straight from memory).  Of a symmetric result the tiles on and above the diagonal are computed, and written twice.
+//
+// What bounds it, with the usual five steps (kernels' time of a call; the matrix cores reach 1.1 PFLOP/s of fp16, a copy
+// 4.7 TB/s): 4096 x 4096, 5.2 ms: the matrix cores, 3.4 ms of products at that rate, and the last 16 of 528 tiles after the
+// 512 that fill the card.  2048 x 2048, 0.98 ms: the same, at half the tiles.  The 73 matrices of a detector, 37.6 M
+// weights, 1.22 ms: a third the memory (norms 86 us, X 100, the last group's R X 207), the rest loads on their way between
+// matrix instructions.  A head's ten, 0.21 ms, and smaller lists: two dozen launches that wait for each other, 5 us at
+// least each.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -43,6 +50,7 @@ typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr float SCALE = 4096.f;  // what stored values are multiplied by
 constexpr float R_SCALE = 512.f; // ... of R
+constexpr int PAD = 128;         // rows and columns of X are multiples of it
 constexpr int WANT = 512;        // workgroups that fill the card
 
 struct Mat {  // one matrix, as the device's table holds it
@@ -61,10 +69,10 @@ __host__ __device__ inline int up(int v, int to) { return (v + to - 1) / to * to
 enum { SQ_A, SQ_FA, SQ_F, SQ_R = SQ_F + 2, SQ = SQ_R + 2 };  // (two of F, two of R)
 struct Dim {  // padded with zeros, which stay zeros
   int n, m, np, mp;
-  __host__ __device__ Dim(int rows, int cols, int pad) {
+  __host__ __device__ Dim(int rows, int cols) {
     n = rows < cols ? rows : cols;
     m = rows < cols ? cols : rows;
-    np = up(n, pad), mp = up(m, pad);
+    np = up(n, PAD), mp = up(m, PAD);
   }
   __host__ __device__ size_t x() const { return (size_t)np * mp; }
   __host__ __device__ size_t a() const { return (size_t)np * np; }
@@ -105,7 +113,7 @@ struct Lists {  // one entry a workgroup
   Tile* fill;       // 64 x 64 pieces of X
   uint2* norm_map;  // (matrix, chunk)
   unsigned n_gram, n_tri, n_rect, n_fill, n_norm;
-  int count, pad, gram_ts, tri_ts, rect_ts;
+  int count, gram_ts, tri_ts, rect_ts;
   int chunk;  // elements a workgroup of the norm's pass takes
 };
 
@@ -141,7 +149,8 @@ __device__ __forceinline__ void triangle(Tile& w, unsigned tile, unsigned wide) 
   w.i = i, w.j = i + tile;
 }
 // Workgroups go to the eight XCDs in turn, and each has an L2 of its own.  The u-th of n pieces of work is taken by that
-// workgroup which makes CHUNK neighbours share one: the tiles of a matrix read the same rows.
+// workgroup which makes CHUNK neighbours share one: the tiles of a matrix read the same rows (a head's X X^t: 12.5 us, 16.9
+// in turn; n x n products of a ragged list: 14.1, 17.2; 8 to 64 of them alike, but a long list's largest matrices on one XCD).
 constexpr unsigned XCDS = 8, CHUNK = 16;
 __device__ __forceinline__ unsigned entry(unsigned u, unsigned n) {
   const unsigned first = u / (XCDS * CHUNK) * (XCDS * CHUNK), v = u - first;
@@ -166,7 +175,7 @@ __global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
   };
   const auto begin = [&](unsigned k) {
     const Mat& t = b.m[k];
-    const Dim d(t.rows, t.cols, l.pad);
+    const Dim d(t.rows, t.cols);
     return Tile{t.at, 0, d.np, d.mp, 0, 0, 0, (unsigned short)t.splits, first + k};
   };
   if (within(&Mat::gram0)) {
@@ -367,7 +376,7 @@ __global__ __launch_bounds__(256) void ortho_start_kernel(Lists l, const double*
   const Mat t = l.table[w.mat];
   const Area o(base, w, l.rect_ts, 0);
   double s = 0;
-  const unsigned chunks = Dim(t.rows, t.cols, l.pad).norms(l.chunk);
+  const unsigned chunks = Dim(t.rows, t.cols).norms(l.chunk);
   for (unsigned i = threadIdx.x; i < chunks; i += 256) s += norms[t.norm0 + i];
   s = block_sum(s, sh);
   const double inv = (double)SCALE / (sqrt(s) + eps);
@@ -427,7 +436,7 @@ __device__ __forceinline__ void spill(const Acc& hh, const Acc& hl, float* E, fl
 // A tile of 128: a quarter a wavefront.  A stage is 32 of the summed index, whole blocks; it comes through registers into
 // shared memory, two stages in turn, two workgroups a compute unit.  The next stage's loads, the writes of the one before
 // it and the reads of the second piece lie between the matrix instructions, in an order that the scheduler is told:
-// left alone it reads an operand where it is needed and waits (4096 x 4096, R X: 395 us, 387 with it; 2048: 74, 61).
+// left alone it reads an operand where it is needed and waits (R X of 4096 x 4096: 395 us, 387 with it; of 2048 x 2048: 74, 61).
 // Nothing is conditional -- the last stage is loaded again where there is no next -- or the compiler could not count the
 // loads in flight and would wait for all of them.  (Loads straight into shared memory do not overlap: before any of it is
 // read, the compiler waits for every such load in flight.)  The 16-byte piece c of row r sits at c ^ (r / 4 % 4): sixteen
@@ -447,7 +456,9 @@ struct Core128 {
     size_t down;  // TURNED: 64 rows further in Q
   };
   static __device__ __forceinline__ int spot(int r, int c) { return r * 4 + (c ^ (r / 4 % 4)); }
-  // TURNED: Q's rows are the summed index.  32 of them lie in shared memory as they come, the 16-byte piece c of row k at
+  // TURNED: Q's rows are the summed index (R X: 390 us at 4096 x 4096 and 70 at 2048 x 2048, 388 and 66 from an X^t that
+  // has to be written and read beside X: the detector's matrices, 162 + 213 us for R X and 99 for the first X, so 184 + 215
+  // and 129).  32 of them lie in shared memory as they come, the 16-byte piece c of row k at
   // this place, and are turned by the reads of it: of sixteen lanes, four each name sixteen columns of a row, and each
   // receives four rows of a column.  Both ways go over all banks.
   static __device__ __forceinline__ int turned_spot(int k, int c) { return k * 16 + (c / 4 ^ k % 4) * 4 + (c % 4 ^ k / 4 % 4); }
@@ -618,7 +629,7 @@ __device__ __forceinline__ void store_gram(float* E, int np, const Area& o, int 
 }
 // A = X X^t: a tile on or above the diagonal, or one part of its sum, which ortho_sum_kernel adds up in their order.
 // (Adding them in the workgroup that ends last needs the other workgroups' tiles flushed through the XCDs' caches: 160 us
-// where this and the launch behind it take 20, at eight 256 x 2304 matrices.)
+// where this and the launch behind it take 17, at eight 256 x 2304 matrices.)
 template <int TS>
 __global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Lists l, _Float16* base, float* parts, int kc, int from) {
   __shared__ typename Core<TS>::Shared sh;
@@ -750,7 +761,7 @@ __global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* 
 
 // ------------------------------------------------------------------------------------------------ small matrices
 // A matrix of at most 64 x 128 stays in one workgroup's shared memory from the first step to the last, so that a list of such
-// is one launch instead of two dozen that wait for each other (64 x 64: XX us against 64).  One step at a time: X and X^t, A
+// is one launch instead of two dozen that wait for each other (64 x 64: 21 us against 127).  One step at a time: X and X^t, A
 // and F, each 32 x 32 of a product a wavefront.  A lane holds four neighbouring entries of a column of the product, which
 // are four of a row of X^t, or of A and F, which are symmetric.
 constexpr int SMALL_N = 64, SMALL_M = 128;
@@ -823,40 +834,35 @@ __device__ __forceinline__ void small_matrix(Small& sh, const Mat& t, const Mome
       in = r < t.rows && c < t.cols;
       return in ? (size_t)r * t.cols + c : 0;
     };
-    const auto read = [&](auto many) {  // (every load before the first use, inside or not)
-      float g[many()], u[many()];
-      bool in;
+    float u[EACH];  // (every load before the first use, inside or not)
+    bool in;
 #pragma unroll
-      for (int k = 0; k < many(); ++k) g[k] = (float)static_cast<const T*>(t.src)[at(k, in)];
+    for (int k = 0; k < EACH; ++k) v[k] = (float)static_cast<const T*>(t.src)[at(k, in)];
+    if (m.update) {
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) u[k] = t.buf[at(k, in)];
+    }
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      const size_t where = at(k, in);
       if (m.update) {
-#pragma unroll
-        for (int k = 0; k < many(); ++k) u[k] = t.buf[at(k, in)];
+        u[k] = fmaf(m.mu, u[k], v[k]);
+        if (in) t.buf[where] = u[k];
+        v[k] = m.nesterov ? fmaf(m.mu, u[k], v[k]) : u[k];
       }
-#pragma unroll
-      for (int k = 0; k < many(); ++k) {
-        const size_t where = at(k, in);
-        if (m.update) {
-          u[k] = fmaf(m.mu, u[k], g[k]);
-          if (in) t.buf[where] = u[k];
-          g[k] = m.nesterov ? fmaf(m.mu, u[k], g[k]) : u[k];
-        }
-        v[k] = in ? g[k] : 0.f;
-        s = fma((double)v[k], (double)v[k], s);
-      }
-    };
-    read(std::integral_constant<int, EACH>());
+      v[k] = in ? v[k] : 0.f;
+      s = fma((double)v[k], (double)v[k], s);
+    }
     s = block_sum(s, sh.norm);
     const double inv = (double)SCALE / (sqrt(s) + eps);
 #pragma unroll
     for (int k = 0; k < EACH; ++k) {
       const int e = k * 256 + threadIdx.x, r = e >> shift, c = e & ((1 << shift) - 1);
-      {
-        const int i = tall ? c : r, j = tall ? r : c;
-        _Float16 h, l;
-        split16((float)((double)v[k] * inv), h, l);
-        const size_t x = place(i, j, mp), y = place(j, i, 64);
-        sh.x[x] = h, sh.x[x + LO] = l, sh.xt[y] = h, sh.xt[y + LO] = l;
-      }
+      const int i = tall ? c : r, j = tall ? r : c;
+      _Float16 h, l;
+      split16((float)((double)v[k] * inv), h, l);
+      const size_t x = place(i, j, mp), y = place(j, i, 64);
+      sh.x[x] = h, sh.x[x + LO] = l, sh.xt[y] = h, sh.xt[y + LO] = l;
     }
   }
   __syncthreads();
@@ -871,11 +877,11 @@ __device__ __forceinline__ void small_matrix(Small& sh, const Mat& t, const Mome
   if (m.update) {
 #pragma unroll
     for (int h = 0; h < mp / 64; ++h)
-        small_fours(i, j + 64 * h, [&](int g, int r, int c) {
-          bool in;
+      small_fours(i, j + 64 * h, [&](int g, int r, int c) {
+        bool in;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) was[h][g][k] = out[target(r + k, c, in)];
-        });
+        for (int k = 0; k < 4; ++k) was[h][g][k] = out[target(r + k, c, in)];
+      });
   }
   float v[mp / 64][4][4];
   const int diagonal = i == j ? (lane & 31) - 4 * (lane >> 5) : -1;  // of this lane's column: its row less 4 (l / 32)
@@ -982,14 +988,15 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   }
   Lists& l = p.l;
   l = Lists{};
-  l.pad = 128;
   // Tiles: 128 needs half the reads of two operands that 64 does, and is taken for a pass that fills the card with such
-  // tiles.
+  // tiles; X X^t, in parts, and R X, with short sums, from half of that on.  The n x n products: at 528 tiles of 128
+  // (4096 x 4096) 273 us, 307 with four times as many of 64; at 292 (the detector's) 45, 35 so.  R X at 2616: 184 us, 256
+  // so; at 256 (2048 x 2048) 70, 71.  X X^t at 730 parts: 95 + 17 us, 113 + 6 so.
   uint64_t tri128 = 0, rect128 = 0, gram128 = 0, elements = 0;
   for (int i = 0; i < count; ++i) {
     if (is_small(rows[i], cols[i])) continue;
     ++l.count;
-    const Dim w(rows[i], cols[i], 128);
+    const Dim w(rows[i], cols[i]);
     elements += (uint64_t)rows[i] * cols[i];
     tri128 += w.tri(128), rect128 += w.rect(128);
     gram128 += (uint64_t)w.tri(128) * ((w.mp + 255) / 256);
@@ -1005,7 +1012,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
     uint64_t blocks = 0;
     for (int i = 0; i < count; ++i) {
       if (is_small(rows[i], cols[i])) continue;
-      const Dim d(rows[i], cols[i], l.pad);
+      const Dim d(rows[i], cols[i]);
       blocks += (uint64_t)d.tri(l.gram_ts) * ((d.mp + p.kc - 1) / p.kc);
     }
     if (blocks >= WANT) break;
@@ -1014,7 +1021,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   p.split = false;
   for (int i = 0; i < count; ++i) {
     if (is_small(rows[i], cols[i])) continue;
-    const Dim d(rows[i], cols[i], l.pad);
+    const Dim d(rows[i], cols[i]);
     const unsigned s = (unsigned)((d.mp + p.kc - 1) / p.kc);
     gram += (uint64_t)d.tri(l.gram_ts) * s;
     tri += d.tri(l.tri_ts);
@@ -1055,8 +1062,8 @@ struct Poly {
 };
 // Groups of steps: twos, the first a three where the number is odd; ones where R of a longer group might leave its range
 int group_length(int left, int steps) { return left == 1 ? 1 : (left == steps && left % 2 ? 3 : 2); }
-// The spectral norms of X, A, F A, F off the diagonal from |X| <= 1 on, step by step, with the polynomials' extremes in between (1 % over, for
-// the roundings).
+// The spectral norms of X, A, F A, F off the diagonal from |X| <= 1 on, step by step, with the polynomials' extremes in
+// between (1 % over, for the roundings).
 Poly polynomial(int steps, double a, double b, double c) {
   Poly r{(float)c, 0.f, (float)a, (float)b, 0};
   if (!(fabs(a) < 1e6) || !(fabs(b) < 1e6) || !(fabs(c) < 1e6)) return r;
@@ -1143,7 +1150,7 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
     const uint64_t was = (uint64_t)gram + tri + rect + fill + norm;
     for (; i < count && batch.count < BATCH; ++i) {
       if (is_small(rows[i], cols[i])) continue;
-      const Dim d(rows[i], cols[i], l.pad);
+      const Dim d(rows[i], cols[i]);
       const unsigned s = (unsigned)((d.mp + p.kc - 1) / p.kc);
       Mat& t = batch.m[batch.count++];
       t = matrix(i);

@@ -71,7 +71,7 @@ def offenders(rows):
 
 
 def main():
-    rows = collect()
+    rows = collect() + collect(os.path.join(CSRC, "train"))
     if not rows:
         print("no csrc/*.ru.txt: build the library first (make -C r3det-pytorch_amd/csrc)")
         return 2
