@@ -30,9 +30,9 @@
 // straight from memory).  Of a symmetric result the tiles on and above the diagonal are computed, and written twice.
 //
 // What bounds it, with the usual five steps (kernels' time of a call; the matrix cores reach 1.1 PFLOP/s of fp16, a copy
-// 4.7 TB/s): 4096 x 4096, 5.2 ms: the matrix cores, 3.4 ms of products at that rate, and the last 16 of 528 tiles after the
-// 512 that fill the card.  2048 x 2048, 0.98 ms: the same, at half the tiles.  The 73 matrices of a detector, 37.6 M
-// weights, 1.22 ms: a third the memory (norms 86 us, X 100, the last group's R X 207), the rest loads on their way between
+// 4.7 TB/s): 4096 x 4096, 4.7 ms: the matrix cores, 3.4 ms of products at that rate.  2048 x 2048, 0.98 ms: the same, with
+// fewer tiles than would keep them busy.  The 73 matrices of a detector, 37.6 M
+// weights, 1.21 ms: a third the memory (norms 86 us, X 100, the last group's R X 205), the rest loads on their way between
 // matrix instructions.  A head's ten, 0.21 ms, and smaller lists: two dozen launches that wait for each other, 5 us at
 // least each.
 #include <hip/hip_runtime.h>
@@ -88,6 +88,7 @@ struct Tile {  // one workgroup's work, with all that it needs of its matrix to 
   size_t part;  // X X^t in parts: where this one goes
   int np, mp;
   unsigned short i, j, split, splits;
+  unsigned short ts;  // 128 or 64 rows and columns (0: none), in units of which i and j are
   unsigned mat;
 };
 struct Area {  // where a matrix's arrays are
@@ -113,6 +114,7 @@ struct Lists {  // one entry a workgroup
   Tile* fill;       // 64 x 64 pieces of X
   uint2* norm_map;  // (matrix, chunk)
   unsigned n_gram, n_tri, n_rect, n_fill, n_norm;
+  unsigned whole_gram, whole_tri;  // tiles that are not quartered
   int count, gram_ts, tri_ts, rect_ts;
   int chunk;  // elements a workgroup of the norm's pass takes
 };
@@ -176,7 +178,21 @@ __global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
   const auto begin = [&](unsigned k) {
     const Mat& t = b.m[k];
     const Dim d(t.rows, t.cols);
-    return Tile{t.at, 0, d.np, d.mp, 0, 0, 0, (unsigned short)t.splits, first + k};
+    return Tile{t.at, 0, d.np, d.mp, 0, 0, 0, (unsigned short)t.splits, 0, first + k};
+  };
+  // the u-th tile of a triangle list, of n as they are and of 64 x 64 quarters behind those
+  const auto put = [&](Tile* list, Tile w, unsigned u, unsigned n, int ts) {
+    w.ts = ts;
+    if (u < n) {
+      list[entry(u, n)] = w;
+      return;
+    }
+    for (unsigned q = 0; q < 4; ++q) {
+      Tile v = w;
+      v.i = 2 * w.i + q / 2, v.j = 2 * w.j + q % 2;
+      v.ts = v.i <= v.j ? 64 : 0;
+      list[n + 4 * (u - n) + q] = v;
+    }
   };
   if (within(&Mat::gram0)) {
     const unsigned k = find(b, &Mat::gram0, e), local = e - b.m[k].gram0;
@@ -185,12 +201,12 @@ __global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
     triangle(w, tile, high);
     w.split = local / tiles;
     w.part = b.m[k].part0 + ((size_t)tile * w.splits + w.split) * (l.gram_ts * l.gram_ts);
-    l.gram[entry(e, l.n_gram)] = w;
+    put(l.gram, w, e, l.whole_gram, l.gram_ts);
   } else if (within(&Mat::tri0)) {
     const unsigned k = find(b, &Mat::tri0, e);
     Tile w = begin(k);
     triangle(w, e - b.m[k].tri0, w.np / l.tri_ts);
-    l.tri[entry(e, l.n_tri)] = w;
+    put(l.tri, w, e, l.whole_tri, l.tri_ts);
   } else if (within(&Mat::rect0)) {
     const unsigned k = find(b, &Mat::rect0, e), local = e - b.m[k].rect0;
     Tile w = begin(k);
@@ -439,8 +455,10 @@ __device__ __forceinline__ void spill(const Acc& hh, const Acc& hl, float* E, fl
 // left alone it reads an operand where it is needed and waits (R X of 4096 x 4096: 395 us, 387 with it; of 2048 x 2048: 74, 61).
 // Nothing is conditional -- the last stage is loaded again where there is no next -- or the compiler could not count the
 // loads in flight and would wait for all of them.  (Loads straight into shared memory do not overlap: before any of it is
-// read, the compiler waits for every such load in flight.)  The 16-byte piece c of row r sits at c ^ (r / 4 % 4): sixteen
-// rows that are read together then lie in different banks.
+// read, the compiler waits for every such load in flight.)  The 16-byte pieces of a row change places
+// with its number: sixteen rows that are read together lie in different banks, and so do eight that are written together
+// in the 32 banks that a write reaches at a time (no conflicts; a third of the cycles with the order that only the reads
+// need, X X^t of 4096 x 4096: 261 us, 255 so).
 struct Stage {
   half8 v[4][512];
 };
@@ -455,13 +473,13 @@ struct Core128 {
     const _Float16 *p[2], *q[2];
     size_t down;  // TURNED: 64 rows further in Q
   };
-  static __device__ __forceinline__ int spot(int r, int c) { return r * 4 + (c ^ (r / 4 % 4)); }
+  static __device__ __forceinline__ int spot(int r, int c) { return r * 4 + (c ^ (r / 4 % 2 + (r / 2 ^ r / 8) % 2 * 2)); }
   // TURNED: Q's rows are the summed index (R X: 390 us at 4096 x 4096 and 70 at 2048 x 2048, 388 and 66 from an X^t that
   // has to be written and read beside X: the detector's matrices, 162 + 213 us for R X and 99 for the first X, so 184 + 215
   // and 129).  32 of them lie in shared memory as they come, the 16-byte piece c of row k at
   // this place, and are turned by the reads of it: of sixteen lanes, four each name sixteen columns of a row, and each
   // receives four rows of a column.  Both ways go over all banks.
-  static __device__ __forceinline__ int turned_spot(int k, int c) { return k * 16 + (c / 4 ^ k % 4) * 4 + (c % 4 ^ k / 4 % 4); }
+  static __device__ __forceinline__ int turned_spot(int k, int c) { return k * 16 + (c / 4 ^ k % 4) * 4 + (c % 4 ^ (k / 4 % 2 + k / 2 % 2 * 2)); }
   template <bool TURNED>
   static __device__ __forceinline__ void fetch(half8 (&to)[8], const Source& s, int stage) {
     const size_t k = (size_t)stage * BLOCK + threadIdx.x * 8;
@@ -608,6 +626,11 @@ struct Core64 {
     __syncthreads();
   }
 };
+template <typename C, typename D>
+union Either {
+  typename C::Shared one;
+  typename D::Shared other;
+};
 template <int TS>
 using Core = std::conditional_t<TS == 128, Core128, Core64<4>>;
 
@@ -631,10 +654,7 @@ __device__ __forceinline__ void store_gram(float* E, int np, const Area& o, int 
 // (Adding them in the workgroup that ends last needs the other workgroups' tiles flushed through the XCDs' caches: 160 us
 // where this and the launch behind it take 17, at eight 256 x 2304 matrices.)
 template <int TS>
-__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Lists l, _Float16* base, float* parts, int kc, int from) {
-  __shared__ typename Core<TS>::Shared sh;
-  const Tile w = l.gram[blockIdx.x];
-  const Area o(base, w, l.rect_ts, from);
+__device__ __forceinline__ void gram_tile(typename Core<TS>::Shared& sh, const Tile& w, const Area& o, float* parts, int kc) {
   const int i0 = w.i * TS, j0 = w.j * TS;
   const int k0 = w.split * kc, k1 = k0 + kc < w.mp ? k0 + kc : w.mp;
   Core<TS>::run(sh, o.x, i0, w.mp, o.x, j0, w.mp, k0, k1, 1.f / SCALE);
@@ -650,6 +670,15 @@ __global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Lists l, _Float16* b
     return;
   }
   store_gram<TS, TS, Core<TS>::PARTS>(sh.E, w.np, o, i0, j0, w.i == w.j);
+}
+template <int TS>
+__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Lists l, _Float16* base, float* parts, int kc, int from) {
+  __shared__ Either<Core<TS>, Core64<4>> sh;
+  const Tile w = l.gram[blockIdx.x];
+  const Area o(base, w, l.rect_ts, from);
+  if (w.ts == TS) gram_tile<TS>(sh.one, w, o, parts, kc);
+  if constexpr (TS == 128)
+    if (w.ts == 64) gram_tile<64>(sh.other, w, o, parts, kc);
 }
 // 32 rows of a tile of A from its parts
 template <int TS>
@@ -682,12 +711,8 @@ struct Op {
   float t, q, l, f, fg, fh, fs, back;  // back: one over out's scale
 };
 template <typename C>
-__global__ __launch_bounds__(C::THREADS, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
+__device__ __forceinline__ void square_tile(typename C::Shared& sh, const Tile& w, const Area& o, const Op& op) {
   constexpr int TS = C::TS;
-  __shared__ typename C::Shared sh;
-  const Tile w = l.tri[blockIdx.x];
-  const Area o(base, w, l.rect_ts, 0);
-  const Op op = blockIdx.y ? second : first;
   const int i0 = w.i * TS, j0 = w.j * TS;
   const _Float16 *g = o.sq + op.g * o.na, *h = o.sq + op.h * o.na;
   const float *gd = o.diag + op.g * w.np, *hd = o.diag + op.h * w.np;
@@ -717,6 +742,16 @@ __global__ __launch_bounds__(C::THREADS, 2) void ortho_square_kernel(Lists l, _F
     __syncthreads();
     store_turned<TS, TS, TS + 1, C::THREADS>(sh.E, out, w.np, j0, i0);
   }
+}
+template <typename C>
+__global__ __launch_bounds__(C::THREADS, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
+  __shared__ Either<C, std::conditional_t<C::TS == 128, Core64<4>, C>> sh;
+  const Tile w = l.tri[blockIdx.x];
+  const Area o(base, w, l.rect_ts, 0);
+  const Op op = blockIdx.y ? second : first;
+  if (w.ts == C::TS) square_tile<C>(sh.one, w, o, op);
+  if constexpr (C::TS == 128)
+    if (w.ts == 64) square_tile<Core64<4>>(sh.other, w, o, op);
 }
 
 // X <- R X; the last group's goes to the caller, as the result or into the weights
@@ -1031,8 +1066,18 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
     if (s > 1) part += (uint64_t)d.tri(l.gram_ts) * s * l.gram_ts * l.gram_ts, p.split = true;
     halves += d.halves(l.rect_ts);
   }
+  // Whole tiles fill the card so many times; a few that are left would each keep a compute unit for a tile's time, alone,
+  // and are quartered (16 of 528, 4096 x 4096: an n x n product 275 -> 234 us, X X^t 255 -> 222).
+  const auto quarter = [](uint64_t& n, bool big) {
+    const unsigned rest = big && n >= WANT && n % WANT <= WANT / 4 ? (unsigned)(n % WANT) : 0;
+    const unsigned whole = (unsigned)n - rest;
+    n = whole + 4 * (uint64_t)rest;
+    return whole;
+  };
+  const uint64_t threads = gram + tri + rect + fill + norm;
+  if (threads > 0xffffff00) return -1;  // (of the lists' kernel)
+  l.whole_gram = quarter(gram, l.gram_ts == 128 && !p.split), l.whole_tri = quarter(tri, l.tri_ts == 128);
   if (gram > 0x7fffffff || tri > 0x7fffffff || rect > 0x7fffffff || fill > 0x7fffffff || norm > 0x7fffffff) return -1;
-  if (gram + tri + rect + fill + norm > 0xffffff00) return -1;  // (the lists' threads)
   l.n_gram = (unsigned)gram, l.n_tri = (unsigned)tri, l.n_rect = (unsigned)rect, l.n_fill = (unsigned)fill;
   l.n_norm = (unsigned)norm;
   size_t at = 0;

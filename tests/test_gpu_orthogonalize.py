@@ -104,6 +104,18 @@ def test_a_ragged_list_of_many():
     check([matrix(*s, seed=i) for i, s in enumerate(shapes)])
 
 
+@pytest.mark.parametrize("count", [170, 171, 172, 213, 214])
+def test_lists_that_just_fill_the_card(count):
+    """Three 128 x 128 tiles a symmetric matrix, 512 of which the card takes at a time: none, one, four, 127 and 130 are left."""
+    shapes = [(200, 300), (256, 129), (130, 140)]
+    check([matrix(*shapes[i % 3], seed=i) for i in range(count)])
+
+
+@pytest.mark.parametrize("shape", [(4100, 4300), (8200, 4097)], ids=str)
+def test_large(shape):
+    check([matrix(*shape, kind="low"), matrix(64, 64)])
+
+
 @pytest.mark.parametrize("steps,co,slope", [(1, COEFFICIENTS, 4.0), (2, COEFFICIENTS, 4.0), (10, COEFFICIENTS, 4.0),
                                             (12, (1.5, -0.5, 0.0), 1.5), (6, (15 / 8, -10 / 8, 3 / 8), 1.9)])
 def test_steps_and_coefficients(steps, co, slope):
