@@ -1041,16 +1041,30 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   l.rect_ts = rect128 >= WANT / 2 ? 128 : 64;
   // The norms: each thread 32 elements, fewer where that would leave compute units without work (2.6 M elements: 20 us, 6 so).
   for (l.chunk = 8192; l.chunk > 1024 && elements / l.chunk < 2 * WANT;) l.chunk /= 2;
-  // X X^t: the longest parts of the sum that still fill the card.  A part is a workgroup's time, so the parts of a ragged
-  // list are of like length, and a short list of wide matrices is spread.
-  for (p.kc = 4096; p.kc > 512; p.kc /= 2) {
-    uint64_t blocks = 0;
+  // Whole tiles fill the card so many times; a few that are left would each keep a compute unit for a tile's time, alone,
+  // and are quartered (16 of 528, 4096 x 4096: an n x n product 275 -> 234 us, X X^t 255 -> 222).
+  const auto quarter = [](uint64_t& n, bool big) {
+    const unsigned rest = big && n >= WANT && n % WANT <= WANT / 4 ? (unsigned)(n % WANT) : 0;
+    const unsigned whole = (unsigned)n - rest;
+    n = whole + 4 * (uint64_t)rest;
+    return whole;
+  };
+  // X X^t: how much of its sum a workgroup takes.  In stages' times: the card takes WANT workgroups at a time, with some 8
+  // in front of and behind their own; where there are parts, their sums are a launch (4) and pass over them (60 tiles of 128
+  // a stage).  (2048 x 2048: parts of 768, 41 + 11 us; of 512, 44 + 11.  The detector's: 768 too, 89 + 20; of 1024,
+  // 98 + 16; of 2048, 104 + 11.  4096 x 4096: whole, 222; of 1024, 231 + 38.)
+  uint64_t least = ~0ull;
+  for (int kc = 4096; kc >= 512; kc -= 128) {
+    uint64_t blocks = 0, whole = 0;
     for (int i = 0; i < count; ++i) {
       if (is_small(rows[i], cols[i])) continue;
       const Dim d(rows[i], cols[i]);
-      blocks += (uint64_t)d.tri(l.gram_ts) * ((d.mp + p.kc - 1) / p.kc);
+      blocks += (uint64_t)d.tri(l.gram_ts) * ((d.mp + kc - 1) / kc), whole += d.tri(l.gram_ts);
     }
-    if (blocks >= WANT) break;
+    const bool split = blocks > whole;
+    if (!split) blocks = quarter(blocks, l.gram_ts == 128);  // (the quarters are done by the way)
+    const uint64_t cost = (blocks + WANT - 1) / WANT * (kc / 32 + 8) + (split ? 4 + blocks / (l.gram_ts == 128 ? 60 : 240) : 0);
+    if (cost <= least) least = cost, p.kc = kc;
   }
   uint64_t gram = 0, tri = 0, rect = 0, fill = 0, norm = 0, part = 0, halves = 0;
   p.split = false;
@@ -1066,14 +1080,6 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
     if (s > 1) part += (uint64_t)d.tri(l.gram_ts) * s * l.gram_ts * l.gram_ts, p.split = true;
     halves += d.halves(l.rect_ts);
   }
-  // Whole tiles fill the card so many times; a few that are left would each keep a compute unit for a tile's time, alone,
-  // and are quartered (16 of 528, 4096 x 4096: an n x n product 275 -> 234 us, X X^t 255 -> 222).
-  const auto quarter = [](uint64_t& n, bool big) {
-    const unsigned rest = big && n >= WANT && n % WANT <= WANT / 4 ? (unsigned)(n % WANT) : 0;
-    const unsigned whole = (unsigned)n - rest;
-    n = whole + 4 * (uint64_t)rest;
-    return whole;
-  };
   const uint64_t threads = gram + tri + rect + fill + norm;
   if (threads > 0xffffff00) return -1;  // (of the lists' kernel)
   l.whole_gram = quarter(gram, l.gram_ts == 128 && !p.split), l.whole_tri = quarter(tri, l.tri_ts == 128);
