@@ -30,7 +30,7 @@
 // straight from memory).  Of a symmetric result the tiles on and above the diagonal are computed, and written twice.
 //
 // What bounds it, with the usual five steps (kernels' time of a call; the matrix cores reach 1.1 PFLOP/s of fp16, a copy
-// 4.7 TB/s): 4096 x 4096, 4.7 ms: the matrix cores, 3.4 ms of products at that rate.  2048 x 2048, 0.98 ms: the same, with
+// 4.7 TB/s): 4096 x 4096, 4.7 ms: the matrix cores, 3.75 ms of products at that rate.  2048 x 2048, 0.98 ms: the same, with
 // fewer tiles than would keep them busy.  The 73 matrices of a detector, 37.6 M
 // weights, 1.21 ms: a third the memory (norms 86 us, X 100, the last group's R X 205), the rest loads on their way between
 // matrix instructions.  A head's ten, 0.21 ms, and smaller lists: two dozen launches that wait for each other, 5 us at

@@ -108,6 +108,8 @@ class RRetinaHead(nn.Module):
         self.assigner = build_assigner(self.train_cfg['assigner'])
         self.bbox_coder = build_from(BBOX_CODERS, _cfg_dict(bbox_coder or dict(type='DeltaXYWHAOBBoxCoder')))
         self.loss_cls = build_loss(loss_cls)
+        if getattr(self.loss_cls, 'use_sigmoid', self.use_sigmoid_cls) != self.use_sigmoid_cls:
+            raise NotImplementedError(f'RRetinaHead: {type(self.loss_cls).__name__} is a sigmoid loss; say use_sigmoid=True')
         self.loss_bbox = build_loss(_cfg_dict(loss_bbox or dict(type='SmoothL1Loss', beta=0.11, loss_weight=1.0)))
         num_anchors = self.num_anchors
         self.cls_convs = nn.ModuleList()

@@ -47,6 +47,14 @@ def test_a_sampler_is_refused():
         head(train_cfg=dict(S0_TRAIN_CFG, sampler=dict(type='RandomSampler')))
 
 
+def test_a_sigmoid_loss_in_a_softmax_head_is_refused():
+    from r3det.models import RRetinaHead
+    with pytest.raises(NotImplementedError, match='use_sigmoid'):
+        RRetinaHead(loss_cls=dict(type='FocalLoss'))
+    with pytest.raises(NotImplementedError, match='softmax form'):
+        RRetinaHead(loss_cls=dict(type='CrossEntropyLoss', use_sigmoid=True))
+
+
 def test_calibration_refuses_softmax():
     from r3det.models import RRetinaNet
     from r3det.models.detectors import calibrate_score_bias
