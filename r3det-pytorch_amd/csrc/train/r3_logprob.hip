@@ -121,7 +121,10 @@ __device__ __forceinline__ float top_value(float x, float m, float ls) {
 
 // ---------------------------------------------------------------------------------------------- few classes
 // LANES neighbouring lanes hold a row in registers, E values a lane.  VEC: 16-byte loads (aligned rows of whole packs).
-// At 16 classes a row is one lane's four 16-byte loads, without an exchange between lanes.
+// Few lanes a row exchange less and keep its best alternatives cheap; many read and write whole lines together, which the
+// gradient needs most.  Values a lane, 4 / 8 / 16, us: forward 785664 x 16 fp32 17.6 / 14.4 / 16.8, 100000 x 32 7.8 / 7.0 /
+// 7.5, 100000 x 64 with the best four 21.7 / 16.1 / 15.0; gradient 392832 x 16 12.5 / 12.7 / 15.6, 200000 x 15 10.5 / 14.5 /
+// 22.4, 50000 x 81 10.8 / 9.6 / 11.2.
 template <typename T, int LANES, int E, bool VEC>
 __device__ __forceinline__ void load_row(const T* x, int lane, int64_t classes, float (&v)[E], int (&at)[E]) {
   constexpr int W = VEC ? (E * (int)sizeof(T) < 16 ? E : 16 / (int)sizeof(T)) : 1;
@@ -577,12 +580,9 @@ __global__ __launch_bounds__(256) void logprob_row_backward_kernel(const T* __re
   if (d_h) dh = d_h[row], h = o.entropy[row];
   if (d_top)
     for (int k = 0; k < o.k; ++k) sum += d_top[row * o.k + k];
-  const auto one = [&](float v, int64_t at) {
+  const auto one = [&](float v, int64_t at, float more) {
     const float lp = (v - m) - ls, p = __builtin_amdgcn_exp2f(lp * LOG2E);
-    float r = (at == y ? dl : 0.f) - p * (sum + dh * (fmaxf(lp, -150.f) + h));
-    if (d_top)
-      for (int k = 0; k < o.k; ++k)
-        if (o.top_ix[row * o.k + k] == at) r += d_top[row * o.k + k];
+    const float r = (at == y ? dl : 0.f) - p * (sum + dh * (fmaxf(lp, -150.f) + h)) + more;
     return (T)(empty ? 0.f : r);
   };
   const int64_t packs = (to - from) / W;
@@ -596,18 +596,35 @@ __global__ __launch_bounds__(256) void logprob_row_backward_kernel(const T* __re
       if (c + u * LANES < packs) {
         const int64_t at = from + (c + u * LANES) * W;
 #pragma unroll
-        for (int j = 0; j < W; ++j) p[u].v[j] = one((float)p[u].v[j], at + j);
+        for (int j = 0; j < W; ++j) p[u].v[j] = one((float)p[u].v[j], at + j, 0.f);
         __builtin_memcpy(out + at, &p[u], sizeof(p[u]));
       }
   }
   const int64_t i = from + packs * W + lane;
-  if (i < to) out[i] = one((float)x[i], i);  // (LANES >= W: one round)
+  if (i < to) out[i] = one((float)x[i], i, 0.f);  // (LANES >= W: one round)
+  if (d_top) {  // the best alternatives' own, written again behind the others (4096 x 65536, 8 of them: 1160 us looked for at
+                // every element, 394 so, 384 without any)
+    if constexpr (LANES == 256) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    for (int k = lane; k < o.k; k += LANES) {
+      const int64_t at = o.top_ix[row * o.k + k];
+      if (at >= from && at < to) out[at] = one((float)x[at], at, d_top[row * o.k + k]);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- launches
-constexpr int SMALL_MAX = 128;     // classes whose row lanes hold in registers
-constexpr int WAVE_MAX = 4096;     // classes that one wavefront walks
-constexpr int64_t PART = 32768;    // classes a workgroup walks at least, where a row is split
+// Rows of up to SMALL_MAX classes stay in registers (50000 x 128: 9.6 us, 29.6 if a wavefront walks each); up to WAVE_MAX a
+// wavefront walks one (300 x 4000 with the best eight: 13.8 us so, 9.1 by four or sixteen; 8000 x 1000: 17); longer ones
+// four wavefronts, or sixteen where those are a workgroup a compute unit at most (67 x 131072 with the best twenty: 34 and
+// 22 us; 8000 x 16000: 100 and 151).  A row is split where rows are fewer than compute units, into parts of PART at least
+// (one row of 1000000 with the best eight: 93 us whole, 19 so, 66 in parts of 8192, whose lists are many).
+constexpr int SMALL_MAX = 128, WAVE_MAX = 1024;
+constexpr int64_t PART = 32768;
 
 int row_split(int64_t rows, int64_t classes) {
   if (classes <= WAVE_MAX) return 1;
@@ -679,8 +696,8 @@ template <typename T>
 int forward(const T* x, int64_t rows, int64_t classes, int64_t stride, const Out& o, void* ws, hipStream_t st) {
   const int c = (int)classes;
   if (c <= 4) return small_forward<T, 1, 4>(x, rows, c, stride, o, st);
-  if (c <= 16) return small_forward<T, 1, 16>(x, rows, c, stride, o, st);
-  if (c <= 32) return small_forward<T, 2, 16>(x, rows, c, stride, o, st);
+  if (c <= 16) return small_forward<T, 2, 8>(x, rows, c, stride, o, st);
+  if (c <= 32) return small_forward<T, 4, 8>(x, rows, c, stride, o, st);
   if (c <= 64) return small_forward<T, 4, 16>(x, rows, c, stride, o, st);
   if (c <= SMALL_MAX) return small_forward<T, 8, 16>(x, rows, c, stride, o, st);
   if (c <= WAVE_MAX) return row_forward<T, 1>(x, rows, classes, stride, 1, nullptr, nullptr, o, st);
@@ -696,10 +713,10 @@ int backward(const T* x, int64_t rows, int64_t classes, int64_t stride, const Ou
              const float* d_top, T* dx, hipStream_t st) {
   const int c = (int)classes;
   if (c <= 4) return small_backward<T, 1, 4>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
-  if (c <= 16) return small_backward<T, 1, 16>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
-  if (c <= 32) return small_backward<T, 2, 16>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
-  if (c <= 64) return small_backward<T, 4, 16>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
-  if (c <= SMALL_MAX) return small_backward<T, 8, 16>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
+  if (c <= 16) return small_backward<T, 4, 4>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
+  if (c <= 32) return small_backward<T, 8, 4>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
+  if (c <= 64) return small_backward<T, 8, 8>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
+  if (c <= SMALL_MAX) return small_backward<T, 16, 8>(x, rows, c, stride, o, d_lp, d_h, d_top, dx, st);
   if (c <= WAVE_MAX) {
     const int64_t blocks = (rows + 3) / 4;
     if (blocks > 0x7fffffff) return -1;

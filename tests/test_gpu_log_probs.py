@@ -195,6 +195,14 @@ def test_nan_and_inf_stay_in_their_rows(classes):
     assert torch.isfinite(dx[clean]).all()
 
 
+@pytest.mark.parametrize("rows,classes", [(9, 4), (9, 5), (9, 15), (9, 32), (9, 33), (9, 64), (9, 65), (9, 128), (9, 129), (5, 1024),
+                                          (5, 1025), (3, 2047), (300, 1500), (3, 4096), (2, 33000), (1, 66000)])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_where_one_form_ends_and_the_next_begins(rows, classes, dtype):
+    x, y = logits(rows, classes, dtype)
+    check(x, y, k=min(classes, 9))
+
+
 @pytest.mark.parametrize("rows,classes", [(5, 1000), (5, 70001), (300, 6000), (2, 300000)])
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_few_classes_left_for_the_best_ones(rows, classes, dtype):
