@@ -145,10 +145,28 @@ __device__ __forceinline__ unsigned find(const Batch& b, unsigned Mat::* first, 
   }
   return lo;
 }
+// The tile-th of the tiles on and above the diagonal, `wide` by `wide` of them: in squares of SIDE, row by row of squares,
+// each row by row.
+constexpr unsigned SIDE = 8;
 __device__ __forceinline__ void triangle(Tile& w, unsigned tile, unsigned wide) {
-  unsigned i = 0;
-  while (tile >= wide - i) tile -= wide - i, ++i;  // (row i has wide - i tiles)
-  w.i = i, w.j = i + tile;
+  unsigned i = 0, j = 0;
+  for (;;) {  // the square whose first tile is (i, j)
+    const unsigned high = wide - i < SIDE ? wide - i : SIDE, across = wide - j < SIDE ? wide - j : SIDE;
+    const unsigned many = i == j ? high * (high + 1) / 2 : high * across;
+    if (tile < many) {
+      if (i == j) {
+        unsigned r = 0;
+        while (tile >= high - r) tile -= high - r, ++r;  // (row r has high - r tiles)
+        w.i = i + r, w.j = j + r + tile;
+      } else {
+        w.i = i + tile / across, w.j = j + tile % across;
+      }
+      return;
+    }
+    tile -= many;
+    j += SIDE;
+    if (j >= wide) i += SIDE, j = i;
+  }
 }
 // Workgroups go to the eight XCDs in turn, and each has an L2 of its own.  The u-th of n pieces of work is taken by that
 // workgroup which makes CHUNK neighbours share one: the tiles of a matrix read the same rows (a head's X X^t: 12.5 us, 16.9
