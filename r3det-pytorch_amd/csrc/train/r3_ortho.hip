@@ -363,31 +363,62 @@ __device__ __forceinline__ void store8(_Float16* at, const float (&v)[8]) {
   *reinterpret_cast<half8*>(at) = h;
   *reinterpret_cast<half8*>(at + LO) = l;
 }
-__device__ __forceinline__ void add8(float (&v)[8], float f, const _Float16* at) {
-  const half8 h = *reinterpret_cast<const half8*>(at), l = *reinterpret_cast<const half8*>(at + LO);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = fmaf(f, (float)h[k] + (float)l[k], v[k]);
+struct Both {
+  half8 h, l;
+  __device__ __forceinline__ float operator[](int k) const { return (float)h[k] + (float)l[k]; }
+};
+__device__ __forceinline__ Both load8(const _Float16* at) {
+  return Both{*reinterpret_cast<const half8*>(at), *reinterpret_cast<const half8*>(at + LO)};
 }
 // ROWS x COLS of fp32 in shared memory, rows of LD: f(row, column, eight values), which may change them; then `f`'s values
 // are in shared memory too.  PARTS > 1: the values are the sum of so many such arrays.  (Neighbouring threads have
 // neighbouring rows: the arrays' order, and LD is odd.)
-template <int ROWS, int COLS, int LD, int PARTS, int THREADS = 256, typename F>
+template <int LD, int PARTS, int STRIDE, typename F>
+__device__ __forceinline__ void eight(float* E, int r, int c, const F& f) {
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = E[r * LD + c + k];
+#pragma unroll
+  for (int s = 1; s < PARTS; ++s)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] += E[s * STRIDE + r * LD + c + k];
+  f(r, c, v);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) E[r * LD + c + k] = v[k];
+}
+template <int ROWS, int COLS, int LD, int PARTS, typename F>
 __device__ __forceinline__ void rows8(float* E, const F& f) {
 #pragma unroll 2
-  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += THREADS) {
-    const int r = q % ROWS, c = q / ROWS * 8;
-    float v[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = E[r * LD + c + k];
-#pragma unroll
-    for (int s = 1; s < PARTS; ++s)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] += E[s * ROWS * LD + r * LD + c + k];
-    f(r, c, v);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) E[r * LD + c + k] = v[k];
-  }
+  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += 256) eight<LD, PARTS, ROWS * LD>(E, q % ROWS, q / ROWS * 8, f);
 }
+// The same for a product's tile, where f takes what `load`(row, column) gives too: loaded for several rows at a time, the
+// first of them before the product's sums are in shared memory.  (What f stores could be what the next row loads, for all
+// that the compiler knows: it would wait for each.)
+template <typename C, typename Load>
+struct Rows {
+  static constexpr int N = C::TS * C::TS / 8 / C::THREADS, BATCH = N < 4 ? N : 4;
+  const Load& load;
+  decltype(load(0, 0)) d[BATCH];
+  __device__ __forceinline__ void fetch(int from) {
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const int q = (from + b) * C::THREADS + threadIdx.x;
+      d[b] = load(q % C::TS, q / C::TS * 8);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void run(float* E, const F& f) {
+    for (int from = 0; from < N; from += BATCH) {
+      if (from) fetch(from);
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        const int q = (from + b) * C::THREADS + threadIdx.x;
+        eight<C::LD, C::PARTS, C::TS * C::LD>(E, q % C::TS, q / C::TS * 8,
+                                              [&](int r, int c, float (&v)[8]) { f(r, c, v, d[b]); });
+      }
+    }
+  }
+};
 // The transpose of ROWS x COLS in shared memory -> an array of `ld` columns, at (r0, c0).
 template <int ROWS, int COLS, int LD, int THREADS = 256>
 __device__ __forceinline__ void store_turned(const float* E, _Float16* p, int ld, int r0, int c0) {
@@ -543,10 +574,10 @@ struct Core128 {
       }
     }
   }
-  // the tile times f in shared memory; TURNED: of P Q
-  template <bool TURNED = false>
+  // the tile times f in shared memory; TURNED: of P Q; `before` is called when the sums are done
+  template <bool TURNED = false, typename Before>
   static __device__ __forceinline__ void run(Shared& sh, const _Float16* p, int prow, int ldp, const _Float16* q, int qrow,
-                                             int ldq, int k0, int k1, float f) {
+                                             int ldq, int k0, int k1, float f, const Before& before) {
     Source src;
     src.down = (size_t)(ldq / 32) * BLOCK;
 #pragma unroll
@@ -593,6 +624,7 @@ struct Core128 {
       Stage* was = now;
       now = then, then = was;
     }
+    before();
     const int wave = threadIdx.x >> 6;
     spill<LD>(hh, hl, sh.E + (wave >> 1) * 64 * LD + (wave & 1) * 64, f);
     __syncthreads();
@@ -619,8 +651,9 @@ struct Core64 {
       f.ql[i] = *reinterpret_cast<const half8*>(q + k + i * 512 + LO);
     }
   }
+  template <typename Before>
   static __device__ __forceinline__ void run(Shared& sh, const _Float16* p, int prow, int ldp, const _Float16* q, int qrow,
-                                             int ldq, int k0, int k1, float f) {
+                                             int ldq, int k0, int k1, float f, const Before& before) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     p += place(prow, k0, ldp), q += place(qrow, k0, ldq);
     const int units = (k1 - k0) / (16 * WAVES), end = units - 1;  // of this wavefront
@@ -640,6 +673,7 @@ struct Core64 {
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
       if (s + u < units) multiply(hh, hl, piece[u]);
+    before();
     spill<LD>(hh, hl, sh.E + wave * TS * LD, f);
     __syncthreads();
   }
@@ -675,7 +709,7 @@ template <int TS>
 __device__ __forceinline__ void gram_tile(typename Core<TS>::Shared& sh, const Tile& w, const Area& o, float* parts, int kc) {
   const int i0 = w.i * TS, j0 = w.j * TS;
   const int k0 = w.split * kc, k1 = k0 + kc < w.mp ? k0 + kc : w.mp;
-  Core<TS>::run(sh, o.x, i0, w.mp, o.x, j0, w.mp, k0, k1, 1.f / SCALE);
+  Core<TS>::run(sh, o.x, i0, w.mp, o.x, j0, w.mp, k0, k1, 1.f / SCALE, [] {});
   if (w.splits > 1) {
     float* mine = parts + w.part;
 #pragma unroll 4
@@ -734,27 +768,36 @@ __device__ __forceinline__ void square_tile(typename C::Shared& sh, const Tile& 
   const int i0 = w.i * TS, j0 = w.j * TS;
   const _Float16 *g = o.sq + op.g * o.na, *h = o.sq + op.h * o.na;
   const float *gd = o.diag + op.g * w.np, *hd = o.diag + op.h * w.np;
-  C::run(sh, g, i0, w.np, h, j0, w.np, 0, w.np, 1.f);
+  struct Loaded {
+    Both g, h;
+    float gi, hj[8];
+  };
+  const auto load = [&](int r, int c) {
+    const size_t at = place(i0 + r, j0 + c, w.np);
+    Loaded d{load8(g + at), load8(h + at), gd[i0 + r]};
+    *reinterpret_cast<float4*>(d.hj) = *reinterpret_cast<const float4*>(hd + j0 + c);
+    *reinterpret_cast<float4*>(d.hj + 4) = *reinterpret_cast<const float4*>(hd + j0 + c + 4);
+    return d;
+  };
+  Rows<C, decltype(load)> rows{load};
+  C::run(sh, g, i0, w.np, h, j0, w.np, 0, w.np, 1.f, [&] { rows.fetch(0); });
   _Float16* out = o.sq + op.out * o.na;
   const bool diagonal = w.i == w.j;
-  rows8<TS, TS, TS + 1, C::PARTS, C::THREADS>(sh.E, [&](int r, int c, float (&v)[8]) {
+  rows.run(sh.E, [&](int r, int c, float (&v)[8], const Loaded& d) {
     const int i = i0 + r, j = j0 + c;
-    const size_t at = place(i, j, w.np);
-    const half8 gh = *reinterpret_cast<const half8*>(g + at), gl = *reinterpret_cast<const half8*>(g + at + LO);
-    const half8 hh = *reinterpret_cast<const half8*>(h + at), hl = *reinterpret_cast<const half8*>(h + at + LO);
-    const float gi = op.fh * (gd[i] - op.t);
+    const float gi = op.fh * (d.gi - op.t);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float hj = hd[j + k] - op.t;
-      float e = fmaf(fmaf(op.fg, hj, op.l), (float)gh[k] + (float)gl[k], op.fs * v[k]);
-      e = fmaf(gi, (float)hh[k] + (float)hl[k], e);
+      const float hj = d.hj[k] - op.t;
+      float e = fmaf(fmaf(op.fg, hj, op.l), d.g[k], op.fs * v[k]);
+      e = fmaf(gi, d.h[k], e);
       if (diagonal && i == j + k) {
-        o.diag[op.out * w.np + i] = fmaf(op.f * (gd[i] - op.t), hj, fmaf(op.l, gd[i], op.q)) + op.fs * op.back * v[k];
+        o.diag[op.out * w.np + i] = fmaf(op.f * (d.gi - op.t), hj, fmaf(op.l, d.gi, op.q)) + op.fs * op.back * v[k];
         e = 0.f;
       }
       v[k] = e;
     }
-    store8(out + at, v);
+    store8(out + place(i, j, w.np), v);
   });
   if (!diagonal) {
     __syncthreads();
@@ -781,12 +824,19 @@ __global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* 
   const Area o(base, w, TS, from);
   const int i0 = w.i * TS, j0 = w.j * TS;
   const _Float16* a = o.sq + R * o.na;
-  if constexpr (TS == 128) Core128::run<true>(sh, a, i0, w.np, o.x, j0, w.mp, 0, w.np, fs);
-  else Core<TS>::run(sh, a, i0, w.np, o.xt, j0, w.np, 0, w.np, fs);
-  rows8<TS, TS, TS + 1, Core<TS>::PARTS>(sh.E, [&](int r, int c, float (&v)[8]) {
-    const size_t at = place(i0 + r, j0 + c, w.mp);
-    add8(v, o.diag[R * w.np + i0 + r], o.x + at);
-    if constexpr (!LAST) store8(o.next + at, v);
+  struct Loaded {
+    Both x;
+    float d;
+  };
+  const auto load = [&](int r, int c) { return Loaded{load8(o.x + place(i0 + r, j0 + c, w.mp)), o.diag[R * w.np + i0 + r]}; };
+  Rows<Core<TS>, decltype(load)> rows{load};
+  const auto before = [&] { rows.fetch(0); };
+  if constexpr (TS == 128) Core128::run<true>(sh, a, i0, w.np, o.x, j0, w.mp, 0, w.np, fs, before);
+  else Core<TS>::run(sh, a, i0, w.np, o.xt, j0, w.np, 0, w.np, fs, before);
+  rows.run(sh.E, [&](int r, int c, float (&v)[8], const Loaded& d) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = fmaf(d.d, d.x[k], v[k]);
+    if constexpr (!LAST) store8(o.next + place(i0 + r, j0 + c, w.mp), v);
   });
   __syncthreads();
   if constexpr (!LAST) {
