@@ -59,8 +59,8 @@ struct Mat {  // one matrix, as the device's table holds it
   float* buf;        // the momentum (update only)
   int rows, cols;    // as the caller has it
   float rate;        // weights <- decay * weights - rate * result
-  unsigned short splits;  // parts of the sum of X X^t
-  unsigned short wide;    // whether four elements of a row are read and written as one
+  unsigned splits;   // parts of the sum of X X^t
+  unsigned wide;     // whether four elements of a row are read and written as one
   unsigned gram0, tri0, rect0, fill0, norm0;  // first entries in the lists, see Lists
   size_t part0;      // floats before this matrix's partial tiles
   size_t at;         // halves before this matrix's arrays
@@ -87,8 +87,8 @@ struct Tile {  // one workgroup's work, with all that it needs of its matrix to 
   size_t at;    // Mat::at
   size_t part;  // X X^t in parts: where this one goes
   int np, mp;
-  unsigned short i, j, split, splits;
-  unsigned short ts;  // 128 or 64 rows and columns (0: none), in units of which i and j are
+  unsigned i, j, split, splits;  // (whole words: scalar loads know no others)
+  unsigned ts;                   // 128 or 64 rows and columns (0: none), in units of which i and j are
   unsigned mat;
 };
 struct Area {  // where a matrix's arrays are
@@ -196,7 +196,7 @@ __global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
   const auto begin = [&](unsigned k) {
     const Mat& t = b.m[k];
     const Dim d(t.rows, t.cols);
-    return Tile{t.at, 0, d.np, d.mp, 0, 0, 0, (unsigned short)t.splits, 0, first + k};
+    return Tile{t.at, 0, d.np, d.mp, 0, 0, 0, t.splits, 0, first + k};
   };
   // the u-th tile of a triangle list, of n as they are and of 64 x 64 quarters behind those
   const auto put = [&](Tile* list, Tile w, unsigned u, unsigned n, int ts) {
@@ -244,9 +244,9 @@ __global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
 }
 
 // ------------------------------------------------------------------------------------------------ momentum, norm, X
-template <typename T>
-struct alignas(4 * sizeof(T)) Four {
-  T v[4];
+template <typename T, int N>
+struct alignas(N * sizeof(T)) Few {
+  T v[N];
 };
 // What is orthogonalised, N elements from i on (N = 4: as one, which Mat::wide allows): the matrix, or the gradient with the
 // momentum (new: after its update, which this is).
@@ -257,7 +257,7 @@ struct Momentum {
 template <typename T, int N, bool NEW>
 __device__ __forceinline__ void direction(float (&v)[N], const Mat& t, size_t i, const Momentum& m) {
   if constexpr (N == 4) {
-    const Four<T> g = *reinterpret_cast<const Four<T>*>(static_cast<const T*>(t.src) + i);
+    const Few<T, 4> g = *reinterpret_cast<const Few<T, 4>*>(static_cast<const T*>(t.src) + i);
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = (float)g.v[k];
   } else {
@@ -316,27 +316,31 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(Lists l, double* __rest
   s = block_sum(s, sh);
   if (threadIdx.x == 0) norms[blockIdx.x] = s;
 }
-// f(row and column of the caller's matrix, row and column of the TS x TS tile at (i0, j0), which of N the first is):
-// N = 4 along the caller's rows where that is allowed, else 1; TALL: the tile is of the transpose
-template <int TS, typename F>
-__device__ __forceinline__ void callers(const Mat& t, int i0, int j0, const F& f) {
+// A TS x TS tile at (i0, j0) in the caller's order, elements N at a time (a constant: 4 along the caller's rows where that is
+// allowed, else 1): x = load(N, place, whether it is inside), then f(N, place, inside, row and column in the tile of the
+// first, TALL, x).  TALL: the tile is of the transpose.  BATCH loads, then as many f.
+template <int TS, int BATCH, int N, typename Load, typename F>
+__device__ __forceinline__ void callers_by(const Mat& t, int i0, int j0, const Load& load, const F& f) {
+  const std::integral_constant<int, N> n;
   const bool tall = t.rows > t.cols;
   const int r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;
-  if (t.wide && t.cols % 4 == 0) {
-#pragma unroll 4
-    for (int q = threadIdx.x; q < TS * TS / 4; q += 256) {
-      const int r = q / (TS / 4), c = q % (TS / 4) * 4;
-      f(std::integral_constant<int, 4>(), (size_t)(r0 + r) * t.cols + c0 + c, r0 + r < t.rows && c0 + c < t.cols, tall ? c : r,
-        tall ? r : c, tall);
-    }
-  } else {
-#pragma unroll 4
-    for (int q = threadIdx.x; q < TS * TS; q += 256) {
-      const int r = q / TS, c = q % TS;
-      f(std::integral_constant<int, 1>(), (size_t)(r0 + r) * t.cols + c0 + c, r0 + r < t.rows && c0 + c < t.cols, tall ? c : r,
-        tall ? r : c, tall);
-    }
+  for (int from = 0; from < TS * TS / N; from += 256 * BATCH) {
+    decltype(load(n, 0, true)) x[BATCH];
+    const auto each = [&](int b, const auto& g) {
+      const int q = from + b * 256 + threadIdx.x, r = q / (TS / N), c = q % (TS / N) * N;
+      g((size_t)(r0 + r) * t.cols + c0 + c, r0 + r < t.rows && c0 + c < t.cols, tall ? c : r, tall ? r : c);
+    };
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) each(b, [&](size_t at, bool in, int, int) { x[b] = load(n, at, in); });
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) each(b, [&](size_t at, bool in, int r, int c) { f(n, at, in, r, c, tall, x[b]); });
   }
+}
+template <int TS, int BATCH, typename Load, typename F>
+__device__ __forceinline__ void callers(const Mat& t, int i0, int j0, const Load& load, const F& f) {
+  constexpr int FOURS = TS * TS / 4 / 256;
+  if (t.wide && t.cols % 4 == 0) callers_by<TS, (BATCH < FOURS ? BATCH : FOURS), 4>(t, i0, j0, load, f);
+  else callers_by<TS, BATCH, 1>(t, i0, j0, load, f);
 }
 
 __device__ __forceinline__ void split16(float v, _Float16& hi, _Float16& lo) {
@@ -446,12 +450,17 @@ __global__ __launch_bounds__(256) void ortho_start_kernel(Lists l, const double*
   s = block_sum(s, sh);
   const double inv = (double)SCALE / (sqrt(s) + eps);
   const int i0 = w.i * 64, j0 = w.j * 64;
-  callers<64>(t, i0, j0, [&](auto N, size_t at, bool in, int r, int c, bool tall) {
-    float v[N()];
-    direction<T, N(), false>(v, t, in ? at : 0, m);  // (inside or not, so that several are on their way)
+  callers<64, 4>(
+      t, i0, j0,
+      [&](auto N, size_t at, bool in) {  // (inside or not, so that several are on their way)
+        Few<float, N()> x;
+        direction<T, N(), false>(x.v, t, in ? at : 0, m);
+        return x;
+      },
+      [&](auto N, size_t, bool in, int r, int c, bool tall, const auto& x) {
 #pragma unroll
-    for (int k = 0; k < N(); ++k) E[(tall ? r + k : r) * 65 + (tall ? c : c + k)] = in ? (float)((double)v[k] * inv) : 0.f;
-  });
+        for (int k = 0; k < N(); ++k) E[(tall ? r + k : r) * 65 + (tall ? c : c + k)] = in ? (float)((double)x.v[k] * inv) : 0.f;
+      });
   __syncthreads();
   rows8<64, 64, 65, 1>(E, [&](int r, int c, float (&v)[8]) { store8(o.x + place(i0 + r, j0 + c, w.mp), v); });
   if (o.xt) store_turned<64, 64, 65>(E, o.xt, w.np, j0, i0);
@@ -844,21 +853,22 @@ __global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* 
   } else {
     const Mat t = l.table[w.mat];
     T* out = static_cast<T*>(t.dst);
-    callers<TS>(t, i0, j0, [&](auto N, size_t at, bool in, int r, int c, bool tall) {
-      if (!in) return;
-      float v[N()];
-      alignas(16) T x[N()];
+    callers<TS, 8>(
+        t, i0, j0,
+        [&](auto N, size_t at, bool in) {  // (the weights, inside or not: eight loads on their way)
+          Few<T, N()> x{};
+          if (update) x = *reinterpret_cast<const Few<T, N()>*>(out + (in ? at : 0));
+          return x;
+        },
+        [&](auto N, size_t at, bool in, int r, int c, bool tall, const auto& x) {
+          Few<T, N()> y;
 #pragma unroll
-      for (int k = 0; k < N(); ++k) v[k] = sh.E[(tall ? r + k : r) * (TS + 1) + (tall ? c : c + k)] * (1.f / SCALE);
-      if (update) {
-        if constexpr (N() == 4) *reinterpret_cast<Four<T>*>(x) = *reinterpret_cast<const Four<T>*>(out + at);
-        else x[0] = out[at];
-#pragma unroll
-        for (int k = 0; k < N(); ++k) v[k] = fmaf(-t.rate, v[k], decay * (float)x[k]);
-      }
-      if constexpr (N() == 4) *reinterpret_cast<Four<T>*>(out + at) = Four<T>{{(T)v[0], (T)v[1], (T)v[2], (T)v[3]}};
-      else out[at] = (T)v[0];
-    });
+          for (int k = 0; k < N(); ++k) {
+            const float v = sh.E[(tall ? r + k : r) * (TS + 1) + (tall ? c : c + k)] * (1.f / SCALE);
+            y.v[k] = (T)(update ? fmaf(-t.rate, v, decay * (float)x.v[k]) : v);
+          }
+          if (in) *reinterpret_cast<Few<T, N()>*>(out + at) = y;
+        });
   }
 }
 
@@ -1273,7 +1283,7 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
       const unsigned s = (unsigned)((d.mp + p.kc - 1) / p.kc);
       Mat& t = batch.m[batch.count++];
       t = matrix(i);
-      t.splits = (unsigned short)s;
+      t.splits = s;
       t.gram0 = gram, t.tri0 = tri, t.rect0 = rect, t.fill0 = fill, t.norm0 = norm, t.part0 = part, t.at = halves;
       gram += d.tri(l.gram_ts) * s;
       tri += d.tri(l.tri_ts);
