@@ -87,8 +87,8 @@ struct Tile {  // one workgroup's work, with all that it needs of its matrix to 
   size_t at;    // Mat::at
   size_t part;  // X X^t in parts: where this one goes
   int np, mp;
-  unsigned i, j, split, splits;  // (whole words: scalar loads know no others)
-  unsigned ts;                   // 128 or 64 rows and columns (0: none), in units of which i and j are
+  unsigned short i, j, split, splits;
+  unsigned short ts;  // 128 or 64 rows and columns (0: none), in units of which i and j are
   unsigned mat;
 };
 struct Area {  // where a matrix's arrays are
@@ -196,7 +196,7 @@ __global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
   const auto begin = [&](unsigned k) {
     const Mat& t = b.m[k];
     const Dim d(t.rows, t.cols);
-    return Tile{t.at, 0, d.np, d.mp, 0, 0, 0, t.splits, 0, first + k};
+    return Tile{t.at, 0, d.np, d.mp, 0, 0, 0, (unsigned short)t.splits, 0, first + k};
   };
   // the u-th tile of a triangle list, of n as they are and of 64 x 64 quarters behind those
   const auto put = [&](Tile* list, Tile w, unsigned u, unsigned n, int ts) {
