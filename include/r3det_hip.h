@@ -638,7 +638,8 @@ int r3det_fr_profile_read(float* records, int capacity);
  * All results fp32 / int64.  A logit of -inf is a class that is not offered; a row with no class left has log_prob and
  * top_log_prob -inf, entropy 0 and the gradient 0.  A row with NaN or +inf has NaN in place of its numbers; NaN is ranked
  * first.
- * The workspace (r3det_label_log_probs_workspace_bytes; 0 for all but few, long rows) need not be initialised. */
+ * The workspace (r3det_label_log_probs_workspace_bytes; 0 for all but few, long rows), 8-byte aligned, need not be
+ * initialised. */
 size_t r3det_label_log_probs_workspace_bytes(int64_t rows, int64_t classes, int top_k);
 int r3det_label_log_probs(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t row_stride,
                           const int64_t* labels, int64_t ignore_index, int has_ignore, int top_k, float* log_prob,

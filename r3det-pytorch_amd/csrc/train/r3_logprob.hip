@@ -748,6 +748,7 @@ int r3k_logprob(const void* x, int dtype, int64_t rows, int64_t classes, int64_t
   if (rows > (1ll << 40) || !x || stride < 0 || (labels && !log_prob) || (k && (!top_lp || !top_ix))) return -1;
   const size_t need = r3k_logprob_workspace_bytes(rows, classes, k);
   if (need && (!ws || ws_bytes < need)) return -3;
+  if (need && (reinterpret_cast<uintptr_t>(ws) & 7)) return -1;
   const Out o{labels, ignore, has_ignore, k, log_prob, entropy, top_lp, top_ix, stats};
   switch (dtype) {
     case 0: return forward(static_cast<const float*>(x), rows, classes, stride, o, ws, st);

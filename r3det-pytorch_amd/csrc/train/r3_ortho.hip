@@ -31,7 +31,7 @@
 //
 // What bounds it, with the usual five steps (kernels' time of a call; the matrix cores reach 1.1 PFLOP/s of fp16, a copy
 // 4.7 TB/s): 4096 x 4096, 4.6 ms: the matrix cores, 3.75 ms of products at that rate.  2048 x 2048, 0.95 ms: the same, with
-// fewer tiles than would keep them busy (0.47).  The 73 matrices of a detector, 37.6 M weights, 1.15 ms: a third the memory
+// fewer tiles than would keep them busy (0.47).  The 73 matrices of a detector, 41.9 M weights, 1.15 ms: a third the memory
 // (norms 86 us, X 100, the last group's R X 185), the rest loads on their way between matrix instructions.  A head's ten,
 // 0.19 ms, and smaller lists: two dozen launches that wait for each other, 5 us at least each.
 #include <hip/hip_runtime.h>
@@ -169,7 +169,8 @@ __device__ __forceinline__ void triangle(Tile& w, unsigned tile, unsigned wide) 
 }
 // Workgroups go to the eight XCDs in turn, and each has an L2 of its own.  The u-th of n pieces of work is taken by that
 // workgroup which makes CHUNK neighbours share one: the tiles of a matrix read the same rows (a head's X X^t: 12.5 us, 16.9
-// in the order as it comes; n x n products of a ragged list: 14.1, 17.2; 8 to 64 of them alike, but a long list's largest matrices on one XCD).
+// in the order as it comes; n x n products of a ragged list: 14.1, 17.2).  8, 32 and 64 of them do as well there, but 64 puts
+// a long list's largest matrices on one XCD.
 constexpr unsigned XCDS = 8, CHUNK = 16;
 __device__ __forceinline__ unsigned entry(unsigned u, unsigned n) {
   const unsigned first = u / (XCDS * CHUNK) * (XCDS * CHUNK), v = u - first;
@@ -536,7 +537,9 @@ struct Core128 {
   // 162 + 213 and 99.)  32 of them lie in shared memory as they come, the 16-byte piece c of row k at
   // this place, and are turned by the reads of it: of sixteen lanes, four each name sixteen columns of a row, and each
   // receives four rows of a column.  Both ways go over all banks.
-  static __device__ __forceinline__ int turned_spot(int k, int c) { return k * 16 + (c / 4 ^ k % 4) * 4 + (c % 4 ^ (k / 4 % 2 + k / 2 % 2 * 2)); }
+  static __device__ __forceinline__ int turned_spot(int k, int c) {
+    return k * 16 + (c / 4 ^ k % 4) * 4 + (c % 4 ^ (k / 4 % 2 + k / 2 % 2 * 2));
+  }
   template <bool TURNED>
   static __device__ __forceinline__ void fetch(half8 (&to)[8], const Source& s, int stage) {
     const size_t k = (size_t)stage * BLOCK + threadIdx.x * 8;
@@ -1102,8 +1105,8 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   l = Lists{};
   // Tiles: 128 needs half the reads of two operands that 64 does, and is taken for a pass that fills the card with such
   // tiles; X X^t, in parts, and R X, with short sums, from half of that on.  The n x n products: at 528 tiles of 128
-  // (4096 x 4096, none quartered) 273 us, 307 with four times as many of 64; at 292 (the detector's) 45, 35 so.  R X at 2616: 184 us, 256
-  // so; at 256 (2048 x 2048) 70, 71.  X X^t at 730 parts: 95 + 17 us, 113 + 6 so.
+  // (4096 x 4096, none quartered) 273 us, 307 with four times as many of 64; at 292 (the detector's) 45, 35 so.  R X at
+  // 2616: 184 us, 256 so; at 256 (2048 x 2048) 70, 71.  X X^t at 730 parts: 95 + 17 us, 113 + 6 so.
   uint64_t tri128 = 0, rect128 = 0, gram128 = 0, elements = 0;
   for (int i = 0; i < count; ++i) {
     if (is_small(rows[i], cols[i])) continue;
