@@ -33,7 +33,7 @@
 // 4.7 TB/s): 4096 x 4096, 4.6 ms: the matrix cores, 3.75 ms of products at that rate.  2048 x 2048, 0.95 ms: the same, with
 // fewer tiles than would keep them busy (0.47).  The 73 matrices of a detector, 41.9 M weights, 1.15 ms: a third the memory
 // (norms 86 us, X 100, the last group's R X 185), the rest loads on their way between matrix instructions.  A head's ten,
-// 0.19 ms, and smaller lists: two dozen launches that wait for each other, 5 us at least each.
+// 0.19 ms, and smaller lists: some twenty launches that wait for each other, 5 us at least each.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -767,25 +767,42 @@ __global__ __launch_bounds__(256) void ortho_sum_kernel(Lists l, _Float16* base,
   store_gram<32, TS, 1>(E, w.np, o, w.i * TS + slice, w.j * TS, w.i == w.j);
 }
 
-// out = q I + l G + f (G - t I) (H - t I) of symmetric matrices that commute (all are polynomials of one): a tile on or above
-// the diagonal.  The scales of what is stored are in the factors: out_ij = fh g_i H_ij + (fg h_j + l) G_ij + fs sum.
-struct Op {
-  int out, g, h;  // which arrays
-  float t, q, l, f, fg, fh, fs, back;  // back: one over out's scale
+// out = q I + l G + f (G - tg I) (H - th I) + m M of symmetric matrices that commute (all are polynomials of one): a tile on
+// or above the diagonal.  The scales of what is stored are in the factors of what lies off the diagonal:
+// out_ij = fh g_i H_ij + (fg h_j + lo) G_ij + mo M_ij + fs sum, with g = diag G - tg, h = diag H - th.  M where ADD.
+struct Stored {
+  int at;       // which array
+  float scale;  // what its entries off the diagonal are multiplied by
 };
-template <typename C>
+struct Op {
+  int out, g, h, m;
+  float tg, th, q, l, f, md, fg, fh, fs, lo, mo, back;  // back: one over out's scale
+  Op() = default;
+  Op(Stored o, Stored a, float ta, Stored b, float tb, float factor)
+      : out(o.at), g(a.at), h(b.at), m(a.at), tg(ta), th(tb), q(0.f), l(0.f), f(factor), md(0.f), fg(factor * (o.scale / a.scale)),
+        fh(factor * (o.scale / b.scale)), fs(factor * (o.scale / (a.scale * b.scale))), lo(0.f), mo(0.f), back(1.f / o.scale) {}
+  Op plus(Stored o, float factor, Stored matrix) const {
+    Op r = *this;
+    r.m = matrix.at, r.md = factor, r.mo = factor * (o.scale / matrix.scale);
+    return r;
+  }
+};
+template <typename C, bool ADD>
 __device__ __forceinline__ void square_tile(typename C::Shared& sh, const Tile& w, const Area& o, const Op& op) {
   constexpr int TS = C::TS;
   const int i0 = w.i * TS, j0 = w.j * TS;
   const _Float16 *g = o.sq + op.g * o.na, *h = o.sq + op.h * o.na;
   const float *gd = o.diag + op.g * w.np, *hd = o.diag + op.h * w.np;
+  const _Float16* m = o.sq + op.m * o.na;
   struct Loaded {
-    Both g, h;
-    float gi, hj[8];
+    Both g, h, m;
+    float gi, mi, hj[8];
   };
   const auto load = [&](int r, int c) {
     const size_t at = place(i0 + r, j0 + c, w.np);
-    Loaded d{load8(g + at), load8(h + at), gd[i0 + r]};
+    Loaded d;
+    d.g = load8(g + at), d.h = load8(h + at), d.gi = gd[i0 + r];
+    if constexpr (ADD) d.m = load8(m + at), d.mi = o.diag[op.m * w.np + i0 + r];
     *reinterpret_cast<float4*>(d.hj) = *reinterpret_cast<const float4*>(hd + j0 + c);
     *reinterpret_cast<float4*>(d.hj + 4) = *reinterpret_cast<const float4*>(hd + j0 + c + 4);
     return d;
@@ -796,14 +813,17 @@ __device__ __forceinline__ void square_tile(typename C::Shared& sh, const Tile& 
   const bool diagonal = w.i == w.j;
   rows.run(sh.E, [&](int r, int c, float (&v)[8], const Loaded& d) {
     const int i = i0 + r, j = j0 + c;
-    const float gi = op.fh * (d.gi - op.t);
+    const float gi = op.fh * (d.gi - op.tg);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float hj = d.hj[k] - op.t;
-      float e = fmaf(fmaf(op.fg, hj, op.l), d.g[k], op.fs * v[k]);
+      const float hj = d.hj[k] - op.th;
+      float e = fmaf(fmaf(op.fg, hj, op.lo), d.g[k], op.fs * v[k]);
       e = fmaf(gi, d.h[k], e);
+      if constexpr (ADD) e = fmaf(op.mo, d.m[k], e);
       if (diagonal && i == j + k) {
-        o.diag[op.out * w.np + i] = fmaf(op.f * (d.gi - op.t), hj, fmaf(op.l, d.gi, op.q)) + op.fs * op.back * v[k];
+        float y = fmaf(op.f * (d.gi - op.tg), hj, fmaf(op.l, d.gi, op.q)) + op.fs * op.back * v[k];
+        if constexpr (ADD) y = fmaf(op.md, d.mi, y);
+        o.diag[op.out * w.np + i] = y;
         e = 0.f;
       }
       v[k] = e;
@@ -815,15 +835,15 @@ __device__ __forceinline__ void square_tile(typename C::Shared& sh, const Tile& 
     store_turned<TS, TS, TS + 1, C::THREADS>(sh.E, out, w.np, j0, i0);
   }
 }
-template <typename C>
+template <typename C, bool ADD>
 __global__ __launch_bounds__(C::THREADS, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
   __shared__ Either<C, std::conditional_t<C::TS == 128, Core64<4>, C>> sh;
   const Tile w = l.tri[blockIdx.x];
   const Area o(base, w, l.rect_ts, 0);
   const Op op = blockIdx.y ? second : first;
-  if (w.ts == C::TS) square_tile<C>(sh.one, w, o, op);
+  if (w.ts == C::TS) square_tile<C, ADD>(sh.one, w, o, op);
   if constexpr (C::TS == 128)
-    if (w.ts == 64) square_tile<Core64<4>>(sh.other, w, o, op);
+    if (w.ts == 64) square_tile<Core64<4>, ADD>(sh.other, w, o, op);
 }
 
 // X <- R X; the last group's goes to the caller, as the result or into the weights
@@ -1190,13 +1210,14 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
 struct Poly {
   float c, t, q, l;
   int longest;  // group; 0: an iterate might leave fp16's range
+  bool brief;   // whether a group's steps can be taken in fewer launches: the products of that stay in range, too
 };
 // Groups of steps: twos, the first a three where the number is odd; ones where R of a longer group might leave its range
 int group_length(int left, int steps) { return left == 1 ? 1 : (left == steps && left % 2 ? 3 : 2); }
 // The spectral norms of X, A, F A, F off the diagonal from |X| <= 1 on, step by step, with the polynomials' extremes in
 // between (1 % over, for the roundings).
 Poly polynomial(int steps, double a, double b, double c) {
-  Poly r{(float)c, 0.f, (float)a, (float)b, 0};
+  Poly r{(float)c, 0.f, (float)a, (float)b, 0, false};
   if (!(fabs(a) < 1e6) || !(fabs(b) < 1e6) || !(fabs(c) < 1e6)) return r;
   const double most = 65504.0 / SCALE / 1.05;
   double t = 0, q = a, f = b;
@@ -1206,7 +1227,7 @@ Poly polynomial(int steps, double a, double b, double c) {
     c = (float)c;
     t = (float)(-b / (2 * c)), q = a - c * t * t, f = 0;
   }
-  double top = 1, high = 0;  // the largest |X|, and |F| so far
+  double top = 1, high = 0, most_a = 0;  // the largest |X|, and |F| and |A| so far
   for (int k = 0; k < steps; ++k) {
     const auto X = [&](double s) { return fabs(s * (a + s * s * (b + s * s * c))); };
     const auto Q = [&](double v) { return a + v * (b + v * c); };
@@ -1224,7 +1245,7 @@ Poly polynomial(int steps, double a, double b, double c) {
     }
     for (double v : z)
       if (v > 0 && v < t1) x = fmax(x, X(sqrt(v)));
-    high = fmax(high, now);
+    high = fmax(high, now), most_a = fmax(most_a, t1);
     if (!(t1 <= most) || !(x <= most) || !(x * top <= most) || !(e <= most)) return r;
     top = 1.01 * x;
   }
@@ -1232,6 +1253,7 @@ Poly polynomial(int steps, double a, double b, double c) {
   const double room = 65504.0 / R_SCALE / 1.05;  // R off its diagonal: that of R - q^g I
   q = fabs(q);
   r.longest = high * high * high + q * q * q <= room ? 3 : high * high + q * q <= room ? 2 : 1;
+  r.brief = f == 0 && r.longest == 3 && high * high * (most_a + fabs(t)) <= room;
   return r;
 }
 
@@ -1305,22 +1327,70 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
   hipLaunchKernelGGL((ortho_start_kernel<T>), dim3(l.n_fill), wg, 0, st, l, norms, base, m, eps);
   if (hipGetLastError() != hipSuccess) return -2;
   const unsigned cus = (unsigned)r3_cu_count();
-  const auto square = [&](const Op& one, const Op* two) {
+  const auto square = [&](const Op& one, const Op* two, bool add = false) {
     const dim3 grid(l.n_tri, two ? 2 : 1);
-    const auto launch = [&](auto core) {
+    const auto launch = [&](auto core, auto ADD) {
       typedef decltype(core) C;
-      hipLaunchKernelGGL((ortho_square_kernel<C>), grid, dim3(C::THREADS), 0, st, l, base, one, two ? *two : one);
+      hipLaunchKernelGGL((ortho_square_kernel<C, ADD()>), grid, dim3(C::THREADS), 0, st, l, base, one, two ? *two : one);
     };
     // A tile a compute unit: eight wavefronts share its sum and its epilogue (eight of 256 x 256: 7.3 us, four 8.4; more
     // tiles than that share the units anyway: 2048 x 2048, 56 against 53).
-    if (l.tri_ts == 128) launch(Core128());
-    else if (grid.x * grid.y <= cus) launch(Core64<8>());
-    else launch(Core64<4>());
+    if (l.tri_ts == 128) launch(Core128(), std::false_type());
+    else if (add) launch(Core64<8>(), std::true_type());
+    else if (grid.x * grid.y <= cus) launch(Core64<8>(), std::false_type());
+    else launch(Core64<4>(), std::false_type());
   };
-  // G H, stored 2^so times from 2^sg and 2^sh times
-  const auto times = [](int out, int g, int h, float so, float sg, float sh) {
-    return Op{out, g, h, 0.f, 0.f, 0.f, 1.f, so / sg, so / sh, so / (sg * sh), 1.f / so};
+  const auto both = [&](const Op& one, const Op& two, bool add = false) { square(one, &two, add); };
+  const auto polynomial_of = [&](Stored out, Stored a) {
+    Op r(out, a, f.t, a, f.t, f.c);
+    r.q = f.q, r.l = f.l, r.lo = f.l * (out.scale / a.scale);
+    return r;
   };
+  const auto times = [](Stored out, Stored g, Stored h) { return Op(out, g, 0.f, h, 0.f, 1.f); };
+  // R of a group of g steps, in launches of at most two products
+  const auto group = [&](int g) {
+    const Stored A{SQ_A, SCALE}, FA{SQ_FA, SCALE};
+    Stored R{SQ_F, SCALE}, spare{SQ_R, R_SCALE};
+    for (int k = 0; k < g; ++k) {
+      const Stored F{SQ_F + (k & 1), SCALE};
+      square(polynomial_of(F, A), nullptr);
+      if (k) {
+        const Op next = times(spare, F, R);
+        if (k + 1 < g) both(next, times(FA, F, A));
+        else square(next, nullptr);
+        R = spare, spare.at = SQ_R + (R.at == SQ_R);
+      } else if (k + 1 < g) {
+        square(times(FA, F, A), nullptr);
+      }
+      if (k + 1 < g) square(times(A, F, FA), nullptr);
+    }
+    return R;
+  };
+  // The same in one launch less for every step but the first, with a product more: where two products' tiles find a compute
+  // unit each, a launch is what counts (one head: 79 us of products, 86 as above; 1025 x 511: 96, 110).  With A' = F F A, the
+  // next step's A, and R so far:
+  //   A' R = (F A) (F R),  H = A' R - t R,  and the next R = F(A') R = q R + c (A' - t I) H.
+  const auto brief_group = [&](int g) {
+    const Stored A{SQ_A, SCALE}, FA{SQ_FA, SCALE};
+    Stored F{SQ_F, SCALE}, R = F, FR{SQ_R + 1, R_SCALE}, H{SQ_F + 1, R_SCALE}, next{SQ_R, R_SCALE};
+    square(polynomial_of(F, A), nullptr);
+    for (int k = 1; k < g; ++k) {
+      both(times(FA, F, A), times(FR, F, R));
+      both(times(A, F, FA), times(H, FA, FR).plus(H, -f.t, R), true);
+      const Op step = Op(next, A, f.t, H, 0.f, f.c).plus(next, f.q, R);
+      const Stored was = F;
+      if (k + 1 < g) {
+        F = Stored{FR.at, SCALE};
+        both(step, polynomial_of(F, A), true);
+        R = next, FR = Stored{was.at, R_SCALE}, next = Stored{F.at, R_SCALE};
+      } else {
+        square(step, nullptr, true);
+        R = next;
+      }
+    }
+    return R;
+  };
+  const bool brief = f.brief && l.tri_ts == 64 && 2 * l.n_tri <= cus;
   int from = 0;
   for (int left = steps; left > 0;) {
     int g = group_length(left, steps);
@@ -1329,30 +1399,15 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
       hipLaunchKernelGGL((ortho_gram_kernel<TS()>), dim3(l.n_gram), wg, 0, st, l, base, parts, p.kc, from);
       if (p.split) hipLaunchKernelGGL((ortho_sum_kernel<TS()>), dim3(l.n_gram, TS() / 32), wg, 0, st, l, base, parts);
     });
-    int R = SQ_F, spare = SQ_R;
-    float scale = SCALE;  // R's
-    for (int k = 0; k < g; ++k) {
-      const int F = SQ_F + (k & 1);
-      square(Op{F, SQ_A, SQ_A, f.t, f.q, f.l, f.c, f.c, f.c, f.c / SCALE, 1.f / SCALE}, nullptr);
-      const Op FA = times(SQ_FA, F, SQ_A, SCALE, SCALE, SCALE);
-      if (k) {
-        const Op next = times(spare, F, R, R_SCALE, SCALE, scale);
-        if (k + 1 < g) square(next, &FA);
-        else square(next, nullptr);
-        R = spare, spare = SQ_R + (R == SQ_R), scale = R_SCALE;
-      } else if (k + 1 < g) {
-        square(FA, nullptr);
-      }
-      if (k + 1 < g) square(times(SQ_A, F, SQ_FA, SCALE, SCALE, SCALE), nullptr);
-    }
+    const Stored R = brief ? brief_group(g) : group(g);
     left -= g;
-    const float fs = 1.f / scale;
+    const float fs = 1.f / R.scale;
     choose(l.rect_ts, [&](auto TS) {
       const dim3 grid(l.n_rect);
       if (left)
-        hipLaunchKernelGGL((ortho_apply_kernel<T, false, TS()>), grid, wg, 0, st, l, base, R, fs, from, update, decay);
+        hipLaunchKernelGGL((ortho_apply_kernel<T, false, TS()>), grid, wg, 0, st, l, base, R.at, fs, from, update, decay);
       else
-        hipLaunchKernelGGL((ortho_apply_kernel<T, true, TS()>), grid, wg, 0, st, l, base, R, fs, from, update, decay);
+        hipLaunchKernelGGL((ortho_apply_kernel<T, true, TS()>), grid, wg, 0, st, l, base, R.at, fs, from, update, decay);
     });
     from ^= 1;
     if (hipGetLastError() != hipSuccess) return -2;

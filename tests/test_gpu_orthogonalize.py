@@ -111,6 +111,14 @@ def test_lists_that_just_fill_the_card(count):
     check([matrix(*shapes[i % 3], seed=i) for i in range(count)])
 
 
+@pytest.mark.parametrize("kind", ["noise", "low"])
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("shape", [(300, 1025), (940, 1000), (1100, 1300), (2100, 1200)], ids=str)
+def test_products_by_one_and_by_two_a_launch(shape, steps, kind):
+    """The n x n products of 21 tiles of 64 go two to a launch where they can; those of 136, 171 and 210 where they must."""
+    check([matrix(*shape, kind=kind)], steps=steps)
+
+
 @pytest.mark.parametrize("shape", [(4100, 4300), (8200, 4097)], ids=str)
 def test_large(shape):
     check([matrix(*shape, kind="low"), matrix(64, 64)])
