@@ -46,6 +46,7 @@ namespace {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
+typedef float float4v __attribute__((ext_vector_type(4)));
 
 constexpr float SCALE = 4096.f;  // what stored values are multiplied by
 constexpr float R_SCALE = 512.f; // ... of R
@@ -280,12 +281,16 @@ __device__ __forceinline__ void direction(float (&v)[N], const Mat& t, size_t i,
 #pragma unroll
   for (int k = 0; k < N; ++k) v[k] = m.nesterov ? fmaf(m.mu, b[k], v[k]) : b[k];
 }
+template <int THREADS = 256>
 __device__ __forceinline__ double block_sum(double v, double* sh) {
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
   __syncthreads();
-  return (sh[0] + sh[1]) + (sh[2] + sh[3]);
+  v = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; w += 4) v += (sh[w] + sh[w + 1]) + (sh[w + 2] + sh[w + 3]);
+  return v;
 }
 // momentum <- mu momentum + gradient, and the squares of the direction summed in 64 bits (no scaling of the matrix is needed
 // against overflow, and the order of the sums is fixed)
@@ -896,44 +901,38 @@ __global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* 
 
 // ------------------------------------------------------------------------------------------------ small matrices
 // A matrix of at most 64 x 128 stays in one workgroup's shared memory from the first step to the last, so that a list of such
-// is one launch instead of two dozen that wait for each other (64 x 64: 21 us against 127).  One step at a time: X and X^t, A
-// and F, each 32 x 32 of a product a wavefront.  A lane holds four neighbouring entries of a column of the product, which
-// are four of a row of X^t, or of A and F, which are symmetric.
-constexpr int SMALL_N = 64, SMALL_M = 128;
+// is one launch instead of two dozen that wait for each other (64 x 64: 15 us against 127).  One step at a time: X and X^t,
+// A and F, each 16 x 16 of a product a wavefront (sixteen; four of 32 x 32 wait for each instruction by themselves: 23 us).
+// A lane holds four neighbouring entries of a column of the product, which are four of a row of X^t, or of A and F, which
+// are symmetric.
+constexpr int SMALL_N = 64, SMALL_M = 128, SMALL_THREADS = 1024;
 __host__ __device__ inline bool is_small(int rows, int cols) {
   return (rows < cols ? rows : cols) <= SMALL_N && (rows < cols ? cols : rows) <= SMALL_M;
 }
 struct Small {
   _Float16 x[SMALL_M / 32 * BLOCK], xt[SMALL_M / 32 * BLOCK], a[2 * BLOCK], f[2 * BLOCK];
   float da[64], df[64];
-  double norm[4];
+  double norm[SMALL_THREADS / 64];
 };
-// 32 x 32 at (i, j) of P Q^t over K columns, which both have
+// 16 x 16 at (i, j) of P Q^t over K columns, which both have
 template <int K>
-__device__ __forceinline__ float16v small_product(const _Float16* p, int i, const _Float16* q, int j) {
-  float16v hh = {}, hl = {}, lh = {};
-  const int lane8 = (threadIdx.x & 63) * 8;
-  half8 ph[K / 16], pl[K / 16], qh[K / 16], ql[K / 16];
+__device__ __forceinline__ float4v small_product(const _Float16* p, int i, const _Float16* q, int j) {
+  float4v hh = {}, hl = {}, lh = {};
+  const int lane = threadIdx.x & 63, r = lane & 15, c = 8 * (lane >> 4);
+  half8 ph[K / 32], pl[K / 32], qh[K / 32], ql[K / 32];
 #pragma unroll
-  for (int k = 0; k < K / 16; ++k) {
-    const _Float16 *u = p + place(i, k * 16, K) + lane8, *v = q + place(j, k * 16, K) + lane8;
+  for (int k = 0; k < K / 32; ++k) {
+    const _Float16 *u = p + place(i + r, k * 32 + c, K), *v = q + place(j + r, k * 32 + c, K);
     ph[k] = *reinterpret_cast<const half8*>(u), pl[k] = *reinterpret_cast<const half8*>(u + LO);
     qh[k] = *reinterpret_cast<const half8*>(v), ql[k] = *reinterpret_cast<const half8*>(v + LO);
   }
 #pragma unroll
-  for (int k = 0; k < K / 16; ++k) {  // (three chains: a matrix instruction waits for the one before it on the same sum)
-    hh = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[k], qh[k], hh, 0, 0, 0);
-    hl = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[k], ql[k], hl, 0, 0, 0);
-    lh = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[k], qh[k], lh, 0, 0, 0);
+  for (int k = 0; k < K / 32; ++k) {  // (three chains: a matrix instruction waits for the one before it on the same sum)
+    hh = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[k], qh[k], hh, 0, 0, 0);
+    hl = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[k], ql[k], hl, 0, 0, 0);
+    lh = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[k], qh[k], lh, 0, 0, 0);
   }
   return hh + (hl + lh);
-}
-// f(place among four, row, column) for the sixteen entries of a lane, four of a column at a time: each four then `done`
-template <typename F>
-__device__ __forceinline__ void small_fours(int i, int j, const F& f) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int g = 0; g < 4; ++g) f(g, i + 8 * g + 4 * (lane >> 5), j + (lane & 31));
 }
 __device__ __forceinline__ void put4(_Float16* at, const float (&v)[4]) {
   half4 h, l;
@@ -961,16 +960,15 @@ __device__ __forceinline__ void small_matrix(Small& sh, const Mat& t, const Mome
   const int shift = tall || mp == 64 ? 6 : 7;  // of the columns of the padded matrix as the caller has it
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   {
-    constexpr int EACH = SMALL_N * mp / 256;
-    float v[EACH];
+    constexpr int EACH = SMALL_N * mp / SMALL_THREADS;
+    float v[EACH], u[EACH];
     double s = 0;
     const auto at = [&](int k, bool& in) {
-      const int e = k * 256 + threadIdx.x, r = e >> shift, c = e & ((1 << shift) - 1);
+      const int e = k * SMALL_THREADS + threadIdx.x, r = e >> shift, c = e & ((1 << shift) - 1);
       in = r < t.rows && c < t.cols;
       return in ? (size_t)r * t.cols + c : 0;
     };
-    float u[EACH];  // (every load before the first use, inside or not)
-    bool in;
+    bool in;  // (every load before the first use, inside or not)
 #pragma unroll
     for (int k = 0; k < EACH; ++k) v[k] = (float)static_cast<const T*>(t.src)[at(k, in)];
     if (m.update) {
@@ -988,11 +986,11 @@ __device__ __forceinline__ void small_matrix(Small& sh, const Mat& t, const Mome
       v[k] = in ? v[k] : 0.f;
       s = fma((double)v[k], (double)v[k], s);
     }
-    s = block_sum(s, sh.norm);
+    s = block_sum<SMALL_THREADS>(s, sh.norm);
     const double inv = (double)SCALE / (sqrt(s) + eps);
 #pragma unroll
     for (int k = 0; k < EACH; ++k) {
-      const int e = k * 256 + threadIdx.x, r = e >> shift, c = e & ((1 << shift) - 1);
+      const int e = k * SMALL_THREADS + threadIdx.x, r = e >> shift, c = e & ((1 << shift) - 1);
       const int i = tall ? c : r, j = tall ? r : c;
       _Float16 h, l;
       split16((float)((double)v[k] * inv), h, l);
@@ -1001,109 +999,95 @@ __device__ __forceinline__ void small_matrix(Small& sh, const Mat& t, const Mome
     }
   }
   __syncthreads();
-  const int i = (wave >> 1) * 32, j = (wave & 1) * 32;
+  // this wavefront's 16 x 16 begin at (i, j); this lane's four at row r of column c
+  const int i = (wave >> 2) * 16, j = (wave & 3) * 16, r = i + 4 * (lane >> 4), c = j + (lane & 15);
   T* out = static_cast<T*>(t.dst);
-  const auto target = [&](int r, int c, bool& in) {
-    const int row = tall ? c : r, col = tall ? r : c;
+  const auto target = [&](int a, int b, bool& in) {
+    const int row = tall ? b : a, col = tall ? a : b;
     in = row < t.rows && col < t.cols;
     return in ? (size_t)row * t.cols + col : 0;
   };
-  T was[mp / 64][4][4];  // the weights: on their way while the steps are taken
+  T was[mp / 64][4];  // the weights: on their way while the steps are taken
   if (m.update) {
+    bool in;
 #pragma unroll
     for (int h = 0; h < mp / 64; ++h)
-      small_fours(i, j + 64 * h, [&](int g, int r, int c) {
-        bool in;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) was[h][g][k] = out[target(r + k, c, in)];
-      });
+      for (int k = 0; k < 4; ++k) was[h][k] = out[target(r + k, c + 64 * h, in)];
   }
-  float v[mp / 64][4][4];
-  const int diagonal = i == j ? (lane & 31) - 4 * (lane >> 5) : -1;  // of this lane's column: its row less 4 (l / 32)
+  float v[mp / 64][4];
+  const int diagonal = c - r;  // the place of this column's diagonal entry among the four, if it is one of them
+  const bool has = diagonal >= 0 && diagonal < 4;
   for (int step = 0;; ++step) {
     {
-      const float16v acc = small_product<mp>(sh.x, i, sh.x, j);
-      float d = 0.f;
-      small_fours(i, j, [&](int g, int r, int c) {
-        float a[4];
+      const float4v acc = small_product<mp>(sh.x, i, sh.x, j);
+      float a[4], d = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bool on = diagonal == 8 * g + k;
-          a[k] = acc[4 * g + k] * (1.f / SCALE);
-          d = on ? a[k] : d;
-          a[k] = on ? 0.f : a[k];
-        }
-        put4(sh.a + place(c, r, 64), a);
-      });
-      if (diagonal >= 0 && diagonal % 8 < 4) sh.da[j + (lane & 31)] = d * (1.f / SCALE);
+      for (int k = 0; k < 4; ++k) {
+        a[k] = acc[k] * (1.f / SCALE);
+        d = diagonal == k ? a[k] : d;
+        a[k] = diagonal == k ? 0.f : a[k];
+      }
+      put4(sh.a + place(c, r, 64), a);
+      if (has) sh.da[c] = d * (1.f / SCALE);
     }
     __syncthreads();
     {
-      const float16v acc = small_product<64>(sh.a, i, sh.a, j);
-      const float aj = sh.da[j + (lane & 31)], dj = aj - p.t, cs = p.c / SCALE;
-      float d = 0.f;
-      small_fours(i, j, [&](int g, int r, int c) {
-        float a[4];
-        get4(a, sh.a + place(c, r, 64));
+      const float4v acc = small_product<64>(sh.a, i, sh.a, j);
+      const float aj = sh.da[c], dj = aj - p.t, cs = p.c / SCALE;
+      float a[4], d = 0.f;
+      get4(a, sh.a + place(c, r, 64));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bool on = diagonal == 8 * g + k;
-          const float sum = cs * acc[4 * g + k];
-          a[k] = fmaf(fmaf(p.c, sh.da[r + k] - p.t + dj, p.l), a[k], sum);
-          d = on ? sum : d;
-          a[k] = on ? 0.f : a[k];
-        }
-        put4(sh.f + place(c, r, 64), a);
-      });
-      if (diagonal >= 0 && diagonal % 8 < 4)
-        sh.df[j + (lane & 31)] = fmaf(p.c * dj, dj, fmaf(p.l, aj, p.q)) + d * (1.f / SCALE);
+      for (int k = 0; k < 4; ++k) {
+        const float sum = cs * acc[k];
+        a[k] = fmaf(fmaf(p.c, sh.da[r + k] - p.t + dj, p.l), a[k], sum);
+        d = diagonal == k ? sum : d;
+        a[k] = diagonal == k ? 0.f : a[k];
+      }
+      put4(sh.f + place(c, r, 64), a);
+      if (has) sh.df[c] = fmaf(p.c * dj, dj, fmaf(p.l, aj, p.q)) + d * (1.f / SCALE);
     }
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < mp / 64; ++h) {
-      const float16v acc = small_product<64>(sh.f, i, sh.xt, j + 64 * h);
-      small_fours(i, j + 64 * h, [&](int g, int r, int c) {
-        float x[4];
-        get4(x, sh.xt + place(c, r, 64));
+      const float4v acc = small_product<64>(sh.f, i, sh.xt, j + 64 * h);
+      float x[4];
+      get4(x, sh.xt + place(c + 64 * h, r, 64));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[h][g][k] = fmaf(sh.df[r + k], x[k], acc[4 * g + k] * (1.f / SCALE));
-      });
+      for (int k = 0; k < 4; ++k) v[h][k] = fmaf(sh.df[r + k], x[k], acc[k] * (1.f / SCALE));
     }
     if (step + 1 == steps) break;
     __syncthreads();
 #pragma unroll
-    for (int h = 0; h < mp / 64; ++h)
-      small_fours(i, j + 64 * h, [&](int g, int r, int c) {
-        half4 hi, lo;
+    for (int h = 0; h < mp / 64; ++h) {
+      half4 hi, lo;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          _Float16 u, w;
-          split16(v[h][g][k], u, w);
-          hi[k] = u, lo[k] = w;
-        }
-        _Float16* at = sh.xt + place(c, r, 64);
-        *reinterpret_cast<half4*>(at) = hi;
-        *reinterpret_cast<half4*>(at + LO) = lo;
-        at = sh.x + place(r, c, mp);  // (rows of eight columns lie behind each other: r + 1 is 8 further)
+      for (int k = 0; k < 4; ++k) {
+        _Float16 u, w;
+        split16(v[h][k], u, w);
+        hi[k] = u, lo[k] = w;
+      }
+      _Float16* at = sh.xt + place(c + 64 * h, r, 64);
+      *reinterpret_cast<half4*>(at) = hi;
+      *reinterpret_cast<half4*>(at + LO) = lo;
+      at = sh.x + place(r, c + 64 * h, mp);  // (rows of eight columns lie behind each other: r + 1 is 8 further)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) at[8 * k] = hi[k], at[8 * k + LO] = lo[k];
-      });
+      for (int k = 0; k < 4; ++k) at[8 * k] = hi[k], at[8 * k + LO] = lo[k];
+    }
     __syncthreads();
   }
 #pragma unroll
   for (int h = 0; h < mp / 64; ++h)
-    small_fours(i, j + 64 * h, [&](int g, int r, int c) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        bool in;
-        const size_t at = target(r + k, c, in);
-        const float y = v[h][g][k] * (1.f / SCALE);
-        if (in) out[at] = (T)(m.update ? fmaf(-t.rate, y, decay * (float)was[h][g][k]) : y);
-      }
-    });
+    for (int k = 0; k < 4; ++k) {
+      bool in;
+      const size_t at = target(r + k, c + 64 * h, in);
+      const float y = v[h][k] * (1.f / SCALE);
+      if (in) out[at] = (T)(m.update ? fmaf(-t.rate, y, decay * (float)was[h][k]) : y);
+    }
 }
 template <typename T>
-__global__ __launch_bounds__(256) void ortho_small_kernel(Batch b, Momentum m, Step p, int steps, double eps, float decay) {
+__global__ __launch_bounds__(SMALL_THREADS) void ortho_small_kernel(Batch b, Momentum m, Step p, int steps, double eps, float decay) {
   __shared__ Small sh;
   const Mat t = b.m[blockIdx.x];
   if (t.rows <= 64 && t.cols <= 64) small_matrix<T, 64>(sh, t, m, p, steps, eps, decay);
@@ -1293,7 +1277,7 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
       for (; i < count && batch.count < BATCH; ++i)
         if (is_small(rows[i], cols[i])) batch.m[batch.count++] = matrix(i);
       if (batch.count)
-        hipLaunchKernelGGL((ortho_small_kernel<T>), dim3(batch.count), wg, 0, st, batch, m, Step{f.c, f.t, f.q, f.l}, steps, eps,
+        hipLaunchKernelGGL((ortho_small_kernel<T>), dim3(batch.count), dim3(SMALL_THREADS), 0, st, batch, m, Step{f.c, f.t, f.q, f.l}, steps, eps,
                            decay);
       if (hipGetLastError() != hipSuccess) return -2;
     }

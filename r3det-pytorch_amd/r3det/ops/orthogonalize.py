@@ -91,9 +91,9 @@ def orthogonalize(tensors, steps=STEPS, coefficients=COEFFICIENTS, eps=1e-7):
     return outs[0] if one else outs
 
 
-def _layout(t):
-    """The strides that say something (a dimension of size one has any)."""
-    return [s for s, n in zip(t.stride(), t.shape) if n > 1]
+def _alike(t, like):
+    """Whether two tensors of one shape have the same strides, where those say something (a dimension of size one has any)."""
+    return t.stride() == like.stride() or all(n < 2 or a == b for a, b, n in zip(t.stride(), like.stride(), t.shape))
 
 
 def _dense(t):
@@ -107,15 +107,16 @@ def _dense(t):
 
 def _apart(params, buffers, grads):
     """All matrices are updated at once: none may share memory with another, nor with a gradient."""
-    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in params + buffers]
-    spans.sort()
+    def span(t):
+        at = t.data_ptr()
+        return at, at + t.numel() * t.element_size()
+
+    spans = sorted(map(span, params + buffers))
     starts = [s[0] for s in spans]
     shared = any(a[1] > b for a, b in zip(spans, starts[1:]))
-    for g in () if shared else grads:
-        at = g.data_ptr()
-        i = bisect.bisect_right(starts, at)
-        if (i and spans[i - 1][1] > at) or (i < len(starts) and starts[i] < at + g.numel() * g.element_size()):
-            shared = True
+    for begin, end in () if shared else map(span, grads):
+        i = bisect.bisect_right(starts, begin)
+        shared = shared or (i > 0 and spans[i - 1][1] > begin) or (i < len(starts) and starts[i] < end)
     if shared:
         raise ValueError("the same weight or buffer comes twice, or shares memory with another one or with a gradient")
 
@@ -150,9 +151,9 @@ def orthogonal_update_(params, grads, buffers, lr, momentum=0.95, nesterov=True,
             raise RuntimeError(f"grads must be of their weight's type {p.dtype}, got {g.dtype}")
         if m.dtype != torch.float32:
             raise RuntimeError(f"buffers must be fp32, got {m.dtype}")
-        if not _dense(p) or (_layout(m) != _layout(p) and p.numel()):
+        if not _dense(p) or not (_alike(m, p) or p.numel() == 0):
             raise RuntimeError("params must be contiguous or channels_last, and their buffers laid out alike")
-    live = [(p, g, m, _layout(g) == _layout(p)) for p, g, m in zip(params, grads, buffers) if p.numel()]
+    live = [(p, g, m, _alike(g, p)) for p, g, m in zip(params, grads, buffers) if p.numel()]
     ps, ms = [t[0] for t in live], [t[2] for t in live]
     _apart(ps, ms, [g for _, g, _, alike in live if alike])
     _same(params, "params")
@@ -171,5 +172,4 @@ def orthogonal_update_(params, grads, buffers, lr, momentum=0.95, nesterov=True,
     _C.run_on(ps[0].device, "r3det_orthogonal_update", _C.lib().r3det_orthogonal_update, len(ps), _pointers(gs), _pointers(ps),
               _pointers(ms), DTYPES[ps[0].dtype], rows, cols, rates, 1.0 - lr * weight_decay, momentum, int(bool(nesterov)), steps,
               a, b, c, eps, ws.data_ptr(), n)
-    for t in ps + ms:
-        torch.autograd.graph.increment_version(t)
+    torch.autograd.graph.increment_version(ps + ms)
