@@ -23,7 +23,8 @@
 //   (G H)_ij = g_i H_ij + h_j G_ij + sum_k G_ik H_kj  with G and H without their diagonals,  (G H)_ii = g_i h_i + the sum.
 //
 // Stored values carry a power of two so that fp16 neither overflows -- spectral norms bound the entries, and the host checks
-// them for the given coefficients -- nor loses lo's bits: 2^12 for X, A, F, F A (norms below 15), 2^9 for R (below 120).
+// them for the given coefficients -- nor loses lo's bits: 2^12 for X, A, F, F A (norms below 15), 2^9 for R and what is made of it
+// (below 120).
 //
 // The matrix instructions want both operands with the summed index contiguous.  The symmetric matrices and X X^t have it;
 // for R X, X is turned on its way out of shared memory (tiles of 128), or X^t is kept beside it (tiles of 64, which come
@@ -125,6 +126,7 @@ struct Plan {
   Lists l;    // (sizes only)
   int kc;     // the summed index of X X^t a workgroup takes at most
   bool split; // whether any matrix has more than one part
+  int narrow; // the smallest n
 };
 
 // ------------------------------------------------------------------------------------------------ the lists
@@ -1107,6 +1109,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   }
   Lists& l = p.l;
   l = Lists{};
+  p.narrow = 1 << 30;
   // Tiles: 128 needs half the reads of two operands that 64 does, and is taken for a pass that fills the card with such
   // tiles; X X^t, in parts, and R X, with short sums, from half of that on.  The n x n products: at 528 tiles of 128
   // (4096 x 4096, none quartered) 273 us, 307 with four times as many of 64; at 292 (the detector's) 45, 35 so.  R X at
@@ -1116,6 +1119,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
     if (is_small(rows[i], cols[i])) continue;
     ++l.count;
     const Dim w(rows[i], cols[i]);
+    if (w.n < p.narrow) p.narrow = w.n;
     elements += (uint64_t)rows[i] * cols[i];
     tri128 += w.tri(128), rect128 += w.rect(128);
     gram128 += (uint64_t)w.tri(128) * ((w.mp + 255) / 256);
@@ -1375,9 +1379,16 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
     return R;
   };
   const bool brief = f.brief && l.tri_ts == 64 && 2 * l.n_tri <= cus;
+  // Where every pass has at most a tile a compute unit, the two passes over X are launches like the others: steps are taken
+  // one by one, if X X^t is a launch as well (250 x 250: 104 us, 111 in groups; 300 x 300: 117, 126) or a matrix is narrow.
+  // (In a group the next A is made of products, whose roundings the largest singular value carries over into the smallest
+  // ones' directions: with two rows, one 40 times the other, a group of three is off by 4e-5 where single steps are by 1e-6,
+  // as the form op by op in fp32 is.  With many rows that form's own error is as large.  60 x 4000: 116 us, 107.)
+  const bool one_by_one = l.gram_ts == 64 && l.tri_ts == 64 && l.rect_ts == 64 && l.n_gram <= cus && l.n_tri <= cus &&
+                          l.n_rect <= cus && (!p.split || p.narrow <= 128);
   int from = 0;
   for (int left = steps; left > 0;) {
-    int g = group_length(left, steps);
+    int g = one_by_one ? 1 : group_length(left, steps);
     if (g > f.longest) g = f.longest;
     choose(l.gram_ts, [&](auto TS) {
       hipLaunchKernelGGL((ortho_gram_kernel<TS()>), dim3(l.n_gram), wg, 0, st, l, base, parts, p.kc, from);
