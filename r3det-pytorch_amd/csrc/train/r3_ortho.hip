@@ -61,7 +61,6 @@ struct Mat {  // one matrix, as the device's table holds it
   int rows, cols;    // as the caller has it
   float rate;        // weights <- decay * weights - rate * result
   unsigned splits;   // parts of the sum of X X^t
-  unsigned wide;     // whether four elements of a row are read and written as one
   unsigned gram0, tri0, rect0, fill0, norm0;  // first entries in the lists, see Lists
   size_t part0;      // floats before this matrix's partial tiles
   size_t at;         // halves before this matrix's arrays
@@ -247,41 +246,41 @@ __global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
 }
 
 // ------------------------------------------------------------------------------------------------ momentum, norm, X
+// N elements as one, from an address that is aligned to one of them: global accesses need no more.
 template <typename T, int N>
-struct alignas(N * sizeof(T)) Few {
+struct Few {
   T v[N];
 };
-// What is orthogonalised, N elements from i on (N = 4: as one, which Mat::wide allows): the matrix, or the gradient with the
-// momentum (new: after its update, which this is).
+template <typename T, int N>
+__device__ __forceinline__ Few<T, N> load_few(const T* at) {
+  Few<T, N> x;
+  __builtin_memcpy(&x, at, sizeof(x));
+  return x;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_few(T* at, const Few<T, N>& x) {
+  __builtin_memcpy(at, &x, sizeof(x));
+}
+// What is orthogonalised, N elements from i on: the matrix, or the gradient with the momentum (new: after its update, which
+// this is).
 struct Momentum {
   int update, nesterov;
   float mu;
 };
 template <typename T, int N, bool NEW>
 __device__ __forceinline__ void direction(float (&v)[N], const Mat& t, size_t i, const Momentum& m) {
-  if constexpr (N == 4) {
-    const Few<T, 4> g = *reinterpret_cast<const Few<T, 4>*>(static_cast<const T*>(t.src) + i);
+  const Few<T, N> g = load_few<T, N>(static_cast<const T*>(t.src) + i);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = (float)g.v[k];
-  } else {
-    v[0] = (float)static_cast<const T*>(t.src)[i];
-  }
+  for (int k = 0; k < N; ++k) v[k] = (float)g.v[k];
   if (!m.update) return;
-  float b[N];
-  if constexpr (N == 4) {
-    const float4 u = *reinterpret_cast<const float4*>(t.buf + i);
-    b[0] = u.x, b[1] = u.y, b[2] = u.z, b[3] = u.w;
-  } else {
-    b[0] = t.buf[i];
-  }
+  Few<float, N> b = load_few<float, N>(t.buf + i);
   if constexpr (NEW) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) b[k] = fmaf(m.mu, b[k], v[k]);
-    if constexpr (N == 4) *reinterpret_cast<float4*>(t.buf + i) = make_float4(b[0], b[1], b[2], b[3]);
-    else t.buf[i] = b[0];
+    for (int k = 0; k < N; ++k) b.v[k] = fmaf(m.mu, b.v[k], v[k]);
+    store_few(t.buf + i, b);
   }
 #pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = m.nesterov ? fmaf(m.mu, b[k], v[k]) : b[k];
+  for (int k = 0; k < N; ++k) v[k] = m.nesterov ? fmaf(m.mu, b.v[k], v[k]) : b.v[k];
 }
 template <int THREADS = 256>
 __device__ __forceinline__ double block_sum(double v, double* sh) {
@@ -304,18 +303,14 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(Lists l, double* __rest
   const size_t all = (size_t)t.rows * t.cols, from = (size_t)w.y * l.chunk;
   const int many = (int)(from + l.chunk < all ? l.chunk : all - from);
   double s = 0;
-  int i = threadIdx.x;
-  if (t.wide) {
 #pragma unroll 4
-    for (int q = threadIdx.x; q < many / 4; q += 256) {
-      float v[4];
-      direction<T, 4, true>(v, t, from + 4 * q, m);
+  for (int q = threadIdx.x; q < many / 4; q += 256) {
+    float v[4];
+    direction<T, 4, true>(v, t, from + 4 * q, m);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s = fma((double)v[k], (double)v[k], s);
-    }
-    i += many / 4 * 4;
+    for (int k = 0; k < 4; ++k) s = fma((double)v[k], (double)v[k], s);
   }
-  for (; i < many; i += 256) {
+  for (int i = many / 4 * 4 + threadIdx.x; i < many; i += 256) {
     float v[1];
     direction<T, 1, true>(v, t, from + i, m);
     s = fma((double)v[0], (double)v[0], s);
@@ -323,31 +318,53 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(Lists l, double* __rest
   s = block_sum(s, sh);
   if (threadIdx.x == 0) norms[blockIdx.x] = s;
 }
-// A TS x TS tile at (i0, j0) in the caller's order, elements N at a time (a constant: 4 along the caller's rows where that is
-// allowed, else 1): x = load(N, place, whether it is inside), then f(N, place, inside, row and column in the tile of the
-// first, TALL, x).  TALL: the tile is of the transpose.  BATCH loads, then as many f.
-template <int TS, int BATCH, int N, typename Load, typename F>
+// A TS x TS tile at (i0, j0) in the caller's order, elements N at a time along the caller's rows (a constant: 4, or 1 where a
+// row has fewer): x = load(N, place, how many are inside), then f(N, place, how many, row and column in the tile of the
+// first, TALL, x).  TALL: the tile is of the transpose.  BATCH loads, then as many f.  PARTS: N may be cut by the row's end.
+template <int N, bool PARTS>
+struct Many {
+  static constexpr bool parts = PARTS;
+  __device__ constexpr int operator()() const { return N; }
+};
+template <int TS, int BATCH, int N, bool PARTS, typename Load, typename F>
 __device__ __forceinline__ void callers_by(const Mat& t, int i0, int j0, const Load& load, const F& f) {
-  const std::integral_constant<int, N> n;
+  const Many<N, PARTS> n;
   const bool tall = t.rows > t.cols;
   const int r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;
   for (int from = 0; from < TS * TS / N; from += 256 * BATCH) {
-    decltype(load(n, 0, true)) x[BATCH];
+    decltype(load(n, 0, 0)) x[BATCH];
     const auto each = [&](int b, const auto& g) {
-      const int q = from + b * 256 + threadIdx.x, r = q / (TS / N), c = q % (TS / N) * N;
-      g((size_t)(r0 + r) * t.cols + c0 + c, r0 + r < t.rows && c0 + c < t.cols, tall ? c : r, tall ? r : c);
+      const int q = from + b * 256 + threadIdx.x, r = q / (TS / N), c = q % (TS / N) * N, left = t.cols - (c0 + c);
+      g((size_t)(r0 + r) * t.cols + c0 + c, r0 + r < t.rows && left > 0 ? (left < N ? left : N) : 0, tall ? c : r, tall ? r : c);
     };
 #pragma unroll
-    for (int b = 0; b < BATCH; ++b) each(b, [&](size_t at, bool in, int, int) { x[b] = load(n, at, in); });
+    for (int b = 0; b < BATCH; ++b) each(b, [&](size_t at, int many, int, int) { x[b] = load(n, at, many); });
 #pragma unroll
-    for (int b = 0; b < BATCH; ++b) each(b, [&](size_t at, bool in, int r, int c) { f(n, at, in, r, c, tall, x[b]); });
+    for (int b = 0; b < BATCH; ++b) each(b, [&](size_t at, int many, int r, int c) { f(n, at, many, r, c, tall, x[b]); });
   }
 }
 template <int TS, int BATCH, typename Load, typename F>
 __device__ __forceinline__ void callers(const Mat& t, int i0, int j0, const Load& load, const F& f) {
   constexpr int FOURS = TS * TS / 4 / 256;
-  if (t.wide && t.cols % 4 == 0) callers_by<TS, (BATCH < FOURS ? BATCH : FOURS), 4>(t, i0, j0, load, f);
-  else callers_by<TS, BATCH, 1>(t, i0, j0, load, f);
+  constexpr int EACH = BATCH < FOURS ? BATCH : FOURS;
+  if (t.cols % 4 == 0) callers_by<TS, EACH, 4, false>(t, i0, j0, load, f);
+  else if (t.cols >= 4) callers_by<TS, EACH, 4, true>(t, i0, j0, load, f);
+  else callers_by<TS, BATCH, 1, false>(t, i0, j0, load, f);
+}
+// What `many` elements of N at `at` are read from, whole and inside the row: so many places before as are missing (0:
+// anywhere, from the array's beginning); then they are the last of the N read.
+template <typename N>
+__device__ __forceinline__ size_t whole(const N& n, size_t at, int many) {
+  return many ? at - (N::parts ? n() - many : 0) : 0;
+}
+template <typename N, typename T, int COUNT>
+__device__ __forceinline__ void to_front(const N&, T (&v)[COUNT], int many) {
+  if constexpr (N::parts) {
+    const T a = v[1], b = v[2], c = v[3];
+    v[0] = many == 3 ? a : many == 2 ? b : many == 1 ? c : v[0];
+    v[1] = many == 3 ? b : many == 2 ? c : a;
+    v[2] = many == 3 ? c : b;
+  }
 }
 
 __device__ __forceinline__ void split16(float v, _Float16& hi, _Float16& lo) {
@@ -459,14 +476,16 @@ __global__ __launch_bounds__(256) void ortho_start_kernel(Lists l, const double*
   const int i0 = w.i * 64, j0 = w.j * 64;
   callers<64, 4>(
       t, i0, j0,
-      [&](auto N, size_t at, bool in) {  // (inside or not, so that several are on their way)
+      [&](auto N, size_t at, int many) {  // (inside or not, so that several are on their way)
         Few<float, N()> x;
-        direction<T, N(), false>(x.v, t, in ? at : 0, m);
+        direction<T, N(), false>(x.v, t, whole(N, at, many), m);
+        to_front(N, x.v, many);
         return x;
       },
-      [&](auto N, size_t, bool in, int r, int c, bool tall, const auto& x) {
+      [&](auto N, size_t, int many, int r, int c, bool tall, const auto& x) {
 #pragma unroll
-        for (int k = 0; k < N(); ++k) E[(tall ? r + k : r) * 65 + (tall ? c : c + k)] = in ? (float)((double)x.v[k] * inv) : 0.f;
+        for (int k = 0; k < N(); ++k)
+          E[(tall ? r + k : r) * 65 + (tall ? c : c + k)] = (decltype(N)::parts ? k < many : many != 0) ? (float)((double)x.v[k] * inv) : 0.f;
       });
   __syncthreads();
   rows8<64, 64, 65, 1>(E, [&](int r, int c, float (&v)[8]) { store8(o.x + place(i0 + r, j0 + c, w.mp), v); });
@@ -884,19 +903,24 @@ __global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* 
     T* out = static_cast<T*>(t.dst);
     callers<TS, 8>(
         t, i0, j0,
-        [&](auto N, size_t at, bool in) {  // (the weights, inside or not: eight loads on their way)
+        [&](auto N, size_t at, int many) {  // (the weights, inside or not: eight loads on their way)
           Few<T, N()> x{};
-          if (update) x = *reinterpret_cast<const Few<T, N()>*>(out + (in ? at : 0));
+          if (update) x = load_few<T, N()>(out + whole(N, at, many));
           return x;
         },
-        [&](auto N, size_t at, bool in, int r, int c, bool tall, const auto& x) {
-          Few<T, N()> y;
+        [&](auto N, size_t at, int many, int r, int c, bool tall, const auto& was) {
+          Few<T, N()> x = was, y;
+          to_front(N, x.v, many);
 #pragma unroll
           for (int k = 0; k < N(); ++k) {
             const float v = sh.E[(tall ? r + k : r) * (TS + 1) + (tall ? c : c + k)] * (1.f / SCALE);
             y.v[k] = (T)(update ? fmaf(-t.rate, v, decay * (float)x.v[k]) : v);
           }
-          if (in) *reinterpret_cast<Few<T, N()>*>(out + at) = y;
+          if (many == N()) store_few(out + at, y);
+          else if constexpr (decltype(N)::parts)
+#pragma unroll
+            for (int k = 0; k < N(); ++k)
+              if (k < many) out[at + k] = y.v[k];
         });
   }
 }
@@ -1271,9 +1295,7 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
   size_t halves = 0, part = 0;
   const dim3 wg(256);
   const auto matrix = [&](int i) {
-    const auto over = [](const void* q, size_t bytes) { return reinterpret_cast<uintptr_t>(q) % bytes != 0; };
-    const bool wide = !over(src[i], 4 * sizeof(T)) && !over(dst[i], 4 * sizeof(T)) && (!update || !over(buf[i], 16));
-    return Mat{src[i], dst[i], update ? buf[i] : nullptr, rows[i], cols[i], rates ? rates[i] : 0.f, 1, wide};
+    return Mat{src[i], dst[i], update ? buf[i] : nullptr, rows[i], cols[i], rates ? rates[i] : 0.f, 1};
   };
   if (l.count < count)
     for (int i = 0; i < count;) {

@@ -269,6 +269,31 @@ def test_update_leaves_its_neighbours_alone():
     assert torch.equal(g, keep) and not (w == 7).all()
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", [(300, 1), (300, 3), (300, 4), (300, 5), (300, 6), (300, 7), (3, 301), (130, 129), (131, 130), (140, 131),
+                                   (50, 61)], ids=str)
+def test_rows_that_end_anywhere_from_any_element_on(shape, dtype):
+    """Rows of any length, weights, gradients and momenta from an odd element on: the same bits as aligned ones, and nothing
+    around them is written."""
+    n, m = shape
+    t = TYPES[dtype]
+    w0, g0, b0 = matrix(n, m, dtype=dtype, seed=1), matrix(n, m, dtype=dtype, seed=2), matrix(n, m, seed=3)
+    stores, views = [], []
+    for k, x in enumerate((w0, g0, b0)):
+        store = torch.full((n * m + 16,), 7.0, dtype=x.dtype, device=DEV)
+        view = store[2 * k + 1:2 * k + 1 + n * m].view(n, m)
+        view.copy_(x)
+        stores.append(store), views.append(view)
+    w, g, b = views
+    assert torch.equal(orthogonalize(g), orthogonalize(g0))
+    orthogonal_update_([w], [g], [b], lr=0.1, weight_decay=0.01)
+    orthogonal_update_([w0], [g0], [b0], lr=0.1, weight_decay=0.01)
+    assert torch.equal(w, w0) and torch.equal(b, b0) and torch.equal(g, g0)
+    for k, store in enumerate(stores):
+        assert (store[:2 * k + 1] == 7).all() and (store[2 * k + 1 + n * m:] == 7).all()
+    check([g0])
+
+
 def test_update_of_weights_that_need_gradients():
     w = torch.nn.Parameter(matrix(20, 30))
     (w * matrix(20, 30, seed=1)).sum().backward()
