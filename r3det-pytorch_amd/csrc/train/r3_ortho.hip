@@ -9,9 +9,9 @@
 // TWO fp16 numbers, hi + lo, 22 bits and lo's sign, and a product is three matrix products on the matrix cores,
 // hi hi + (hi lo + lo hi), summed in fp32 in two accumulators.
 //
-// Steps are taken in groups of two (the first of three where their number is odd) that touch X only twice.  Everything
-// inside a group is a polynomial of its first A, n x n and symmetric, written without cancellation: with the square
-// completed, t = -b / 2c and q = a - c t^2, a step multiplies X by
+// Steps are taken in groups of two (the first of three where their number is odd) that touch X only twice; short lists take
+// them one by one.  Everything inside a group is a polynomial of its first A, n x n and symmetric, written without
+// cancellation: with the square completed, t = -b / 2c and q = a - c t^2, a step multiplies X by
 //   F = a I + b A + c A A = q I + c (A - t I)^2,
 // which for the usual coefficients is 0.64 I and a positive matrix (the three terms cancel six to one where singular values
 // are near 1).  The next A is F (F A), and the group's steps together are X <- R X with R the product of the F.
@@ -31,8 +31,8 @@
 // straight from memory).  Of a symmetric result the tiles on and above the diagonal are computed, and written twice.
 //
 // What bounds it, with the usual five steps (kernels' time of a call; the matrix cores reach 1.1 PFLOP/s of fp16, a copy
-// 4.7 TB/s): 4096 x 4096, 4.5 ms: the matrix cores, 3.75 ms of products at that rate.  2048 x 2048, 0.92 ms: the same, with
-// fewer tiles than would keep them busy (0.47).  The 73 matrices of a detector, 41.9 M weights, 1.14 ms: a third the memory
+// 4.7 TB/s): 4096 x 4096, 4.6 ms: the matrix cores, 3.75 ms of products at that rate.  2048 x 2048, 0.94 ms: the same, with
+// fewer tiles than would keep them busy (0.47).  The 73 matrices of a detector, 41.9 M weights, 1.17 ms: a third the memory
 // (norms 86 us, X 100, the last group's R X 185), the rest loads on their way between matrix instructions.  A head's ten,
 // 0.19 ms, and smaller lists: some twenty launches that wait for each other, 5 us at least each.
 #include <hip/hip_runtime.h>
