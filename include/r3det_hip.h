@@ -661,9 +661,9 @@ int r3det_label_log_probs_backward(const void* logits, int dtype, int64_t rows, 
 /* Newton-Schulz products for `count` matrices at once.  For each matrix G (rows[i] x cols[i], contiguous, of type dtype;
  * at least 1 x 1, at most 2^31 - 1 elements, the smaller side at most 32768):
  *   X = G / (|G|_F + eps), then `steps` (1 .. 64) times  A = X X^t,  X <- a X + (b A + c A A) X   (for rows > cols: of G^t);
- * dst[i] (rows x cols, contiguous, of the same type; may be src[i]) receives X.  In fp32's accuracy whatever the type: off by
- * 1e-6 of its norm, as the products in fp32 one by one are; by up to 5e-5 for a matrix of few rows, one singular value far
- * above the others, in a list of many tiles.
+ * dst[i] (rows x cols, contiguous, of the same type; may be src[i]) receives X.  In fp32's accuracy whatever the type,
+ * and whatever else is in the list: as far from 64 bits as the products in fp32 one by one are, within a factor of three (some
+ * 1e-6 of its norm; up to 1e-5 of those and of these where one singular value is far above the others).
  * A zero matrix stays zero where eps > 0.  The arrays of pointers and sizes are HOST arrays and are read before the call
  * returns.  With P = a I + b A + c A A, the coefficients have to keep the spectral norms of X, A, P A and of P less its
  * vertex a - b b / (4 c) (less a, where |b| > 14 |c|) below 15 in every step, for singular values of up to 1 at first

@@ -9,8 +9,8 @@
 // TWO fp16 numbers, hi + lo, 22 bits and lo's sign, and a product is three matrix products on the matrix cores,
 // hi hi + (hi lo + lo hi), summed in fp32 in two accumulators.
 //
-// Steps are taken in groups of two (the first of three where their number is odd) that touch X only twice; short lists take
-// them one by one.  Everything inside a group is a polynomial of its first A, n x n and symmetric, written without
+// Steps are taken in groups of two (the first of three where their number is odd) that touch X only twice; short lists and
+// matrices of fewer than 256 rows take them one by one (NARROW below).  Everything inside a group is a polynomial of its first A, n x n and symmetric, written without
 // cancellation: with the square completed, t = -b / 2c and q = a - c t^2, a step multiplies X by
 //   F = a I + b A + c A A = q I + c (A - t I)^2,
 // which for the usual coefficients is 0.64 I and a positive matrix (the three terms cancel six to one where singular values
@@ -1123,14 +1123,30 @@ __global__ __launch_bounds__(SMALL_THREADS) void ortho_small_kernel(Batch b, Mom
 // ------------------------------------------------------------------------------------------------ the host
 size_t round256(size_t v) { return (v + 255) / 256 * 256; }
 
-// 0: fine, -1: a shape that is not taken
-int plan(int count, const int* rows, const int* cols, Plan& p) {
-  if (count < 0 || count > (1 << 16) || (count && (!rows || !cols))) return -1;
+// Matrices are taken in chains of launches by what their accuracy allows.  In a group of steps the next A is made of products,
+// whose roundings the largest singular value carries over into the smallest ones' directions, where every later step
+// multiplies them by a a: with one value 12 to 40 times the others, groups of 3 + 2 leave an error of 56e-6 with 2 rows, 50e-6
+// with 5, 15e-6 with 65, 14e-6 with 135, 10e-6 with 192, 7e-6 with 256 (any columns), where the form op by op in fp32 has
+// 2e-6, 2e-6, 3e-6, 4e-6, 6e-6 and 8e-6, and single steps 1e-6 throughout.  So from NARROW rows on groups are no worse than
+// that form at its worst, and matrices of fewer take single steps whatever else is in the list.
+constexpr int NARROW = 256;
+enum { SMALLS = 1, NARROWS = 2, WIDES = 4 };
+int kind(int rows, int cols) {
+  return is_small(rows, cols) ? SMALLS : (rows < cols ? rows : cols) < NARROW ? NARROWS : WIDES;
+}
+// a list that is taken
+bool taken(int count, const int* rows, const int* cols) {
+  if (count < 0 || count > (1 << 16) || (count && (!rows || !cols))) return false;
   for (int i = 0; i < count; ++i) {
-    if (rows[i] < 1 || cols[i] < 1 || (int64_t)rows[i] * cols[i] > 0x7fffffff) return -1;
-    if ((rows[i] < cols[i] ? rows[i] : cols[i]) > 32768) return -1;
-    if ((rows[i] > cols[i] ? rows[i] : cols[i]) > 65535 * 64) return -1;  // (a tile's place has 16 bits)
+    if (rows[i] < 1 || cols[i] < 1 || (int64_t)rows[i] * cols[i] > 0x7fffffff) return false;
+    if ((rows[i] < cols[i] ? rows[i] : cols[i]) > 32768) return false;
+    if ((rows[i] > cols[i] ? rows[i] : cols[i]) > 65535 * 64) return false;  // (a tile's place has 16 bits)
   }
+  return true;
+}
+// One chain, for the matrices of these kinds.  0: fine, -1: too many tiles
+int plan(int count, const int* rows, const int* cols, int kinds, Plan& p) {
+  const auto skip = [&](int i) { return !(kind(rows[i], cols[i]) & kinds); };
   Lists& l = p.l;
   l = Lists{};
   p.narrow = 1 << 30;
@@ -1140,7 +1156,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   // 2616: 184 us, 256 so; at 256 (2048 x 2048) 70, 71.  X X^t at 730 parts: 95 + 17 us, 113 + 6 so.
   uint64_t tri128 = 0, rect128 = 0, gram128 = 0, elements = 0;
   for (int i = 0; i < count; ++i) {
-    if (is_small(rows[i], cols[i])) continue;
+    if (skip(i)) continue;
     ++l.count;
     const Dim w(rows[i], cols[i]);
     if (w.n < p.narrow) p.narrow = w.n;
@@ -1169,7 +1185,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   for (int kc = 4096; kc >= 512; kc -= 128) {
     uint64_t blocks = 0, whole = 0;
     for (int i = 0; i < count; ++i) {
-      if (is_small(rows[i], cols[i])) continue;
+      if (skip(i)) continue;
       const Dim d(rows[i], cols[i]);
       blocks += (uint64_t)d.tri(l.gram_ts) * ((d.mp + kc - 1) / kc), whole += d.tri(l.gram_ts);
     }
@@ -1181,7 +1197,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   uint64_t gram = 0, tri = 0, rect = 0, fill = 0, norm = 0, part = 0, halves = 0;
   p.split = false;
   for (int i = 0; i < count; ++i) {
-    if (is_small(rows[i], cols[i])) continue;
+    if (skip(i)) continue;
     const Dim d(rows[i], cols[i]);
     const unsigned s = (unsigned)((d.mp + p.kc - 1) / p.kc);
     gram += (uint64_t)d.tri(l.gram_ts) * s;
@@ -1213,7 +1229,7 @@ int plan(int count, const int* rows, const int* cols, Plan& p) {
   p.norms = take(sizeof(double) * norm);
   p.parts = take(sizeof(float) * part);
   p.halves = take(sizeof(_Float16) * halves);
-  p.total = at ? at : 256;  // (nothing but small matrices needs nothing)
+  p.total = at;
   return 0;
 }
 
@@ -1275,10 +1291,51 @@ void choose(int ts, const F& f) {  // f(tile) with the tile a constant
   else f(std::integral_constant<int, 64>());
 }
 
-template <typename T>
-int run(int count, const void* const* src, void* const* dst, float* const* buf, const int* rows, const int* cols,
-        const float* rates, float decay, float mu, int nesterov, int steps, const Poly& f, double eps, const Plan& p, char* ws,
-        hipStream_t st) {
+// Where every pass has at most a tile a compute unit, the two passes over X are launches like the others: steps are taken
+// one by one, if X X^t is a launch as well (250 x 250: 104 us, 111 in groups; 300 x 300: 117, 126) or a matrix is narrow.
+bool one_by_one(const Plan& p) {
+  const Lists& l = p.l;
+  const unsigned most = WANT / 2;
+  return l.gram_ts == 64 && l.tri_ts == 64 && l.rect_ts == 64 && l.n_gram <= most && l.n_tri <= most && l.n_rect <= most &&
+         (!p.split || p.narrow < NARROW);
+}
+// The chains of a list, one behind the other in one workspace: all but the small ones together in single steps, where that is
+// as fast; else the wide ones in groups and the narrow ones in single steps.
+struct Chains {
+  struct {
+    int kinds;
+    bool single;
+    Plan p;
+  } of[2];
+  int many;
+  size_t total;
+};
+int chains(int count, const int* rows, const int* cols, Chains& c) {
+  c.many = 0, c.total = 256;  // (nothing but small matrices needs nothing)
+  if (!taken(count, rows, cols)) return -1;
+  const auto add = [&](int kinds, bool single, const Plan& p) {
+    c.of[c.many++] = {kinds, single, p};
+    if (p.total > c.total) c.total = p.total;
+  };
+  int kinds = 0;
+  for (int i = 0; i < count; ++i) kinds |= kind(rows[i], cols[i]) & (NARROWS | WIDES);
+  if (!kinds) return 0;
+  Plan p;
+  if (plan(count, rows, cols, kinds, p) != 0) return -1;
+  if (kinds != (NARROWS | WIDES) || one_by_one(p)) {
+    add(kinds, kinds == NARROWS || one_by_one(p), p);
+    return 0;
+  }
+  for (int k : {WIDES, NARROWS}) {
+    if (plan(count, rows, cols, k, p) != 0) return -1;
+    add(k, k == NARROWS, p);
+  }
+  return 0;
+}
+
+template <typename T, typename Matrix>
+int chain(int count, const Matrix& matrix, const int* rows, const int* cols, int kinds, bool single, const Momentum& m,
+          float decay, int steps, const Poly& f, double eps, const Plan& p, char* ws, hipStream_t st) {
   Lists l = p.l;
   l.table = reinterpret_cast<Mat*>(ws + p.table);
   l.gram = reinterpret_cast<Tile*>(ws + p.gram);
@@ -1289,30 +1346,14 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
   double* norms = reinterpret_cast<double*>(ws + p.norms);
   float* parts = reinterpret_cast<float*>(ws + p.parts);
   _Float16* base = reinterpret_cast<_Float16*>(ws + p.halves);
-  const int update = buf != nullptr;
-  const Momentum m{update, nesterov, mu};
   unsigned gram = 0, tri = 0, rect = 0, fill = 0, norm = 0;
   size_t halves = 0, part = 0;
   const dim3 wg(256);
-  const auto matrix = [&](int i) {
-    return Mat{src[i], dst[i], update ? buf[i] : nullptr, rows[i], cols[i], rates ? rates[i] : 0.f, 1};
-  };
-  if (l.count < count)
-    for (int i = 0; i < count;) {
-      Batch batch{};
-      for (; i < count && batch.count < BATCH; ++i)
-        if (is_small(rows[i], cols[i])) batch.m[batch.count++] = matrix(i);
-      if (batch.count)
-        hipLaunchKernelGGL((ortho_small_kernel<T>), dim3(batch.count), dim3(SMALL_THREADS), 0, st, batch, m, Step{f.c, f.t, f.q, f.l}, steps, eps,
-                           decay);
-      if (hipGetLastError() != hipSuccess) return -2;
-    }
-  if (l.count == 0) return 0;
   for (int i = 0, first = 0; first < l.count;) {
     Batch batch{};
     const uint64_t was = (uint64_t)gram + tri + rect + fill + norm;
     for (; i < count && batch.count < BATCH; ++i) {
-      if (is_small(rows[i], cols[i])) continue;
+      if (!(kind(rows[i], cols[i]) & kinds)) continue;
       const Dim d(rows[i], cols[i]);
       const unsigned s = (unsigned)((d.mp + p.kc - 1) / p.kc);
       Mat& t = batch.m[batch.count++];
@@ -1401,16 +1442,9 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
     return R;
   };
   const bool brief = f.brief && l.tri_ts == 64 && 2 * l.n_tri <= cus;
-  // Where every pass has at most a tile a compute unit, the two passes over X are launches like the others: steps are taken
-  // one by one, if X X^t is a launch as well (250 x 250: 104 us, 111 in groups; 300 x 300: 117, 126) or a matrix is narrow.
-  // (In a group the next A is made of products, whose roundings the largest singular value carries over into the smallest
-  // ones' directions: with two rows, one 40 times the other, a group of three is off by 4e-5 where single steps are by 1e-6,
-  // as the form op by op in fp32 is.  With many rows that form's own error is as large.  60 x 4000: 116 us, 107.)
-  const bool one_by_one = l.gram_ts == 64 && l.tri_ts == 64 && l.rect_ts == 64 && l.n_gram <= cus && l.n_tri <= cus &&
-                          l.n_rect <= cus && (!p.split || p.narrow <= 128);
   int from = 0;
   for (int left = steps; left > 0;) {
-    int g = one_by_one ? 1 : group_length(left, steps);
+    int g = single ? 1 : group_length(left, steps);
     if (g > f.longest) g = f.longest;
     choose(l.gram_ts, [&](auto TS) {
       hipLaunchKernelGGL((ortho_gram_kernel<TS()>), dim3(l.n_gram), wg, 0, st, l, base, parts, p.kc, from);
@@ -1422,9 +1456,9 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
     choose(l.rect_ts, [&](auto TS) {
       const dim3 grid(l.n_rect);
       if (left)
-        hipLaunchKernelGGL((ortho_apply_kernel<T, false, TS()>), grid, wg, 0, st, l, base, R.at, fs, from, update, decay);
+        hipLaunchKernelGGL((ortho_apply_kernel<T, false, TS()>), grid, wg, 0, st, l, base, R.at, fs, from, m.update, decay);
       else
-        hipLaunchKernelGGL((ortho_apply_kernel<T, true, TS()>), grid, wg, 0, st, l, base, R.at, fs, from, update, decay);
+        hipLaunchKernelGGL((ortho_apply_kernel<T, true, TS()>), grid, wg, 0, st, l, base, R.at, fs, from, m.update, decay);
     });
     from ^= 1;
     if (hipGetLastError() != hipSuccess) return -2;
@@ -1432,30 +1466,54 @@ int run(int count, const void* const* src, void* const* dst, float* const* buf, 
   return 0;
 }
 
+template <typename T>
+int run(int count, const void* const* src, void* const* dst, float* const* buf, const int* rows, const int* cols,
+        const float* rates, float decay, float mu, int nesterov, int steps, const Poly& f, double eps, const Chains& c, char* ws,
+        hipStream_t st) {
+  const int update = buf != nullptr;
+  const Momentum m{update, nesterov, mu};
+  const auto matrix = [&](int i) {
+    return Mat{src[i], dst[i], update ? buf[i] : nullptr, rows[i], cols[i], rates ? rates[i] : 0.f, 1};
+  };
+  for (int i = 0; i < count;) {
+    Batch batch{};
+    for (; i < count && batch.count < BATCH; ++i)
+      if (kind(rows[i], cols[i]) == SMALLS) batch.m[batch.count++] = matrix(i);
+    if (batch.count)
+      hipLaunchKernelGGL((ortho_small_kernel<T>), dim3(batch.count), dim3(SMALL_THREADS), 0, st, batch, m, Step{f.c, f.t, f.q, f.l}, steps, eps,
+                         decay);
+    if (hipGetLastError() != hipSuccess) return -2;
+  }
+  for (int k = 0; k < c.many; ++k) {
+    const int rc = chain<T>(count, matrix, rows, cols, c.of[k].kinds, c.of[k].single, m, decay, steps, f, eps, c.of[k].p, ws, st);
+    if (rc != 0) return rc;
+  }
+  return 0;
+}
 }  // namespace
 
 size_t r3k_ortho_workspace_bytes(int count, const int* rows, const int* cols) {
-  Plan p;
-  return count > 0 && plan(count, rows, cols, p) == 0 ? p.total : 0;
+  Chains c;
+  return count > 0 && chains(count, rows, cols, c) == 0 ? c.total : 0;
 }
 
 int r3k_ortho(int count, const void* const* src, void* const* dst, float* const* buf, int dtype, const int* rows,
               const int* cols, const float* rates, float decay, float mu, int nesterov, int steps, float a, float b, float c,
               double eps, void* ws, size_t ws_bytes, hipStream_t st) {
-  Plan p;
-  if (plan(count, rows, cols, p) != 0 || dtype < 0 || dtype > 2 || steps < 1 || steps > 64 || !(eps >= 0)) return -1;
+  Chains plans;
+  if (chains(count, rows, cols, plans) != 0 || dtype < 0 || dtype > 2 || steps < 1 || steps > 64 || !(eps >= 0)) return -1;
   const Poly f = polynomial(steps, a, b, c);
   if (!f.longest) return -1;
   if (count == 0) return 0;
   if (!src || !dst || (buf && !rates)) return -1;
   for (int i = 0; i < count; ++i)
     if (!src[i] || !dst[i] || (buf && !buf[i])) return -1;
-  if (!ws || ws_bytes < p.total) return -3;
+  if (!ws || ws_bytes < plans.total) return -3;
   char* w = static_cast<char*>(ws);
   if (reinterpret_cast<uintptr_t>(w) & 15) return -1;
   switch (dtype) {
-    case 0: return run<float>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, p, w, st);
-    case 1: return run<_Float16>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, p, w, st);
-    default: return run<__bf16>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, p, w, st);
+    case 0: return run<float>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, plans, w, st);
+    case 1: return run<_Float16>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, plans, w, st);
+    default: return run<__bf16>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, plans, w, st);
   }
 }

@@ -69,12 +69,13 @@ def orthogonalize(tensors, steps=STEPS, coefficients=COEFFICIENTS, eps=1e-7):
     """One matrix or a list of matrices (fp32, fp16 or bf16, all alike; more than two dimensions: (size(0), rest)) ->
     new, contiguous tensors of the same shapes and type: ``X = G / (|G| + eps)``, then ``steps`` times
     ``X = a X + (b A + c A A) X`` with ``A = X X^t`` (of the transpose where there are more rows than columns), which moves
-    every singular value towards 1 and keeps the singular vectors.  Computed to fp32's accuracy whatever the type, and
-    rounded once (in a long list, a matrix of few rows whose largest singular value is 40 times the others is off by up to
-    5e-5 of its norm, elsewhere by 1e-6).  A zero matrix stays zero (with eps = 0: NaN); NaN or an infinity in a matrix makes that matrix NaN and no other.  The
-    coefficients must keep the spectral norms of X, A and P A, with P = a + b A + c A A, and of P less its vertex
-    a - b b / 4 c below 15 (RuntimeError otherwise).  No gradient flows through it.  Runs on the
-    current stream of the tensors' device, without a host synchronisation."""
+    every singular value towards 1 and keeps the singular vectors.  Computed to fp32's accuracy whatever the type and
+    whatever else is in the list, and rounded once: as far from 64 bits as the formula op by op in fp32 is, within a factor of
+    three (some 1e-6 of its norm; up to 1e-5 both ways where one singular value is far above the others).  A zero matrix stays
+    zero (with eps = 0: NaN); NaN or an infinity in a matrix makes that matrix NaN and no other.  The coefficients must keep
+    the spectral norms of X, A and P A, with P = a + b A + c A A, and of P less its vertex a - b b / 4 c below 15
+    (RuntimeError otherwise).  No gradient flows through it.  Runs on the current stream of the tensors' device, without a
+    host synchronisation."""
     one = isinstance(tensors, torch.Tensor)
     ts = [tensors] if one else list(tensors)
     steps, a, b, c, eps = _numbers(steps, coefficients, eps)

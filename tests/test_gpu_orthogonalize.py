@@ -341,3 +341,31 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         for x, y in zip(ws + ms, e_ws + e_ms):
             assert torch.equal(x, y)
+
+
+def one_large(rows, cols, large):
+    g = matrix(rows, cols, seed=rows)
+    u, _, v = torch.linalg.svd(g.double().cpu(), full_matrices=False)
+    s = torch.ones(min(rows, cols), dtype=torch.float64)
+    s[0] = large
+    return ((u * s) @ v).float().to(DEV)
+
+
+@pytest.mark.parametrize("steps", [3, 5, 7])
+@pytest.mark.parametrize("rows", [2, 5, 15, 45, 65, 135, 192, 255, 256, 300])
+def test_a_large_singular_value_in_a_long_list(rows, steps):
+    """Beside as many tiles as a head's tower has, where wide matrices take their steps in groups: every matrix stays as close as
+    it is alone.  (What a step rounds in the large value's direction is what a group carries over, see above.)"""
+    tower = [matrix(256, 2304, seed=i) for i in range(8)]
+    check([one_large(rows, cols, large) for cols in (600, 2304) for large in (9.0, 12.0, 20.0, 40.0)] + tower, steps=steps)
+
+
+def test_neighbours_in_a_list_change_nothing_of_a_narrow_matrix_s_accuracy():
+    """A head's predictions, their towers beside them: no further from 64 bits than 4 times what the same matrices alone are
+    (single steps both times; parts of X X^t may differ), which their errors' random signs leave room for."""
+    preds = [one_large(rows, 2304, 20.0) for rows in (5, 15, 45, 135)]
+    tower = [matrix(256, 2304, seed=i) for i in range(8)]
+    for g, beside, alone in zip(preds, orthogonalize(preds + tower), (orthogonalize(g) for g in preds)):
+        want, norms = iterate(g)
+        off = [(o.double() - want).norm().item() for o in (beside, alone)]
+        assert off[0] <= 4 * off[1] + 4 * U * norms[-1], (tuple(g.shape), off)
