@@ -88,7 +88,7 @@ struct Tile {  // one workgroup's work, with all that it needs of its matrix to 
   size_t part;  // X X^t in parts: where this one goes
   int np, mp;
   unsigned short i, j, split, splits;
-  unsigned short ts;  // 128 or 64 rows and columns (0: none), in units of which i and j are
+  unsigned short ts;  // 128 or 64 rows and columns (0: none), in units of which i and j are; fill: the chain's rect_ts
   unsigned mat;
 };
 struct Area {  // where a matrix's arrays are
@@ -106,26 +106,23 @@ struct Area {  // where a matrix's arrays are
     else xt = next_t = nullptr, x += from ? nx : 0, next += from ? 0 : nx;
   }
 };
-struct Lists {  // one entry a workgroup
-  Mat* table;
-  Tile* gram;       // X X^t: triangle tiles times parts of the sum
-  Tile* tri;        // triangle tiles of the other n x n products
-  Tile* rect;       // tiles of X
+struct Chain {  // lists of a chain of launches, one entry a workgroup
+  Tile* gram;  // X X^t: triangle tiles times parts of the sum
+  Tile* tri;   // triangle tiles of the other n x n products
+  Tile* rect;  // tiles of X
+  unsigned n_gram, n_tri, n_rect;
+  unsigned whole_gram, whole_tri;  // tiles that are not quartered
+  int gram_ts, tri_ts, rect_ts;
+  unsigned gram0, tri0, rect0;     // of its first matrix, see Mat
+};
+struct Lists {
+  Mat* table;       // of one chain's matrices behind the other's
   Tile* fill;       // 64 x 64 pieces of X
   uint2* norm_map;  // (matrix, chunk)
-  unsigned n_gram, n_tri, n_rect, n_fill, n_norm;
-  unsigned whole_gram, whole_tri;  // tiles that are not quartered
-  int count, gram_ts, tri_ts, rect_ts;
-  int chunk;  // elements a workgroup of the norm's pass takes
-};
-
-// the whole workspace; every part is a multiple of 256 bytes
-struct Plan {
-  size_t table, gram, tri, rect, fill, norm_map, norms, parts, halves, total;
-  Lists l;    // (sizes only)
-  int kc;     // the summed index of X X^t a workgroup takes at most
-  bool split; // whether any matrix has more than one part
-  int narrow; // the smallest n
+  unsigned n_fill, n_norm;
+  unsigned second;  // the second chain's first matrix
+  int chunk;        // elements a workgroup of the norm's pass takes
+  Chain c[2];
 };
 
 // ------------------------------------------------------------------------------------------------ the lists
@@ -214,30 +211,35 @@ __global__ void ortho_lists_kernel(Lists l, Batch b, unsigned first) {
       list[n + 4 * (u - n) + q] = v;
     }
   };
+  const auto chain = [&](unsigned k) -> const Chain& { return l.c[first + k >= l.second]; };
   if (within(&Mat::gram0)) {
     const unsigned k = find(b, &Mat::gram0, e), local = e - b.m[k].gram0;
+    const Chain& c = chain(k);
     Tile w = begin(k);
-    const unsigned high = w.np / l.gram_ts, tiles = high * (high + 1) / 2, tile = local % tiles;
+    const unsigned high = w.np / c.gram_ts, tiles = high * (high + 1) / 2, tile = local % tiles;
     triangle(w, tile, high);
     w.split = local / tiles;
-    w.part = b.m[k].part0 + ((size_t)tile * w.splits + w.split) * (l.gram_ts * l.gram_ts);
-    put(l.gram, w, e, l.whole_gram, l.gram_ts);
+    w.part = b.m[k].part0 + ((size_t)tile * w.splits + w.split) * (c.gram_ts * c.gram_ts);
+    put(c.gram, w, e - c.gram0, c.whole_gram, c.gram_ts);
   } else if (within(&Mat::tri0)) {
     const unsigned k = find(b, &Mat::tri0, e);
+    const Chain& c = chain(k);
     Tile w = begin(k);
-    triangle(w, e - b.m[k].tri0, w.np / l.tri_ts);
-    put(l.tri, w, e, l.whole_tri, l.tri_ts);
+    triangle(w, e - b.m[k].tri0, w.np / c.tri_ts);
+    put(c.tri, w, e - c.tri0, c.whole_tri, c.tri_ts);
   } else if (within(&Mat::rect0)) {
     const unsigned k = find(b, &Mat::rect0, e), local = e - b.m[k].rect0;
+    const Chain& c = chain(k);
     Tile w = begin(k);
-    const unsigned high = w.np / l.rect_ts;
+    const unsigned high = w.np / c.rect_ts;
     w.i = local % high, w.j = local / high;
-    l.rect[entry(e, l.n_rect)] = w;
+    c.rect[entry(e - c.rect0, c.n_rect)] = w;
   } else if (within(&Mat::fill0)) {
     const unsigned k = find(b, &Mat::fill0, e), local = e - b.m[k].fill0;
     Tile w = begin(k);
     const unsigned wide = w.mp / 64;
     w.i = local / wide, w.j = local % wide;
+    w.ts = chain(k).rect_ts;
     l.fill[e] = w;
   } else if (within(&Mat::norm0)) {
     const unsigned k = find(b, &Mat::norm0, e);
@@ -414,10 +416,10 @@ __device__ __forceinline__ void eight(float* E, int r, int c, const F& f) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) E[r * LD + c + k] = v[k];
 }
-template <int ROWS, int COLS, int LD, int PARTS, typename F>
+template <int ROWS, int COLS, int LD, int PARTS, int THREADS = 256, typename F>
 __device__ __forceinline__ void rows8(float* E, const F& f) {
 #pragma unroll 2
-  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += 256) eight<LD, PARTS, ROWS * LD>(E, q % ROWS, q / ROWS * 8, f);
+  for (int q = threadIdx.x; q < ROWS * COLS / 8; q += THREADS) eight<LD, PARTS, ROWS * LD>(E, q % ROWS, q / ROWS * 8, f);
 }
 // The same for a product's tile, where f takes what `load`(row, column) gives too: loaded for several rows at a time, the
 // first of them before the product's sums are in shared memory.  (What f stores could be what the next row loads, for all
@@ -467,7 +469,7 @@ __global__ __launch_bounds__(256) void ortho_start_kernel(Lists l, const double*
   __shared__ float E[64 * 65];
   const Tile w = l.fill[blockIdx.x];
   const Mat t = l.table[w.mat];
-  const Area o(base, w, l.rect_ts, 0);
+  const Area o(base, w, w.ts, 0);
   double s = 0;
   const unsigned chunks = Dim(t.rows, t.cols).norms(l.chunk);
   for (unsigned i = threadIdx.x; i < chunks; i += 256) s += norms[t.norm0 + i];
@@ -722,12 +724,14 @@ union Either {
 };
 template <int TS>
 using Core = std::conditional_t<TS == 128, Core128, Core64<4>>;
+template <typename C>
+using Quarter = std::conditional_t<C::TS == 128, Core64<4>, C>;  // what works on 64 x 64 in the same workgroup
 
 // A from ROWS rows of a tile in shared memory
-template <int ROWS, int TS, int PARTS>
+template <int ROWS, int TS, int PARTS, int THREADS>
 __device__ __forceinline__ void store_gram(float* E, int np, const Area& o, int i0, int j0, bool diagonal) {
   _Float16* a = o.sq + SQ_A * o.na;
-  rows8<ROWS, TS, TS + 1, PARTS>(E, [&](int r, int c, float (&v)[8]) {
+  rows8<ROWS, TS, TS + 1, PARTS, THREADS>(E, [&](int r, int c, float (&v)[8]) {
     if (diagonal)
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -736,50 +740,37 @@ __device__ __forceinline__ void store_gram(float* E, int np, const Area& o, int 
   });
   if (!diagonal) {
     __syncthreads();
-    store_turned<ROWS, TS, TS + 1>(E, a, np, j0, i0);
+    store_turned<ROWS, TS, TS + 1, THREADS>(E, a, np, j0, i0);
   }
 }
 // A = X X^t: a tile on or above the diagonal, or one part of its sum, which ortho_sum_kernel adds up in their order.
 // (Adding them in the workgroup that ends last needs the other workgroups' tiles flushed through the XCDs' caches: 160 us
 // where this and the launch behind it take 17, at eight 256 x 2304 matrices.)
-template <int TS>
-__device__ __forceinline__ void gram_tile(typename Core<TS>::Shared& sh, const Tile& w, const Area& o, float* parts, int kc) {
+template <typename C>
+__device__ __forceinline__ void gram_tile(typename C::Shared& sh, const Tile& w, const Area& o, float* parts, int kc) {
+  constexpr int TS = C::TS;
   const int i0 = w.i * TS, j0 = w.j * TS;
   const int k0 = w.split * kc, k1 = k0 + kc < w.mp ? k0 + kc : w.mp;
-  Core<TS>::run(sh, o.x, i0, w.mp, o.x, j0, w.mp, k0, k1, 1.f / SCALE, [] {});
+  C::run(sh, o.x, i0, w.mp, o.x, j0, w.mp, k0, k1, 1.f / SCALE, [] {});
   if (w.splits > 1) {
     float* mine = parts + w.part;
 #pragma unroll 4
-    for (int q = threadIdx.x; q < TS * TS; q += 256) {
+    for (int q = threadIdx.x; q < TS * TS; q += C::THREADS) {
       float v = 0.f;
 #pragma unroll
-      for (int k = 0; k < Core<TS>::PARTS; ++k) v += sh.E[k * TS * (TS + 1) + q / TS * (TS + 1) + q % TS];
+      for (int k = 0; k < C::PARTS; ++k) v += sh.E[k * TS * (TS + 1) + q / TS * (TS + 1) + q % TS];
       mine[q] = v;
     }
     return;
   }
-  store_gram<TS, TS, Core<TS>::PARTS>(sh.E, w.np, o, i0, j0, w.i == w.j);
-}
-template <int TS>
-__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Lists l, _Float16* base, float* parts, int kc, int from) {
-  __shared__ Either<Core<TS>, Core64<4>> sh;
-  const Tile w = l.gram[blockIdx.x];
-  const Area o(base, w, l.rect_ts, from);
-  if (w.ts == TS) gram_tile<TS>(sh.one, w, o, parts, kc);
-  if constexpr (TS == 128)
-    if (w.ts == 64) gram_tile<64>(sh.other, w, o, parts, kc);
+  store_gram<TS, TS, C::PARTS, C::THREADS>(sh.E, w.np, o, i0, j0, w.i == w.j);
 }
 // 32 rows of a tile of A from its parts
-template <int TS>
-__global__ __launch_bounds__(256) void ortho_sum_kernel(Lists l, _Float16* base, const float* __restrict__ parts) {
-  __shared__ float E[32 * (TS + 1)];
-  const Tile w = l.gram[blockIdx.x];
-  if (w.split || w.splits == 1) return;
-  const Area o(base, w, l.rect_ts, 0);
-  const int slice = blockIdx.y * 32;
+template <int TS, int THREADS>
+__device__ __forceinline__ void sum_tile(float* E, const Tile& w, const Area& o, const float* parts, int slice) {
   const float* mine = parts + w.part + slice * TS;
 #pragma unroll
-  for (int q = threadIdx.x * 4; q < 32 * TS; q += 1024) {
+  for (int q = threadIdx.x * 4; q < 32 * TS; q += THREADS * 4) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int s = 0; s < w.splits; ++s) {
@@ -790,7 +781,14 @@ __global__ __launch_bounds__(256) void ortho_sum_kernel(Lists l, _Float16* base,
     e[0] = v.x, e[1] = v.y, e[2] = v.z, e[3] = v.w;
   }
   __syncthreads();
-  store_gram<32, TS, 1>(E, w.np, o, w.i * TS + slice, w.j * TS, w.i == w.j);
+  store_gram<32, TS, 1, THREADS>(E, w.np, o, w.i * TS + slice, w.j * TS, w.i == w.j);
+}
+template <int TS>
+__global__ __launch_bounds__(256) void ortho_sum_kernel(Chain l, _Float16* base, const float* __restrict__ parts) {
+  __shared__ float E[32 * (TS + 1)];
+  const Tile w = l.gram[blockIdx.x];
+  if (w.split || w.splits == 1) return;
+  sum_tile<TS, 256>(E, w, Area(base, w, l.rect_ts, 0), parts, blockIdx.y * 32);
 }
 
 // out = q I + l G + f (G - tg I) (H - th I) + m M of symmetric matrices that commute (all are polynomials of one): a tile on
@@ -861,24 +859,10 @@ __device__ __forceinline__ void square_tile(typename C::Shared& sh, const Tile& 
     store_turned<TS, TS, TS + 1, C::THREADS>(sh.E, out, w.np, j0, i0);
   }
 }
-template <typename C, bool ADD>
-__global__ __launch_bounds__(C::THREADS, 2) void ortho_square_kernel(Lists l, _Float16* base, Op first, Op second) {
-  __shared__ Either<C, std::conditional_t<C::TS == 128, Core64<4>, C>> sh;
-  const Tile w = l.tri[blockIdx.x];
-  const Area o(base, w, l.rect_ts, 0);
-  const Op op = blockIdx.y ? second : first;
-  if (w.ts == C::TS) square_tile<C, ADD>(sh.one, w, o, op);
-  if constexpr (C::TS == 128)
-    if (w.ts == 64) square_tile<Core64<4>, ADD>(sh.other, w, o, op);
-}
-
-// X <- R X; the last group's goes to the caller, as the result or into the weights
-template <typename T, bool LAST, int TS>
-__global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* base, int R, float fs, int from, int update,
-                                                             float decay) {
-  __shared__ typename Core<TS>::Shared sh;
-  const Tile w = l.rect[blockIdx.x];
-  const Area o(base, w, TS, from);
+// X <- R X of a tile, in shared memory; as the next X unless it is the LAST
+template <typename C, bool LAST>
+__device__ __forceinline__ void apply_tile(typename C::Shared& sh, const Tile& w, const Area& o, int R, float fs) {
+  constexpr int TS = C::TS;
   const int i0 = w.i * TS, j0 = w.j * TS;
   const _Float16* a = o.sq + R * o.na;
   struct Loaded {
@@ -886,43 +870,121 @@ __global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Lists l, _Float16* 
     float d;
   };
   const auto load = [&](int r, int c) { return Loaded{load8(o.x + place(i0 + r, j0 + c, w.mp)), o.diag[R * w.np + i0 + r]}; };
-  Rows<Core<TS>, decltype(load)> rows{load};
+  Rows<C, decltype(load)> rows{load};
   const auto before = [&] { rows.fetch(0); };
-  if constexpr (TS == 128) Core128::run<true>(sh, a, i0, w.np, o.x, j0, w.mp, 0, w.np, fs, before);
-  else Core<TS>::run(sh, a, i0, w.np, o.xt, j0, w.np, 0, w.np, fs, before);
+  if constexpr (TS == 128) C::template run<true>(sh, a, i0, w.np, o.x, j0, w.mp, 0, w.np, fs, before);
+  else C::run(sh, a, i0, w.np, o.xt, j0, w.np, 0, w.np, fs, before);
   rows.run(sh.E, [&](int r, int c, float (&v)[8], const Loaded& d) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = fmaf(d.d, d.x[k], v[k]);
     if constexpr (!LAST) store8(o.next + place(i0 + r, j0 + c, w.mp), v);
   });
   __syncthreads();
-  if constexpr (!LAST) {
-    if constexpr (TS == 64) store_turned<TS, TS, TS + 1>(sh.E, o.next_t, w.np, j0, i0);
-  } else {
-    const Mat t = l.table[w.mat];
-    T* out = static_cast<T*>(t.dst);
-    callers<TS, 8>(
-        t, i0, j0,
-        [&](auto N, size_t at, int many) {  // (the weights, inside or not: eight loads on their way)
-          Few<T, N()> x{};
-          if (update) x = load_few<T, N()>(out + whole(N, at, many));
-          return x;
-        },
-        [&](auto N, size_t at, int many, int r, int c, bool tall, const auto& was) {
-          Few<T, N()> x = was, y;
-          to_front(N, x.v, many);
+  if constexpr (!LAST && TS == 64) store_turned<TS, TS, TS + 1, C::THREADS>(sh.E, o.next_t, w.np, j0, i0);
+}
+// The last one's to the caller, as the result or into the weights
+template <typename T, int TS>
+__device__ __forceinline__ void hand_over(const float* E, const Mat& t, int i0, int j0, int update, float decay) {
+  T* out = static_cast<T*>(t.dst);
+  callers<TS, 8>(
+      t, i0, j0,
+      [&](auto N, size_t at, int many) {  // (the weights, inside or not: eight loads on their way)
+        Few<T, N()> x{};
+        if (update) x = load_few<T, N()>(out + whole(N, at, many));
+        return x;
+      },
+      [&](auto N, size_t at, int many, int r, int c, bool tall, const auto& was) {
+        Few<T, N()> x = was, y;
+        to_front(N, x.v, many);
 #pragma unroll
-          for (int k = 0; k < N(); ++k) {
-            const float v = sh.E[(tall ? r + k : r) * (TS + 1) + (tall ? c : c + k)] * (1.f / SCALE);
-            y.v[k] = (T)(update ? fmaf(-t.rate, v, decay * (float)x.v[k]) : v);
-          }
-          if (many == N()) store_few(out + at, y);
-          else if constexpr (decltype(N)::parts)
+        for (int k = 0; k < N(); ++k) {
+          const float v = E[(tall ? r + k : r) * (TS + 1) + (tall ? c : c + k)] * (1.f / SCALE);
+          y.v[k] = (T)(update ? fmaf(-t.rate, v, decay * (float)x.v[k]) : v);
+        }
+        if (many == N()) store_few(out + at, y);
+        else if constexpr (decltype(N)::parts)
 #pragma unroll
-            for (int k = 0; k < N(); ++k)
-              if (k < many) out[at + k] = y.v[k];
-        });
+          for (int k = 0; k < N(); ++k)
+            if (k < many) out[at + k] = y.v[k];
+      });
+}
+
+// A launch of one chain takes a piece of the other along: the first `blocks` workgroups' work.  (The narrow matrices' chain
+// has as many launches as the wide ones' and little work in each: a call for one head takes 309 us with that chain behind,
+// 231 with it riding; the detector's 1218 and 1100, the ragged list 373 and 268.)
+enum { RIDE_GRAM, RIDE_SUM, RIDE_POLY, RIDE_APPLY };
+struct Rider {
+  const Tile* list;
+  unsigned blocks;
+  int what, from, kc;
+  Op op;  // RIDE_POLY
+};
+template <typename C>
+__device__ __forceinline__ void ride(typename C::Shared& sh, const Rider& r, _Float16* base, float* parts) {
+  static_assert(C::TS == 64, "the chain that rides is in tiles of 64");
+  const bool sum = r.what == RIDE_SUM;
+  const Tile w = r.list[sum ? blockIdx.x / 2 : blockIdx.x];
+  const Area o(base, w, 64, r.from);
+  if (r.what == RIDE_GRAM) gram_tile<C>(sh, w, o, parts, r.kc);
+  else if (r.what == RIDE_POLY) square_tile<C, false>(sh, w, o, r.op);
+  else if (r.what == RIDE_APPLY) apply_tile<C, false>(sh, w, o, r.op.out, 1.f / SCALE);
+  else if (w.split == 0 && w.splits > 1) sum_tile<64, C::THREADS>(sh.E, w, o, parts, blockIdx.x % 2 * 32);
+}
+
+template <int TS, bool RIDE>
+__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(Chain l, Rider r, _Float16* base, float* parts, int kc, int from) {
+  __shared__ Either<Core<TS>, Core64<4>> sh;
+  if constexpr (RIDE)
+    if (blockIdx.x < r.blocks) return ride<Core64<4>>(sh.other, r, base, parts);
+  const Tile w = l.gram[blockIdx.x - (RIDE ? r.blocks : 0)];
+  const Area o(base, w, l.rect_ts, from);
+  if (w.ts == TS) gram_tile<Core<TS>>(sh.one, w, o, parts, kc);
+  if constexpr (TS == 128)
+    if (w.ts == 64) gram_tile<Core64<4>>(sh.other, w, o, parts, kc);
+}
+template <typename C, bool ADD, bool RIDE>
+__global__ __launch_bounds__(C::THREADS, 2) void ortho_square_kernel(Chain l, Rider r, _Float16* base, float* parts, Op first,
+                                                                     Op second) {
+  __shared__ Either<C, Quarter<C>> sh;
+  if constexpr (RIDE)
+    if (blockIdx.x < r.blocks) {
+      if (blockIdx.y == 0) ride<Quarter<C>>(sh.other, r, base, parts);
+      return;
+    }
+  const Tile w = l.tri[blockIdx.x - (RIDE ? r.blocks : 0)];
+  const Area o(base, w, l.rect_ts, 0);
+  const Op op = blockIdx.y ? second : first;
+  if (w.ts == C::TS) square_tile<C, ADD>(sh.one, w, o, op);
+  if constexpr (C::TS == 128)
+    if (w.ts == 64) square_tile<Core64<4>, ADD>(sh.other, w, o, op);
+}
+template <int TS, bool RIDE>
+__global__ __launch_bounds__(256, 2) void ortho_apply_kernel(Chain l, Rider r, _Float16* base, float* parts, int R, float fs,
+                                                             int from) {
+  __shared__ Either<Core<TS>, Core64<4>> sh;
+  if constexpr (RIDE)
+    if (blockIdx.x < r.blocks) return ride<Core64<4>>(sh.other, r, base, parts);
+  const Tile w = l.rect[blockIdx.x - (RIDE ? r.blocks : 0)];
+  apply_tile<Core<TS>, false>(sh.one, w, Area(base, w, TS, from), R, fs);
+}
+struct Product {  // what the last X is made of
+  int R, from;
+  float fs;
+};
+// (the other chain's tiles, of 64, are the first `others`)
+template <typename T, int TS>
+__global__ __launch_bounds__(256, 2) void ortho_apply_last_kernel(const Mat* table, Chain l, Product p, const Tile* other,
+                                                            unsigned others, Product q, _Float16* base, int update, float decay) {
+  __shared__ Either<Core<TS>, Core64<4>> sh;
+  if (blockIdx.x < others) {
+    const Tile w = other[blockIdx.x];
+    apply_tile<Core64<4>, true>(sh.other, w, Area(base, w, 64, q.from), q.R, q.fs);
+    hand_over<T, 64>(sh.other.E, table[w.mat], w.i * 64, w.j * 64, update, decay);
+    return;
   }
+  const Tile w = l.rect[blockIdx.x - others];
+  apply_tile<Core<TS>, true>(sh.one, w, Area(base, w, TS, p.from), p.R, p.fs);
+  hand_over<T, TS>(sh.one.E, table[w.mat], w.i * TS, w.j * TS, update, decay);
 }
 
 // ------------------------------------------------------------------------------------------------ small matrices
@@ -1144,31 +1206,42 @@ bool taken(int count, const int* rows, const int* cols) {
   }
   return true;
 }
-// One chain, for the matrices of these kinds.  0: fine, -1: too many tiles
-int plan(int count, const int* rows, const int* cols, int kinds, Plan& p) {
+// One chain of launches: the matrices of some kinds.
+struct Work {
+  int kinds;
+  bool single;  // steps one by one
+  int kc;       // the summed index of X X^t a workgroup takes at most
+  bool split;   // whether any matrix has more than one part
+  int narrow;   // the smallest n
+  unsigned count;
+  uint64_t part, halves, fill, elements;
+  Chain c;      // (sizes only)
+  unsigned parts_of(const Dim& d) const { return (unsigned)((d.mp + kc - 1) / kc); }
+};
+// 0: fine, -1: too many tiles
+int work(int count, const int* rows, const int* cols, int kinds, Work& p) {
   const auto skip = [&](int i) { return !(kind(rows[i], cols[i]) & kinds); };
-  Lists& l = p.l;
-  l = Lists{};
+  p = Work{};
+  p.kinds = kinds;
   p.narrow = 1 << 30;
+  Chain& l = p.c;
   // Tiles: 128 needs half the reads of two operands that 64 does, and is taken for a pass that fills the card with such
   // tiles; X X^t, in parts, and R X, with short sums, from half of that on.  The n x n products: at 528 tiles of 128
   // (4096 x 4096, none quartered) 273 us, 307 with four times as many of 64; at 292 (the detector's) 45, 35 so.  R X at
   // 2616: 184 us, 256 so; at 256 (2048 x 2048) 70, 71.  X X^t at 730 parts: 95 + 17 us, 113 + 6 so.
-  uint64_t tri128 = 0, rect128 = 0, gram128 = 0, elements = 0;
+  uint64_t tri128 = 0, rect128 = 0, gram128 = 0;
   for (int i = 0; i < count; ++i) {
     if (skip(i)) continue;
-    ++l.count;
+    ++p.count;
     const Dim w(rows[i], cols[i]);
     if (w.n < p.narrow) p.narrow = w.n;
-    elements += (uint64_t)rows[i] * cols[i];
+    p.elements += (uint64_t)rows[i] * cols[i];
     tri128 += w.tri(128), rect128 += w.rect(128);
     gram128 += (uint64_t)w.tri(128) * ((w.mp + 255) / 256);
   }
   l.gram_ts = gram128 >= WANT / 2 ? 128 : 64;
   l.tri_ts = tri128 >= WANT ? 128 : 64;
   l.rect_ts = rect128 >= WANT / 2 ? 128 : 64;
-  // The norms: each thread 32 elements, fewer where that would leave compute units without work (2.6 M elements: 20 us, 6 so).
-  for (l.chunk = 8192; l.chunk > 1024 && elements / l.chunk < 2 * WANT;) l.chunk /= 2;
   // Whole tiles fill the card so many times; a few that are left would each keep a compute unit for a tile's time, alone,
   // and are quartered (16 of 528, 4096 x 4096: an n x n product 275 -> 234 us, X X^t 255 -> 222).
   const auto quarter = [](uint64_t& n, bool big) {
@@ -1194,36 +1267,81 @@ int plan(int count, const int* rows, const int* cols, int kinds, Plan& p) {
     const uint64_t cost = (blocks + WANT - 1) / WANT * (kc / 32 + 8) + (split ? 4 + blocks / (l.gram_ts == 128 ? 60 : 240) : 0);
     if (cost <= least) least = cost, p.kc = kc;
   }
-  uint64_t gram = 0, tri = 0, rect = 0, fill = 0, norm = 0, part = 0, halves = 0;
-  p.split = false;
+  uint64_t gram = 0, tri = 0, rect = 0;
   for (int i = 0; i < count; ++i) {
     if (skip(i)) continue;
     const Dim d(rows[i], cols[i]);
-    const unsigned s = (unsigned)((d.mp + p.kc - 1) / p.kc);
+    const unsigned s = p.parts_of(d);
     gram += (uint64_t)d.tri(l.gram_ts) * s;
     tri += d.tri(l.tri_ts);
     rect += d.rect(l.rect_ts);
-    fill += d.rect(64);
-    norm += d.norms(l.chunk);
-    if (s > 1) part += (uint64_t)d.tri(l.gram_ts) * s * l.gram_ts * l.gram_ts, p.split = true;
-    halves += d.halves(l.rect_ts);
+    p.fill += d.rect(64);
+    if (s > 1) p.part += (uint64_t)d.tri(l.gram_ts) * s * l.gram_ts * l.gram_ts, p.split = true;
+    p.halves += d.halves(l.rect_ts);
   }
-  const uint64_t threads = gram + tri + rect + fill + norm;
-  if (threads > 0xffffff00) return -1;  // (of the lists' kernel)
   l.whole_gram = quarter(gram, l.gram_ts == 128 && !p.split), l.whole_tri = quarter(tri, l.tri_ts == 128);
-  if (gram > 0x7fffffff || tri > 0x7fffffff || rect > 0x7fffffff || fill > 0x7fffffff || norm > 0x7fffffff) return -1;
-  l.n_gram = (unsigned)gram, l.n_tri = (unsigned)tri, l.n_rect = (unsigned)rect, l.n_fill = (unsigned)fill;
-  l.n_norm = (unsigned)norm;
+  if (gram > 0x3fffffff || tri > 0x3fffffff || rect > 0x3fffffff || p.fill > 0x3fffffff) return -1;
+  l.n_gram = (unsigned)gram, l.n_tri = (unsigned)tri, l.n_rect = (unsigned)rect;
+  return 0;
+}
+// Where every pass has at most a tile a compute unit, the two passes over X are launches like the others: steps are taken
+// one by one, if X X^t is a launch as well (250 x 250: 104 us, 111 in groups; 300 x 300: 117, 126) or a matrix is narrow.
+bool one_by_one(const Work& p) {
+  const Chain& l = p.c;
+  const unsigned most = WANT / 2;
+  return l.gram_ts == 64 && l.tri_ts == 64 && l.rect_ts == 64 && l.n_gram <= most && l.n_tri <= most && l.n_rect <= most &&
+         (!p.split || p.narrow < NARROW);
+}
+
+// The whole list: all but the small matrices in one chain, in single steps, where that is as fast; else the wide ones in
+// groups and the narrow ones in single steps.  Every part of the workspace is a multiple of 256 bytes.
+struct Plan {
+  size_t table, gram[2], tri[2], rect[2], fill, norm_map, norms, parts, halves, total;
+  Lists l;  // (sizes only)
+  Work w[2];
+  int chains;
+};
+// 0: fine, -1: a list that is not taken
+int plan(int count, const int* rows, const int* cols, Plan& p) {
+  p.chains = 0, p.total = 256;  // (nothing but small matrices needs nothing)
+  if (!taken(count, rows, cols)) return -1;
+  int kinds = 0;
+  for (int i = 0; i < count; ++i) kinds |= kind(rows[i], cols[i]) & (NARROWS | WIDES);
+  if (!kinds) return 0;
+  if (work(count, rows, cols, kinds, p.w[0]) != 0) return -1;
+  p.w[0].single = kinds == NARROWS || one_by_one(p.w[0]);
+  p.chains = 1;
+  if (kinds == (NARROWS | WIDES) && !p.w[0].single) {
+    if (work(count, rows, cols, WIDES, p.w[0]) != 0 || work(count, rows, cols, NARROWS, p.w[1]) != 0) return -1;
+    p.w[1].single = true;
+    p.chains = 2;
+  }
+  Lists& l = p.l;
+  l = Lists{};
+  uint64_t elements = 0, norm = 0, fill = 0, part = 0, halves = 0, entries = 0;
+  for (int k = 0; k < p.chains; ++k) elements += p.w[k].elements;
+  // The norms: each thread 32 elements, fewer where that would leave compute units without work (2.6 M elements: 20 us, 6 so).
+  for (l.chunk = 8192; l.chunk > 1024 && elements / l.chunk < 2 * WANT;) l.chunk /= 2;
+  for (int i = 0; i < count; ++i)
+    if (kind(rows[i], cols[i]) != SMALLS) norm += Dim(rows[i], cols[i]).norms(l.chunk);
   size_t at = 0;
   const auto take = [&](size_t bytes) {
     const size_t was = at;
     at += round256(bytes);
     return was;
   };
-  p.table = take(sizeof(Mat) * (size_t)l.count);
-  p.gram = take(sizeof(Tile) * gram);
-  p.tri = take(sizeof(Tile) * tri);
-  p.rect = take(sizeof(Tile) * rect);
+  for (int k = 0; k < p.chains; ++k) {
+    const Work& w = p.w[k];
+    fill += w.fill, part += w.part, halves += w.halves;
+    entries += (uint64_t)w.c.n_gram + w.c.n_tri + w.c.n_rect;
+    p.gram[k] = take(sizeof(Tile) * (size_t)w.c.n_gram);
+    p.tri[k] = take(sizeof(Tile) * (size_t)w.c.n_tri);
+    p.rect[k] = take(sizeof(Tile) * (size_t)w.c.n_rect);
+  }
+  if (entries + fill + norm > 0x7fffffff) return -1;  // (of the lists' kernel)
+  l.n_fill = (unsigned)fill, l.n_norm = (unsigned)norm;
+  l.second = p.w[0].count;
+  p.table = take(sizeof(Mat) * (size_t)(p.w[0].count + (p.chains > 1 ? p.w[1].count : 0)));
   p.fill = take(sizeof(Tile) * fill);
   p.norm_map = take(sizeof(uint2) * norm);
   p.norms = take(sizeof(double) * norm);
@@ -1291,113 +1409,147 @@ void choose(int ts, const F& f) {  // f(tile) with the tile a constant
   else f(std::integral_constant<int, 64>());
 }
 
-// Where every pass has at most a tile a compute unit, the two passes over X are launches like the others: steps are taken
-// one by one, if X X^t is a launch as well (250 x 250: 104 us, 111 in groups; 300 x 300: 117, 126) or a matrix is narrow.
-bool one_by_one(const Plan& p) {
-  const Lists& l = p.l;
-  const unsigned most = WANT / 2;
-  return l.gram_ts == 64 && l.tri_ts == 64 && l.rect_ts == 64 && l.n_gram <= most && l.n_tri <= most && l.n_rect <= most &&
-         (!p.split || p.narrow < NARROW);
-}
-// The chains of a list, one behind the other in one workspace: all but the small ones together in single steps, where that is
-// as fast; else the wide ones in groups and the narrow ones in single steps.
-struct Chains {
-  struct {
-    int kinds;
-    bool single;
-    Plan p;
-  } of[2];
-  int many;
-  size_t total;
+// The narrow chain's launches but its last, one after the other, for those of the wide one to take along.
+struct Rides {
+  const Chain* c;  // (null: none)
+  int kc;
+  bool split;
+  int steps;  // that are left
+  Op op;      // of its products
+  int what = RIDE_GRAM, from = 0;
+  bool left() const { return c && (steps > 1 || what != RIDE_APPLY); }
+  Rider next() {
+    if (!left()) return Rider{};
+    Rider r{c->gram, c->n_gram, what, from, kc, op};
+    if (what == RIDE_GRAM) {
+      what = split ? RIDE_SUM : RIDE_POLY;
+    } else if (what == RIDE_SUM) {
+      r.blocks *= 2, what = RIDE_POLY;
+    } else if (what == RIDE_POLY) {
+      r.list = c->tri, r.blocks = c->n_tri, what = RIDE_APPLY;
+    } else {
+      r.list = c->rect, r.blocks = c->n_rect, what = RIDE_GRAM;
+      from ^= 1, --steps;
+    }
+    return r;
+  }
 };
-int chains(int count, const int* rows, const int* cols, Chains& c) {
-  c.many = 0, c.total = 256;  // (nothing but small matrices needs nothing)
-  if (!taken(count, rows, cols)) return -1;
-  const auto add = [&](int kinds, bool single, const Plan& p) {
-    c.of[c.many++] = {kinds, single, p};
-    if (p.total > c.total) c.total = p.total;
-  };
-  int kinds = 0;
-  for (int i = 0; i < count; ++i) kinds |= kind(rows[i], cols[i]) & (NARROWS | WIDES);
-  if (!kinds) return 0;
-  Plan p;
-  if (plan(count, rows, cols, kinds, p) != 0) return -1;
-  if (kinds != (NARROWS | WIDES) || one_by_one(p)) {
-    add(kinds, kinds == NARROWS || one_by_one(p), p);
-    return 0;
-  }
-  for (int k : {WIDES, NARROWS}) {
-    if (plan(count, rows, cols, k, p) != 0) return -1;
-    add(k, k == NARROWS, p);
-  }
-  return 0;
-}
 
-template <typename T, typename Matrix>
-int chain(int count, const Matrix& matrix, const int* rows, const int* cols, int kinds, bool single, const Momentum& m,
-          float decay, int steps, const Poly& f, double eps, const Plan& p, char* ws, hipStream_t st) {
-  Lists l = p.l;
-  l.table = reinterpret_cast<Mat*>(ws + p.table);
-  l.gram = reinterpret_cast<Tile*>(ws + p.gram);
-  l.tri = reinterpret_cast<Tile*>(ws + p.tri);
-  l.rect = reinterpret_cast<Tile*>(ws + p.rect);
-  l.fill = reinterpret_cast<Tile*>(ws + p.fill);
-  l.norm_map = reinterpret_cast<uint2*>(ws + p.norm_map);
+template <typename T>
+int run(int count, const void* const* src, void* const* dst, float* const* buf, const int* rows, const int* cols,
+        const float* rates, float decay, float mu, int nesterov, int steps, const Poly& f, double eps, const Plan& p, char* ws,
+        hipStream_t st) {
+  const int update = buf != nullptr;
+  const Momentum m{update, nesterov, mu};
+  const dim3 wg(256);
+  const auto matrix = [&](int i) {
+    return Mat{src[i], dst[i], update ? buf[i] : nullptr, rows[i], cols[i], rates ? rates[i] : 0.f, 1};
+  };
+  for (int i = 0; i < count;) {
+    Batch batch{};
+    for (; i < count && batch.count < BATCH; ++i)
+      if (kind(rows[i], cols[i]) == SMALLS) batch.m[batch.count++] = matrix(i);
+    if (batch.count)
+      hipLaunchKernelGGL((ortho_small_kernel<T>), dim3(batch.count), dim3(SMALL_THREADS), 0, st, batch, m, Step{f.c, f.t, f.q, f.l}, steps, eps,
+                         decay);
+    if (hipGetLastError() != hipSuccess) return -2;
+  }
+  if (p.chains == 0) return 0;
+  Lists lists = p.l;
+  lists.table = reinterpret_cast<Mat*>(ws + p.table);
+  lists.fill = reinterpret_cast<Tile*>(ws + p.fill);
+  lists.norm_map = reinterpret_cast<uint2*>(ws + p.norm_map);
+  for (int k = 0; k < p.chains; ++k) {
+    lists.c[k] = p.w[k].c;
+    lists.c[k].gram = reinterpret_cast<Tile*>(ws + p.gram[k]);
+    lists.c[k].tri = reinterpret_cast<Tile*>(ws + p.tri[k]);
+    lists.c[k].rect = reinterpret_cast<Tile*>(ws + p.rect[k]);
+  }
   double* norms = reinterpret_cast<double*>(ws + p.norms);
   float* parts = reinterpret_cast<float*>(ws + p.parts);
   _Float16* base = reinterpret_cast<_Float16*>(ws + p.halves);
-  unsigned gram = 0, tri = 0, rect = 0, fill = 0, norm = 0;
-  size_t halves = 0, part = 0;
-  const dim3 wg(256);
-  for (int i = 0, first = 0; first < l.count;) {
-    Batch batch{};
-    const uint64_t was = (uint64_t)gram + tri + rect + fill + norm;
-    for (; i < count && batch.count < BATCH; ++i) {
-      if (!(kind(rows[i], cols[i]) & kinds)) continue;
-      const Dim d(rows[i], cols[i]);
-      const unsigned s = (unsigned)((d.mp + p.kc - 1) / p.kc);
-      Mat& t = batch.m[batch.count++];
-      t = matrix(i);
-      t.splits = s;
-      t.gram0 = gram, t.tri0 = tri, t.rect0 = rect, t.fill0 = fill, t.norm0 = norm, t.part0 = part, t.at = halves;
-      gram += d.tri(l.gram_ts) * s;
-      tri += d.tri(l.tri_ts);
-      rect += d.rect(l.rect_ts);
-      fill += d.rect(64);
-      norm += d.norms(l.chunk);
-      if (s > 1) part += (size_t)d.tri(l.gram_ts) * s * l.gram_ts * l.gram_ts;
-      halves += d.halves(l.rect_ts);
+  {
+    Mat next{};  // (what the next matrix's entries begin at)
+    if (p.chains > 1) {  // (the second chain's begin behind the first's, before those were quartered)
+      Chain& c = lists.c[1];
+      for (int i = 0; i < count; ++i) {
+        if (!(kind(rows[i], cols[i]) & p.w[0].kinds)) continue;
+        const Dim d(rows[i], cols[i]);
+        c.gram0 += d.tri(lists.c[0].gram_ts) * p.w[0].parts_of(d), c.tri0 += d.tri(lists.c[0].tri_ts);
+        c.rect0 += d.rect(lists.c[0].rect_ts);
+      }
     }
-    batch.end.gram0 = gram, batch.end.tri0 = tri, batch.end.rect0 = rect, batch.end.fill0 = fill, batch.end.norm0 = norm;
-    const uint64_t entries = (uint64_t)gram + tri + rect + fill + norm - was;
-    hipLaunchKernelGGL(ortho_lists_kernel, dim3((unsigned)((entries + 255) / 256)), wg, 0, st, l, batch, (unsigned)first);
+    unsigned first = 0;
+    Batch batch{};
+    const auto flush = [&] {
+      batch.end = next;
+      const Mat& was = batch.m[0];
+      const unsigned entries = next.gram0 - was.gram0 + (next.tri0 - was.tri0) + (next.rect0 - was.rect0) +
+                               (next.fill0 - was.fill0) + (next.norm0 - was.norm0);
+      hipLaunchKernelGGL(ortho_lists_kernel, dim3((entries + 255) / 256), wg, 0, st, lists, batch, first);
+      first += batch.count;
+      batch.count = 0;
+    };
+    for (int k = 0; k < p.chains; ++k)
+      for (int i = 0; i < count; ++i) {
+        const Work& w = p.w[k];
+        if (!(kind(rows[i], cols[i]) & w.kinds)) continue;
+        const Dim d(rows[i], cols[i]);
+        Mat& t = batch.m[batch.count++];
+        t = matrix(i);
+        t.splits = w.parts_of(d);
+        t.gram0 = next.gram0, t.tri0 = next.tri0, t.rect0 = next.rect0, t.fill0 = next.fill0, t.norm0 = next.norm0;
+        t.part0 = next.part0, t.at = next.at;
+        next.gram0 += d.tri(w.c.gram_ts) * t.splits;
+        next.tri0 += d.tri(w.c.tri_ts);
+        next.rect0 += d.rect(w.c.rect_ts);
+        next.fill0 += d.rect(64);
+        next.norm0 += d.norms(lists.chunk);
+        if (t.splits > 1) next.part0 += (size_t)d.tri(w.c.gram_ts) * t.splits * w.c.gram_ts * w.c.gram_ts;
+        next.at += d.halves(w.c.rect_ts);
+        if (batch.count == BATCH) flush();
+      }
+    if (batch.count) flush();
     if (hipGetLastError() != hipSuccess) return -2;
-    first += batch.count;
   }
-  hipLaunchKernelGGL((ortho_norm_kernel<T>), dim3(l.n_norm), wg, 0, st, l, norms, m);
-  hipLaunchKernelGGL((ortho_start_kernel<T>), dim3(l.n_fill), wg, 0, st, l, norms, base, m, eps);
+  hipLaunchKernelGGL((ortho_norm_kernel<T>), dim3(lists.n_norm), wg, 0, st, lists, norms, m);
+  hipLaunchKernelGGL((ortho_start_kernel<T>), dim3(lists.n_fill), wg, 0, st, lists, norms, base, m, eps);
   if (hipGetLastError() != hipSuccess) return -2;
   const unsigned cus = (unsigned)r3_cu_count();
-  const auto square = [&](const Op& one, const Op* two, bool add = false) {
-    const dim3 grid(l.n_tri, two ? 2 : 1);
-    const auto launch = [&](auto core, auto ADD) {
-      typedef decltype(core) C;
-      hipLaunchKernelGGL((ortho_square_kernel<C, ADD()>), grid, dim3(C::THREADS), 0, st, l, base, one, two ? *two : one);
-    };
-    // A tile a compute unit: eight wavefronts share its sum and its epilogue (eight of 256 x 256: 7.3 us, four 8.4; more
-    // tiles than that share the units anyway: 2048 x 2048, 56 against 53).
-    if (l.tri_ts == 128) launch(Core128(), std::false_type());
-    else if (add) launch(Core64<8>(), std::true_type());
-    else if (grid.x * grid.y <= cus) launch(Core64<8>(), std::false_type());
-    else launch(Core64<4>(), std::false_type());
-  };
-  const auto both = [&](const Op& one, const Op& two, bool add = false) { square(one, &two, add); };
   const auto polynomial_of = [&](Stored out, Stored a) {
     Op r(out, a, f.t, a, f.t, f.c);
     r.q = f.q, r.l = f.l, r.lo = f.l * (out.scale / a.scale);
     return r;
   };
   const auto times = [](Stored out, Stored g, Stored h) { return Op(out, g, 0.f, h, 0.f, 1.f); };
+  const auto of_step = [&] { return polynomial_of(Stored{SQ_F, SCALE}, Stored{SQ_A, SCALE}); };
+  // The narrow chain rides where it is in tiles of 64 throughout (one in larger ones has work for the card by itself).
+  const Chain& second = lists.c[1];
+  const bool riding = p.chains > 1 && second.gram_ts == 64 && second.tri_ts == 64 && second.rect_ts == 64;
+  Rides rides{riding ? &second : nullptr, p.w[1].kc, p.w[1].split, steps, of_step()};
+  const auto chain = [&](const Chain& l, const Work& w) {
+  const auto square = [&](const Op& one, const Op* two, bool add = false) {
+    const Rider r = rides.next();
+    const dim3 grid(r.blocks + l.n_tri, two ? 2 : 1);
+    const auto launch_as = [&](auto core, auto ADD, auto RIDE) {
+      typedef decltype(core) C;
+      hipLaunchKernelGGL((ortho_square_kernel<C, ADD(), RIDE()>), grid, dim3(C::THREADS), 0, st, l, r, base, parts, one,
+                         two ? *two : one);
+    };
+    const auto launch = [&](auto core, auto ADD) {
+      if (r.blocks) launch_as(core, ADD, std::true_type());
+      else launch_as(core, ADD, std::false_type());
+    };
+    // A tile a compute unit: eight wavefronts share its sum and its epilogue (eight of 256 x 256: 7.3 us, four 8.4; more
+    // tiles than that share the units anyway: 2048 x 2048, 56 against 53).
+    const bool eight = r.blocks + l.n_tri * grid.y <= cus;
+    if (l.tri_ts == 128) launch(Core128(), std::false_type());
+    else if (add && eight) launch(Core64<8>(), std::true_type());
+    else if (add) launch(Core64<4>(), std::true_type());
+    else if (eight) launch(Core64<8>(), std::false_type());
+    else launch(Core64<4>(), std::false_type());
+  };
+  const auto both = [&](const Op& one, const Op& two, bool add = false) { square(one, &two, add); };
   // R of a group of g steps, in launches of at most two products
   const auto group = [&](int g) {
     const Stored A{SQ_A, SCALE}, FA{SQ_FA, SCALE};
@@ -1444,76 +1596,78 @@ int chain(int count, const Matrix& matrix, const int* rows, const int* cols, int
   const bool brief = f.brief && l.tri_ts == 64 && 2 * l.n_tri <= cus;
   int from = 0;
   for (int left = steps; left > 0;) {
-    int g = single ? 1 : group_length(left, steps);
+    int g = w.single ? 1 : group_length(left, steps);
     if (g > f.longest) g = f.longest;
     choose(l.gram_ts, [&](auto TS) {
-      hipLaunchKernelGGL((ortho_gram_kernel<TS()>), dim3(l.n_gram), wg, 0, st, l, base, parts, p.kc, from);
-      if (p.split) hipLaunchKernelGGL((ortho_sum_kernel<TS()>), dim3(l.n_gram, TS() / 32), wg, 0, st, l, base, parts);
+      const Rider r = rides.next();
+      const auto launch = [&](auto RIDE) {
+        hipLaunchKernelGGL((ortho_gram_kernel<TS(), RIDE()>), dim3(r.blocks + l.n_gram), wg, 0, st, l, r, base, parts, w.kc, from);
+      };
+      if (r.blocks) launch(std::true_type());
+      else launch(std::false_type());
+      if (w.split) hipLaunchKernelGGL((ortho_sum_kernel<TS()>), dim3(l.n_gram, TS() / 32), wg, 0, st, l, base, parts);
     });
     const Stored R = brief ? brief_group(g) : group(g);
     left -= g;
-    const float fs = 1.f / R.scale;
-    choose(l.rect_ts, [&](auto TS) {
-      const dim3 grid(l.n_rect);
-      if (left)
-        hipLaunchKernelGGL((ortho_apply_kernel<T, false, TS()>), grid, wg, 0, st, l, base, R.at, fs, from, m.update, decay);
-      else
-        hipLaunchKernelGGL((ortho_apply_kernel<T, true, TS()>), grid, wg, 0, st, l, base, R.at, fs, from, m.update, decay);
-    });
+    if (left) {
+      choose(l.rect_ts, [&](auto TS) {
+        const Rider r = rides.next();
+        const auto launch = [&](auto RIDE) {
+          hipLaunchKernelGGL((ortho_apply_kernel<TS(), RIDE()>), dim3(r.blocks + l.n_rect), wg, 0, st, l, r, base, parts, R.at,
+                             1.f / R.scale, from);
+        };
+        if (r.blocks) launch(std::true_type());
+        else launch(std::false_type());
+      });
+    } else {
+      while (rides.left()) {
+        const Rider r = rides.next();
+        hipLaunchKernelGGL((ortho_square_kernel<Core64<8>, false, true>), dim3(r.blocks), dim3(512), 0, st, l, r, base, parts, Op{},
+                           Op{});
+      }
+      choose(l.rect_ts, [&](auto TS) {
+        const unsigned others = rides.c ? rides.c->n_rect : 0;
+        hipLaunchKernelGGL((ortho_apply_last_kernel<T, TS()>), dim3(others + l.n_rect), wg, 0, st, lists.table, l,
+                           Product{R.at, from, 1.f / R.scale}, second.rect, others, Product{SQ_F, rides.from, 1.f / SCALE}, base,
+                           update, decay);
+      });
+    }
     from ^= 1;
     if (hipGetLastError() != hipSuccess) return -2;
   }
   return 0;
-}
-
-template <typename T>
-int run(int count, const void* const* src, void* const* dst, float* const* buf, const int* rows, const int* cols,
-        const float* rates, float decay, float mu, int nesterov, int steps, const Poly& f, double eps, const Chains& c, char* ws,
-        hipStream_t st) {
-  const int update = buf != nullptr;
-  const Momentum m{update, nesterov, mu};
-  const auto matrix = [&](int i) {
-    return Mat{src[i], dst[i], update ? buf[i] : nullptr, rows[i], cols[i], rates ? rates[i] : 0.f, 1};
   };
-  for (int i = 0; i < count;) {
-    Batch batch{};
-    for (; i < count && batch.count < BATCH; ++i)
-      if (kind(rows[i], cols[i]) == SMALLS) batch.m[batch.count++] = matrix(i);
-    if (batch.count)
-      hipLaunchKernelGGL((ortho_small_kernel<T>), dim3(batch.count), dim3(SMALL_THREADS), 0, st, batch, m, Step{f.c, f.t, f.q, f.l}, steps, eps,
-                         decay);
-    if (hipGetLastError() != hipSuccess) return -2;
-  }
-  for (int k = 0; k < c.many; ++k) {
-    const int rc = chain<T>(count, matrix, rows, cols, c.of[k].kinds, c.of[k].single, m, decay, steps, f, eps, c.of[k].p, ws, st);
+  for (int k = 0; k < (riding ? 1 : p.chains); ++k) {
+    const int rc = chain(lists.c[k], p.w[k]);
     if (rc != 0) return rc;
   }
   return 0;
 }
+
 }  // namespace
 
 size_t r3k_ortho_workspace_bytes(int count, const int* rows, const int* cols) {
-  Chains c;
-  return count > 0 && chains(count, rows, cols, c) == 0 ? c.total : 0;
+  Plan p;
+  return count > 0 && plan(count, rows, cols, p) == 0 ? p.total : 0;
 }
 
 int r3k_ortho(int count, const void* const* src, void* const* dst, float* const* buf, int dtype, const int* rows,
               const int* cols, const float* rates, float decay, float mu, int nesterov, int steps, float a, float b, float c,
               double eps, void* ws, size_t ws_bytes, hipStream_t st) {
-  Chains plans;
-  if (chains(count, rows, cols, plans) != 0 || dtype < 0 || dtype > 2 || steps < 1 || steps > 64 || !(eps >= 0)) return -1;
+  Plan p;
+  if (plan(count, rows, cols, p) != 0 || dtype < 0 || dtype > 2 || steps < 1 || steps > 64 || !(eps >= 0)) return -1;
   const Poly f = polynomial(steps, a, b, c);
   if (!f.longest) return -1;
   if (count == 0) return 0;
   if (!src || !dst || (buf && !rates)) return -1;
   for (int i = 0; i < count; ++i)
     if (!src[i] || !dst[i] || (buf && !buf[i])) return -1;
-  if (!ws || ws_bytes < plans.total) return -3;
+  if (!ws || ws_bytes < p.total) return -3;
   char* w = static_cast<char*>(ws);
   if (reinterpret_cast<uintptr_t>(w) & 15) return -1;
   switch (dtype) {
-    case 0: return run<float>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, plans, w, st);
-    case 1: return run<_Float16>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, plans, w, st);
-    default: return run<__bf16>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, plans, w, st);
+    case 0: return run<float>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, p, w, st);
+    case 1: return run<_Float16>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, p, w, st);
+    default: return run<__bf16>(count, src, dst, buf, rows, cols, rates, decay, mu, nesterov, steps, f, eps, p, w, st);
   }
 }

@@ -369,3 +369,44 @@ def test_neighbours_in_a_list_change_nothing_of_a_narrow_matrix_s_accuracy():
         want, norms = iterate(g)
         off = [(o.double() - want).norm().item() for o in (beside, alone)]
         assert off[0] <= 4 * off[1] + 4 * U * norms[-1], (tuple(g.shape), off)
+
+
+MIXED = [(300, 500), (100, 900), (5, 700), (64, 64), (1100, 1300), (200, 210), (4097, 65), (15, 2304), (256, 256), (1, 5000)]
+
+
+@pytest.mark.parametrize("steps,co,slope", [(s, COEFFICIENTS, 4.0) for s in (1, 2, 3, 4, 5, 6, 9)] +
+                         [(7, (1.5, -0.5, 0.0), 1.5), (5, (15 / 8, -10 / 8, 3 / 8), 1.9)])
+def test_narrow_and_wide_matrices_together(steps, co, slope):
+    """Two chains of launches, the narrow one's pieces among the wide one's: more, as many and fewer of them than launches."""
+    check([matrix(*s, seed=i) for i, s in enumerate(MIXED)], steps=steps, co=co, slope=slope)
+    check([matrix(*s, dtype="bf16", seed=i) for i, s in enumerate(MIXED[::-1])], steps=steps, co=co, slope=slope)
+
+
+@pytest.mark.parametrize("wide", [39, 40, 41])
+def test_chains_that_end_anywhere_in_a_table(wide):
+    shapes = [(260, 300 + i) for i in range(wide)]
+    shapes[7:7] = [(100, 300), (64, 50), (3, 999)]
+    check([matrix(*s, seed=i) for i, s in enumerate(shapes + [(200, 222)])])
+
+
+def test_many_narrow_matrices_beside_a_wide_one():
+    """A chain of its own work for the whole card, in tiles of 128, behind the wide one's."""
+    check([matrix(200, 300, seed=i) for i in range(90)] + [matrix(1100, 1300)] + [matrix(130, 1000, seed=i) for i in range(90)])
+
+
+def test_many_wide_matrices_beside_narrow_ones():
+    """The wide ones in tiles of 128, quartered ones among them, with pieces of 64 along."""
+    check([matrix(300, 400, seed=i) for i in range(52)] + [matrix(100, 700), matrix(9, 2000)] +
+          [matrix(700, 900, seed=i) for i in range(13)])
+
+
+def test_update_of_a_head():
+    shapes = [(256, 2304)] * 8 + [(135, 2304), (45, 2304), (64, 100)]
+    gen = torch.Generator().manual_seed(6)
+    ws, gs, ms = ([torch.randn(s, generator=gen).to(DEV) for s in shapes] for _ in range(3))
+    before = [(w.clone(), m.clone()) for w, m in zip(ws, ms)]
+    orthogonal_update_(ws, gs, ms, lr=0.05, momentum=0.9, weight_decay=0.01)
+    for w, g, m, (w0, m0) in zip(ws, gs, ms, before):
+        want_w, want_m, tol = update_by_formula(w0, g, m0, 0.05, 0.9, True, 0.01, "rms")
+        assert ((m.double() - want_m).abs() <= 3 * U * (want_m.abs() + m0.abs().double() + g.abs().double())).all()
+        assert (w.double() - want_w).norm() <= tol + 5 * U * want_w.norm().item()
