@@ -8,6 +8,7 @@ which the rotated heads' ``use_sigmoid_cls=False`` branch selects) and the ranki
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _C
 
@@ -101,8 +102,8 @@ def label_log_probs(logits, labels=None, top_k=0, entropy=True, ignore_index=Non
     label is outside [0, classes) -- nothing here reads labels on the host), ``entropy`` the row's -sum p log p, the top
     ones its ``top_k`` <= min(classes, 64) best classes in order, ties to the lowest index.  Logits of -inf are classes
     that are not offered: a row with none left has log probabilities of -inf, the entropy 0 and no gradient.  NaN or +inf
-    in a row makes its numbers NaN; NaN is ranked first.  Differentiable (once) through all but ``top_index``; the logits must stay as they
-    are until the backward pass.  Rows may be any distance apart; other strides are copied first.  Works on the current
+    in a row makes its numbers NaN; NaN is ranked first.  Differentiable (once, backwards; dual tensors are refused) through all but
+    ``top_index``; the logits must stay as they are until the backward pass.  Rows may be any distance apart; other strides are copied first.  Works on the current
     stream of the logits' device; nothing synchronises with the host."""
     if not isinstance(logits, torch.Tensor) or logits.dim() < 1:
         raise TypeError("logits must be a tensor of at least one dimension")
@@ -124,6 +125,8 @@ def label_log_probs(logits, labels=None, top_k=0, entropy=True, ignore_index=Non
             raise RuntimeError(f"labels are on {labels.device}, logits on {logits.device}")
         if labels.shape != logits.shape[:-1]:
             raise ValueError(f"labels must have the shape {tuple(logits.shape[:-1])}, got {tuple(labels.shape)}")
+    if forward_ad.unpack_dual(logits).tangent is not None:  # (requires_grad says nothing of these)
+        raise RuntimeError("label_log_probs has no forward-mode derivative: its result would have no tangent")
     if not logits.is_cuda:
         raise RuntimeError("logits must be a CUDA tensor (HIP device tensor on ROCm)")
     if logits.requires_grad and torch.is_grad_enabled():

@@ -374,3 +374,20 @@ def test_captured_and_replayed(rows, classes):
         torch.cuda.synchronize()
         for a, b in zip(out, eager):
             assert torch.equal(a, b)
+
+
+def test_forward_mode_is_refused_and_not_lost():
+    from torch.autograd import forward_ad
+
+    from r3det.models.losses import CrossEntropyLoss
+    x, y = torch.randn(6, 9, device=DEV), torch.arange(6, device=DEV)
+    want = label_log_probs(x, y)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: label_log_probs(dual, y), lambda: CrossEntropyLoss()(dual, y)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        got = label_log_probs(x, y)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: label_log_probs(t, y).log_prob, (x,), (torch.ones_like(x),))
+    assert torch.equal(got.log_prob, want.log_prob) and torch.equal(got.entropy, want.entropy)

@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from r3det import _C
 from r3det.ops.log_probs import label_log_probs
@@ -61,3 +62,17 @@ def test_refusals_of_the_c_entries():
     for bad in (dict(x=None), dict(dtype=3), dict(rows=-1), dict(classes=0), dict(stats=None), dict(dx=None), dict(labels=None),
                 dict(h=None), dict(dtop=p), dict(k=2, dtop=p, ix=None)):
         assert backward(**bad) == -1, bad
+
+
+def test_dual_tensors_are_refused():
+    """A dual tensor needs no gradient: computed all the same, its result would have no tangent, which reads as zero."""
+    x, y = torch.randn(3, 5), torch.zeros(3, dtype=torch.int64)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        assert not dual.requires_grad
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            label_log_probs(dual, y)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            label_log_probs(dual, y)
+        with pytest.raises(RuntimeError, match="CUDA tensor"):  # (no tangent: the next check's)
+            label_log_probs(x, y)
