@@ -264,9 +264,11 @@ struct Best {
   unsigned long long bound = 0;  // what k keys are known to pass, the list's or not (uniform)
   unsigned long long least = 0;  // what a key has to pass: the k-th best, or `bound`
   float floor = -__builtin_inff();  // its value
-  // The j-th greatest of the lanes' `high`, by its upper 16 bits (0: fewer have `any`).
-  static __device__ __forceinline__ unsigned of_lanes(bool any, float high, int j) {
-    const unsigned mine = any ? ord(high) >> 16 : 0u;
+  // A value by the upper 16 bits of its place in the order (0: a masked class, which is no key).  They stay numbers from here
+  // on: widened to a float's 32 bits again, those of an infinity would be a NaN's, and those of a tiny negative number's -0's.
+  static __device__ __forceinline__ unsigned upper(float x) { return x != -__builtin_inff() ? ord(x) >> 16 : 0u; }
+  // The j-th greatest of the lanes' (0: fewer have any).
+  static __device__ __forceinline__ unsigned of_lanes(unsigned mine, int j) {
     unsigned t = 0;
 #pragma unroll
     for (int b = 15; b >= 0; --b) {
@@ -402,18 +404,17 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void logprob_row_ker
 #pragma unroll
         for (int u = 1; u < UNROLL; ++u) most = __builtin_elementwise_maximum(most, high[u]);  // (packs that are not there are -inf)
         if constexpr (WAVES == 1) {
-          best.seed(Best::of_lanes(most != -__builtin_inff(), most, o.k));
+          best.seed(Best::of_lanes(Best::upper(most), o.k));
         } else {
           constexpr int EACH = 64 / WAVES;
           const int whole = packs / 64 < WAVES ? (int)(packs / 64) : WAVES;  // wavefronts with a pack for every lane
           if (whole * EACH >= o.k) {
-            const unsigned mine = most != -__builtin_inff() ? ord(most) >> 16 : 0u, t = Best::of_lanes(mine != 0, most, EACH);
+            const unsigned mine = Best::upper(most), t = Best::of_lanes(mine, EACH);
             const unsigned long long in = __ballot(mine >= t);
             const int rank = __popcll(in & ((1ull << lane) - 1));
             if (mine >= t && rank < EACH) reached[wave * EACH + rank] = mine;  // (t = 0: zeros among them)
             __syncthreads();
-            const unsigned best_of = lane < whole * EACH ? reached[lane] : 0u;
-            best.seed(Best::of_lanes(best_of != 0, unord(best_of << 16 | 0xffffu), o.k));
+            best.seed(Best::of_lanes(lane < whole * EACH ? reached[lane] : 0u, o.k));
           }
         }
       }

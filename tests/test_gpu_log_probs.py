@@ -391,3 +391,38 @@ def test_forward_mode_is_refused_and_not_lost():
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda t: label_log_probs(t, y).log_prob, (x,), (torch.ones_like(x),))
     assert torch.equal(got.log_prob, want.log_prob) and torch.equal(got.entropy, want.entropy)
+
+
+@pytest.mark.parametrize("k", [1, 2, 3, 20])
+@pytest.mark.parametrize("rows,classes", [(9, 40), (9, 100), (9, 900), (9, 1025), (9, 4000), (9, 70000), (300, 4000)])
+def test_infinities_are_ranked_as_values(rows, classes, k):
+    """One, two and many of +inf at a row's beginning, in its middle and at its end: their places come first, in order."""
+    x = torch.randn(rows, classes, generator=torch.Generator().manual_seed(3)).to(DEV)
+    x[0, 5] = math.inf
+    x[1, classes // 2] = math.inf
+    x[2, classes - 1] = math.inf
+    x[3, 7] = x[3, 30] = math.inf
+    x[4, ::3] = math.inf
+    x[5] = math.inf
+    x[6] = -math.inf
+    x[6, 11] = math.inf
+    x[7, 8:] = -math.inf
+    x[7, 3] = math.inf
+    for t in (torch.float32, torch.bfloat16):
+        got = label_log_probs(x.to(t), top_k=k)
+        want = reference(x.to(t), k=k)["top_index"]
+        assert torch.equal(got.top_index.cpu(), want)
+        assert got.top_log_prob[:6].isnan().all() and got.entropy[:8].isnan().all()
+        assert torch.equal(got.top_index[5].cpu(), torch.arange(k))
+
+
+@pytest.mark.parametrize("k", [1, 3, 20])
+@pytest.mark.parametrize("rows,classes", [(3, 100), (3, 900), (3, 4000), (3, 70000), (300, 4000)])
+def test_smallest_negative_numbers_are_ranked_as_values(rows, classes, k):
+    """Subnormal logits below zero, next to -0 in the order."""
+    step = torch.randint(1, 30000, (rows, classes), generator=torch.Generator().manual_seed(4))
+    x = -(step * 2.0 ** -149).to(torch.float32).to(DEV)
+    assert (x < 0).all()
+    got = label_log_probs(x, top_k=k)
+    assert torch.equal(got.top_index.cpu(), reference(x, k=k)["top_index"])
+    assert (got.top_log_prob + math.log(classes)).abs().max() <= (classes / 64 + 60) * U + 2e-6
