@@ -14,7 +14,7 @@ import torch.distributed as dist
 from torch.nn.parallel import DistributedDataParallel
 
 from .models.detectors import parse_losses
-from .ops.orthogonalize import COEFFICIENTS, DTYPES, STEPS, orthogonal_update_
+from .ops.orthogonalize import COEFFICIENTS, DTYPES, STEPS, alike, orthogonal_update_
 
 # xGMI is point to point (7 links x ~153 GB/s per GPU): a ring all-reduce is bound per link, and the
 # 168 MB of fp32 gradients of R3Det-R50 go out in few, large buckets -- 4 x ~48 MB instead of torch's
@@ -77,15 +77,15 @@ class Muon(torch.optim.Optimizer):
                 raise ValueError('Muon: weights are fp32, fp16 or bf16, and of two and more dimensions in an orthogonal '
                                  'group; put the others into a group with orthogonal=False')
 
-    def _momentum(self, p):
+    def _momentum(self, p, orthogonal):
         state = self.state[p]
         m = state.get('momentum_buffer')
-        if m is None:
-            if p.is_cuda and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError('Muon: take one step before the capture (a replay would begin without momentum again)')
-            m = torch.zeros_like(p, dtype=torch.float32)
-        elif m.stride() != p.stride() or m.device != p.device:  # (the weight was laid out anew, or the state loaded)
-            m = torch.empty_like(p, dtype=torch.float32).copy_(m)
+        # (laid out as the weight is where both are one matrix; the others' may be any way)
+        if m is not None and m.device == p.device and (not orthogonal or alike(m, p)):
+            return m
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('Muon: take one step before the capture (every replay would begin with the momentum as it is now)')
+        m = torch.zeros_like(p, dtype=torch.float32) if m is None else torch.empty_like(p, dtype=torch.float32).copy_(m)
         state['momentum_buffer'] = m
         return m
 
@@ -96,14 +96,14 @@ class Muon(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for g in self.param_groups:
-            alike = {}  # (one call takes weights of one type on one device)
+            kinds = {}  # (one call takes weights of one type on one device)
             for p in g['params']:
                 if p.grad is not None:
                     if p.grad.is_sparse:
                         raise RuntimeError('Muon: sparse gradients are not taken')
-                    alike.setdefault((p.device, p.dtype), []).append(p)
-            for ps in alike.values():
-                grads, buffers = [p.grad for p in ps], [self._momentum(p) for p in ps]
+                    kinds.setdefault((p.device, p.dtype), []).append(p)
+            for ps in kinds.values():
+                grads, buffers = [p.grad for p in ps], [self._momentum(p, g['orthogonal']) for p in ps]
                 if g['orthogonal']:
                     orthogonal_update_(ps, grads, buffers, g['lr'], g['momentum'], g['nesterov'], g['weight_decay'], g['steps'],
                                        g['coefficients'], g['eps'], g['scale'])

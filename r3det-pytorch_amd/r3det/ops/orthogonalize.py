@@ -93,7 +93,7 @@ def orthogonalize(tensors, steps=STEPS, coefficients=COEFFICIENTS, eps=1e-7):
     return outs[0] if one else outs
 
 
-def _alike(t, like):
+def alike(t, like):
     """Whether two tensors of one shape have the same strides, where those say something (a dimension of size one has any)."""
     return t.stride() == like.stride() or all(n < 2 or a == b for a, b, n in zip(t.stride(), like.stride(), t.shape))
 
@@ -153,9 +153,9 @@ def orthogonal_update_(params, grads, buffers, lr, momentum=0.95, nesterov=True,
             raise RuntimeError(f"grads must be of their weight's type {p.dtype}, got {g.dtype}")
         if m.dtype != torch.float32:
             raise RuntimeError(f"buffers must be fp32, got {m.dtype}")
-        if not _dense(p) or not (_alike(m, p) or p.numel() == 0):
+        if not _dense(p) or not (alike(m, p) or p.numel() == 0):
             raise RuntimeError("params must be contiguous or channels_last, and their buffers laid out alike")
-    live = [(p, g, m, _alike(g, p)) for p, g, m in zip(params, grads, buffers) if p.numel()]
+    live = [(p, g, m, alike(g, p)) for p, g, m in zip(params, grads, buffers) if p.numel()]
     ps, ms = [t[0] for t in live], [t[2] for t in live]
     _apart(ps, ms, [g for _, g, _, alike in live if alike])
     _same(params, "params")

@@ -306,3 +306,59 @@ def test_gradient_of_the_class_biases_against_differences():
         # (the differences' share, and n additions of gradients of at most 1 / avg by the convolution's backward pass)
         share = float(w[:, a::A].sum()) / avg
         assert abs(float(h.retina_cls.bias.grad[channel]) - want) <= step ** 2 / 6 / (6 * 3 ** 0.5) * share + 1e-5
+
+
+def captured(opt):
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        opt.step()
+    return graph
+
+
+def test_momentum_of_a_strided_weight_goes_on_through_replays():
+    """A weight that no tensor is laid out like (every second element of another): its momentum stays where it is."""
+    from r3det.dist_train import Muon
+    g = torch.randn(12, device=DEV)
+    pair = [torch.nn.Parameter(torch.arange(24.0, device=DEV)[::2]) for _ in range(2)]
+    opts = [Muon([dict(params=[p], orthogonal=False)], lr=0.1) for p in pair]
+    assert pair[0].stride() == (2,)
+    for p, o in zip(pair, opts):
+        p.grad = g.clone()
+        o.step()
+        at = o.state[p]['momentum_buffer']
+        o.step()
+        assert o.state[p]['momentum_buffer'] is at
+    graph = captured(opts[0])
+    for _ in range(4):
+        graph.replay()
+        opts[1].step()
+        torch.cuda.synchronize()
+        assert torch.equal(pair[0], pair[1])
+        assert torch.equal(*(o.state[p]['momentum_buffer'] for p, o in zip(pair, opts)))
+
+
+def test_a_layout_that_changed_before_a_capture_is_refused_inside_it():
+    """The momentum would be copied out of its old place by every replay, and none would go on from the one before."""
+    from r3det.dist_train import Muon
+    w = torch.nn.Parameter(torch.randn(16, 8, 3, 3, device=DEV))
+    opt = Muon([w])
+    w.grad = torch.randn_like(w)
+    opt.step()
+    w.data = w.data.contiguous(memory_format=torch.channels_last)
+    w.grad = torch.randn_like(w)
+    before = w.detach().clone()
+    with pytest.raises(RuntimeError, match='before the capture'):
+        captured(opt)
+    assert torch.equal(w, before)
+    opt.step()
+    other = torch.nn.Parameter(w.detach().clone())
+    eager = Muon([other])
+    eager.load_state_dict(opt.state_dict())
+    other.grad = w.grad.clone()
+    graph = captured(opt)
+    for _ in range(3):
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert torch.equal(w, other)
