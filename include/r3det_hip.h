@@ -658,8 +658,8 @@ int r3det_label_log_probs_backward(const void* logits, int dtype, int64_t rows, 
  * Training: orthogonalised updates of weight matrices
  * ------------------------------------------------------------------------------------- */
 
-/* Newton-Schulz products for `count` matrices at once.  For each matrix G (rows[i] x cols[i], contiguous, of type dtype;
- * at least 1 x 1, at most 2^31 - 1 elements, the smaller side at most 32768):
+/* Newton-Schulz products for `count` (at most 65536) matrices at once.  For each matrix G (rows[i] x cols[i], contiguous, of
+ * type dtype; at least 1 x 1, at most 2^31 - 1 elements, the smaller side at most 32768, the longer 4194240):
  *   X = G / (|G|_F + eps), then `steps` (1 .. 64) times  A = X X^t,  X <- a X + (b A + c A A) X   (for rows > cols: of G^t);
  * dst[i] (rows x cols, contiguous, of the same type; may be src[i]) receives X.  In fp32's accuracy whatever the type,
  * and whatever else is in the list: as far from 64 bits as the products in fp32 one by one are, within a factor of three (some
@@ -668,7 +668,8 @@ int r3det_label_log_probs_backward(const void* logits, int dtype, int64_t rows, 
  * returns.  With P = a I + b A + c A A, the coefficients have to keep the spectral norms of X, A, P A and of P less its
  * vertex a - b b / (4 c) (less a, where |b| > 14 |c|) below 15 in every step, for singular values of up to 1 at first
  * (R3DET_EINVAL otherwise).  A workspace of r3det_orthogonalize_workspace_bytes (0: a shape that is not taken, or no
- * matrix), 16-byte aligned, need not be initialised. */
+ * matrix), 16-byte aligned, need not be initialised.  With n and m the smaller and the longer side, rounded up to multiples of
+ * 128, it has 8 to 12 n m + 24 n n bytes a matrix and up to 4 n n for every 512 of m (matrices of at most 64 x 128: nothing). */
 size_t r3det_orthogonalize_workspace_bytes(int count, const int* rows, const int* cols);
 int r3det_orthogonalize(int count, const void* const* src, void* const* dst, int dtype, const int* rows, const int* cols,
                         int steps, float a, float b, float c, double eps, void* ws, size_t ws_bytes, void* stream);

@@ -15,6 +15,7 @@ from .log_probs import DTYPES
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 STEPS = 5
+MOST_ROWS, MOST_COLUMNS, MOST_MATRICES = 32768, 65535 * 64, 65536  # (the C entries', too)
 
 
 def _numbers(steps, coefficients, eps):
@@ -42,8 +43,11 @@ def _same(ts, name):
         if t.dtype != ts[0].dtype or t.device != ts[0].device:
             raise RuntimeError(f"{name} must be of one type and on one device")
         rows, cols = t.size(0), t.numel() // max(t.size(0), 1)
-        if t.numel() >= 2 ** 31 or min(rows, cols) > 32768:
-            raise ValueError(f"{name}: a matrix of {rows} x {cols} is not taken (at most 2^31 - 1 elements, 32768 on the smaller side)")
+        if t.numel() >= 2 ** 31 or min(rows, cols) > MOST_ROWS or (t.numel() and max(rows, cols) > MOST_COLUMNS):
+            raise ValueError(f"{name}: a matrix of {rows} x {cols} is not taken (at most 2^31 - 1 elements, {MOST_ROWS} on the "
+                             f"smaller side, {MOST_COLUMNS} on the longer)")
+    if len(ts) > MOST_MATRICES and sum(t.numel() > 0 for t in ts) > MOST_MATRICES:
+        raise ValueError(f"{name}: at most {MOST_MATRICES} matrices are taken at once, got {len(ts)}")
     for t in ts:
         if not t.is_cuda:
             raise RuntimeError(f"{name} must be CUDA tensors (HIP device tensors on ROCm)")
@@ -75,7 +79,12 @@ def orthogonalize(tensors, steps=STEPS, coefficients=COEFFICIENTS, eps=1e-7):
     zero (with eps = 0: NaN); NaN or an infinity in a matrix makes that matrix NaN and no other.  The coefficients must keep
     the spectral norms of X, A and P A, with P = a + b A + c A A, and of P less its vertex a - b b / 4 c below 15
     (RuntimeError otherwise).  No gradient flows through it.  Runs on the current stream of the tensors' device, without a
-    host synchronisation."""
+    host synchronisation.
+
+    At most 65536 matrices at a time, of at most 2^31 - 1 elements, 32768 on the smaller side and 4194240 on the longer
+    (ValueError otherwise).  The call takes a workspace: for a matrix of n x m, n the smaller, both rounded up to a multiple of
+    128, 8 to 12 n m + 24 n n bytes and up to 4 n n more for every 512 of m (14 bytes an element for a detector's weights, 0.6 GB;
+    a single row counts as 128: 1.06 GB for one of a million); nothing for matrices of at most 64 x 128."""
     one = isinstance(tensors, torch.Tensor)
     ts = [tensors] if one else list(tensors)
     steps, a, b, c, eps = _numbers(steps, coefficients, eps)
@@ -134,8 +143,9 @@ def orthogonal_update_(params, grads, buffers, lr, momentum=0.95, nesterov=True,
     with ``s = 0.2 sqrt(max(rows, cols))`` for ``scale="rms"`` (the update's entries are then of about the size of an adaptive
     optimiser's) or ``sqrt(max(1, rows / cols))`` for ``"spectral"``, or a number.  ``params`` and ``grads`` fp32, fp16 or bf16,
     all alike; ``buffers`` fp32.  A weight must be contiguous or channels_last, its momentum laid out alike; a gradient
-    laid out otherwise is copied.  No weight or buffer may share memory with another or with a gradient.  ``lr`` and the other numbers are read when the
-    call is made (a captured graph keeps them)."""
+    laid out otherwise is copied.  No weight or buffer may share memory with another or with a gradient.  ``lr`` and the
+    other numbers are read when the call is made (a captured graph keeps them).  Sizes and workspace as for
+    ``orthogonalize``."""
     params, grads, buffers = list(params), list(grads), list(buffers)
     if not len(params) == len(grads) == len(buffers):
         raise ValueError(f"{len(params)} params, {len(grads)} grads and {len(buffers)} buffers")

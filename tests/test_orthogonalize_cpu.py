@@ -108,3 +108,43 @@ def test_refusals_of_the_c_entries():
                                          1, 5, 3.4445, -4.775, 2.0315, 1e-7, ws, n, None)
     assert update() == -3
     assert update(bufs=None) == -1 and update(rates=None) == -1 and update(bufs=ptrs(far, None)) == -1
+
+
+def test_every_limit_is_refused_with_its_reason():
+    """What the C entries do not take is refused by name in front of them, and nothing else is."""
+    one = torch.empty(1, 1)
+    L = _C.lib()
+    for rows, cols, taken in ((1, 4194240, True), (1, 4194241, False), (4194241, 1, False), (5000000, 2, False), (32768, 65535, True),
+                              (32769, 32769, False), (32768, 65536, False), (4194240, 511, True)):
+        wide = (ctypes.c_int * 1)(rows), (ctypes.c_int * 1)(cols)
+        assert (L.r3det_orthogonalize_workspace_bytes(1, *wide) > 0) == taken, (rows, cols)
+        w = one.expand(rows, cols)
+        with pytest.raises(RuntimeError if taken else ValueError, match="CUDA tensor" if taken else "not taken.*4194240"):
+            orthogonalize([W, w])
+    long = [torch.empty(1, 4194241) for _ in range(3)]
+    with pytest.raises(ValueError, match="not taken"):
+        orthogonal_update_(*([t] for t in long), lr=0.1)
+    many = [torch.zeros(1, 1)] * 65537
+    with pytest.raises(ValueError, match="at most 65536 matrices"):
+        orthogonalize(many)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        orthogonalize(many[1:] + [torch.zeros(0, 3)])
+    sizes = (ctypes.c_int * 65537)(*[1] * 65537)
+    assert L.r3det_orthogonalize_workspace_bytes(65537, sizes, sizes) == 0
+    assert L.r3det_orthogonalize_workspace_bytes(65536, sizes, sizes) > 0
+
+
+def test_the_workspace_is_what_the_documentation_says():
+    L = _C.lib()
+
+    def size(*shapes):
+        rows, cols = zip(*shapes)
+        return L.r3det_orthogonalize_workspace_bytes(len(shapes), (ctypes.c_int * len(shapes))(*rows), (ctypes.c_int * len(shapes))(*cols))
+    for shapes in ([(1, 1000000)], [(2048, 2048)], [(4096, 4096)], [(256, 2304)] * 8 + [(135, 2304)], [(300, 40000)], [(100, 70)] * 500):
+        least = most = 0
+        for r, c in shapes:
+            n, m = (-(-s // 128) * 128 for s in sorted((r, c)))
+            least += 8 * n * m + 24 * n * n
+            most += 12 * n * m + 24 * n * n + 4 * n * n * -(-m // 512) + 4096 + n * m // 16  # (lists, diagonals, norms)
+        assert least <= size(*shapes) <= most, (shapes, least, size(*shapes), most)
+    assert size((64, 128), (128, 64), (5, 5)) == 256
