@@ -410,3 +410,37 @@ def test_update_of_a_head():
         want_w, want_m, tol = update_by_formula(w0, g, m0, 0.05, 0.9, True, 0.01, "rms")
         assert ((m.double() - want_m).abs() <= 3 * U * (want_m.abs() + m0.abs().double() + g.abs().double())).all()
         assert (w.double() - want_w).norm() <= tol + 5 * U * want_w.norm().item()
+
+
+@pytest.mark.parametrize("steps,co", [(1, COEFFICIENTS), (5, COEFFICIENTS), (1, (1.5, -0.5, 0.0)), (6, (1.5, -0.5, 0.0))])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_a_bad_value_makes_its_whole_matrix_nan_and_no_other(bad, steps, co):
+    """In every form: one launch for all steps, single steps, groups, tiles of 64 and of 128, pieces of one chain along with
+    another's.  (An infinity leaves one NaN among zeros in the first X; its row and column of A are NaN, and so all of F X.)"""
+    for shapes in ([(64, 64), (30, 100), (1, 9)], [(70, 200), (1, 4097), (300, 40)], [(300, 500), (257, 256)], MIXED,
+                   [(256, 2304)] * 8 + [(135, 2304), (5, 2304)], [(300, 400)] * 60):
+        ts = [matrix(*s, seed=i) for i, s in enumerate(shapes)]
+        clean = orthogonalize(ts, steps=steps, coefficients=co)
+        for k in {0, len(ts) // 2, len(ts) - 1}:
+            n, m = shapes[k]
+            one = list(ts)
+            one[k] = ts[k].clone()
+            one[k][n // 2, m - 1] = bad
+            for i, (got, want) in enumerate(zip(orthogonalize(one, steps=steps, coefficients=co), clean)):
+                if i == k:
+                    assert torch.isnan(got).all(), (shapes[k], torch.isnan(got).sum())
+                else:
+                    assert torch.equal(got, want), (shapes[k], shapes[i])
+
+
+def test_a_bad_gradient_spoils_its_weight_alone():
+    shapes = [(64, 64), (135, 700), (300, 500), (1100, 1300)]
+    ws, gs = [matrix(*s, seed=1) for s in shapes], [matrix(*s, seed=2) for s in shapes]
+    clean, ms = [w.clone() for w in ws], [torch.zeros_like(w) for w in ws]
+    orthogonal_update_(clean, gs, [m.clone() for m in ms], lr=0.1)
+    for k in range(len(shapes)):
+        got, bad = [w.clone() for w in ws], [g.clone() for g in gs]
+        bad[k][2, 3] = math.inf
+        orthogonal_update_(got, bad, [m.clone() for m in ms], lr=0.1)
+        for i, (a, b) in enumerate(zip(got, clean)):
+            assert torch.isnan(a).all() if i == k else torch.equal(a, b)
