@@ -57,7 +57,7 @@ class Muon(torch.optim.Optimizer):
                      W = W - lr U
 
     The momentum is fp32 whatever the weights' type and is laid out as its weight is.  The same gradients give the same
-    bits, so replicas that exchange gradients stay equal.  ``lr`` and the others are read from the group at every step
+    bits on cards alike, so replicas that exchange gradients stay equal.  ``lr`` and the others are read from the group at every step
     (schedulers work; a captured step keeps them).  Device tensors only."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, orthogonal=True, scale='rms',
