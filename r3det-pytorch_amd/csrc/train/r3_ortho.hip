@@ -53,6 +53,7 @@ constexpr float SCALE = 4096.f;  // what stored values are multiplied by
 constexpr float R_SCALE = 512.f; // ... of R
 constexpr int PAD = 128;         // rows and columns of X are multiples of it
 constexpr int WANT = 512;        // workgroups that fill the card
+constexpr unsigned CARD = 256;   // its compute units
 
 struct Mat {  // one matrix, as the device's table holds it
   const void* src;   // the matrix / the gradient
@@ -1288,8 +1289,7 @@ int work(int count, const int* rows, const int* cols, int kinds, Work& p) {
 // one by one, if X X^t is a launch as well (250 x 250: 104 us, 111 in groups; 300 x 300: 117, 126) or a matrix is narrow.
 bool one_by_one(const Work& p) {
   const Chain& l = p.c;
-  const unsigned most = WANT / 2;
-  return l.gram_ts == 64 && l.tri_ts == 64 && l.rect_ts == 64 && l.n_gram <= most && l.n_tri <= most && l.n_rect <= most &&
+  return l.gram_ts == 64 && l.tri_ts == 64 && l.rect_ts == 64 && l.n_gram <= CARD && l.n_tri <= CARD && l.n_rect <= CARD &&
          (!p.split || p.narrow < NARROW);
 }
 
@@ -1304,14 +1304,23 @@ struct Plan {
 // 0: fine, -1: a list that is not taken
 int plan(int count, const int* rows, const int* cols, Plan& p) {
   p.chains = 0, p.total = 256;  // (nothing but small matrices needs nothing)
+  p.w[0].single = false;
   if (!taken(count, rows, cols)) return -1;
   int kinds = 0;
-  for (int i = 0; i < count; ++i) kinds |= kind(rows[i], cols[i]) & (NARROWS | WIDES);
+  uint64_t tiles = 0;  // (of 64)
+  for (int i = 0; i < count; ++i) {
+    const int k = kind(rows[i], cols[i]) & (NARROWS | WIDES);
+    kinds |= k;
+    if (k) tiles += Dim(rows[i], cols[i]).rect(64);
+  }
   if (!kinds) return 0;
-  if (work(count, rows, cols, kinds, p.w[0]) != 0) return -1;
-  p.w[0].single = kinds == NARROWS || one_by_one(p.w[0]);
+  const bool both = kinds == (NARROWS | WIDES);
   p.chains = 1;
-  if (kinds == (NARROWS | WIDES) && !p.w[0].single) {
+  if (!both || tiles <= CARD) {  // (more are not taken one by one)
+    if (work(count, rows, cols, kinds, p.w[0]) != 0) return -1;
+    p.w[0].single = kinds == NARROWS || one_by_one(p.w[0]);
+  }
+  if (both && !p.w[0].single) {
     if (work(count, rows, cols, WIDES, p.w[0]) != 0 || work(count, rows, cols, NARROWS, p.w[1]) != 0) return -1;
     p.w[1].single = true;
     p.chains = 2;
