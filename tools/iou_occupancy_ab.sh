@@ -16,11 +16,12 @@ mkdir -p $(dirname $OUT)
 export TMPDIR=/tmp
 C=$R/r3det-pytorch_amd/csrc
 mkdir -p /tmp/r3_iou_ab
-hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -munsafe-fp-atomics -fvisibility=hidden \
+hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC -ffp-contract=off -munsafe-fp-atomics -fvisibility=hidden \
       -fvisibility-inlines-hidden -Wno-pass-failed -DR3_COMPACT_WAVES=1 -DR3_VEC_WAVES=1 -DR3_DRAIN3_V3_WAVES=4 \
       -c $C/r3_iou.hip -o /tmp/r3_iou_ab/r3_iou.o
 hipcc --offload-arch=gfx950 -shared -fPIC -Wl,--version-script=$C/exports.map -o /tmp/r3_iou_ab/libr3det_hip_iou_ab.so \
-      $C/r3_api.o /tmp/r3_iou_ab/r3_iou.o $C/r3_nms.o $C/r3_fr.o $C/r3_frb.o $C/r3_boxes.o $C/r3_pool.o $C/r3_epilogue.o $C/r3_poly.o
+      $C/r3_api.o /tmp/r3_iou_ab/r3_iou.o $C/r3_nms.o $C/r3_fr.o $C/r3_frb.o $C/r3_boxes.o $C/r3_pool.o $C/r3_epilogue.o $C/r3_poly.o \
+      $C/train/r3_logprob.o $C/train/r3_ortho.o
 cd /tmp
 : > $OUT
 for lib in A B; do

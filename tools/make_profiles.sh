@@ -54,7 +54,7 @@ unset NMS_PROF_N
 cd $R
 { for n in 8576 10240 12288 14336 16384 20000 24576 32768; do for impl in 7 6; do echo -n "nms_impl $impl: "; NMS_PROF_nms_impl=$impl NMS_PROF_N=$n python3 tools/nms_prof.py 2>&1 | grep batched; done; done; } > $O/${TAG}_nms_sorted_chunks_ab.txt
 python3 tools/nms_suppressor_stats.py 8576 16384 32768 2>&1 | grep "^n=" > $O/${TAG}_nms_suppressors.txt
-hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -I r3det-pytorch_amd/csrc -I include -o /tmp/nrp tools/probes/nms_reduce_probe.hip > /dev/null 2>&1
+hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -ffp-contract=off -I r3det-pytorch_amd/csrc -I include -o /tmp/nrp tools/probes/nms_reduce_probe.hip > /dev/null 2>&1
 DUMP_POOL=/tmp/pool32k.bin NMS_PROF_N=32768 python3 tools/nms_prof.py > /dev/null 2>&1
 { echo "# tools/probes/nms_reduce_probe 32768 <the pool of tools/nms_prof.py> <label group>: s_memtime stamps of one reducer workgroup and of workgroup 0 of the ranking kernel"; for g in 0 5 9; do echo "# label group $g"; /tmp/nrp 32768 /tmp/pool32k.bin $g 2>&1 | tail -8; done; } > $O/${TAG}_nms_reduce_stamps.txt
 cd /tmp

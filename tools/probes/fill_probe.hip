@@ -1,6 +1,6 @@
 // Probe: how fast can 128 x 196416 fp32 zeros be written, as a function of the tile shape a workgroup owns?
 // (The IoU stream kernel writes 16 x 1024 tiles; a plain fill of the same 100 MB is twice as fast.)
-// build: hipcc --offload-arch=gfx950 -O3 -o fill_probe fill_probe.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o fill_probe fill_probe.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -3,7 +3,7 @@
 //   V0 copy through LDS (pitch 129)                         V1 + 80-byte per-quad table loads (unused)
 //   V2 + 16 transposed LDS gathers + bilinear math          V3 = V2 with conflict-free lane mapping
 //   V4 = V2 without the table loads (taps synthesised)
-// build: hipcc --offload-arch=gfx950 -O3 -o fr_stage_probe fr_stage_probe.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o fr_stage_probe fr_stage_probe.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 

@@ -1,7 +1,7 @@
 // Probe: where the time of frb_index_sort_kernel (csrc/r3_frb.hip) goes -- s_memtime stamps of one workgroup at
 // the phase boundaries (A scan of the sample rows | B taps of the reaching sources | C bitonic sort | D write),
 // level 0 of a 1024^2 input (N = 4, 128 x 128), regular box field.
-// build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -I r3det-pytorch_amd/csrc -I include -o tools/probes/frb_index_probe tools/probes/frb_index_probe.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -ffp-contract=off -I r3det-pytorch_amd/csrc -I include -o tools/probes/frb_index_probe tools/probes/frb_index_probe.hip
 #include "../../r3det-pytorch_amd/csrc/r3_frb.hip"
 #include <cstdio>
 #include <cstdlib>

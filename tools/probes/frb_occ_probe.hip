@@ -1,5 +1,5 @@
 // Probe: what the runtime says about the residency of the channels_last FR backward gather (512 threads, 32 KB LDS).
-// build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -I r3det-pytorch_amd/csrc -I include -o tools/probes/frb_occ_probe tools/probes/frb_occ_probe.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -ffp-contract=off -I r3det-pytorch_amd/csrc -I include -o tools/probes/frb_occ_probe tools/probes/frb_occ_probe.hip
 #include "../../r3det-pytorch_amd/csrc/r3_frb.hip"
 #include <cstdio>
 int g_r3_fr_walk = 8;

@@ -1,6 +1,6 @@
 // Probe: how fast can "load tile -> LDS -> barrier -> LDS -> store" run on MI355X compared with a
 // plain copy, as a function of workgroup size / tile size / LDS write form?
-// build: hipcc --offload-arch=gfx950 -O3 -o lds_copy_probe lds_copy_probe.hip ; run: ./lds_copy_probe
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o lds_copy_probe lds_copy_probe.hip ; run: ./lds_copy_probe
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

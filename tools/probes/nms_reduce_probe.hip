@@ -1,7 +1,7 @@
 // Probe: where the time of nms_reduce_groups_kernel (csrc/r3_nms.hip) goes -- s_memtime stamps of reducer workgroup
 // (group 0, image 0) at the phase boundaries (label compaction | prologue loads | rounds | keep bits), on a
 // clustered pool like tools/nms_prof.py's (n boxes around n / 12 objects, 15 labels), through r3k_batched_nms.
-// build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -I r3det-pytorch_amd/csrc -I include -o tools/probes/nms_reduce_probe tools/probes/nms_reduce_probe.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -ffp-contract=off -I r3det-pytorch_amd/csrc -I include -o tools/probes/nms_reduce_probe tools/probes/nms_reduce_probe.hip
 #include "../../r3det-pytorch_amd/csrc/r3_nms.hip"
 #include <cstdio>
 #include <cstdlib>

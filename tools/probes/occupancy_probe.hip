@@ -1,6 +1,6 @@
 // Probe: how many workgroups of a given size / LDS footprint does the runtime say a compute unit holds, and how many
 // actually run at once (workgroups record start stamps; those that start within 2 us of the first are resident).
-// build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -o tools/probes/occupancy_probe tools/probes/occupancy_probe.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -o tools/probes/occupancy_probe tools/probes/occupancy_probe.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

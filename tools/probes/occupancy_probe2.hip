@@ -1,4 +1,4 @@
-// build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -o tools/probes/occupancy_probe2 tools/probes/occupancy_probe2.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -o tools/probes/occupancy_probe2 tools/probes/occupancy_probe2.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -1,7 +1,7 @@
 // Probe: what does a PERSISTENT workgroup (one per CU, looping over G planes of 64 KB) cost in
 // HBM throughput compared with one-plane-per-workgroup launches?  Isolates the memory-system side
 // of fr_forward_chan / _cell (no sampling math at all).
-// build: hipcc --offload-arch=gfx950 -O3 -o persist_copy_probe persist_copy_probe.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o persist_copy_probe persist_copy_probe.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 

@@ -1,6 +1,6 @@
 // Probe: where the time of pool_select_kernel (csrc/r3_pool.hip) goes -- s_memtime stamps of workgroup 0 at the phase
 // boundaries: 0-1 histogram digits | 1-2 the pass over the keys (entries to the two lists) | the rest: meta write.  N = 4 images of L keys (argv[1], default 16384), k = 2000, detector-like score distribution.
-// build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -I r3det-pytorch_amd/csrc -I include -o tools/probes/pool_select_probe tools/probes/pool_select_probe.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -ffp-contract=off -I r3det-pytorch_amd/csrc -I include -o tools/probes/pool_select_probe tools/probes/pool_select_probe.hip
 #include "../../r3det-pytorch_amd/csrc/r3_pool.hip"
 #include <cmath>
 #include <cstdio>

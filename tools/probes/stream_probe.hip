@@ -1,7 +1,7 @@
 // Probe: the streaming floor of the FeatureRefineModule tail: out = a + b + r (3 reads + 1 write per element)
 // on N x 256 x 128 x 128 fp32 tensors, rotating over buffer sets beyond the Infinity Cache.  Variants: linear
 // float4 grid-stride; one wave per 1 KB row with 4 rows in flight per wave (the sampler kernel's shape).
-// build: hipcc --offload-arch=gfx950 -O3 -o stream_probe stream_probe.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o stream_probe stream_probe.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #define CK(x) do { hipError_t e = (x); if (e != hipSuccess) { printf("HIP error %s at %d\n", hipGetErrorString(e), __LINE__); return 1; } } while (0)

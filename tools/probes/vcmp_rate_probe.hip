@@ -1,6 +1,6 @@
 // Probe: issue rate of the compare-and-count idiom of mc_sort_prepare_kernel (v_cmp_ge_u32 + v_addc / v_cndmask)
 // against plain v_add_u32, per wavefront and SIMD.  One workgroup of 256 threads per CU x 4, long loops, events.
-// build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -o tools/probes/vcmp_rate_probe tools/probes/vcmp_rate_probe.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -o tools/probes/vcmp_rate_probe tools/probes/vcmp_rate_probe.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #define CK(x) do { hipError_t e = (x); if (e != hipSuccess) { printf("HIP error %s at %d\n", hipGetErrorString(e), __LINE__); return 1; } } while (0)

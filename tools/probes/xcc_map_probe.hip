@@ -1,6 +1,6 @@
 // Probe: which XCD (XCC_ID) and when a workgroup of a 1-D grid runs -- the assumption behind the "XCD-contiguous
 // band" remaps of the tile kernels (t = (b & 7) * (T / 8) + (b >> 3): blockIdx b is dispatched to XCD b % 8).
-// build: hipcc --offload-arch=gfx950 -O3 -o tools/probes/xcc_map_probe tools/probes/xcc_map_probe.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/probes/xcc_map_probe tools/probes/xcc_map_probe.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>
