@@ -663,7 +663,8 @@ int r3det_label_log_probs_backward(const void* logits, int dtype, int64_t rows, 
  *   X = G / (|G|_F + eps), then `steps` (1 .. 64) times  A = X X^t,  X <- a X + (b A + c A A) X   (for rows > cols: of G^t);
  * dst[i] (rows x cols, contiguous, of the same type; may be src[i]) receives X.  In fp32's accuracy whatever the type,
  * and whatever else is in the list: as far from 64 bits as the products in fp32 one by one are, within a factor of three (some
- * 1e-6 of its norm; up to 1e-5 of those and of these where one singular value is far above the others).
+ * 1e-6 of its norm; up to 1e-5 of those and of these where one singular value is far above the others).  What a norm far
+ * below eps leaves small is exact to 2^-37 (1 + a + ... + a^steps) an entry only (5e-9 with the usual five steps).
  * A zero matrix stays zero where eps > 0.  The arrays of pointers and sizes are HOST arrays and are read before the call
  * returns.  With P = a I + b A + c A A, the coefficients have to keep the spectral norms of X, A, P A and of P less its
  * vertex a - b b / (4 c) (less a, where |b| > 14 |c|) below 15 in every step, for singular values of up to 1 at first

@@ -444,3 +444,18 @@ def test_a_bad_gradient_spoils_its_weight_alone():
         orthogonal_update_(got, bad, [m.clone() for m in ms], lr=0.1)
         for i, (a, b) in enumerate(zip(got, clean)):
             assert torch.isnan(a).all() if i == k else torch.equal(a, b)
+
+
+@pytest.mark.parametrize("shape", [(64, 64), (5, 700), (256, 2304), (1100, 1300)], ids=str)
+def test_norms_far_below_eps(shape):
+    """Values are held times 2^12 in fp16 pairs, whose second has steps of 2^-24: an entry is off by up to 2^-37 at first and
+    after every step, and each step multiplies that by a (the cubic and quintic terms are nothing there)."""
+    a = COEFFICIENTS[0]
+    least = 2.0 ** -37 * sum(a ** k for k in range(6)) * math.sqrt(shape[0] * shape[1])
+    for norm in (1e-8, 1e-9, 1e-10, 1e-12, 1e-15):
+        g = matrix(*shape)
+        g *= norm / g.norm()
+        want, norms = iterate(g)
+        plain = (iterate(g, dtype=torch.float32)[0].double() - want).norm().item()
+        got = orthogonalize([g, matrix(256, 300)])[0]
+        assert (got.double() - want).norm().item() <= tolerances(g, norms, plain, 5, torch.float32) + least, norm
