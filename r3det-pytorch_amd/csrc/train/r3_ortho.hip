@@ -31,10 +31,10 @@
 // straight from memory).  Of a symmetric result the tiles on and above the diagonal are computed, and written twice.
 //
 // What bounds it, with the usual five steps (kernels' time of a call; the matrix cores reach 1.1 PFLOP/s of fp16, a copy
-// 4.7 TB/s): 4096 x 4096, 4.6 ms: the matrix cores, 3.75 ms of products at that rate.  2048 x 2048, 0.94 ms: the same, with
-// fewer tiles than would keep them busy (0.47).  The 73 matrices of a detector, 41.9 M weights, 1.17 ms: a third the memory
-// (norms 86 us, X 100, the last group's R X 185), the rest loads on their way between matrix instructions.  A head's ten,
-// 0.19 ms, and smaller lists: some twenty launches that wait for each other, 5 us at least each.
+// 4.7 TB/s): 4096 x 4096, 4.6 ms: the matrix cores, 3.75 ms of products at that rate.  2048 x 2048, 0.95 ms: the same, with
+// fewer tiles than would keep them busy (0.47).  The 73 matrices of a detector, 41.9 M weights, 1.27 ms: a third the memory
+// (norms 87 us, X 105, the last launch 213), the rest loads on their way between matrix instructions.  A head's ten,
+// 0.25 ms, and smaller lists: some twenty-five launches that wait for each other, 5 us at least each.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
