@@ -663,7 +663,7 @@ int r3det_label_log_probs_backward(const void* logits, int dtype, int64_t rows, 
  *   X = G / (|G|_F + eps), then `steps` (1 .. 64) times  A = X X^t,  X <- a X + (b A + c A A) X   (for rows > cols: of G^t);
  * dst[i] (rows x cols, contiguous, of the same type; may be src[i]) receives X.  In fp32's accuracy whatever the type,
  * and whatever else is in the list: as far from 64 bits as the products in fp32 one by one are, within a factor of three and
- * 1e-6 of its norm (some 1e-6; up to 1e-5 both ways where one singular value is far above the others).  What a norm far
+ * 1e-6 of its norm (some 1e-6; more both ways where one singular value is far above the others).  What a norm far
  * below eps leaves small is exact to 2^-37 (1 + a + ... + a^steps) an entry only (5e-9 with the usual five steps).
  * A zero matrix stays zero where eps > 0.  The arrays of pointers and sizes are HOST arrays and are read before the call
  * returns.  With P = a I + b A + c A A, the coefficients have to keep the spectral norms of X, A, P A and of P less its

@@ -75,7 +75,7 @@ def orthogonalize(tensors, steps=STEPS, coefficients=COEFFICIENTS, eps=1e-7):
     ``X = a X + (b A + c A A) X`` with ``A = X X^t`` (of the transpose where there are more rows than columns), which moves
     every singular value towards 1 and keeps the singular vectors.  Computed to fp32's accuracy whatever the type and
     whatever else is in the list, and rounded once: as far from 64 bits as the formula op by op in fp32 is, within a factor of
-    three and 1e-6 of its norm (some 1e-6; up to 1e-5 both ways where one singular value is far above the others).  What a norm far
+    three and 1e-6 of its norm (some 1e-6; more both ways where one singular value is far above the others).  What a norm far
     below ``eps`` leaves small is exact to 5e-9 an entry only (with the usual steps).  A zero matrix stays zero (with eps = 0:
     NaN); NaN or an infinity in a matrix makes that matrix NaN and no other.  The coefficients must keep the spectral norms of
     X, A and P A, with P = a + b A + c A A, and of P less its vertex a - b b / 4 c below 15 (RuntimeError otherwise).  No
