@@ -92,6 +92,16 @@ struct Out {
   float* top_lp;
   int64_t* top_ix;
   float* stats;  // (rows, 2): m, log S
+  Out from(int64_t row) const {  // of the rows from this one on
+    Out o = *this;
+    if (labels) o.labels += row;
+    if (log_prob) o.log_prob += row;
+    if (entropy) o.entropy += row;
+    if (top_lp) o.top_lp += row * k;
+    if (top_ix) o.top_ix += row * k;
+    if (stats) o.stats += 2 * row;
+    return o;
+  }
 };
 
 // One thread per row: what the row's triple says.  S = 0 only where every class is -inf: log p is -inf there and the
@@ -693,8 +703,12 @@ int row_forward(const T* x, int64_t rows, int64_t classes, int64_t stride, int s
   return 0;
 }
 
+// A launch has fewer than 2^32 threads, and one of more is cut short without an error: of many rows so many are taken at a time
+// (at 256 threads a row 2^30; the gradient's split rows take 256 more for every 16384 classes, which memory bounds).
+constexpr int64_t ROWS = 1 << 22;
+
 template <typename T>
-int forward(const T* x, int64_t rows, int64_t classes, int64_t stride, const Out& o, void* ws, hipStream_t st) {
+int forward(const T* x, int64_t rows, int64_t classes, int64_t stride, int split, const Out& o, void* ws, hipStream_t st) {
   const int c = (int)classes;
   if (c <= 4) return small_forward<T, 1, 4>(x, rows, c, stride, o, st);
   if (c <= 16) return small_forward<T, 2, 8>(x, rows, c, stride, o, st);
@@ -702,7 +716,6 @@ int forward(const T* x, int64_t rows, int64_t classes, int64_t stride, const Out
   if (c <= 64) return small_forward<T, 4, 16>(x, rows, c, stride, o, st);
   if (c <= SMALL_MAX) return small_forward<T, 8, 16>(x, rows, c, stride, o, st);
   if (c <= WAVE_MAX) return row_forward<T, 1>(x, rows, classes, stride, 1, nullptr, nullptr, o, st);
-  const int split = row_split(rows, classes);
   unsigned long long* keys = static_cast<unsigned long long*>(ws);
   float* part = reinterpret_cast<float*>(keys + (size_t)rows * split * o.k);
   if (rows * split <= r3_cu_count()) return row_forward<T, 16>(x, rows, classes, stride, split, part, keys, o, st);
@@ -750,12 +763,16 @@ int r3k_logprob(const void* x, int dtype, int64_t rows, int64_t classes, int64_t
   const size_t need = r3k_logprob_workspace_bytes(rows, classes, k);
   if (need && (!ws || ws_bytes < need)) return -3;
   if (need && (reinterpret_cast<uintptr_t>(ws) & 7)) return -1;
-  const Out o{labels, ignore, has_ignore, k, log_prob, entropy, top_lp, top_ix, stats};
-  switch (dtype) {
-    case 0: return forward(static_cast<const float*>(x), rows, classes, stride, o, ws, st);
-    case 1: return forward(static_cast<const _Float16*>(x), rows, classes, stride, o, ws, st);
-    default: return forward(static_cast<const __bf16*>(x), rows, classes, stride, o, ws, st);
+  const int split = row_split(rows, classes);  // (of the whole call: the last few rows of many have no workspace)
+  const Out all{labels, ignore, has_ignore, k, log_prob, entropy, top_lp, top_ix, stats};
+  for (int64_t at = 0; at < rows; at += ROWS) {
+    const int64_t n = rows - at < ROWS ? rows - at : ROWS;
+    const Out o = all.from(at);
+    const auto run = [&](auto type) { return forward(static_cast<const decltype(type)*>(x) + at * stride, n, classes, stride, split, o, ws, st); };
+    const int rc = dtype == 0 ? run(0.f) : dtype == 1 ? run((_Float16)0) : run((__bf16)0);
+    if (rc != 0) return rc;
   }
+  return 0;
 }
 
 int r3k_logprob_backward(const void* x, int dtype, int64_t rows, int64_t classes, int64_t stride, const int64_t* labels,
@@ -766,14 +783,18 @@ int r3k_logprob_backward(const void* x, int dtype, int64_t rows, int64_t classes
   if (rows == 0) return 0;
   if (rows > (1ll << 40) || !x || stride < 0 || !stats || !dx || (d_lp && !labels) || (d_h && !entropy) || (d_top && (!k || !top_ix)))
     return -1;
-  const Out o{labels, ignore, has_ignore, k, nullptr, const_cast<float*>(entropy), nullptr, const_cast<int64_t*>(top_ix),
-              const_cast<float*>(stats)};
-  switch (dtype) {
-    case 0:
-      return backward(static_cast<const float*>(x), rows, classes, stride, o, d_lp, d_h, d_top, static_cast<float*>(dx), st);
-    case 1:
-      return backward(static_cast<const _Float16*>(x), rows, classes, stride, o, d_lp, d_h, d_top, static_cast<_Float16*>(dx), st);
-    default:
-      return backward(static_cast<const __bf16*>(x), rows, classes, stride, o, d_lp, d_h, d_top, static_cast<__bf16*>(dx), st);
+  const Out all{labels, ignore, has_ignore, k, nullptr, const_cast<float*>(entropy), nullptr, const_cast<int64_t*>(top_ix),
+                const_cast<float*>(stats)};
+  for (int64_t at = 0; at < rows; at += ROWS) {
+    const int64_t n = rows - at < ROWS ? rows - at : ROWS;
+    const Out o = all.from(at);
+    const float *lp = d_lp ? d_lp + at : nullptr, *h = d_h ? d_h + at : nullptr, *top = d_top ? d_top + at * k : nullptr;
+    const auto run = [&](auto type) {
+      typedef decltype(type) T;
+      return backward(static_cast<const T*>(x) + at * stride, n, classes, stride, o, lp, h, top, static_cast<T*>(dx) + at * classes, st);
+    };
+    const int rc = dtype == 0 ? run(0.f) : dtype == 1 ? run((_Float16)0) : run((__bf16)0);
+    if (rc != 0) return rc;
   }
+  return 0;
 }

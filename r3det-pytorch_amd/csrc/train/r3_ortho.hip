@@ -1281,7 +1281,8 @@ int work(int count, const int* rows, const int* cols, int kinds, Work& p) {
     p.halves += d.halves(l.rect_ts);
   }
   l.whole_gram = quarter(gram, l.gram_ts == 128 && !p.split), l.whole_tri = quarter(tri, l.tri_ts == 128);
-  if (gram > 0x3fffffff || tri > 0x3fffffff || rect > 0x3fffffff || p.fill > 0x3fffffff) return -1;
+  const uint64_t most = (1 << 23) - 1;  // (a launch has fewer than 2^32 threads: two chains' tiles by 256)
+  if (gram > most || tri > most || rect > most || p.fill > most) return -1;  // (workspaces of 274 GB and more)
   l.n_gram = (unsigned)gram, l.n_tri = (unsigned)tri, l.n_rect = (unsigned)rect;
   return 0;
 }

@@ -426,3 +426,29 @@ def test_smallest_negative_numbers_are_ranked_as_values(rows, classes, k):
     got = label_log_probs(x, top_k=k)
     assert torch.equal(got.top_index.cpu(), reference(x, k=k)["top_index"])
     assert (got.top_log_prob + math.log(classes)).abs().max() <= (classes / 64 + 60) * U + 2e-6
+
+
+@pytest.mark.parametrize("rows,classes", [((1 << 22) + 3, 5), ((1 << 22) + 3, 1030), ((1 << 26) + 5, 129)])
+def test_more_rows_than_a_launch_takes(rows, classes):
+    """Rows are independent: those at the ends and around every border are what they are by themselves, and none is left out."""
+    x = torch.empty(rows, classes, dtype=torch.bfloat16, device=DEV).normal_()
+    y = torch.arange(rows, device=DEV) % classes
+    y[-2] = IGNORE
+    leaf = x.requires_grad_(True)
+    got = label_log_probs(leaf, y, top_k=2, ignore_index=IGNORE)
+    weight = torch.linspace(-1, 1, rows, device=DEV)
+    d, = torch.autograd.grad([got.log_prob, got.top_log_prob], [leaf], [weight, weight[:, None].expand(rows, 2)])
+    assert got.log_prob.max() <= 0 and (got.top_index >= 0).all() and (got.top_index < classes).all()
+    at = sorted({r for b in range(0, rows, 1 << 22) for r in (b - 1, b, b + 1) if 0 <= r < rows} | set(range(rows - 5, rows)))
+    at = torch.tensor(at, device=DEV)
+    few = x.detach()[at].clone().requires_grad_(True)
+    want = label_log_probs(few, y[at], top_k=2, ignore_index=IGNORE)
+    dw, = torch.autograd.grad([want.log_prob, want.top_log_prob], [few], [weight[at], weight[at][:, None].expand(len(at), 2)])
+    for a, b in zip(got, want):
+        assert torch.equal(a[at], b)
+    assert torch.equal(d[at], dw)
+    # the gradient of a row sums to nothing, whatever its place
+    sums = torch.cat([part.float().sum(1) for part in d.split(1 << 22)])
+    assert sums.abs().max() <= 3 * 2.0 ** -8 * 2
+    del x, leaf, d, got, sums
+    torch.cuda.empty_cache()
