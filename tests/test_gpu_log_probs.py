@@ -452,3 +452,51 @@ def test_more_rows_than_a_launch_takes(rows, classes):
     assert sums.abs().max() <= 3 * 2.0 ** -8 * 2
     del x, leaf, d, got, sums
     torch.cuda.empty_cache()
+
+
+def test_the_most_classes():
+    """2^31 - 1 of them in one row, zeros but for a peak at the last and a masked one: log S is known.  256 workgroups of sixteen
+    wavefronts add at most 8192 terms a lane, so S is off by 8300 u relatively."""
+    n = 2 ** 31 - 1
+    x = torch.zeros(1, n, dtype=torch.bfloat16, device=DEV)
+    x[0, -1] = 5
+    x[0, 7] = -math.inf
+    leaf = x.requires_grad_(True)
+    got = label_log_probs(leaf, torch.tensor([n - 1], device=DEV), top_k=9)
+    total = n - 2 + math.exp(5)
+    lp = 5 - math.log(total)
+    assert abs(got.log_prob.item() - lp) <= (8300 + 2 * abs(lp)) * U
+    assert abs(got.entropy.item() - (math.log(total) - 5 * math.exp(5) / total)) <= (2 * 8300 + 3 * abs(lp)) * U
+    assert got.top_index.tolist() == [[n - 1, 0, 1, 2, 3, 4, 5, 6, 8]]
+    d, = torch.autograd.grad(got.log_prob.sum(), leaf)
+    some = d[0, [0, 6, 7, 8, n // 2, n - 2, n - 1]].double().cpu()
+    want = torch.tensor([-1 / total] * 7, dtype=torch.float64)
+    want[2], want[6] = 0, 1 - math.exp(lp)
+    assert ((some - want).abs() <= want.abs() * (2.0 ** -8 + 9000 * U)).all()
+    assert bool((d[0, 8:-1].view(torch.int16).split(1 << 28)[3] == d[0, 8].view(torch.int16)).all())
+    del x, leaf, d
+    torch.cuda.empty_cache()
+
+
+def test_two_threads_at_once():
+    """Calls on two streams from two threads, long rows with workspaces among them."""
+    import threading
+    cases = [logits(r, c, t) for r, c, t in ((3, 70000, "fp32"), (300, 4000, "bf16"), (5000, 16, "fp32"), (67, 33000, "fp16"))]
+    want = [label_log_probs(x, y, top_k=8) for x, y in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(k):
+        stream = torch.cuda.Stream(device=DEV)
+        with torch.cuda.stream(stream):
+            for i in range(40):
+                x, y = cases[(i + k) % 4]
+                got = label_log_probs(x, y, top_k=8)
+                bad.extend([(k, i)] * (not all(torch.equal(a, b) for a, b in zip(got, want[(i + k) % 4]))))
+        stream.synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

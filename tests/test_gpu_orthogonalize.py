@@ -459,3 +459,50 @@ def test_norms_far_below_eps(shape):
         plain = (iterate(g, dtype=torch.float32)[0].double() - want).norm().item()
         got = orthogonalize([g, matrix(256, 300)])[0]
         assert (got.double() - want).norm().item() <= tolerances(g, norms, plain, 5, torch.float32) + least, norm
+
+
+@pytest.mark.parametrize("shape", [(65535, 32767), (1, 4194240), (4194240, 400)], ids=str)
+def test_the_largest_matrices(shape):
+    """Against the formula in 64 bits on three vectors, one step; the result is rounded to bf16, at most half a step an entry (a
+    vector meets that error as a matrix of random signs: its norm is what it is of the entries)."""
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    g = torch.empty(shape, dtype=torch.bfloat16, device=DEV).normal_(generator=gen)
+    o = orthogonalize(g, steps=1)
+    norm = math.sqrt(sum(float(p.double().pow(2).sum()) for p in g.split(4096))) + 1e-7
+
+    def of(m, v):
+        return torch.cat([p.double() @ v for p in m.split(4096)])
+
+    def turned(u):
+        return sum(p.double().t() @ q for p, q in zip(g.split(4096), u.split(4096)))
+    a, b, c = COEFFICIENTS
+    v = torch.randn(shape[1], 3, generator=gen, device=DEV, dtype=torch.float64)
+    x = of(g, v) / norm
+    once = of(g, turned(x)) / norm ** 2
+    want = a * x + b * once + c * of(g, turned(once)) / norm ** 2
+    assert (of(o, v) - want).norm() <= want.norm() * (2.0 ** -8 + 64 * U)
+    del g, o
+    torch.cuda.empty_cache()
+
+
+def test_two_threads_at_once():
+    """Calls on two streams from two threads: mixed lists, small ones, updates in place."""
+    import threading
+    lists = [[matrix(*s, seed=i) for i, s in enumerate(shapes)] for shapes in (MIXED, [(64, 64), (20, 100)], [(256, 2304)] * 8 + [(135, 2304)])]
+    want = [orthogonalize(l) for l in lists]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(k):
+        stream = torch.cuda.Stream(device=DEV)
+        with torch.cuda.stream(stream):
+            for i in range(12):
+                got = orthogonalize(lists[(i + k) % 3])
+                bad.extend([(k, i)] * (not all(torch.equal(x, y) for x, y in zip(got, want[(i + k) % 3]))))
+        stream.synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
